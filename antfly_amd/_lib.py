@@ -32,6 +32,7 @@ ERR_TENSOR_NOT_FOUND = -17
 ERR_IO = -18
 
 TYPE_F32, TYPE_Q4_0, TYPE_Q8_0, TYPE_Q4_K = 0, 2, 8, 12
+TYPE_F16, TYPE_BF16 = 1, 30  # of a paged cache and what is attended with it
 ACTIVATION_NONE, ACTIVATION_RELU, ACTIVATION_QUICK_GELU, ACTIVATION_GELU = 0, 1, 2, 3
 LAYOUT_RAW, LAYOUT_PREPARED = 0, 1
 # a launcher's `dispatch` besides a kind (0 .. 3): choose by rows; ... and keep Q4_K on f32 activations everywhere
@@ -71,6 +72,28 @@ class PlannedRequest(C.Structure):
         ("out_dim", C.c_size_t),
         ("operator_plan", OperatorPlan),
     ]
+
+
+class PagedCache(C.Structure):
+    """afhip_paged_cache: blocks of slots of keys and values (strides in elements)."""
+
+    _fields_ = ([("keys", Buffer), ("values", Buffer), ("type", C.c_int)] +
+                [(n, C.c_size_t) for n in ("blocks", "block_size", "kv_heads", "head_dim", "block_stride", "slot_stride",
+                                           "head_stride")])
+
+
+class BatchPlan(C.Structure):
+    _fields_ = ([(n, C.c_size_t) for n in ("requests", "table_columns", "block_size", "blocks", "tokens", "mask_words")] +
+                [(n, Buffer) for n in ("context_lens", "query_lens", "free_blocks", "parents", "block_tables", "query_starts",
+                                       "slots", "positions", "masks", "blocks_taken")])
+
+
+class TreeAttention(C.Structure):
+    _fields_ = ([("cache", PagedCache), ("type", C.c_int), ("scale", C.c_float)] +
+                [(n, C.c_size_t) for n in ("requests", "tokens", "heads", "max_query_len", "max_key_len", "table_columns",
+                                           "mask_words", "query_token_stride", "query_head_stride", "out_token_stride",
+                                           "out_head_stride")] +
+                [(n, Buffer) for n in ("query", "out", "query_starts", "context_lens", "block_tables", "masks")])
 
 
 class DebugStats(C.Structure):
@@ -146,6 +169,15 @@ SIGNATURES = {
     "afhip_launch_gemm_stamps": (_st, [_vp, Buffer, Buffer, Buffer, Buffer, _sz, _sz, _sz]),
     "afhip_launch_rate_probe": (_st, [_vp, _i, _i, _i, Buffer, Buffer]),
     "afhip_rate_probe_wavefronts": (_sz, [_i]),
+    "afhip_launch_quantize_fp8": (_st, [_vp, Buffer, Buffer, Buffer, _sz, _sz]),
+    "afhip_linear_fp8_workspace_bytes": (_sz, [_sz, _sz, _sz]),
+    "afhip_launch_matmul_fp8_f32": (_st, [_vp, Buffer, Buffer, Buffer, Buffer, Buffer, Buffer, Buffer, _i, _sz, _sz, _sz, Buffer]),
+    "afhip_launch_linear_fp8_f32": (_st, [_vp, Buffer, Buffer, Buffer, Buffer, Buffer, Buffer, _i, _sz, _sz, _sz, Buffer]),
+    "afhip_launch_batch_plan": (_st, [_vp, C.POINTER(BatchPlan)]),
+    "afhip_launch_cache_store": (_st, [_vp, C.POINTER(PagedCache), _i, Buffer, Buffer, _sz, _sz, Buffer, _sz]),
+    "afhip_launch_cache_move": (_st, [_vp, C.POINTER(PagedCache), Buffer, _sz, Buffer, Buffer, Buffer, _sz, _sz]),
+    "afhip_tree_attention_workspace_bytes": (_sz, [C.POINTER(TreeAttention)]),
+    "afhip_launch_tree_attention": (_st, [_vp, C.POINTER(TreeAttention), Buffer]),
     "afhip_compute_create": (_st, [C.POINTER(_vp)]),
     "afhip_compute_destroy": (None, [_vp]),
     "afhip_compute_backend_kind": (_i, [_vp]),

@@ -141,6 +141,31 @@ def launchQuantizeRows(stream, tensor_type, dst_raw: Buffer, input: Buffer, rows
                                                 rows if dst_rows is None else dst_rows))
 
 
+def launchQuantizeFp8(stream, q: Buffer, scales: Buffer, input: Buffer, rows, in_dim) -> None:
+    """f32 [rows, in_dim] as e4m3 codes with one f32 scale per row and 128 columns."""
+    check(_lib.lib().afhip_launch_quantize_fp8(stream, q, scales, input, rows, in_dim))
+
+
+def linearFp8WorkspaceBytes(rows: int, in_dim: int, out_dim: int) -> int:
+    return _lib.lib().afhip_linear_fp8_workspace_bytes(rows, in_dim, out_dim)
+
+
+def launchMatmulFp8F32(stream, dst: Buffer, q: Buffer, q_scales: Buffer, weight: Buffer, weight_scales: Buffer, rows, in_dim,
+                       out_dim, bias: Buffer = NO_BUFFER, residual: Buffer = NO_BUFFER, activation: int = 0,
+                       workspace: Buffer = NO_BUFFER) -> None:
+    """Y = act(X @ W^T + bias) + residual, both operands e4m3 codes with f32 scales per block of 128."""
+    check(_lib.lib().afhip_launch_matmul_fp8_f32(stream, dst, q, q_scales, weight, weight_scales, bias, residual, activation,
+                                                 rows, in_dim, out_dim, workspace))
+
+
+def launchLinearFp8F32(stream, dst: Buffer, input: Buffer, weight: Buffer, weight_scales: Buffer, rows, in_dim, out_dim,
+                       bias: Buffer = NO_BUFFER, residual: Buffer = NO_BUFFER, activation: int = 0,
+                       workspace: Buffer = NO_BUFFER) -> None:
+    """The same on f32 activations, quantized within the call; `workspace` of linearFp8WorkspaceBytes bytes."""
+    check(_lib.lib().afhip_launch_linear_fp8_f32(stream, dst, input, weight, weight_scales, bias, residual, activation, rows,
+                                                 in_dim, out_dim, workspace))
+
+
 def launchDecodeFp16(stream, dst_f32: Buffer, src_u16: Buffer, n: int) -> None:
     check(_lib.lib().afhip_launch_decode_fp16(stream, dst_f32, src_u16, n))
 

@@ -59,6 +59,8 @@ const char *afhip_status_string(afhip_status status);
 
 /* GGUF tensor-type ids (gguf/tensor_types.zig). */
 enum afhip_tensor_type { AFHIP_TYPE_F32 = 0, AFHIP_TYPE_Q4_0 = 2, AFHIP_TYPE_Q8_0 = 8, AFHIP_TYPE_Q4_K = 12 };
+/* Two more ids of the same table, for the paged key / value cache and what is attended with it; no linear op takes them. */
+enum afhip_half_type { AFHIP_TYPE_F16 = 1, AFHIP_TYPE_BF16 = 30 };
 /* Q4_K (144-byte super-blocks of 256 weights) is computed on f32 activations against the
  * dequantized weights, as the engine does on the CPU (ops/native_compute.zig:31075-31144)
  * and in its CUDA backend (ops/cuda/cuda_compute.zig:708) -- except on the CPU engine's gated
@@ -340,6 +342,132 @@ afhip_status afhip_launch_block_dots(void *stream, int tensor_type, int layout, 
 /* fp16 -> f32 of n little-endian halves with the device's conversion
  * (gguf/quant_codec.zig:35-39).  Parity probe for subnormal scales. */
 afhip_status afhip_launch_decode_fp16(void *stream, afhip_buffer dst_f32, afhip_buffer src_u16, size_t n);
+
+/* ------------------------------------------------------------------------
+ * Matrix product in 8-bit floating point (e4m3: 4 exponent and 3 mantissa bits, finite up to 448) with one f32 scale
+ * per block of 128.  No counterpart in the reference.
+ *
+ *   weight         e4m3 [out_dim][in_dim], row-major;  weight_scales f32 [ceil(out_dim / 128)][ceil(in_dim / 128)]:
+ *                  the value of weight[o][k] is its code's times weight_scales[o / 128][k / 128]
+ *   activations    e4m3 [rows][in_dim];  scales f32 [rows][ceil(in_dim / 128)]
+ *
+ *   Y[r][o] = sum over blocks b of  x_scale[r][b] * weight_scale[o / 128][b] * (sum over k in b of  x[r][k] * w[o][k])
+ *
+ * with every sum in f32.  in_dim is a non-zero multiple of 16 (the last block may be shorter than 128), out_dim and rows
+ * are any numbers (rows up to 2^20 - 16, else AFHIP_ERR_OP_UNSUPPORTED); everything is contiguous; codes and f32 activations are 16-byte aligned, the other
+ * buffers 4-byte (else AFHIP_ERR_INVALID_STATE).  rows * out_dim == 0 is a successful no-op.  Results must not overlap
+ * what is read, except that the residual may be Y itself.
+ * ---------------------------------------------------------------------- */
+#define AFHIP_FP8_BLOCK 128
+/* f32 [rows][in_dim] -> codes and scales: with m the largest |x| of a row's block, at least 2^-100,
+ * scale = m / 448 and code = e4m3(x * (448 / m)), f32 operations rounded to nearest, ties to even; a value that is no
+ * number stays one, and an infinite one makes its block's values no numbers. */
+afhip_status afhip_launch_quantize_fp8(void *stream, afhip_buffer q, afhip_buffer scales, afhip_buffer input, size_t rows,
+                                       size_t in_dim);
+/* Scratch of the two products below, 256-byte aligned.  afhip_launch_matmul_fp8_f32 runs with less or none (then K is not
+ * shared out over workgroups: the same sums in another order); afhip_launch_linear_fp8_f32 refuses less. */
+size_t afhip_linear_fp8_workspace_bytes(size_t rows, size_t in_dim, size_t out_dim);
+/* Y = act(X W^T + bias) + residual on activations that are codes already (several projections of one input quantize it
+ * once).  bias f32 [out_dim] and residual f32 [rows][out_dim] are optional (.ptr == 0); activation: afhip_activation. */
+afhip_status afhip_launch_matmul_fp8_f32(void *stream, afhip_buffer dst, afhip_buffer q, afhip_buffer q_scales,
+                                         afhip_buffer weight, afhip_buffer weight_scales, afhip_buffer bias,
+                                         afhip_buffer residual, int activation, size_t rows, size_t in_dim, size_t out_dim,
+                                         afhip_buffer workspace);
+/* The same on f32 activations: quantized as by afhip_launch_quantize_fp8, in the product's own launch where the rows are
+ * few, into the workspace otherwise. */
+afhip_status afhip_launch_linear_fp8_f32(void *stream, afhip_buffer dst, afhip_buffer input, afhip_buffer weight,
+                                         afhip_buffer weight_scales, afhip_buffer bias, afhip_buffer residual,
+                                         int activation, size_t rows, size_t in_dim, size_t out_dim,
+                                         afhip_buffer workspace);
+
+/* ------------------------------------------------------------------------
+ * A paged key / value cache and what a speculative decode step does with it: plan the batch, store the drafted tokens'
+ * keys and values, attend over context and draft tree, move the accepted path behind the context.  The engine's own
+ * cache is host code (runtime/kv); these take device buffers only, never wait and allocate nothing.
+ *
+ * The cache holds `blocks` blocks of `block_size` slots; a slot holds one token's key (value) of `head_dim` values for
+ * each of `kv_heads` heads.  Key d of head h in slot s of block b is keys[b * block_stride + s * slot_stride +
+ * h * head_stride + d] (strides in elements, so blocks may hold slots of heads or heads of slots).  A token's slot
+ * number is b * block_size + s.  A request's block table row names the blocks of its tokens 0 .. block_size - 1,
+ * block_size .. 2 block_size - 1, and so on; -1 (and any number outside [0, blocks)) names none.
+ * head_dim and the strides are multiples of 8, keys and values 16-byte aligned; blocks * block_size < 2^31, and a cache
+ * tensor spans less than 64 GiB (else AFHIP_ERR_INVALID_STATE; a type other than F16 / BF16 ->
+ * AFHIP_ERR_UNSUPPORTED_TENSOR_TYPE).
+ * All int32 / uint64 arrays are device memory, aligned to their element.
+ * ---------------------------------------------------------------------- */
+typedef struct afhip_paged_cache {
+    afhip_buffer keys, values;
+    int type; /* AFHIP_TYPE_F16 or AFHIP_TYPE_BF16 */
+    size_t blocks, block_size, kv_heads, head_dim;
+    size_t block_stride, slot_stride, head_stride;
+} afhip_paged_cache;
+
+/* The plan of a batch, from the lengths of its requests: request r holds context_lens[r] cached tokens and brings
+ * query_lens[r] new ones.  Its new tokens take the positions behind its context, and where these need blocks that it does
+ * not own yet (it owns the first ceil(context_lens[r] / block_size) of its row), the next ones of `free_blocks`, in
+ * request order.  Written in one launch:
+ *   block_tables  int32 [requests][table_columns], read and written: the new blocks' entries; others stay
+ *   query_starts  int32 [requests + 1]: where a request's tokens begin among all new ones, and their number
+ *   slots         int32 [tokens]: each new token's slot, -1 where there is none (a table row or the free list too short,
+ *                 a table entry that is -1) and past the batch's tokens
+ *   positions     int32 [tokens]: context_lens[r] plus the token's depth in its tree (its index without parents); -1 past
+ *                 the batch's tokens
+ *   masks         uint64 [tokens][mask_words], optional: bit p of a token's words says that it sees token p of its
+ *                 request: itself and its ancestors (without parents: itself and the tokens before it); 0 past the batch
+ *   blocks_taken  int32 [1]: the blocks that the batch needs from the list (more than it holds: the batch does not fit)
+ * parents, int32 [tokens], optional: the index within its request of the draft that a token follows, -1 behind the
+ * context; an index that is not smaller than the token's own counts as -1.  At most mask_words * 64 (without masks:
+ * 1024) tokens of a request are walked; later ones see nothing of their tree and keep depth 0.
+ * Lengths below zero count as zero.  requests <= 8192, mask_words <= 16, else AFHIP_ERR_OP_UNSUPPORTED.  `tokens` is the
+ * capacity of the token arrays: a batch of more tokens has the rest left out (query_starts still holds the sums, which
+ * have to stay below 2^31).  The same call again gives the same result: the free list is not changed. */
+typedef struct afhip_batch_plan {
+    size_t requests, table_columns, block_size, blocks, tokens, mask_words;
+    afhip_buffer context_lens, query_lens, free_blocks, parents;
+    afhip_buffer block_tables, query_starts, slots, positions, masks, blocks_taken;
+} afhip_batch_plan;
+afhip_status afhip_launch_batch_plan(void *stream, const afhip_batch_plan *plan);
+
+/* Keys and values of `tokens` new tokens into their slots: type F32, F16 or BF16 (converted to the cache's type, to
+ * nearest, ties to even), [tokens][kv_heads][head_dim] with the given strides (elements; multiples of 4 for F32 and of 8
+ * otherwise, 16-byte aligned).  A slot outside the cache writes nothing; two tokens of one slot race. */
+afhip_status afhip_launch_cache_store(void *stream, const afhip_paged_cache *cache, int type, afhip_buffer keys,
+                                      afhip_buffer values, size_t token_stride, size_t head_stride, afhip_buffer slots,
+                                      size_t tokens);
+/* After a verification: for i = 0 .. path_lens[r] - 1 in this order, the cache's token at position
+ * context_lens[r] + paths[r][i] becomes the one at context_lens[r] + i.  paths int32 [requests][path_columns] with
+ * paths[r][i] >= i, ascending (a tree's path from its root).  Steps whose index is negative, or whose slots the table does
+ * not name, move nothing. */
+afhip_status afhip_launch_cache_move(void *stream, const afhip_paged_cache *cache, afhip_buffer block_tables,
+                                     size_t table_columns, afhip_buffer context_lens, afhip_buffer paths,
+                                     afhip_buffer path_lens, size_t requests, size_t path_columns);
+
+/* Attention of every request's new tokens over the cache.  Token t of request r (row query_starts[r] + t of query) sees
+ * the context_lens[r] cached tokens, and new token p of its request (cached at position context_lens[r] + p) where bit p of
+ * its mask words is set; without masks, where p <= t.  Head h reads key head h / (heads / kv_heads).
+ *
+ *   out[t][h] = sum over seen j of  softmax_j(scale * q[t][h] . k[j]) v[j],   zero where nothing is seen
+ *
+ * What is not seen does not count, whatever it holds (an infinity or no number included).  query and out: F32, or the
+ * cache's own type; [tokens][heads][head_dim] with strides in elements (multiples of 4 for F32, of 8 otherwise; 16-byte
+ * aligned).  F32 queries keep their bits (they are multiplied as two or three terms of the cache's type) and so do the
+ * softmax's weights (two terms); 16-bit queries take one term of each.  Sums are f32.
+ * max_query_len and max_key_len bound what the batch holds (new tokens; context plus new tokens) and choose the launch's
+ * shape; tokens past the first and keys past the second are left out.  A key whose block the table does not name is not
+ * seen.  head_dim <= 256, heads a multiple of kv_heads, mask_words <= 16, max_key_len * block_size < 2^32, else
+ * AFHIP_ERR_OP_UNSUPPORTED.
+ * `workspace` (256-byte aligned, afhip_tree_attention_workspace_bytes) holds the parts of rows whose keys are shared out
+ * over workgroups; less than asked for is refused (AFHIP_ERR_INVALID_STATE). */
+typedef struct afhip_tree_attention {
+    afhip_paged_cache cache;
+    int type; /* of query and out */
+    float scale;
+    size_t requests, tokens, heads, max_query_len, max_key_len, table_columns, mask_words;
+    size_t query_token_stride, query_head_stride, out_token_stride, out_head_stride;
+    afhip_buffer query, out, query_starts, context_lens, block_tables, masks;
+} afhip_tree_attention;
+size_t afhip_tree_attention_workspace_bytes(const afhip_tree_attention *attention);
+afhip_status afhip_launch_tree_attention(void *stream, const afhip_tree_attention *attention, afhip_buffer workspace);
 
 /* ------------------------------------------------------------------------
  * Backend object: ops/cuda/cuda_compute.zig (CudaCompute + the ComputeBackend
