@@ -12,9 +12,11 @@
 // keys 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3).  V comes row-major and is needed column-major: it goes through LDS and
 // is read with the transposing ds_read_b64_tr_b16.  K goes from memory into the operand registers, no LDS.
 //
-// A wavefront works alone on tiles of 32 keys (its own part of LDS, no barrier in the loop); the four wavefronts of a
-// workgroup take tiles in turn and add up at the end.  Few rows on long contexts are split over workgroups as well, and a
-// second kernel joins the parts.
+// Keys and values of a tile of 32 keys come from memory straight into LDS (no registers in between), the next tile's while
+// this one is worked on.  A workgroup's four wavefronts are kKeyGroups groups that take tiles in turn; the wavefronts of one
+// group share its tiles and have 16 kQ rows each.  Few rows: four groups that need no barrier in the loop and add up at the
+// end; many rows: one group, every key read once for 128 rows.  Few rows on long contexts are split over workgroups as well,
+// and a second kernel joins the parts.
 #include "paged_launch.h"
 
 #include <hip/hip_runtime.h>
@@ -113,19 +115,52 @@ __device__ __forceinline__ uint32_t seen_bits(int first, int context, int token,
     return static_cast<uint32_t>(bits);
 }
 
-// kDim: the head's values, rounded up to a size that is here (the rest are zeros that are not read).  kF32: query and out
-// are f32.  kQ: sixteens of rows.
-template <int kDim, bool kBf16, bool kF32, int kQ>
-__global__ __launch_bounds__(kThreads) void tree_attention_kernel(TreeAttentionArgs a, uint32_t row_tiles, uint32_t splits,
+// Whether one of the two values of a register is no finite number.
+template <bool kBf16>
+__device__ __forceinline__ bool is_odd(uint32_t w) {
+    constexpr uint32_t kExponent = kBf16 ? 0x7F80u : 0x7C00u;
+    return (w & kExponent) == kExponent || (w >> 16 & kExponent) == kExponent;
+}
+template <bool kBf16>
+__device__ __forceinline__ bool is_odd(short v) {
+    constexpr short kExponent = kBf16 ? 0x7F80 : 0x7C00;
+    return (v & kExponent) == kExponent;
+}
+
+__device__ const uint4 kNothing{0, 0, 0, 0};  // what keys without a place and values past a head's end are loaded from
+
+// 16 bytes a lane from memory to 1 KiB of LDS from `to` on (a uniform address).
+__device__ __forceinline__ void load_to_lds(uint32_t to, const uint4* from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "memory", "m0");
+}
+
+// Where 16-byte piece `piece` of row `row` of a tile lies in LDS, in pieces.  The pieces of a row are in an order of its own,
+// so that the same piece of 16 rows (what the lanes of an operand read) falls on all banks: 256 bytes of them.
+template <int kDim>
+__device__ __forceinline__ int lds_piece(int row, int piece) {
+    constexpr int kPieces = kDim / 8;
+    return row * kPieces + (kPieces == 8 ? piece ^ (row >> 1 & 7) : piece ^ (row & 15));
+}
+
+template <int kDim, int kQ, int kKeyGroups>
+constexpr size_t attention_lds_bytes() {
+    constexpr int kRows = 16 * kQ * (kWaves / kKeyGroups);
+    constexpr size_t tiles = static_cast<size_t>(kKeyGroups) * 2 * 2 * kTile * kDim * 2;
+    constexpr size_t sums = kKeyGroups == 1 ? 0 : static_cast<size_t>(kKeyGroups) * kRows * ((kDim + 4) * sizeof(float) + sizeof(Part));
+    return tiles > sums ? tiles : sums;
+}
+
+// kDim: the head's values, rounded up to a size that is here (the rest are zeros).  kF32: query and out are f32.
+template <int kDim, bool kBf16, bool kF32, int kQ, int kKeyGroups>
+__global__ __launch_bounds__(kThreads, kF32 ? 1 : 2) void tree_attention_kernel(TreeAttentionArgs a, uint32_t row_tiles, uint32_t splits,
                                                                  uint32_t split_keys, float* part_out, Part* parts) {
     constexpr int kSteps = kDim / 32;                            // products of K Q^T along the head
-    constexpr int kTerms = kF32 ? (kBf16 ? 3 : 2) : 1;           // of a query value: 24 bits of three bf16, 22 of two f16
-    constexpr int kParts = kTerms;                               // of a weight
-    constexpr int kRows = 16 * kQ;
-    constexpr int kRowBytes = kDim * 2 + 32;  // of V in LDS: four rows of a lane group and the four groups fall on other banks
-    constexpr int kLoads = kTile * kDim / 8 / 64;                // 16-byte loads of V a lane
-    constexpr int kChunks = kDim / 8;                            // 16-byte parts of a row
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int kTerms = kF32 ? (kBf16 ? 3 : 2) : 1;           // of a query value or a weight: 24 bits of three bf16, 22 of two f16
+    constexpr int kRowGroups = kWaves / kKeyGroups, kRows = 16 * kQ * kRowGroups;
+    constexpr int kPieces = kDim / 8;                            // 16-byte pieces of a row
+    constexpr int kTileBytes = kTile * kDim * 2;                 // of K, and of V behind it
+    constexpr int kLoads = kTile * kPieces / 64 / kRowGroups;    // of a wavefront, 1 KiB each, for K and for V
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
 
     // the row tiles of a key head's split lie on one XCD (workgroups go round them in turn): they share its L2
     const uint32_t item = (blockIdx.x >> 3) / row_tiles * 8 + (blockIdx.x & 7), row_tile = (blockIdx.x >> 3) % row_tiles;
@@ -147,11 +182,14 @@ __global__ __launch_bounds__(kThreads) void tree_attention_kernel(TreeAttentionA
     const int key_begin = static_cast<int>(min(static_cast<unsigned long long>(split) * split_keys, static_cast<unsigned long long>(keys)));
     const int key_end = static_cast<int>(min(static_cast<unsigned long long>(key_begin) + split_keys, static_cast<unsigned long long>(keys)));
 
-    const int tid = static_cast<int>(threadIdx.x), wave = tid >> 6, lane = tid & 63, column = lane & 15, quarter = lane >> 4;
-    char* v_lds = lds + wave * (kTile * kRowBytes);
+    const int tid = static_cast<int>(threadIdx.x), wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int column = lane & 15, quarter = lane >> 4;
+    const int key_group = wave / kRowGroups, row_group = wave % kRowGroups;
+    char* const tiles = lds + key_group * (4 * kTileBytes);
+    const uint32_t tiles_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)tiles));
     const int* table = a.block_tables + static_cast<size_t>(request) * a.table_columns;
     const uint32_t head_at = kv_head * a.cache.head_stride;
-    const int chunks = static_cast<int>(a.cache.head_dim / 8);  // that hold something
+    const int pieces = static_cast<int>(a.cache.head_dim / 8);  // that hold something
 
     // where a key's values lie, in 16-byte units
     auto place = [&](int key) -> uint32_t {
@@ -161,36 +199,56 @@ __global__ __launch_bounds__(kThreads) void tree_attention_kernel(TreeAttentionA
         if (block >= a.cache.blocks) return kNowhere;
         return block * a.cache.block_stride + (static_cast<uint32_t>(key) - col * a.block_size.by) * a.cache.slot_stride + head_at;
     };
+    // this wavefront's part of a tile's K and V; `at`: lane l % 32 has the place of key l % 32
+    auto request_tile = [&](uint32_t at, int stage) {
+        const uint32_t to = tiles_at + stage * (2 * kTileBytes) + row_group * (kLoads * 1024);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int slot = (row_group * kLoads + i) * 64 + lane, row = slot / kPieces, piece = lds_piece<kDim>(row, slot % kPieces) % kPieces;
+            const uint32_t from = static_cast<uint32_t>(__shfl(static_cast<int>(at), row));
+            const bool there = from != kNowhere && piece < pieces;
+            load_to_lds(to + i * 1024, there ? a.cache.keys + from + piece : &kNothing);
+            load_to_lds(to + kTileBytes + i * 1024, there ? a.cache.values + from + piece : &kNothing);
+        }
+    };
+    const int step = kKeyGroups * kTile, first_tile = key_begin + key_group * kTile;
+    uint32_t at = place(first_tile + (lane & 31));
+    request_tile(at, 0);
+    uint32_t at_next = place(first_tile + step + (lane & 31));
 
     // ---- the rows
     s16x8 query[kQ][kSteps][kTerms];
-    float unit[kQ];  // what a product of the row is multiplied by: scale, log2(e), and for f32 on f16 the row's power of two
+    float unit[kQ];  // what a product of the row is multiplied by: |scale|, log2(e), and for f32 on f16 the row's power of two
     const unsigned long long* words[kQ];
     int row_token[kQ];
     bool real[kQ];
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale turns the queries round
 #pragma unroll
     for (int qt = 0; qt < kQ; ++qt) {
-        const int row = first_row + qt * 16 + column;
+        const int row = first_row + (row_group * kQ + qt) * 16 + column;
         real[qt] = row < rows;
         row_token[qt] = real[qt] ? row / group : 0;
         const int head = static_cast<int>(kv_head) * group + (real[qt] ? row % group : 0);
         const size_t token = static_cast<size_t>(begin + row_token[qt]);
         words[qt] = a.masks != nullptr ? a.masks + token * a.mask_words : nullptr;
-        unit[qt] = a.scale * kLog2e;
-        const size_t at = token * a.query_token_stride + static_cast<size_t>(head) * a.query_head_stride;
+        unit[qt] = fmaxf(__builtin_fabsf(a.scale) * kLog2e, 1e-30f);  // (never 0, which would make minus infinity no number)
+        const size_t from = token * a.query_token_stride + static_cast<size_t>(head) * a.query_head_stride;
         if (kF32) {
             float v[kSteps][8];
             float most = 0.0f;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
-                const int chunk = s * 4 + quarter;
-                const bool held = real[qt] && chunk < chunks;
-                const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.query) + at) + 2 * chunk;
+                const int piece = s * 4 + quarter;
+                const bool held = real[qt] && piece < pieces;
+                const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.query) + from) + 2 * piece;
                 const float4 x = held ? p[0] : float4{0, 0, 0, 0}, y = held ? p[1] : float4{0, 0, 0, 0};
                 v[s][0] = x.x; v[s][1] = x.y; v[s][2] = x.z; v[s][3] = x.w;
                 v[s][4] = y.x; v[s][5] = y.y; v[s][6] = y.z; v[s][7] = y.w;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) most = fmaxf(most, __builtin_fabsf(v[s][j]));
+                for (int j = 0; j < 8; ++j) {
+                    if (flip != 0) v[s][j] = -v[s][j];
+                    most = fmaxf(most, __builtin_fabsf(v[s][j]));
+                }
             }
             if (!kBf16) {  // f16 has 5 exponent bits: the row's largest value goes to [0.5, 1)
                 most = row_max(most);
@@ -218,16 +276,17 @@ __global__ __launch_bounds__(kThreads) void tree_attention_kernel(TreeAttentionA
         } else {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
-                const int chunk = s * 4 + quarter;
-                const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.query) + at) + chunk;
-                const uint4 raw = real[qt] && chunk < chunks ? *p : uint4{0, 0, 0, 0};
+                const int piece = s * 4 + quarter;
+                const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.query) + from) + piece;
+                uint4 raw = real[qt] && piece < pieces ? *p : uint4{0, 0, 0, 0};
+                raw = uint4{raw.x ^ flip, raw.y ^ flip, raw.z ^ flip, raw.w ^ flip};
                 query[qt][s][0] = __builtin_bit_cast(s16x8, raw);
             }
         }
     }
 
     f32x4 out[kQ][kDim / 16];
-    float most[kQ], sum[kQ];
+    float most[kQ], sum[kQ];  // the largest product so far (before `unit`), and this lane's part of the weights' sum
 #pragma unroll
     for (int qt = 0; qt < kQ; ++qt) {
         most[qt] = -__builtin_inff();
@@ -237,111 +296,76 @@ __global__ __launch_bounds__(kThreads) void tree_attention_kernel(TreeAttentionA
     }
 
     // ---- the keys
-    uint4 key_regs[2][kSteps], value_regs[kLoads];
-    auto load = [&](uint32_t at) {  // `at`: lane l % 32 has the place of key l % 32
+    int stage = 0;
+    for (int first = key_begin; first < key_end; first += step, stage ^= 1) {
+        const int tile = first + key_group * kTile;
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // this wavefront's part of the tile is there
+        if (kRowGroups > 1) __syncthreads();                // everyone's is, and the other stage has been read
+        const uint32_t at_now = at;
+        at = at_next;
+        if (tile + step < key_end) {
+            request_tile(at, stage ^ 1);
+            at_next = place(tile + 2 * step + (lane & 31));
+        }
+        if (tile >= key_end) continue;
+        const char* k_lds = tiles + stage * (2 * kTileBytes);
+        char* v_lds = tiles + stage * (2 * kTileBytes) + kTileBytes;
+
+        const uint32_t held = static_cast<uint32_t>(__ballot(at_now != kNowhere));  // keys of the tile that have a place
+        const bool clean = tile + kTile <= context && held == ~0u;                   // every row sees every key
+
+        f32x4 score[kQ][2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const uint32_t from = static_cast<uint32_t>(__shfl(static_cast<int>(at), half * 16 + column));
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
-                const int chunk = s * 4 + quarter;
-                const uint4 zero{0, 0, 0, 0};
-                key_regs[half][s] = from != kNowhere && chunk < chunks ? a.cache.keys[static_cast<size_t>(from) + chunk] : zero;
+                const s16x8 k = *reinterpret_cast<const s16x8*>(k_lds + lds_piece<kDim>(half * 16 + column, s * 4 + quarter) * 16);
+#pragma unroll
+                for (int qt = 0; qt < kQ; ++qt) {
+#pragma unroll
+                    for (int term = kTerms - 1; term >= 0; --term)  // the small terms first
+                        score[qt][half] = mfma<kBf16>(k, query[qt][s][term], s == 0 && term == kTerms - 1 ? f32x4{0, 0, 0, 0} : score[qt][half]);
+                }
             }
         }
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int slot = i * 64 + lane, chunk = slot % kChunks;
-            const uint32_t from = static_cast<uint32_t>(__shfl(static_cast<int>(at), slot / kChunks));
-            const uint4 zero{0, 0, 0, 0};
-            value_regs[i] = from != kNowhere && chunk < chunks ? a.cache.values[static_cast<size_t>(from) + chunk] : zero;
-        }
-    };
-    int tile = key_begin + wave * kTile;
-    uint32_t at = place(tile + (lane & 31));
-    load(at);
-    uint32_t at_next = place(tile + kWaves * kTile + (lane & 31));
-    for (; tile < key_end; tile += kWaves * kTile) {
-        const uint32_t held = static_cast<uint32_t>(__ballot(at != kNowhere));  // keys of the tile that have a place
-        const bool clean = tile + kTile <= context && held == ~0u;               // every row sees every key
         uint32_t odd = 0;  // keys with a value that is no finite number (looked for only where some row may not see them)
+        uint32_t seen[kQ];
         if (!clean) {
-            constexpr uint32_t kExponent = kBf16 ? 0x7F80u : 0x7C00u;
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                uint32_t* w = reinterpret_cast<uint32_t*>(&value_regs[i]);
-                bool found = false;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if ((w[j] & kExponent) == kExponent) {
-                        found = true;
-                        w[j] &= 0xFFFF0000u;
-                    }
-                    if ((w[j] >> 16 & kExponent) == kExponent) {
-                        found = true;
-                        w[j] &= 0x0000FFFFu;
-                    }
-                }
-                unsigned long long which = __ballot(found);
+            for (int slot = lane; slot < kTile * kPieces; slot += 64) {
+                const uint4 v = *reinterpret_cast<const uint4*>(v_lds + slot * 16);
+                unsigned long long which = __ballot(is_odd<kBf16>(v.x) || is_odd<kBf16>(v.y) || is_odd<kBf16>(v.z) || is_odd<kBf16>(v.w));
                 while (which != 0) {
                     const int l = __builtin_ctzll(which);
                     which &= which - 1;
-                    odd |= 1u << ((i * 64 + l) / kChunks);
+                    odd |= 1u << __builtin_amdgcn_readlane(slot / kPieces, l);
+                }
+            }
+#pragma unroll
+            for (int qt = 0; qt < kQ; ++qt) {
+                seen[qt] = real[qt] ? seen_bits(tile, context, row_token[qt], words[qt], static_cast<int>(a.mask_words)) & held : 0u;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if ((seen[qt] >> (half * 16 + quarter * 4 + j) & 1) == 0) score[qt][half][j] = -__builtin_inff();
+                    }
                 }
             }
         }
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int slot = i * 64 + lane;
-            *reinterpret_cast<uint4*>(v_lds + slot / kChunks * kRowBytes + slot % kChunks * 16) = value_regs[i];
-        }
-        f32x4 score[kQ][2];
-#pragma unroll
-        for (int qt = 0; qt < kQ; ++qt) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                score[qt][half] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-                    for (int term = kTerms - 1; term >= 0; --term)  // the small terms first
-                        score[qt][half] = mfma<kBf16>(__builtin_bit_cast(s16x8, key_regs[half][s]), query[qt][s][term], score[qt][half]);
-                }
-            }
-        }
-        const uint32_t at_now = at;
-        at = at_next;
-        if (tile + kWaves * kTile < key_end) {
-            load(at);
-            at_next = place(tile + 2 * kWaves * kTile + (lane & 31));
-        }
-
         float peak[kQ];
         bool passes = false;
-        uint32_t seen[kQ];
 #pragma unroll
         for (int qt = 0; qt < kQ; ++qt) {
-            seen[qt] = ~0u;
-            if (!clean) seen[qt] = real[qt] ? seen_bits(tile, context, row_token[qt], words[qt], static_cast<int>(a.mask_words)) & held : 0u;
-            peak[qt] = -__builtin_inff();
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float x = score[qt][half][j] * unit[qt];
-                    if (!clean && (seen[qt] >> (half * 16 + quarter * 4 + j) & 1) == 0) x = -__builtin_inff();
-                    score[qt][half][j] = x;
-                    peak[qt] = fmaxf(peak[qt], x);
-                }
-            }
-            peak[qt] = row_max(peak[qt]);
-            passes |= peak[qt] > most[qt] + kSlack;
+            const f32x4 x = score[qt][0], y = score[qt][1];
+            peak[qt] = row_max(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]))));
+            passes |= (peak[qt] - most[qt]) * unit[qt] > kSlack;
         }
         if (__any(passes)) {
 #pragma unroll
             for (int qt = 0; qt < kQ; ++qt) {
-                const float next = peak[qt] > most[qt] + kSlack ? peak[qt] : most[qt];  // each row by itself: no other row's keys move its bits
-                const float by = exp2_between(most[qt], next);
+                // each row by itself: no other row's keys move its bits
+                const float next = (peak[qt] - most[qt]) * unit[qt] > kSlack ? peak[qt] : most[qt];
+                const float by = most[qt] == next ? 1.0f : __builtin_amdgcn_exp2f((most[qt] - next) * unit[qt]);
                 most[qt] = next;
                 sum[qt] *= by;
 #pragma unroll
@@ -351,21 +375,19 @@ __global__ __launch_bounds__(kThreads) void tree_attention_kernel(TreeAttentionA
                 }
             }
         }
-        s16x8 weight[kQ][kParts];
-        float weights[kQ][8];
+        s16x8 weight[kQ][kTerms];
 #pragma unroll
         for (int qt = 0; qt < kQ; ++qt) {
-            const float from = most[qt] == -__builtin_inff() ? 0.0f : most[qt];
+            const float from = most[qt] == -__builtin_inff() ? 0.0f : -most[qt] * unit[qt];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float p = __builtin_amdgcn_exp2f(score[qt][j >> 2][j & 3] - from);
-                weights[qt][j] = p;
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(score[qt][j >> 2][j & 3], unit[qt], from));
                 sum[qt] += p;
                 float rest = p;
 #pragma unroll
-                for (int part = 0; part < kParts; ++part) {
-                    weight[qt][part][j] = narrow<kBf16>(rest);
-                    rest -= widen<kBf16>(weight[qt][part][j]);
+                for (int term = 0; term < kTerms; ++term) {
+                    weight[qt][term][j] = narrow<kBf16>(rest);
+                    if (term + 1 < kTerms) rest -= widen<kBf16>(weight[qt][term][j]);
                 }
             }
         }
@@ -375,111 +397,65 @@ __global__ __launch_bounds__(kThreads) void tree_attention_kernel(TreeAttentionA
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int row = half * 16 + quarter * 4 + (column >> 2);
-                const char* from = v_lds + row * kRowBytes + d * 32 + (column & 3) * 8;
+                const char* from = v_lds + lds_piece<kDim>(row, d * 2 + (column >> 1 & 1)) * 16 + (column & 1) * 8;
                 const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)from);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[half * 4 + j] = four[j];
             }
+            if (odd != 0) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = is_odd<kBf16>(static_cast<short>(v[j])) ? static_cast<short>(0) : v[j];
+            }
 #pragma unroll
             for (int qt = 0; qt < kQ; ++qt) {
 #pragma unroll
-                for (int part = kParts - 1; part >= 0; --part) out[qt][d] = mfma<kBf16>(v, weight[qt][part], out[qt][d]);
+                for (int term = kTerms - 1; term >= 0; --term) out[qt][d] = mfma<kBf16>(v, weight[qt][term], out[qt][d]);
             }
         }
         // A row that does not see a key must not get 0 * inf from it: the products above took such values as zeros, and the
-        // rows that see them add them here, one by one.
+        // rows that see them add them here, key by key.
         while (odd != 0) {
             const int key = __builtin_ctz(odd);
             odd &= odd - 1;
-            const uint32_t from = static_cast<uint32_t>(__shfl(static_cast<int>(at_now), key));
             const int holder = key % 16 / 4, index = key / 16 * 4 + key % 4;
 #pragma unroll
             for (int qt = 0; qt < kQ; ++qt) {
                 float p = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float other = __shfl(weights[qt][j], holder * 16 + column);
+                    const float other = __shfl(widen<kBf16>(weight[qt][0][j]), holder * 16 + column);
                     if (j == index) p = other;
                 }
                 if ((seen[qt] >> key & 1) == 0) continue;
 #pragma unroll
                 for (int d = 0; d < kDim / 16; ++d) {
+                    const char* from = v_lds + lds_piece<kDim>(key, d * 2 + (quarter >> 1)) * 16 + (quarter & 1) * 8;
+                    const s16x4 four = *reinterpret_cast<const s16x4*>(from);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const int dim = d * 16 + quarter * 4 + j;
-                        if (dim >= chunks * 8) continue;
-                        const float v = widen<kBf16>(reinterpret_cast<const short*>(a.cache.values)[static_cast<size_t>(from) * 8 + dim]);
-                        if (!(__builtin_fabsf(v) < __builtin_inff())) out[qt][d][j] = __builtin_fmaf(p, v, out[qt][d][j]);
+                        if (is_odd<kBf16>(static_cast<short>(four[j]))) out[qt][d][j] = __builtin_fmaf(p, widen<kBf16>(four[j]), out[qt][d][j]);
                     }
                 }
             }
         }
     }
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // (of a workgroup without keys: its first request)
 
-    // ---- the four wavefronts' sums
-#pragma unroll
-    for (int qt = 0; qt < kQ; ++qt) sum[qt] = row_sum(sum[qt]);
-    constexpr int kPitch = kDim + 4;                       // floats of a row in LDS
-    float* sums = reinterpret_cast<float*>(lds);           // [2][kRows][kPitch]
-    Part* wave_parts = reinterpret_cast<Part*>(sums + 2 * kRows * kPitch);  // [kWaves][kRows]
-    __syncthreads();  // V is done with
-    if (quarter == 0) {
-#pragma unroll
-        for (int qt = 0; qt < kQ; ++qt) wave_parts[wave * kRows + qt * 16 + column] = Part{most[qt], sum[qt]};
-    }
-    __syncthreads();
+    // ---- the key groups' sums, and out: four values a lane
+    float all[kQ];  // the row's maximum in units of log2
 #pragma unroll
     for (int qt = 0; qt < kQ; ++qt) {
-        float all = -__builtin_inff();
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) all = fmaxf(all, wave_parts[w * kRows + qt * 16 + column].most);
-        const float by = exp2_between(most[qt], all);
-#pragma unroll
-        for (int d = 0; d < kDim / 16; ++d) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) out[qt][d][j] *= by;
-        }
+        sum[qt] = row_sum(sum[qt]);
+        all[qt] = most[qt] == -__builtin_inff() ? most[qt] : most[qt] * unit[qt];
     }
-    auto cell = [&](int region, int qt, int d) {
-        return reinterpret_cast<f32x4*>(sums + (region * kRows + qt * 16 + column) * kPitch + d * 16 + quarter * 4);
-    };
-#pragma unroll
-    for (int round = 0; round < 2; ++round) {  // wavefronts 2 and 3 to 0 and 1, then 0 and 1 side by side
-        if (round == 0 ? wave >= 2 : wave < 2) {
-#pragma unroll
-            for (int qt = 0; qt < kQ; ++qt) {
-#pragma unroll
-                for (int d = 0; d < kDim / 16; ++d) *cell(wave & 1, qt, d) = out[qt][d];
-            }
-        }
-        __syncthreads();
-        if (round == 0 && wave < 2) {
-#pragma unroll
-            for (int qt = 0; qt < kQ; ++qt) {
-#pragma unroll
-                for (int d = 0; d < kDim / 16; ++d) out[qt][d] += *cell(wave, qt, d);
-            }
-        }
-        // (a wavefront writes only the region it alone has read: no barrier between)
-    }
-
-    // ---- out: four values a thread
-    constexpr int kFours = kDim / 4;
-    for (int i = tid; i < kRows * kFours; i += kThreads) {
-        const int r = i / kFours, d = i % kFours * 4, row = first_row + r;
-        if (row >= rows || d >= chunks * 8) continue;
-        const f32x4 x = *reinterpret_cast<const f32x4*>(sums + r * kPitch + d) + *reinterpret_cast<const f32x4*>(sums + (kRows + r) * kPitch + d);
-        float all = -__builtin_inff(), total = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) all = fmaxf(all, wave_parts[w * kRows + r].most);
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) total += wave_parts[w * kRows + r].sum * exp2_between(wave_parts[w * kRows + r].most, all);
+    auto put = [&](int row, int d, f32x4 x, float highest, float total) {
+        if (row >= rows || d >= pieces * 8) return;
         const size_t token = static_cast<size_t>(begin + row / group);
         const int head = static_cast<int>(kv_head) * group + row % group;
         if (splits > 1) {
             const size_t index = (static_cast<size_t>(split) * a.tokens + token) * a.heads + head;
             *reinterpret_cast<f32x4*>(part_out + index * a.cache.head_dim + d) = x;
-            if (d == 0) parts[index] = Part{all, total};
+            if (d == 0) parts[index] = Part{highest, total};
         } else {
             const size_t to = token * a.out_token_stride + static_cast<size_t>(head) * a.out_head_stride + d;
             const float by = total == 0.0f ? 0.0f : 1.0f / total;
@@ -492,6 +468,44 @@ __global__ __launch_bounds__(kThreads) void tree_attention_kernel(TreeAttentionA
                 *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(a.out) + to) = y;
             }
         }
+    };
+    if (kKeyGroups == 1) {
+#pragma unroll
+        for (int qt = 0; qt < kQ; ++qt) {
+#pragma unroll
+            for (int d = 0; d < kDim / 16; ++d)
+                put(first_row + (row_group * kQ + qt) * 16 + column, d * 16 + quarter * 4, out[qt][d], all[qt], sum[qt]);
+        }
+        return;
+    }
+    constexpr int kPitch = kDim + 4;                                                   // floats of a row in LDS
+    float* sums = reinterpret_cast<float*>(lds);                                       // [kKeyGroups][kRows][kPitch]
+    Part* group_parts = reinterpret_cast<Part*>(sums + kKeyGroups * kRows * kPitch);   // [kKeyGroups][kRows]
+    __syncthreads();  // the tiles are done with
+#pragma unroll
+    for (int qt = 0; qt < kQ; ++qt) {
+        const int r = key_group * kRows + (row_group * kQ + qt) * 16 + column;
+        if (quarter == 0) group_parts[r] = Part{all[qt], sum[qt]};
+#pragma unroll
+        for (int d = 0; d < kDim / 16; ++d) *reinterpret_cast<f32x4*>(sums + r * kPitch + d * 16 + quarter * 4) = out[qt][d];
+    }
+    __syncthreads();
+    constexpr int kFours = kDim / 4;
+    for (int i = tid; i < kRows * kFours; i += kThreads) {
+        const int r = i / kFours, d = i % kFours * 4;
+        float highest = -__builtin_inff(), total = 0.0f;
+#pragma unroll
+        for (int g = 0; g < kKeyGroups; ++g) highest = fmaxf(highest, group_parts[g * kRows + r].most);
+        f32x4 x{0, 0, 0, 0};
+#pragma unroll
+        for (int g = 0; g < kKeyGroups; ++g) {
+            const float by = exp2_between(group_parts[g * kRows + r].most, highest);
+            total = __builtin_fmaf(group_parts[g * kRows + r].sum, by, total);
+            const f32x4 y = *reinterpret_cast<const f32x4*>(sums + (g * kRows + r) * kPitch + d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(y[j], by, x[j]);
+        }
+        put(first_row + r, d, x, highest, total);
     }
 }
 
@@ -538,7 +552,7 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(TreeAttentionArgs 
 }
 
 struct Shape {
-    int dim, sixteens;  // kDim, kQ
+    int dim, sixteens, key_groups;  // kDim, kQ, kKeyGroups
     uint32_t row_tiles, splits, split_keys;
 };
 
@@ -548,10 +562,15 @@ Shape shape_of(const TreeAttentionArgs& a, int compute_units) {
     Shape s;
     s.dim = a.cache.head_dim <= 64 ? 64 : a.cache.head_dim <= 128 ? 128 : 256;
     const uint64_t rows = static_cast<uint64_t>(a.max_query_len) * a.group;
-    // sixteens of rows as the queries' registers allow: three terms of f32 queries, or heads of 256, take two
-    const int most = a.f32 || s.dim == 256 ? 2 : 4;
-    s.sixteens = rows <= 16 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
-    s.row_tiles = static_cast<uint32_t>((rows + 16 * s.sixteens - 1) / (16 * s.sixteens));
+    if (s.dim == 256) {  // two stages of four groups' tiles would not fit LDS, and two sixteens of rows not the registers
+        s.sixteens = 1;
+        s.key_groups = rows <= 32 ? 2 : 1;
+    } else {
+        s.sixteens = rows <= 16 ? 1 : 2;
+        s.key_groups = rows <= 32 ? 4 : rows <= 64 ? 2 : 1;
+    }
+    const uint64_t tile_rows = 16 * s.sixteens * (kWaves / s.key_groups);
+    s.row_tiles = static_cast<uint32_t>((rows + tile_rows - 1) / tile_rows);
     const uint64_t base = static_cast<uint64_t>(a.requests) * a.cache.kv_heads * s.row_tiles;
     const uint64_t wanted = base == 0 ? 1 : (4 * static_cast<uint64_t>(compute_units) + base - 1) / base;
     uint64_t splits = wanted < kMostSplits ? wanted : kMostSplits;
@@ -570,13 +589,11 @@ size_t part_out_bytes(const TreeAttentionArgs& a, const Shape& s) {
     return (static_cast<size_t>(s.splits) * a.tokens * a.heads * a.cache.head_dim * sizeof(float) + 255) / 256 * 256;
 }
 
-template <int kDim, bool kBf16, bool kF32, int kQ>
+template <int kDim, bool kBf16, bool kF32, int kQ, int kKeyGroups>
 hipError_t attend(hipStream_t stream, const TreeAttentionArgs& a, const Shape& s, void* workspace) {
     static LdsLimit limit;
-    const size_t v_bytes = static_cast<size_t>(kWaves) * kTile * (kDim * 2 + 32);
-    const size_t sum_bytes = 2 * 16 * kQ * (kDim + 4) * sizeof(float) + kWaves * 16 * kQ * sizeof(Part);
-    const size_t lds = v_bytes > sum_bytes ? v_bytes : sum_bytes;
-    const auto kernel = tree_attention_kernel<kDim, kBf16, kF32, kQ>;
+    constexpr size_t lds = attention_lds_bytes<kDim, kQ, kKeyGroups>();
+    const auto kernel = tree_attention_kernel<kDim, kBf16, kF32, kQ, kKeyGroups>;
     hipError_t e = allow_lds(kernel, lds, &limit);
     if (e != hipSuccess) return e;
     float* part_out = static_cast<float*>(workspace);
@@ -592,11 +609,15 @@ hipError_t attend(hipStream_t stream, const TreeAttentionArgs& a, const Shape& s
 
 template <int kDim, bool kBf16, bool kF32>
 hipError_t attend_rows(hipStream_t stream, const TreeAttentionArgs& a, const Shape& s, void* workspace) {
-    if (s.sixteens == 1) return attend<kDim, kBf16, kF32, 1>(stream, a, s, workspace);
-    if constexpr (!kF32 && kDim < 256) {
-        if (s.sixteens == 4) return attend<kDim, kBf16, kF32, 4>(stream, a, s, workspace);
+    if constexpr (kDim == 256) {
+        if (s.key_groups == 2) return attend<kDim, kBf16, kF32, 1, 2>(stream, a, s, workspace);
+        return attend<kDim, kBf16, kF32, 1, 1>(stream, a, s, workspace);
+    } else {
+        if (s.sixteens == 1) return attend<kDim, kBf16, kF32, 1, 4>(stream, a, s, workspace);
+        if (s.key_groups == 4) return attend<kDim, kBf16, kF32, 2, 4>(stream, a, s, workspace);
+        if (s.key_groups == 2) return attend<kDim, kBf16, kF32, 2, 2>(stream, a, s, workspace);
+        return attend<kDim, kBf16, kF32, 2, 1>(stream, a, s, workspace);
     }
-    return attend<kDim, kBf16, kF32, 2>(stream, a, s, workspace);
 }
 
 template <int kDim>
