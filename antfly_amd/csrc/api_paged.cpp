@@ -208,6 +208,7 @@ afhip_status afhip_launch_tree_attention(void* stream, const afhip_tree_attentio
     const afhip_status s = attention_args(attention, &args, &empty);
     if (s != AFHIP_OK || empty) return s;
     const int units = gemv_compute_units();
+    if (!tree_attention_fits_a_launch(args, units)) return AFHIP_ERR_OP_UNSUPPORTED;
     const size_t needed = tree_attention_workspace_bytes(args, units);
     if (needed > workspace.len || (needed != 0 && !aligned(workspace, 256))) return AFHIP_ERR_INVALID_STATE;
     return status_of(launch_tree_attention(static_cast<hipStream_t>(stream), args, reinterpret_cast<void*>(workspace.ptr), units));

@@ -12,11 +12,11 @@
 // keys 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3).  V comes row-major and is needed column-major: it goes through LDS and
 // is read with the transposing ds_read_b64_tr_b16.  K goes from memory into the operand registers, no LDS.
 //
-// Keys and values of a tile of 32 keys come from memory straight into LDS (no registers in between), the next tile's while
-// this one is worked on.  A workgroup's four wavefronts are kKeyGroups groups that take tiles in turn; the wavefronts of one
-// group share its tiles and have 16 kQ rows each.  Few rows: four groups that need no barrier in the loop and add up at the
-// end; many rows: one group, every key read once for 128 rows.  Few rows on long contexts are split over workgroups as well,
-// and a second kernel joins the parts.
+// Keys and values come in tiles of 32 keys from memory straight into a ring of tiles in LDS (no registers in between),
+// requested kStages - 1 tiles ahead.  The wavefronts of a workgroup share its tiles and have 16 kQ rows each: a lone wavefront
+// (no barrier anywhere) up to 32 rows, four of them, and every key read once, for 128.  Long contexts are shared out over
+// workgroups by the lengths that the device holds, so that ragged requests keep all of them busy to the end, and a second
+// kernel joins the parts.
 #include "paged_launch.h"
 
 #include <hip/hip_runtime.h>
@@ -31,7 +31,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kThreads = 256, kWaves = 4;
 constexpr int kTile = 32;             // keys of one wavefront's step
 constexpr uint32_t kNowhere = ~0u;    // of a key that has no place in the cache
 constexpr float kLog2e = 1.4426950408889634f;
@@ -135,86 +134,200 @@ __device__ __forceinline__ void load_to_lds(uint32_t to, const uint4* from) {
 }
 
 // Where 16-byte piece `piece` of row `row` of a tile lies in LDS, in pieces.  The pieces of a row are in an order of its own,
-// so that the same piece of 16 rows (what the lanes of an operand read) falls on all banks: 256 bytes of them.
+// so that what the lanes of an operand read falls on all banks (256 bytes of them): one piece of 16 rows of K, two
+// neighbouring pieces of eight rows of V.
 template <int kDim>
-__device__ __forceinline__ int lds_piece(int row, int piece) {
+__device__ __forceinline__ int key_piece(int row, int piece) {
     constexpr int kPieces = kDim / 8;
     return row * kPieces + (kPieces == 8 ? piece ^ (row >> 1 & 7) : piece ^ (row & 15));
 }
+template <int kDim>
+__device__ __forceinline__ int value_piece(int row, int piece) {
+    constexpr int kPieces = kDim / 8;
+    return row * kPieces + (kPieces == 8 ? piece ^ (row & 6) : piece ^ (row << 1 & 14));
+}
 
-template <int kDim, int kQ, int kKeyGroups>
-constexpr size_t attention_lds_bytes() {
-    constexpr int kRows = 16 * kQ * (kWaves / kKeyGroups);
-    constexpr size_t tiles = static_cast<size_t>(kKeyGroups) * 2 * 2 * kTile * kDim * 2;
-    constexpr size_t sums = kKeyGroups == 1 ? 0 : static_cast<size_t>(kKeyGroups) * kRows * ((kDim + 4) * sizeof(float) + sizeof(Part));
-    return tiles > sums ? tiles : sums;
+// s_waitcnt for "at most kLeft vector memory operations outstanding" (nothing else waited for).
+template <int kLeft>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kLeft) : "memory");
+}
+
+// What the launch's shape and the lengths on the device say of one request.
+struct Share {
+    int begin, tokens, context, keys;   // its first row of query, new tokens, cached tokens, both together
+    uint32_t row_tiles, splits, tiles;  // workgroups' rows, parts of its keys, tiles of keys in a part
+    uint32_t first, first_slot;         // number of its first workgroup, and of its first part
+};
+
+__device__ __forceinline__ Share lengths_of(const TreeAttentionArgs& a, uint32_t request, int rows_a_tile) {
+    Share s{};
+    s.begin = min(max(a.query_starts[request], 0), static_cast<int>(a.tokens));
+    const int end = min(max(a.query_starts[request + 1], s.begin), static_cast<int>(a.tokens));
+    s.tokens = min(end - s.begin, static_cast<int>(a.max_query_len));
+    s.context = max(a.context_lens[request], 0);
+    const unsigned long long most = min(static_cast<unsigned long long>(a.table_columns) * a.block_size.by, static_cast<unsigned long long>(a.max_key_len));
+    s.keys = static_cast<int>(min(static_cast<unsigned long long>(s.context) + s.tokens, most));
+    s.row_tiles = (static_cast<uint32_t>(s.tokens) * a.group + rows_a_tile - 1) / rows_a_tile;
+    return s;
+}
+
+template <typename T>
+__device__ __forceinline__ T sum_up_to(T v, int lane) {  // over the wavefront's lanes up to this one
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const T other = __shfl_up(v, d);
+        if (lane >= d) v += other;
+    }
+    return v;
+}
+
+// How the keys are shared out.  A part has the same number of tiles for all requests (rounded to whole tiles and evened out
+// within a request): all the batch's tiles of keys, counted once for every row tile and key head, over plan.target
+// workgroups, `least` tiles at least.  Workgroups are numbered by request, key head, part, row tile; parts of requests that
+// have several are numbered the same way.  Every wavefront works this out for itself from the lengths.
+struct SharePlan {
+    uint32_t target, least;
+    uint32_t row_tiles;  // of the largest request
+    bool even;           // otherwise every request is one part, and has as many workgroups as the largest may need
+};
+
+// `of`: a workgroup's number (by_request false) or a request's.  False: there is no such workgroup.
+template <bool kByRequest>
+__device__ __forceinline__ bool find_share(const TreeAttentionArgs& a, const SharePlan& plan, int rows_a_tile, uint32_t of, uint32_t* request, Share* out) {
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    const uint32_t heads = a.cache.kv_heads;
+    if (!plan.even) {
+        const uint32_t r = kByRequest ? of : of / (heads * plan.row_tiles);
+        if (r >= a.requests) return false;
+        *request = r;
+        *out = lengths_of(a, r, rows_a_tile);
+        out->splits = 1;
+        out->tiles = (out->keys + kTile - 1) / kTile;
+        out->first = r * heads * plan.row_tiles;
+        out->row_tiles = plan.row_tiles;  // (its numbering; rows past its own are empty)
+        return true;
+    }
+    Share mine{};
+    unsigned long long work = 0;
+    for (uint32_t r0 = 0; r0 < a.requests; r0 += 64) {
+        if (r0 + lane < a.requests) {
+            mine = lengths_of(a, r0 + lane, rows_a_tile);
+            work += static_cast<unsigned long long>((mine.keys + kTile - 1) / kTile) * mine.row_tiles;
+        }
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) work += __shfl_xor(work, d);
+    const unsigned long long each = (work * heads + plan.target - 1) / plan.target;
+    const uint32_t tiles = static_cast<uint32_t>(min(max(each, static_cast<unsigned long long>(plan.least)), 0x7fffffffull));
+    uint32_t before = 0, slots_before = 0;
+    for (uint32_t r0 = 0; r0 < a.requests; r0 += 64) {
+        uint32_t count = 0, slots = 0;
+        mine.splits = 0;
+        if (r0 + lane < a.requests) {
+            if (a.requests > 64) mine = lengths_of(a, r0 + lane, rows_a_tile);
+            const uint32_t all = (mine.keys + kTile - 1) / kTile;
+            mine.splits = max((all + tiles - 1) / tiles, 1u);
+            mine.tiles = (all + mine.splits - 1) / mine.splits;
+            count = mine.row_tiles * mine.splits * heads;
+            slots = mine.splits > 1 ? count : 0;
+        }
+        const uint32_t upto = sum_up_to(count, lane), slots_upto = sum_up_to(slots, lane);
+        mine.first = before + upto - count;
+        mine.first_slot = slots_before + slots_upto - slots;
+        const unsigned long long here = kByRequest ? (of >= r0 && of < r0 + 64 ? 1ull << (of - r0) : 0ull)
+                                                   : __ballot(of >= mine.first && of < mine.first + count);
+        if (here != 0) {
+            const int l = __builtin_ctzll(here);
+            *request = r0 + l;
+            out->begin = __builtin_amdgcn_readlane(mine.begin, l);
+            out->tokens = __builtin_amdgcn_readlane(mine.tokens, l);
+            out->context = __builtin_amdgcn_readlane(mine.context, l);
+            out->keys = __builtin_amdgcn_readlane(mine.keys, l);
+            out->row_tiles = __builtin_amdgcn_readlane(mine.row_tiles, l);
+            out->splits = __builtin_amdgcn_readlane(mine.splits, l);
+            out->tiles = __builtin_amdgcn_readlane(mine.tiles, l);
+            out->first = __builtin_amdgcn_readlane(mine.first, l);
+            out->first_slot = __builtin_amdgcn_readlane(mine.first_slot, l);
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+        slots_before += __builtin_amdgcn_readlane(slots_upto, 63);
+    }
+    return false;
 }
 
 // kDim: the head's values, rounded up to a size that is here (the rest are zeros).  kF32: query and out are f32.
-template <int kDim, bool kBf16, bool kF32, int kQ, int kKeyGroups>
-__global__ __launch_bounds__(kThreads, kF32 ? 1 : 2) void tree_attention_kernel(TreeAttentionArgs a, uint32_t row_tiles, uint32_t splits,
-                                                                 uint32_t split_keys, float* part_out, Part* parts) {
+template <int kDim, bool kBf16, bool kF32, int kQ, int kWaves, int kStages>
+__global__ __launch_bounds__(kWaves * 64, kF32 || kDim == 256 ? 1 : 2) void tree_attention_kernel(TreeAttentionArgs a, SharePlan plan, float* part_out,
+                                                                                                 Part* parts) {
     constexpr int kSteps = kDim / 32;                            // products of K Q^T along the head
     constexpr int kTerms = kF32 ? (kBf16 ? 3 : 2) : 1;           // of a query value or a weight: 24 bits of three bf16, 22 of two f16
-    constexpr int kRowGroups = kWaves / kKeyGroups, kRows = 16 * kQ * kRowGroups;
+    constexpr int kRows = 16 * kQ * kWaves;
     constexpr int kPieces = kDim / 8;                            // 16-byte pieces of a row
     constexpr int kTileBytes = kTile * kDim * 2;                 // of K, and of V behind it
-    constexpr int kLoads = kTile * kPieces / 64 / kRowGroups;    // of a wavefront, 1 KiB each, for K and for V
+    constexpr int kLoads = kTile * kPieces / 64 / kWaves;        // of a wavefront, 1 KiB each, for K and for V
     extern __shared__ __attribute__((aligned(1024))) char lds[];
 
-    // the row tiles of a key head's split lie on one XCD (workgroups go round them in turn): they share its L2
-    const uint32_t item = (blockIdx.x >> 3) / row_tiles * 8 + (blockIdx.x & 7), row_tile = (blockIdx.x >> 3) % row_tiles;
-    if (item >= a.requests * a.cache.kv_heads * splits) return;
-    const uint32_t request = item / (a.cache.kv_heads * splits), kv_head = item % a.cache.kv_heads;
-    const uint32_t split = item / a.cache.kv_heads % splits;
-
-    const int begin = min(max(a.query_starts[request], 0), static_cast<int>(a.tokens));
-    const int end = min(max(a.query_starts[request + 1], begin), static_cast<int>(a.tokens));
-    const int tokens = min(end - begin, static_cast<int>(a.max_query_len));
-    const int group = static_cast<int>(a.group), rows = tokens * group, first_row = static_cast<int>(row_tile) * kRows;
+    // workgroups go round the eight XCDs in turn: the row tiles of a part, which share its keys, lie on one and share its L2
+    const uint32_t number = ((blockIdx.x >> 3) / plan.row_tiles * 8 + (blockIdx.x & 7)) * plan.row_tiles + (blockIdx.x >> 3) % plan.row_tiles;
+    uint32_t request;
+    Share share;
+    if (!find_share<false>(a, plan, kRows, number, &request, &share)) return;
+    const uint32_t inside = number - share.first, row_tile = inside % share.row_tiles, split = inside / share.row_tiles % share.splits;
+    const uint32_t kv_head = inside / share.row_tiles / share.splits, slot = share.first_slot + inside;
+    const int begin = share.begin, context = share.context, group = static_cast<int>(a.group), rows = share.tokens * group;
+    const int first_row = static_cast<int>(row_tile) * kRows;
     if (first_row >= rows) return;
-    const int context = max(a.context_lens[request], 0);
-    const unsigned long long most_keys = min(static_cast<unsigned long long>(a.table_columns) * a.block_size.by,
-                                             static_cast<unsigned long long>(a.max_key_len));
-    int keys = static_cast<int>(min(static_cast<unsigned long long>(context) + tokens, most_keys));
+    int keys = share.keys;
     const int last_token = min(first_row + kRows - 1, rows - 1) / group;
     if (a.masks == nullptr) keys = static_cast<int>(min(static_cast<unsigned long long>(keys), static_cast<unsigned long long>(context) + last_token + 1));
-    const int key_begin = static_cast<int>(min(static_cast<unsigned long long>(split) * split_keys, static_cast<unsigned long long>(keys)));
-    const int key_end = static_cast<int>(min(static_cast<unsigned long long>(key_begin) + split_keys, static_cast<unsigned long long>(keys)));
+    const int split_keys = static_cast<int>(share.tiles) * kTile;  // (splits * split_keys < keys + splits * kTile: far from 2^31)
+    const int key_begin = min(static_cast<int>(split) * split_keys, keys), key_end = min(key_begin + split_keys, keys);
 
     const int tid = static_cast<int>(threadIdx.x), wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int column = lane & 15, quarter = lane >> 4;
-    const int key_group = wave / kRowGroups, row_group = wave % kRowGroups;
-    char* const tiles = lds + key_group * (4 * kTileBytes);
-    const uint32_t tiles_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)tiles));
-    const int* table = a.block_tables + static_cast<size_t>(request) * a.table_columns;
-    const uint32_t head_at = kv_head * a.cache.head_stride;
+    const int my_row = first_row + wave * 16 * kQ;  // of this wavefront's first
+    const bool works = my_row < rows;               // otherwise it only helps to load
+    if (share.splits > 1 && key_begin >= key_end) {  // none of this part's keys is there for these rows: the part says so
+        for (int r = tid; r < kRows; r += kWaves * 64) parts[static_cast<size_t>(slot) * kRows + r] = Part{-__builtin_inff(), 0.0f};
+        return;
+    }
+    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
     const int pieces = static_cast<int>(a.cache.head_dim / 8);  // that hold something
 
-    // where a key's values lie, in 16-byte units
-    auto place = [&](int key) -> uint32_t {
-        if (key >= key_end) return kNowhere;
-        const uint32_t col = divide(static_cast<uint32_t>(key), a.block_size);
-        const uint32_t block = static_cast<uint32_t>(table[col]);
-        if (block >= a.cache.blocks) return kNowhere;
-        return block * a.cache.block_stride + (static_cast<uint32_t>(key) - col * a.block_size.by) * a.cache.slot_stride + head_at;
+    // where 64 blocks from `window_at` on lie, in 16-byte units, one a lane
+    const int* table = a.block_tables + static_cast<size_t>(request) * a.table_columns;
+    const uint32_t last_block = key_begin < key_end ? divide(static_cast<uint32_t>(key_end - 1), a.block_size) : 0;
+    uint32_t window = kNowhere, window_at = 0, window_end = 0;  // (keys from window_end on are not in it)
+    auto place = [&](int tile) -> uint32_t {  // of key tile + lane % 32
+        if (static_cast<uint32_t>(tile) + kTile > window_end) {
+            window_at = divide(static_cast<uint32_t>(tile), a.block_size);
+            const uint32_t column = window_at + lane;
+            const uint32_t block = column <= last_block ? static_cast<uint32_t>(table[column]) : kNowhere;
+            window = block < a.cache.blocks ? block * a.cache.block_stride + kv_head * a.cache.head_stride : kNowhere;
+            window_end = (window_at + 64) * a.block_size.by;  // (below 2^32: a bound of the keys times the block size)
+        }
+        const uint32_t key = static_cast<uint32_t>(tile) + (lane & 31), block = divide(key, a.block_size);
+        const uint32_t at = static_cast<uint32_t>(__shfl(static_cast<int>(window), static_cast<int>(block - window_at)));
+        return at == kNowhere || static_cast<int>(key) >= key_end ? kNowhere : at + (key - block * a.block_size.by) * a.cache.slot_stride;
     };
-    // this wavefront's part of a tile's K and V; `at`: lane l % 32 has the place of key l % 32
-    auto request_tile = [&](uint32_t at, int stage) {
-        const uint32_t to = tiles_at + stage * (2 * kTileBytes) + row_group * (kLoads * 1024);
+    // Requests this wavefront's part of a tile's K and V; which of its keys have a place.
+    auto request_tile = [&](int tile, int stage) -> uint32_t {
+        const uint32_t at = place(tile);  // lane l % 32 has the place of key l % 32
+        const uint32_t to = lds_at + stage * (2 * kTileBytes) + wave * (kLoads * 1024);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int slot = (row_group * kLoads + i) * 64 + lane, row = slot / kPieces, piece = lds_piece<kDim>(row, slot % kPieces) % kPieces;
+            const int slot = (wave * kLoads + i) * 64 + lane, row = slot / kPieces, kp = key_piece<kDim>(row, slot % kPieces) % kPieces, vp = value_piece<kDim>(row, slot % kPieces) % kPieces;
             const uint32_t from = static_cast<uint32_t>(__shfl(static_cast<int>(at), row));
-            const bool there = from != kNowhere && piece < pieces;
-            load_to_lds(to + i * 1024, there ? a.cache.keys + from + piece : &kNothing);
-            load_to_lds(to + kTileBytes + i * 1024, there ? a.cache.values + from + piece : &kNothing);
+            load_to_lds(to + i * 1024, from != kNowhere && kp < pieces ? a.cache.keys + (from + kp) : &kNothing);
+            load_to_lds(to + kTileBytes + i * 1024, from != kNowhere && vp < pieces ? a.cache.values + (from + vp) : &kNothing);
         }
+        return static_cast<uint32_t>(__ballot(at != kNowhere));
     };
-    const int step = kKeyGroups * kTile, first_tile = key_begin + key_group * kTile;
-    uint32_t at = place(first_tile + (lane & 31));
-    request_tile(at, 0);
-    uint32_t at_next = place(first_tile + step + (lane & 31));
+    uint32_t held_ahead[kStages - 1];  // of the tiles on their way, the next one's first
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) held_ahead[i] = key_begin + i * kTile < key_end ? request_tile(key_begin + i * kTile, i) : 0u;
 
     // ---- the rows
     s16x8 query[kQ][kSteps][kTerms];
@@ -225,7 +338,7 @@ __global__ __launch_bounds__(kThreads, kF32 ? 1 : 2) void tree_attention_kernel(
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale turns the queries round
 #pragma unroll
     for (int qt = 0; qt < kQ; ++qt) {
-        const int row = first_row + (row_group * kQ + qt) * 16 + column;
+        const int row = my_row + qt * 16 + column;
         real[qt] = row < rows;
         row_token[qt] = real[qt] ? row / group : 0;
         const int head = static_cast<int>(kv_head) * group + (real[qt] ? row % group : 0);
@@ -296,30 +409,29 @@ __global__ __launch_bounds__(kThreads, kF32 ? 1 : 2) void tree_attention_kernel(
     }
 
     // ---- the keys
-    int stage = 0;
-    for (int first = key_begin; first < key_end; first += step, stage ^= 1) {
-        const int tile = first + key_group * kTile;
-        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // this wavefront's part of the tile is there
-        if (kRowGroups > 1) __syncthreads();                // everyone's is, and the other stage has been read
-        const uint32_t at_now = at;
-        at = at_next;
-        if (tile + step < key_end) {
-            request_tile(at, stage ^ 1);
-            at_next = place(tile + 2 * step + (lane & 31));
-        }
-        if (tile >= key_end) continue;
-        const char* k_lds = tiles + stage * (2 * kTileBytes);
-        char* v_lds = tiles + stage * (2 * kTileBytes) + kTileBytes;
-
-        const uint32_t held = static_cast<uint32_t>(__ballot(at_now != kNowhere));  // keys of the tile that have a place
-        const bool clean = tile + kTile <= context && held == ~0u;                   // every row sees every key
+    int stage = 0, free_stage = kStages - 1;
+    for (int tile = key_begin; tile < key_end; tile += kTile) {
+        // this wavefront's part of the tile is there: all but what was requested behind it, all of it near the end
+        if (tile + (kStages - 2) * kTile < key_end) wait_loads<2 * kLoads * (kStages - 2)>();
+        else wait_loads<0>();
+        if (kWaves > 1) __syncthreads();           // everyone's is, and the stage to be filled has been read
+        const uint32_t held = held_ahead[0];
+#pragma unroll
+        for (int i = 0; i + 1 < kStages - 1; ++i) held_ahead[i] = held_ahead[i + 1];
+        if (tile + (kStages - 1) * kTile < key_end) held_ahead[kStages - 2] = request_tile(tile + (kStages - 1) * kTile, free_stage);
+        const char* k_lds = lds + stage * (2 * kTileBytes);
+        const char* v_lds = k_lds + kTileBytes;
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+        free_stage = free_stage + 1 == kStages ? 0 : free_stage + 1;
+        if (!works) continue;
+        const bool clean = tile + kTile <= context && held == ~0u;  // every row sees every key
 
         f32x4 score[kQ][2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
-                const s16x8 k = *reinterpret_cast<const s16x8*>(k_lds + lds_piece<kDim>(half * 16 + column, s * 4 + quarter) * 16);
+                const s16x8 k = *reinterpret_cast<const s16x8*>(k_lds + key_piece<kDim>(half * 16 + column, s * 4 + quarter) * 16);
 #pragma unroll
                 for (int qt = 0; qt < kQ; ++qt) {
 #pragma unroll
@@ -331,13 +443,13 @@ __global__ __launch_bounds__(kThreads, kF32 ? 1 : 2) void tree_attention_kernel(
         uint32_t odd = 0;  // keys with a value that is no finite number (looked for only where some row may not see them)
         uint32_t seen[kQ];
         if (!clean) {
-            for (int slot = lane; slot < kTile * kPieces; slot += 64) {
-                const uint4 v = *reinterpret_cast<const uint4*>(v_lds + slot * 16);
+            for (int at = lane; at < kTile * kPieces; at += 64) {
+                const uint4 v = *reinterpret_cast<const uint4*>(v_lds + at * 16);
                 unsigned long long which = __ballot(is_odd<kBf16>(v.x) || is_odd<kBf16>(v.y) || is_odd<kBf16>(v.z) || is_odd<kBf16>(v.w));
                 while (which != 0) {
                     const int l = __builtin_ctzll(which);
                     which &= which - 1;
-                    odd |= 1u << __builtin_amdgcn_readlane(slot / kPieces, l);
+                    odd |= 1u << __builtin_amdgcn_readlane(at / kPieces, l);
                 }
             }
 #pragma unroll
@@ -391,13 +503,14 @@ __global__ __launch_bounds__(kThreads, kF32 ? 1 : 2) void tree_attention_kernel(
                 }
             }
         }
+        odd = __builtin_amdgcn_readfirstlane(odd);
 #pragma unroll
         for (int d = 0; d < kDim / 16; ++d) {
             s16x8 v;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int row = half * 16 + quarter * 4 + (column >> 2);
-                const char* from = v_lds + lds_piece<kDim>(row, d * 2 + (column >> 1 & 1)) * 16 + (column & 1) * 8;
+                const char* from = v_lds + value_piece<kDim>(row, d * 2 + (column >> 1 & 1)) * 16 + (column & 1) * 8;
                 const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)from);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[half * 4 + j] = four[j];
@@ -429,7 +542,7 @@ __global__ __launch_bounds__(kThreads, kF32 ? 1 : 2) void tree_attention_kernel(
                 if ((seen[qt] >> key & 1) == 0) continue;
 #pragma unroll
                 for (int d = 0; d < kDim / 16; ++d) {
-                    const char* from = v_lds + lds_piece<kDim>(key, d * 2 + (quarter >> 1)) * 16 + (quarter & 1) * 8;
+                    const char* from = v_lds + value_piece<kDim>(key, d * 2 + (quarter >> 1)) * 16 + (quarter & 1) * 8;
                     const s16x4 four = *reinterpret_cast<const s16x4*>(from);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -439,184 +552,181 @@ __global__ __launch_bounds__(kThreads, kF32 ? 1 : 2) void tree_attention_kernel(
             }
         }
     }
-    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // (of a workgroup without keys: its first request)
 
-    // ---- the key groups' sums, and out: four values a lane
-    float all[kQ];  // the row's maximum in units of log2
+    // ---- out: a lane has four consecutive values of its row in each register group
 #pragma unroll
     for (int qt = 0; qt < kQ; ++qt) {
-        sum[qt] = row_sum(sum[qt]);
-        all[qt] = most[qt] == -__builtin_inff() ? most[qt] : most[qt] * unit[qt];
-    }
-    auto put = [&](int row, int d, f32x4 x, float highest, float total) {
-        if (row >= rows || d >= pieces * 8) return;
-        const size_t token = static_cast<size_t>(begin + row / group);
+        const float total = row_sum(sum[qt]);
+        if (!real[qt]) continue;
+        const int row = my_row + qt * 16 + column;
+        const size_t token = static_cast<size_t>(begin + row_token[qt]);
         const int head = static_cast<int>(kv_head) * group + row % group;
-        if (splits > 1) {
-            const size_t index = (static_cast<size_t>(split) * a.tokens + token) * a.heads + head;
-            *reinterpret_cast<f32x4*>(part_out + index * a.cache.head_dim + d) = x;
-            if (d == 0) parts[index] = Part{highest, total};
-        } else {
-            const size_t to = token * a.out_token_stride + static_cast<size_t>(head) * a.out_head_stride + d;
-            const float by = total == 0.0f ? 0.0f : 1.0f / total;
-            if (kF32) {
-                *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to) = x * by;
+        const size_t part = static_cast<size_t>(slot) * kRows + (row - first_row);
+        if (share.splits > 1 && quarter == 0) parts[part] = Part{most[qt] == -__builtin_inff() ? most[qt] : most[qt] * unit[qt], total};
+        const size_t to = token * a.out_token_stride + static_cast<size_t>(head) * a.out_head_stride;
+        const float by = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+        for (int dt = 0; dt < kDim / 16; ++dt) {
+            const int d = dt * 16 + quarter * 4;
+            if (d >= pieces * 8) continue;
+            if (share.splits > 1) {
+                *reinterpret_cast<f32x4*>(part_out + part * a.cache.head_dim + d) = out[qt][dt];
+            } else if (kF32) {
+                *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to + d) = out[qt][dt] * by;
             } else {
                 s16x4 y;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) y[j] = narrow<kBf16>(x[j] * by);
-                *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(a.out) + to) = y;
+                for (int j = 0; j < 4; ++j) y[j] = narrow<kBf16>(out[qt][dt][j] * by);
+                *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(a.out) + to + d) = y;
             }
         }
-    };
-    if (kKeyGroups == 1) {
-#pragma unroll
-        for (int qt = 0; qt < kQ; ++qt) {
-#pragma unroll
-            for (int d = 0; d < kDim / 16; ++d)
-                put(first_row + (row_group * kQ + qt) * 16 + column, d * 16 + quarter * 4, out[qt][d], all[qt], sum[qt]);
-        }
-        return;
-    }
-    constexpr int kPitch = kDim + 4;                                                   // floats of a row in LDS
-    float* sums = reinterpret_cast<float*>(lds);                                       // [kKeyGroups][kRows][kPitch]
-    Part* group_parts = reinterpret_cast<Part*>(sums + kKeyGroups * kRows * kPitch);   // [kKeyGroups][kRows]
-    __syncthreads();  // the tiles are done with
-#pragma unroll
-    for (int qt = 0; qt < kQ; ++qt) {
-        const int r = key_group * kRows + (row_group * kQ + qt) * 16 + column;
-        if (quarter == 0) group_parts[r] = Part{all[qt], sum[qt]};
-#pragma unroll
-        for (int d = 0; d < kDim / 16; ++d) *reinterpret_cast<f32x4*>(sums + r * kPitch + d * 16 + quarter * 4) = out[qt][d];
-    }
-    __syncthreads();
-    constexpr int kFours = kDim / 4;
-    for (int i = tid; i < kRows * kFours; i += kThreads) {
-        const int r = i / kFours, d = i % kFours * 4;
-        float highest = -__builtin_inff(), total = 0.0f;
-#pragma unroll
-        for (int g = 0; g < kKeyGroups; ++g) highest = fmaxf(highest, group_parts[g * kRows + r].most);
-        f32x4 x{0, 0, 0, 0};
-#pragma unroll
-        for (int g = 0; g < kKeyGroups; ++g) {
-            const float by = exp2_between(group_parts[g * kRows + r].most, highest);
-            total = __builtin_fmaf(group_parts[g * kRows + r].sum, by, total);
-            const f32x4 y = *reinterpret_cast<const f32x4*>(sums + (g * kRows + r) * kPitch + d);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(y[j], by, x[j]);
-        }
-        put(first_row + r, d, x, highest, total);
     }
 }
 
-// The parts of a row from `splits` workgroups, one wavefront a row: each part is brought to the common maximum.
-template <bool kBf16, bool kF32>
-__global__ __launch_bounds__(kThreads) void join_parts_kernel(TreeAttentionArgs a, uint32_t splits, const float* part_out, const Part* parts) {
-    const uint32_t request = blockIdx.y, row = blockIdx.x * kWaves + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    const int begin = min(max(a.query_starts[request], 0), static_cast<int>(a.tokens));
-    const int end = min(max(a.query_starts[request + 1], begin), static_cast<int>(a.tokens));
-    const uint32_t tokens = min(static_cast<uint32_t>(end - begin), a.max_query_len);
-    if (row >= tokens * a.heads) return;
-    const size_t token = static_cast<size_t>(begin) + row / a.heads;
-    const uint32_t head = row % a.heads;
-    const size_t stride = static_cast<size_t>(a.tokens) * a.heads, index = token * a.heads + head;
-    const Part mine = lane < static_cast<int>(splits) ? parts[index + lane * stride] : Part{-__builtin_inff(), 0.0f};
-    float most = mine.most;
+// The parts of a row, brought to their common maximum.  kLanes lanes have four values of the row each, four groups of them
+// take the parts in turn and add up in LDS.
+constexpr int kJoinThreads = 256, kJoinGroups = 4;
+template <bool kBf16, bool kF32, int kLanes>
+__global__ __launch_bounds__(kJoinThreads) void join_parts_kernel(TreeAttentionArgs a, SharePlan plan, int rows_a_tile, const float* part_out,
+                                                                 const Part* parts) {
+    constexpr int kJoinRows = kJoinThreads / (kLanes * kJoinGroups);
+    __shared__ f32x4 sums[kJoinGroups][kJoinRows][kLanes];
+    __shared__ Part group_parts[kJoinGroups][kJoinRows];
+    uint32_t request;
+    Share share;
+    if (!find_share<true>(a, plan, rows_a_tile, blockIdx.y, &request, &share) || share.splits == 1) return;
+    const int tid = static_cast<int>(threadIdx.x), piece = tid % kLanes, group = tid / kLanes % kJoinGroups, mine = tid / (kLanes * kJoinGroups);
+    const uint32_t rows = static_cast<uint32_t>(share.tokens) * a.group;   // of one key head
+    const uint32_t all = blockIdx.x * kJoinRows + mine, kv_head = all / rows, row = all % rows;
+    if (blockIdx.x * kJoinRows >= rows * a.cache.kv_heads) return;
+    const bool real = kv_head < a.cache.kv_heads;
+    const uint32_t row_tile = row / rows_a_tile;
+    const size_t slot = share.first_slot + static_cast<size_t>(real ? kv_head : 0) * share.splits * share.row_tiles + row_tile;
+    const size_t first = slot * rows_a_tile + row % rows_a_tile, stride = static_cast<size_t>(share.row_tiles) * rows_a_tile;
+    const uint32_t d = piece * 4;
+    float most = -__builtin_inff(), total = 0.0f;
+    f32x4 x{0, 0, 0, 0};
+    for (uint32_t s = group; s < share.splits; s += kJoinGroups) most = fmaxf(most, parts[first + s * stride].most);
+#pragma unroll 4
+    for (uint32_t s = group; s < share.splits; s += kJoinGroups) {
+        const Part part = parts[first + s * stride];
+        if (part.most == -__builtin_inff() || d >= a.cache.head_dim) continue;  // (a part that saw no key is not written)
+        const float by = exp2_between(part.most, most);
+        total = __builtin_fmaf(part.sum, by, total);
+        const f32x4 y = *reinterpret_cast<const f32x4*>(part_out + (first + s * stride) * a.cache.head_dim + d);
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-    const float by = exp2_between(mine.most, most);
-    float total = mine.sum * by;
+        for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(y[j], by, x[j]);
+    }
+    sums[group][mine][piece] = x;
+    if (piece == 0) group_parts[group][mine] = Part{most, total};
+    __syncthreads();
+    if (group != 0 || !real || d >= a.cache.head_dim) return;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
+    for (int g = 0; g < kJoinGroups; ++g) most = fmaxf(most, group_parts[g][mine].most);
+    total = 0.0f;
+    x = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int g = 0; g < kJoinGroups; ++g) {
+        const float by = exp2_between(group_parts[g][mine].most, most);
+        total = __builtin_fmaf(group_parts[g][mine].sum, by, total);
+        const f32x4 y = sums[g][mine][piece];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(y[j], by, x[j]);
+    }
     const float over = total == 0.0f ? 0.0f : 1.0f / total;
-    for (uint32_t d = lane * 4; d < a.cache.head_dim; d += 256) {
-        f32x4 x{0, 0, 0, 0};
-        for (uint32_t s = 0; s < splits; ++s) {
-            // (by readlane: lanes past the head's end are not in this loop, and a shuffle would not read them)
-            const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, by), s));
-            const f32x4 y = *reinterpret_cast<const f32x4*>(part_out + (index + s * stride) * a.cache.head_dim + d);
+    const size_t token = static_cast<size_t>(share.begin) + row / a.group;
+    const size_t to = token * a.out_token_stride + static_cast<size_t>(kv_head * a.group + row % a.group) * a.out_head_stride + d;
+    if (kF32) {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to) = x * over;
+    } else {
+        s16x4 y;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(y[j], f, x[j]);
-        }
-        const size_t to = token * a.out_token_stride + static_cast<size_t>(head) * a.out_head_stride + d;
-        if (kF32) {
-            *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to) = x * over;
-        } else {
-            s16x4 y;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = narrow<kBf16>(x[j] * over);
-            *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(a.out) + to) = y;
-        }
+        for (int j = 0; j < 4; ++j) y[j] = narrow<kBf16>(x[j] * over);
+        *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(a.out) + to) = y;
     }
 }
 
 struct Shape {
-    int dim, sixteens, key_groups;  // kDim, kQ, kKeyGroups
-    uint32_t row_tiles, splits, split_keys;
+    int dim, sixteens, waves;  // kDim, kQ, kWaves
+    SharePlan plan;
+    uint64_t groups, slots;  // most workgroups, and parts of requests that have several
+    int rows_a_tile() const { return 16 * sixteens * waves; }
 };
 
-constexpr uint32_t kMostSplits = 64;  // a lane of the joining wavefront each
+constexpr uint32_t kMostEvened = 1024;  // requests: every wavefront reads their lengths, 64 at a time
 
 Shape shape_of(const TreeAttentionArgs& a, int compute_units) {
     Shape s;
     s.dim = a.cache.head_dim <= 64 ? 64 : a.cache.head_dim <= 128 ? 128 : 256;
     const uint64_t rows = static_cast<uint64_t>(a.max_query_len) * a.group;
-    if (s.dim == 256) {  // two stages of four groups' tiles would not fit LDS, and two sixteens of rows not the registers
+    if (s.dim == 256) {  // (two sixteens of rows would not fit the registers)
         s.sixteens = 1;
-        s.key_groups = rows <= 32 ? 2 : 1;
+        s.waves = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     } else {
         s.sixteens = rows <= 16 ? 1 : 2;
-        s.key_groups = rows <= 32 ? 4 : rows <= 64 ? 2 : 1;
+        s.waves = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
     }
-    const uint64_t tile_rows = 16 * s.sixteens * (kWaves / s.key_groups);
-    s.row_tiles = static_cast<uint32_t>((rows + tile_rows - 1) / tile_rows);
-    const uint64_t base = static_cast<uint64_t>(a.requests) * a.cache.kv_heads * s.row_tiles;
-    const uint64_t wanted = base == 0 ? 1 : (4 * static_cast<uint64_t>(compute_units) + base - 1) / base;
-    uint64_t splits = wanted < kMostSplits ? wanted : kMostSplits;
-    const uint64_t least = 256;  // keys that are worth a workgroup
-    if (splits > (a.max_key_len + least - 1) / least) splits = (a.max_key_len + least - 1) / least;
-    if (splits == 0) splits = 1;
-    const uint64_t step = kWaves * kTile;
-    const uint64_t keys = ((a.max_key_len + splits - 1) / splits + step - 1) / step * step;
-    s.split_keys = static_cast<uint32_t>(keys == 0 ? step : keys);
-    s.splits = static_cast<uint32_t>((a.max_key_len + s.split_keys - 1) / s.split_keys);
-    if (s.splits == 0) s.splits = 1;
+    const uint64_t tile_rows = s.rows_a_tile(), most_row_tiles = (rows + tile_rows - 1) / tile_rows;
+    // row tiles of the whole batch: every request's last one may be part empty
+    uint64_t row_tiles = static_cast<uint64_t>(a.tokens) * a.group / tile_rows + a.requests;
+    if (row_tiles > a.requests * most_row_tiles) row_tiles = a.requests * most_row_tiles;
+    const uint64_t tiles = (static_cast<uint64_t>(a.max_key_len) + kTile - 1) / kTile;
+    s.plan.even = a.requests <= kMostEvened;
+    s.plan.row_tiles = static_cast<uint32_t>(most_row_tiles);
+    s.plan.least = 2;  // fewer tiles are not worth a workgroup
+    s.plan.target = static_cast<uint32_t>(compute_units * (s.waves == 1 ? 10 : s.waves == 2 ? 6 : 2));
+    const uint64_t heads = a.cache.kv_heads;
+    if (!s.plan.even) {
+        s.groups = a.requests * most_row_tiles * heads;
+        s.slots = 0;
+    } else {
+        // in parts of p tiles a request of t has at most t / p + 1, and fewer than 2 t / p if it has several; the tiles of all over
+        // p are no more than the target
+        const uint64_t finest = row_tiles * heads * (tiles <= s.plan.least ? 1 : (tiles + s.plan.least - 1) / s.plan.least);
+        s.groups = row_tiles * heads + s.plan.target;
+        if (s.groups > finest) s.groups = finest;
+        s.slots = tiles <= s.plan.least ? 0 : 2 * static_cast<uint64_t>(s.plan.target) < s.groups ? 2 * static_cast<uint64_t>(s.plan.target) : s.groups;
+    }
+    s.groups = (s.groups + 8 * most_row_tiles - 1) / (8 * most_row_tiles) * (8 * most_row_tiles);
     return s;
 }
 
 size_t part_out_bytes(const TreeAttentionArgs& a, const Shape& s) {
-    return (static_cast<size_t>(s.splits) * a.tokens * a.heads * a.cache.head_dim * sizeof(float) + 255) / 256 * 256;
+    return (s.slots * s.rows_a_tile() * a.cache.head_dim * sizeof(float) + 255) / 256 * 256;
 }
 
-template <int kDim, bool kBf16, bool kF32, int kQ, int kKeyGroups>
+template <int kDim, bool kBf16, bool kF32, int kQ, int kWaves, int kStages>
 hipError_t attend(hipStream_t stream, const TreeAttentionArgs& a, const Shape& s, void* workspace) {
     static LdsLimit limit;
-    constexpr size_t lds = attention_lds_bytes<kDim, kQ, kKeyGroups>();
-    const auto kernel = tree_attention_kernel<kDim, kBf16, kF32, kQ, kKeyGroups>;
+    constexpr size_t lds = static_cast<size_t>(kStages) * 2 * kTile * kDim * 2;
+    const auto kernel = tree_attention_kernel<kDim, kBf16, kF32, kQ, kWaves, kStages>;
     hipError_t e = allow_lds(kernel, lds, &limit);
     if (e != hipSuccess) return e;
     float* part_out = static_cast<float*>(workspace);
-    Part* parts = s.splits > 1 ? reinterpret_cast<Part*>(static_cast<char*>(workspace) + part_out_bytes(a, s)) : nullptr;
-    const uint32_t items = a.requests * a.cache.kv_heads * s.splits;
-    kernel<<<(items + 7) / 8 * 8 * s.row_tiles, kThreads, lds, stream>>>(a, s.row_tiles, s.splits, s.split_keys, part_out, parts);
+    Part* parts = s.slots != 0 ? reinterpret_cast<Part*>(static_cast<char*>(workspace) + part_out_bytes(a, s)) : nullptr;
+    kernel<<<static_cast<uint32_t>(s.groups), kWaves * 64, lds, stream>>>(a, s.plan, part_out, parts);
     e = hipGetLastError();
-    if (e != hipSuccess || s.splits == 1) return e;
-    const dim3 grid(static_cast<uint32_t>((static_cast<uint64_t>(a.max_query_len) * a.heads + kWaves - 1) / kWaves), a.requests);
-    join_parts_kernel<kBf16, kF32><<<grid, kThreads, 0, stream>>>(a, s.splits, part_out, parts);
+    if (e != hipSuccess || s.slots == 0) return e;
+    constexpr int kLanes = kDim / 4;
+    constexpr int kJoinRows = kJoinThreads / (kLanes * kJoinGroups);
+    const dim3 grid(static_cast<uint32_t>((static_cast<uint64_t>(a.max_query_len) * a.heads + kJoinRows - 1) / kJoinRows), a.requests);
+    join_parts_kernel<kBf16, kF32, kLanes><<<grid, kJoinThreads, 0, stream>>>(a, s.plan, s.rows_a_tile(), part_out, parts);
     return hipGetLastError();
 }
 
+// The ring's length: as many stages as let two workgroups of four wavefronts, or five of one, on a unit's 160 KiB of LDS.
 template <int kDim, bool kBf16, bool kF32>
 hipError_t attend_rows(hipStream_t stream, const TreeAttentionArgs& a, const Shape& s, void* workspace) {
     if constexpr (kDim == 256) {
-        if (s.key_groups == 2) return attend<kDim, kBf16, kF32, 1, 2>(stream, a, s, workspace);
-        return attend<kDim, kBf16, kF32, 1, 1>(stream, a, s, workspace);
+        if (s.waves == 1) return attend<kDim, kBf16, kF32, 1, 1, 2>(stream, a, s, workspace);
+        if (s.waves == 2) return attend<kDim, kBf16, kF32, 1, 2, 2>(stream, a, s, workspace);
+        return attend<kDim, kBf16, kF32, 1, 4, 2>(stream, a, s, workspace);
     } else {
-        if (s.sixteens == 1) return attend<kDim, kBf16, kF32, 1, 4>(stream, a, s, workspace);
-        if (s.key_groups == 4) return attend<kDim, kBf16, kF32, 2, 4>(stream, a, s, workspace);
-        if (s.key_groups == 2) return attend<kDim, kBf16, kF32, 2, 2>(stream, a, s, workspace);
-        return attend<kDim, kBf16, kF32, 2, 1>(stream, a, s, workspace);
+        constexpr int kAlone = kDim == 64 ? 3 : 2;
+        if (s.sixteens == 1) return attend<kDim, kBf16, kF32, 1, 1, kAlone>(stream, a, s, workspace);
+        if (s.waves == 1) return attend<kDim, kBf16, kF32, 2, 1, kAlone>(stream, a, s, workspace);
+        if (s.waves == 2) return attend<kDim, kBf16, kF32, 2, 2, 3>(stream, a, s, workspace);
+        return attend<kDim, kBf16, kF32, 2, 4, 4>(stream, a, s, workspace);
     }
 }
 
@@ -630,8 +740,10 @@ hipError_t attend_types(hipStream_t stream, const TreeAttentionArgs& a, const Sh
 
 size_t tree_attention_workspace_bytes(const TreeAttentionArgs& args, int compute_units) {
     const Shape s = shape_of(args, compute_units);
-    return s.splits == 1 ? 0 : part_out_bytes(args, s) + static_cast<size_t>(s.splits) * args.tokens * args.heads * sizeof(Part);
+    return s.slots == 0 ? 0 : part_out_bytes(args, s) + s.slots * s.rows_a_tile() * sizeof(Part);
 }
+
+bool tree_attention_fits_a_launch(const TreeAttentionArgs& args, int compute_units) { return shape_of(args, compute_units).groups <= 0x7fffffff; }
 
 hipError_t launch_tree_attention(hipStream_t stream, const TreeAttentionArgs& args, void* workspace, int compute_units) {
     const Shape s = shape_of(args, compute_units);

@@ -59,6 +59,7 @@ struct TreeAttentionArgs {
     bool cache_bf16, f32;  // f32: query and out; otherwise they are of the cache's type
 };
 size_t tree_attention_workspace_bytes(const TreeAttentionArgs& args, int compute_units);
+bool tree_attention_fits_a_launch(const TreeAttentionArgs& args, int compute_units);
 hipError_t launch_tree_attention(hipStream_t stream, const TreeAttentionArgs& args, void* workspace, int compute_units);
 
 }  // namespace afhip
