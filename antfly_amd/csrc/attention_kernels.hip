@@ -34,9 +34,11 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 constexpr int kTile = 32;             // keys of one wavefront's step
 constexpr uint32_t kNowhere = ~0u;    // of a key that has no place in the cache
 constexpr float kLog2e = 1.4426950408889634f;
-// A row's maximum follows its scores only when they pass it by more than 2^kSlack: the weights stay below 2^kSlack, far
-// inside every type here, and most tiles leave the sums as they are.
+// The number that is taken off a row's scores follows their maximum only when that passes it by more than kSlack: the weights
+// stay below 2^kSlack, far inside every type here, most tiles leave the sums as they are, and no lane has to know the others'
+// scores to see that.
 constexpr float kSlack = 8.0f;
+constexpr float kUnset = 1e38f;
 
 template <bool kBf16>
 __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
@@ -126,7 +128,7 @@ __device__ __forceinline__ bool is_odd(short v) {
     return (v & kExponent) == kExponent;
 }
 
-__device__ const uint4 kNothing{0, 0, 0, 0};  // what keys without a place and values past a head's end are loaded from
+__device__ const uint4 kNothing{0, 0, 0, 0};  // what values past a head's end are loaded from
 
 // 16 bytes a lane from memory to 1 KiB of LDS from `to` on (a uniform address).
 __device__ __forceinline__ void load_to_lds(uint32_t to, const uint4* from) {
@@ -184,7 +186,7 @@ __device__ __forceinline__ T sum_up_to(T v, int lane) {  // over the wavefront's
 
 // How the keys are shared out.  A part has the same number of tiles for all requests (rounded to whole tiles and evened out
 // within a request): all the batch's tiles of keys, counted once for every row tile and key head, over plan.target
-// workgroups, `least` tiles at least.  Workgroups are numbered by request, key head, part, row tile; parts of requests that
+// workgroups, and `least` tiles at least.  Workgroups are numbered by request, key head, part, row tile; parts of requests that
 // have several are numbered the same way.  Every wavefront works this out for itself from the lengths.
 struct SharePlan {
     uint32_t target, least;
@@ -209,17 +211,17 @@ __device__ __forceinline__ bool find_share(const TreeAttentionArgs& a, const Sha
         return true;
     }
     Share mine{};
-    unsigned long long work = 0;
+    float work = 0.0f;  // (a float's error is far below the whole tiles that parts are rounded to: 2^-10 more covers it)
     for (uint32_t r0 = 0; r0 < a.requests; r0 += 64) {
         if (r0 + lane < a.requests) {
             mine = lengths_of(a, r0 + lane, rows_a_tile);
-            work += static_cast<unsigned long long>((mine.keys + kTile - 1) / kTile) * mine.row_tiles;
+            work += static_cast<float>((mine.keys + kTile - 1) / kTile) * static_cast<float>(mine.row_tiles);
         }
     }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) work += __shfl_xor(work, d);
-    const unsigned long long each = (work * heads + plan.target - 1) / plan.target;
-    const uint32_t tiles = static_cast<uint32_t>(min(max(each, static_cast<unsigned long long>(plan.least)), 0x7fffffffull));
+    const float each = work * (static_cast<float>(heads) * 1.001f) / static_cast<float>(plan.target);
+    const uint32_t tiles = max(static_cast<uint32_t>(fminf(each, 0x1p30f)) + 1, plan.least);
     uint32_t before = 0, slots_before = 0;
     for (uint32_t r0 = 0; r0 < a.requests; r0 += 64) {
         uint32_t count = 0, slots = 0;
@@ -295,6 +297,7 @@ __global__ __launch_bounds__(kWaves * 64, kF32 || kDim == 256 ? 1 : 2) void tree
     }
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
     const int pieces = static_cast<int>(a.cache.head_dim / 8);  // that hold something
+    const bool whole_heads = pieces == kPieces;
 
     // where 64 blocks from `window_at` on lie, in 16-byte units, one a lane
     const int* table = a.block_tables + static_cast<size_t>(request) * a.table_columns;
@@ -315,13 +318,21 @@ __global__ __launch_bounds__(kWaves * 64, kF32 || kDim == 256 ? 1 : 2) void tree
     // Requests this wavefront's part of a tile's K and V; which of its keys have a place.
     auto request_tile = [&](int tile, int stage) -> uint32_t {
         const uint32_t at = place(tile);  // lane l % 32 has the place of key l % 32
+        // a key without a place is not seen by any row: what is loaded for it may be anything
+        const int there = static_cast<int>(at == kNowhere ? 0u : at);
         const uint32_t to = lds_at + stage * (2 * kTileBytes) + wave * (kLoads * 1024);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int slot = (wave * kLoads + i) * 64 + lane, row = slot / kPieces, kp = key_piece<kDim>(row, slot % kPieces) % kPieces, vp = value_piece<kDim>(row, slot % kPieces) % kPieces;
-            const uint32_t from = static_cast<uint32_t>(__shfl(static_cast<int>(at), row));
-            load_to_lds(to + i * 1024, from != kNowhere && kp < pieces ? a.cache.keys + (from + kp) : &kNothing);
-            load_to_lds(to + kTileBytes + i * 1024, from != kNowhere && vp < pieces ? a.cache.values + (from + vp) : &kNothing);
+            const int slot = (wave * kLoads + i) * 64 + lane, row = slot / kPieces;
+            const int kp = key_piece<kDim>(row, slot % kPieces) % kPieces, vp = value_piece<kDim>(row, slot % kPieces) % kPieces;
+            const uint32_t from = static_cast<uint32_t>(__shfl(there, row));
+            const uint4 *k = a.cache.keys + (from + kp), *v = a.cache.values + (from + vp);
+            if (!whole_heads) {
+                if (kp >= pieces) k = &kNothing;
+                if (vp >= pieces) v = &kNothing;
+            }
+            load_to_lds(to + i * 1024, k);
+            load_to_lds(to + kTileBytes + i * 1024, v);
         }
         return static_cast<uint32_t>(__ballot(at != kNowhere));
     };
@@ -399,10 +410,12 @@ __global__ __launch_bounds__(kWaves * 64, kF32 || kDim == 256 ? 1 : 2) void tree
     }
 
     f32x4 out[kQ][kDim / 16];
-    float most[kQ], sum[kQ];  // the largest product so far (before `unit`), and this lane's part of the weights' sum
+    // A weight is exp2(product * unit + shift): the shift takes off the row's largest score (up to kSlack more than it), kUnset
+    // until the row has seen a key.  And this lane's part of the weights' sum.
+    float shift[kQ], sum[kQ];
 #pragma unroll
     for (int qt = 0; qt < kQ; ++qt) {
-        most[qt] = -__builtin_inff();
+        shift[qt] = kUnset;
         sum[qt] = 0.0f;
 #pragma unroll
         for (int d = 0; d < kDim / 16; ++d) out[qt][d] = f32x4{0, 0, 0, 0};
@@ -431,7 +444,8 @@ __global__ __launch_bounds__(kWaves * 64, kF32 || kDim == 256 ? 1 : 2) void tree
         for (int half = 0; half < 2; ++half) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
-                const s16x8 k = *reinterpret_cast<const s16x8*>(k_lds + key_piece<kDim>(half * 16 + column, s * 4 + quarter) * 16);
+                // (rows 16 apart have their pieces in the same order)
+                const s16x8 k = *reinterpret_cast<const s16x8*>(k_lds + key_piece<kDim>(column, s * 4 + quarter) * 16 + half * (16 * kDim * 2));
 #pragma unroll
                 for (int qt = 0; qt < kQ; ++qt) {
 #pragma unroll
@@ -443,7 +457,9 @@ __global__ __launch_bounds__(kWaves * 64, kF32 || kDim == 256 ? 1 : 2) void tree
         uint32_t odd = 0;  // keys with a value that is no finite number (looked for only where some row may not see them)
         uint32_t seen[kQ];
         if (!clean) {
-            for (int at = lane; at < kTile * kPieces; at += 64) {
+            // (all rows see the context's keys)
+            const int from_row = held != ~0u ? 0 : max(context - tile, 0);
+            for (int at = from_row * kPieces + lane; at < kTile * kPieces; at += 64) {
                 const uint4 v = *reinterpret_cast<const uint4*>(v_lds + at * 16);
                 unsigned long long which = __ballot(is_odd<kBf16>(v.x) || is_odd<kBf16>(v.y) || is_odd<kBf16>(v.z) || is_odd<kBf16>(v.w));
                 while (which != 0) {
@@ -464,36 +480,39 @@ __global__ __launch_bounds__(kWaves * 64, kF32 || kDim == 256 ? 1 : 2) void tree
                 }
             }
         }
-        float peak[kQ];
+        float x[kQ][8];
         bool passes = false;
 #pragma unroll
         for (int qt = 0; qt < kQ; ++qt) {
-            const f32x4 x = score[qt][0], y = score[qt][1];
-            peak[qt] = row_max(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]))));
-            passes |= (peak[qt] - most[qt]) * unit[qt] > kSlack;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[qt][j] = __builtin_fmaf(score[qt][j >> 2][j & 3], unit[qt], shift[qt]);
+            passes |= fmaxf(fmaxf(fmaxf(x[qt][0], x[qt][1]), fmaxf(x[qt][2], x[qt][3])), fmaxf(fmaxf(x[qt][4], x[qt][5]), fmaxf(x[qt][6], x[qt][7]))) > kSlack;
         }
         if (__any(passes)) {
 #pragma unroll
             for (int qt = 0; qt < kQ; ++qt) {
+                const f32x4 lo = score[qt][0], hi = score[qt][1];
+                const float peak = row_max(fmaxf(fmaxf(fmaxf(lo[0], lo[1]), fmaxf(lo[2], lo[3])), fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3]))));
                 // each row by itself: no other row's keys move its bits
-                const float next = (peak[qt] - most[qt]) * unit[qt] > kSlack ? peak[qt] : most[qt];
-                const float by = most[qt] == next ? 1.0f : __builtin_amdgcn_exp2f((most[qt] - next) * unit[qt]);
-                most[qt] = next;
+                const float next = __builtin_fmaf(peak, unit[qt], shift[qt]) > kSlack ? -peak * unit[qt] : shift[qt];
+                const float by = next == shift[qt] ? 1.0f : __builtin_amdgcn_exp2f(next - shift[qt]);
+                shift[qt] = next;
                 sum[qt] *= by;
 #pragma unroll
                 for (int d = 0; d < kDim / 16; ++d) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) out[qt][d][j] *= by;
                 }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[qt][j] = __builtin_fmaf(score[qt][j >> 2][j & 3], unit[qt], next);
             }
         }
         s16x8 weight[kQ][kTerms];
 #pragma unroll
         for (int qt = 0; qt < kQ; ++qt) {
-            const float from = most[qt] == -__builtin_inff() ? 0.0f : -most[qt] * unit[qt];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(score[qt][j >> 2][j & 3], unit[qt], from));
+                const float p = __builtin_amdgcn_exp2f(x[qt][j]);
                 sum[qt] += p;
                 float rest = p;
 #pragma unroll
@@ -509,8 +528,8 @@ __global__ __launch_bounds__(kWaves * 64, kF32 || kDim == 256 ? 1 : 2) void tree
             s16x8 v;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const int row = half * 16 + quarter * 4 + (column >> 2);
-                const char* from = v_lds + value_piece<kDim>(row, d * 2 + (column >> 1 & 1)) * 16 + (column & 1) * 8;
+                const int row = quarter * 4 + (column >> 2);
+                const char* from = v_lds + value_piece<kDim>(row, d * 2 + (column >> 1 & 1)) * 16 + (column & 1) * 8 + half * (16 * kDim * 2);
                 const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)from);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[half * 4 + j] = four[j];
@@ -562,7 +581,7 @@ __global__ __launch_bounds__(kWaves * 64, kF32 || kDim == 256 ? 1 : 2) void tree
         const size_t token = static_cast<size_t>(begin + row_token[qt]);
         const int head = static_cast<int>(kv_head) * group + row % group;
         const size_t part = static_cast<size_t>(slot) * kRows + (row - first_row);
-        if (share.splits > 1 && quarter == 0) parts[part] = Part{most[qt] == -__builtin_inff() ? most[qt] : most[qt] * unit[qt], total};
+        if (share.splits > 1 && quarter == 0) parts[part] = Part{shift[qt] == kUnset ? -__builtin_inff() : -shift[qt], total};
         const size_t to = token * a.out_token_stride + static_cast<size_t>(head) * a.out_head_stride;
         const float by = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
@@ -583,71 +602,72 @@ __global__ __launch_bounds__(kWaves * 64, kF32 || kDim == 256 ? 1 : 2) void tree
     }
 }
 
-// The parts of a row, brought to their common maximum.  kLanes lanes have four values of the row each, four groups of them
-// take the parts in turn and add up in LDS.
-constexpr int kJoinThreads = 256, kJoinGroups = 4;
+// The parts of a row, brought to their common maximum: a wavefront takes rows of one request in turn.  kLanes lanes have four
+// values of the row each, 64 / kLanes groups of them every so many-th part; kBatch parts are requested at a time.
+constexpr int kJoinWaves = 4, kBatch = 8;
 template <bool kBf16, bool kF32, int kLanes>
-__global__ __launch_bounds__(kJoinThreads) void join_parts_kernel(TreeAttentionArgs a, SharePlan plan, int rows_a_tile, const float* part_out,
-                                                                 const Part* parts) {
-    constexpr int kJoinRows = kJoinThreads / (kLanes * kJoinGroups);
-    __shared__ f32x4 sums[kJoinGroups][kJoinRows][kLanes];
-    __shared__ Part group_parts[kJoinGroups][kJoinRows];
+__global__ __launch_bounds__(kJoinWaves * 64) void join_parts_kernel(TreeAttentionArgs a, SharePlan plan, int rows_a_tile, const float* part_out,
+                                                                    const Part* parts) {
+    constexpr uint32_t kGroups = 64 / kLanes;
     uint32_t request;
     Share share;
     if (!find_share<true>(a, plan, rows_a_tile, blockIdx.y, &request, &share) || share.splits == 1) return;
-    const int tid = static_cast<int>(threadIdx.x), piece = tid % kLanes, group = tid / kLanes % kJoinGroups, mine = tid / (kLanes * kJoinGroups);
-    const uint32_t rows = static_cast<uint32_t>(share.tokens) * a.group;   // of one key head
-    const uint32_t all = blockIdx.x * kJoinRows + mine, kv_head = all / rows, row = all % rows;
-    if (blockIdx.x * kJoinRows >= rows * a.cache.kv_heads) return;
-    const bool real = kv_head < a.cache.kv_heads;
-    const uint32_t row_tile = row / rows_a_tile;
-    const size_t slot = share.first_slot + static_cast<size_t>(real ? kv_head : 0) * share.splits * share.row_tiles + row_tile;
-    const size_t first = slot * rows_a_tile + row % rows_a_tile, stride = static_cast<size_t>(share.row_tiles) * rows_a_tile;
-    const uint32_t d = piece * 4;
-    float most = -__builtin_inff(), total = 0.0f;
-    f32x4 x{0, 0, 0, 0};
-    for (uint32_t s = group; s < share.splits; s += kJoinGroups) most = fmaxf(most, parts[first + s * stride].most);
-#pragma unroll 4
-    for (uint32_t s = group; s < share.splits; s += kJoinGroups) {
-        const Part part = parts[first + s * stride];
-        if (part.most == -__builtin_inff() || d >= a.cache.head_dim) continue;  // (a part that saw no key is not written)
-        const float by = exp2_between(part.most, most);
-        total = __builtin_fmaf(part.sum, by, total);
-        const f32x4 y = *reinterpret_cast<const f32x4*>(part_out + (first + s * stride) * a.cache.head_dim + d);
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    const uint32_t group = lane / kLanes, d = lane % kLanes * 4;
+    const uint32_t rows = static_cast<uint32_t>(share.tokens) * a.group;  // of one key head
+    const size_t stride = static_cast<size_t>(share.row_tiles) * rows_a_tile;
+    for (uint32_t at = blockIdx.x * kJoinWaves + (threadIdx.x >> 6); at < rows * a.cache.kv_heads; at += gridDim.x * kJoinWaves) {
+        const uint32_t kv_head = at / rows, row = at % rows;
+        const size_t slot = share.first_slot + static_cast<size_t>(kv_head) * share.splits * share.row_tiles + row / rows_a_tile;
+        const size_t first = slot * rows_a_tile + row % rows_a_tile;
+        float most = -__builtin_inff(), total = 0.0f;
+        for (uint32_t s = lane; s < share.splits; s += 64) most = fmaxf(most, parts[first + s * stride].most);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(y[j], by, x[j]);
-    }
-    sums[group][mine][piece] = x;
-    if (piece == 0) group_parts[group][mine] = Part{most, total};
-    __syncthreads();
-    if (group != 0 || !real || d >= a.cache.head_dim) return;
+        for (int w = 1; w < 64; w *= 2) most = fmaxf(most, __shfl_xor(most, w));
+        f32x4 x{0, 0, 0, 0};
+        for (uint32_t s0 = group; s0 < share.splits; s0 += kBatch * kGroups) {
+            f32x4 y[kBatch];
+            Part part[kBatch];
 #pragma unroll
-    for (int g = 0; g < kJoinGroups; ++g) most = fmaxf(most, group_parts[g][mine].most);
-    total = 0.0f;
-    x = f32x4{0, 0, 0, 0};
+            for (int i = 0; i < kBatch; ++i) {  // (past the end: the last part again, not counted)
+                const size_t from = first + min(s0 + i * kGroups, share.splits - 1) * stride;
+                part[i] = parts[from];
+                y[i] = *reinterpret_cast<const f32x4*>(part_out + from * a.cache.head_dim + (d < a.cache.head_dim ? d : 0));
+            }
 #pragma unroll
-    for (int g = 0; g < kJoinGroups; ++g) {
-        const float by = exp2_between(group_parts[g][mine].most, most);
-        total = __builtin_fmaf(group_parts[g][mine].sum, by, total);
-        const f32x4 y = sums[g][mine][piece];
+            for (int i = 0; i < kBatch; ++i) {
+                // (a part that saw no key has not been written)
+                const bool counts = s0 + i * kGroups < share.splits && part[i].most != -__builtin_inff();
+                const float by = counts ? exp2_between(part[i].most, most) : 0.0f;
+                total = __builtin_fmaf(part[i].sum, by, total);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(y[j], by, x[j]);
-    }
-    const float over = total == 0.0f ? 0.0f : 1.0f / total;
-    const size_t token = static_cast<size_t>(share.begin) + row / a.group;
-    const size_t to = token * a.out_token_stride + static_cast<size_t>(kv_head * a.group + row % a.group) * a.out_head_stride + d;
-    if (kF32) {
-        *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to) = x * over;
-    } else {
-        s16x4 y;
+                for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(counts ? y[i][j] : 0.0f, by, x[j]);
+            }
+        }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = narrow<kBf16>(x[j] * over);
-        *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(a.out) + to) = y;
+        for (int w = kLanes; w < 64; w *= 2) {
+            total += __shfl_xor(total, w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] += __shfl_xor(x[j], w);
+        }
+        if (group != 0 || d >= a.cache.head_dim) continue;
+        const float over = total == 0.0f ? 0.0f : 1.0f / total;
+        const size_t token = static_cast<size_t>(share.begin) + row / a.group;
+        const size_t to = token * a.out_token_stride + static_cast<size_t>(kv_head * a.group + row % a.group) * a.out_head_stride + d;
+        if (kF32) {
+            *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to) = x * over;
+        } else {
+            s16x4 y;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = narrow<kBf16>(x[j] * over);
+            *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(a.out) + to) = y;
+        }
     }
 }
 
 struct Shape {
     int dim, sixteens, waves;  // kDim, kQ, kWaves
+    int compute_units;
     SharePlan plan;
     uint64_t groups, slots;  // most workgroups, and parts of requests that have several
     int rows_a_tile() const { return 16 * sixteens * waves; }
@@ -657,14 +677,15 @@ constexpr uint32_t kMostEvened = 1024;  // requests: every wavefront reads their
 
 Shape shape_of(const TreeAttentionArgs& a, int compute_units) {
     Shape s;
+    s.compute_units = compute_units;
     s.dim = a.cache.head_dim <= 64 ? 64 : a.cache.head_dim <= 128 ? 128 : 256;
     const uint64_t rows = static_cast<uint64_t>(a.max_query_len) * a.group;
     if (s.dim == 256) {  // (two sixteens of rows would not fit the registers)
         s.sixteens = 1;
         s.waves = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     } else {
-        s.sixteens = rows <= 16 ? 1 : 2;
-        s.waves = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+        s.sixteens = rows <= 64 ? 1 : 2;
+        s.waves = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     }
     const uint64_t tile_rows = s.rows_a_tile(), most_row_tiles = (rows + tile_rows - 1) / tile_rows;
     // row tiles of the whole batch: every request's last one may be part empty
@@ -674,8 +695,13 @@ Shape shape_of(const TreeAttentionArgs& a, int compute_units) {
     s.plan.even = a.requests <= kMostEvened;
     s.plan.row_tiles = static_cast<uint32_t>(most_row_tiles);
     s.plan.least = 2;  // fewer tiles are not worth a workgroup
-    s.plan.target = static_cast<uint32_t>(compute_units * (s.waves == 1 ? 10 : s.waves == 2 ? 6 : 2));
-    const uint64_t heads = a.cache.kv_heads;
+    const uint64_t heads = a.cache.kv_heads, base = row_tiles * heads;
+    // One round of what the compute units hold at once (by LDS and registers), the workgroups that rounding adds among them; a
+    // batch that fills more than half of that anyway shares out over half a round more.
+    const uint64_t resident = static_cast<uint64_t>(compute_units) * (s.waves == 1 ? 5 : s.waves == 2 ? 3 : 2);
+    uint64_t target = resident > base ? resident - base : 0;
+    if (target < resident / 2) target = resident / 2;
+    s.plan.target = static_cast<uint32_t>(target);
     if (!s.plan.even) {
         s.groups = a.requests * most_row_tiles * heads;
         s.slots = 0;
@@ -707,10 +733,11 @@ hipError_t attend(hipStream_t stream, const TreeAttentionArgs& a, const Shape& s
     kernel<<<static_cast<uint32_t>(s.groups), kWaves * 64, lds, stream>>>(a, s.plan, part_out, parts);
     e = hipGetLastError();
     if (e != hipSuccess || s.slots == 0) return e;
-    constexpr int kLanes = kDim / 4;
-    constexpr int kJoinRows = kJoinThreads / (kLanes * kJoinGroups);
-    const dim3 grid(static_cast<uint32_t>((static_cast<uint64_t>(a.max_query_len) * a.heads + kJoinRows - 1) / kJoinRows), a.requests);
-    join_parts_kernel<kBf16, kF32, kLanes><<<grid, kJoinThreads, 0, stream>>>(a, s.plan, s.rows_a_tile(), part_out, parts);
+    // eight workgroups a compute unit over all requests, or one wavefront a row
+    const uint64_t rows = static_cast<uint64_t>(a.max_query_len) * a.heads, most = (8 * static_cast<uint64_t>(s.compute_units) + a.requests - 1) / a.requests;
+    const uint64_t groups = (rows + kJoinWaves - 1) / kJoinWaves;
+    const dim3 grid(static_cast<uint32_t>(groups < most ? groups : most), a.requests);
+    join_parts_kernel<kBf16, kF32, kDim / 4><<<grid, kJoinWaves * 64, 0, stream>>>(a, s.plan, s.rows_a_tile(), part_out, parts);
     return hipGetLastError();
 }
 
@@ -723,9 +750,9 @@ hipError_t attend_rows(hipStream_t stream, const TreeAttentionArgs& a, const Sha
         return attend<kDim, kBf16, kF32, 1, 4, 2>(stream, a, s, workspace);
     } else {
         constexpr int kAlone = kDim == 64 ? 3 : 2;
-        if (s.sixteens == 1) return attend<kDim, kBf16, kF32, 1, 1, kAlone>(stream, a, s, workspace);
-        if (s.waves == 1) return attend<kDim, kBf16, kF32, 2, 1, kAlone>(stream, a, s, workspace);
-        if (s.waves == 2) return attend<kDim, kBf16, kF32, 2, 2, 3>(stream, a, s, workspace);
+        if (s.waves == 1) return attend<kDim, kBf16, kF32, 1, 1, kAlone>(stream, a, s, workspace);
+        if (s.waves == 2) return attend<kDim, kBf16, kF32, 1, 2, 3>(stream, a, s, workspace);
+        if (s.sixteens == 1) return attend<kDim, kBf16, kF32, 1, 4, 3>(stream, a, s, workspace);
         return attend<kDim, kBf16, kF32, 2, 4, 4>(stream, a, s, workspace);
     }
 }
