@@ -70,7 +70,9 @@ afhip_status afhip_launch_quantize_fp8(void* stream, afhip_buffer q, afhip_buffe
 
 size_t afhip_linear_fp8_workspace_bytes(size_t rows, size_t in_dim, size_t out_dim) {
     if (!dims_fit(rows, in_dim, out_dim) || rows == 0 || out_dim == 0) return 0;
-    return codes_bytes(rows, in_dim) + scales_bytes(rows, in_dim);
+    const int r = static_cast<int>(rows), k = static_cast<int>(in_dim), n = static_cast<int>(out_dim);
+    if (linear_fp8_is_fused(r, k)) return 0;
+    return codes_bytes(rows, in_dim) + scales_bytes(rows, in_dim) + plan_matmul_fp8(r, k, n, gemv_compute_units(), SIZE_MAX).sums_bytes(r, n);
 }
 
 afhip_status afhip_launch_matmul_fp8_f32(void* stream, afhip_buffer dst, afhip_buffer q, afhip_buffer q_scales, afhip_buffer weight,
@@ -83,7 +85,9 @@ afhip_status afhip_launch_matmul_fp8_f32(void* stream, afhip_buffer dst, afhip_b
     if (rows == 0 || out_dim == 0) return AFHIP_OK;
     call.x = reinterpret_cast<const uint8_t*>(q.ptr);
     call.x_scales = reinterpret_cast<const float*>(q_scales.ptr);
-    return status_of(launch_matmul_fp8(static_cast<hipStream_t>(stream), call));
+    const bool lent = workspace.ptr != 0 && workspace.ptr % 256 == 0;
+    const Fp8Plan plan = plan_matmul_fp8(call.rows, call.in_dim, call.out_dim, gemv_compute_units(), lent ? workspace.len : 0);
+    return status_of(launch_matmul_fp8(static_cast<hipStream_t>(stream), call, plan, reinterpret_cast<float*>(workspace.ptr)));
 }
 
 afhip_status afhip_launch_linear_fp8_f32(void* stream, afhip_buffer dst, afhip_buffer input, afhip_buffer weight, afhip_buffer weight_scales,
@@ -94,7 +98,11 @@ afhip_status afhip_launch_linear_fp8_f32(void* stream, afhip_buffer dst, afhip_b
     if (s != AFHIP_OK) return s;
     if (!holds(input, rows * in_dim, 4, 16)) return AFHIP_ERR_INVALID_STATE;
     if (rows == 0 || out_dim == 0) return AFHIP_OK;
-    if (!holds(workspace, afhip_linear_fp8_workspace_bytes(rows, in_dim, out_dim), 1, 256)) return AFHIP_ERR_INVALID_STATE;
+    if (linear_fp8_is_fused(call.rows, call.in_dim))
+        return status_of(launch_linear_fp8_fused(static_cast<hipStream_t>(stream), call, reinterpret_cast<const float*>(input.ptr)));
+    const Fp8Plan plan = plan_matmul_fp8(call.rows, call.in_dim, call.out_dim, gemv_compute_units(), SIZE_MAX);
+    const size_t quantized = codes_bytes(rows, in_dim) + scales_bytes(rows, in_dim);
+    if (!holds(workspace, quantized + plan.sums_bytes(call.rows, call.out_dim), 1, 256)) return AFHIP_ERR_INVALID_STATE;
     uint8_t* codes = reinterpret_cast<uint8_t*>(workspace.ptr);
     float* scales = reinterpret_cast<float*>(workspace.ptr + codes_bytes(rows, in_dim));
     const hipError_t e = launch_quantize_fp8(static_cast<hipStream_t>(stream), codes, scales, reinterpret_cast<const float*>(input.ptr), rows,
@@ -102,7 +110,7 @@ afhip_status afhip_launch_linear_fp8_f32(void* stream, afhip_buffer dst, afhip_b
     if (e != hipSuccess) return static_cast<afhip_status>(e);
     call.x = codes;
     call.x_scales = scales;
-    return status_of(launch_matmul_fp8(static_cast<hipStream_t>(stream), call));
+    return status_of(launch_matmul_fp8(static_cast<hipStream_t>(stream), call, plan, reinterpret_cast<float*>(workspace.ptr + quantized)));
 }
 
 }  // extern "C"

@@ -17,6 +17,7 @@
 #include "fp8_launch.h"
 
 #include <hip/hip_runtime.h>
+#include <math.h>
 
 namespace afhip {
 
@@ -38,229 +39,425 @@ __device__ __forceinline__ f16x8 widen(uint32_t lo, uint32_t hi) {
 }
 
 // ---- quantizer: eight lanes a block, four values of each 32 to a lane
+struct BlockPart {
+    float4 v[4];
+    __device__ __forceinline__ void load(const float* row, int block, int part, int in_dim) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int k = block * kFp8Block + i * 32 + part * 4;
+            v[i] = k < in_dim ? *reinterpret_cast<const float4*>(row + k) : float4{0, 0, 0, 0};
+        }
+    }
+    // four codes for each of the four parts; returns the block's scale
+    __device__ __forceinline__ float quantize(int* codes) const {
+        float most = kTiniest;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            most = fmaxf(most, fmaxf(fmaxf(__builtin_fabsf(v[i].x), __builtin_fabsf(v[i].y)), fmaxf(__builtin_fabsf(v[i].z), __builtin_fabsf(v[i].w))));
+        most = max_over_8(most);
+        const float by = kMost / most;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int low = __builtin_amdgcn_cvt_pk_fp8_f32(v[i].x * by, v[i].y * by, 0, false);
+            codes[i] = __builtin_amdgcn_cvt_pk_fp8_f32(v[i].z * by, v[i].w * by, low, true);
+        }
+        return most / kMost;
+    }
+};
+
 __global__ __launch_bounds__(256) void quantize_fp8_kernel(uint8_t* q, float* scales, const float* x, size_t blocks, int row_blocks, int in_dim) {
     const size_t at = static_cast<size_t>(blockIdx.x) * 32 + threadIdx.x / 8;
     if (at >= blocks) return;
     const size_t row = at / row_blocks;
     const int block = static_cast<int>(at % row_blocks), part = threadIdx.x & 7;
-    const size_t from = row * in_dim;
-    float4 v[4];
-    float most = kTiniest;
+    BlockPart x_part;
+    x_part.load(x + row * in_dim, block, part, in_dim);
+    int codes[4];
+    const float scale = x_part.quantize(codes);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int k = block * kFp8Block + i * 32 + part * 4;
-        v[i] = k < in_dim ? *reinterpret_cast<const float4*>(x + from + k) : float4{0, 0, 0, 0};
-        most = fmaxf(most, fmaxf(fmaxf(__builtin_fabsf(v[i].x), __builtin_fabsf(v[i].y)), fmaxf(__builtin_fabsf(v[i].z), __builtin_fabsf(v[i].w))));
+        if (k < in_dim) *reinterpret_cast<int*>(q + row * in_dim + k) = codes[i];
     }
-    most = max_over_8(most);
-    const float by = kMost / most;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int k = block * kFp8Block + i * 32 + part * 4;
-        int code = __builtin_amdgcn_cvt_pk_fp8_f32(v[i].x * by, v[i].y * by, 0, false);
-        code = __builtin_amdgcn_cvt_pk_fp8_f32(v[i].z * by, v[i].w * by, code, true);
-        if (k < in_dim) *reinterpret_cast<int*>(q + from + k) = code;
-    }
-    if (part == 0) scales[at] = most / kMost;
+    if (part == 0) scales[at] = scale;
 }
 
-// ---- few rows: operands from memory into registers
+// ---- what both kernels share
 //
-// A workgroup has 16 kN columns of W and 16 kM rows of X; its wavefronts share out the blocks of K (in turn) and add up in
-// LDS.  kAhead blocks are requested at a time.
-template <int kM, int kN, int kWaves, int kAhead>
+// Codes come from memory straight into LDS, whole 128-byte blocks of a row, 1 KiB (eight rows) an instruction.  16-byte piece p
+// of row r lies at place p ^ (r / 2 % 8) of the row's 128 bytes: the same piece of 16 rows, what an operand's lanes read, falls
+// on all banks (two rows to 256 bytes).
+__device__ const uint4 kNothing{0, 0, 0, 0};  // what pieces past in_dim are loaded from
+
+__device__ __forceinline__ void load_to_lds(uint32_t to, const void* from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ void load_dword_to_lds(uint32_t to, const void* from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(to), "v"(from) : "memory", "m0");
+}
+// s_waitcnt for "at most kLeft vector memory operations outstanding" (nothing else waited for).
+template <int kLeft>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kLeft) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p));
+}
+
+// One float by a scalar load (a vector load would stand in the queue behind the blocks on their way, and wait for them).  The
+// address is the same for the whole wavefront.
+__device__ __forceinline__ float load_uniform(const float* p) { return *(const __attribute__((address_space(4))) float*)p; }
+
+// Rows [first, first + 8) of a block to LDS (eight lanes a row); `rows`: how many the matrix has, `pieces`: of a row.
+__device__ __forceinline__ void request_rows(uint32_t to, const uint8_t* matrix, int first, int in_tile, int rows, int in_dim, int block, int lane) {
+    const int row = lane >> 3, piece = block * 8 + ((lane & 7) ^ ((in_tile + row) >> 1 & 7));
+    const uint8_t* from = matrix + static_cast<size_t>(min(first + row, rows - 1)) * in_dim + piece * 16;
+    load_to_lds(to, piece * 16 < in_dim ? static_cast<const void*>(from) : &kNothing);
+}
+__device__ __forceinline__ uint4 read_piece(const char* tile, int row, int piece) {
+    return *reinterpret_cast<const uint4*>(tile + row * 128 + (piece ^ (row >> 1 & 7)) * 16);
+}
+
+// ---- few rows
+//
+// A workgroup has 16 columns of W and 16 kM rows of X.  Its wavefronts share out the blocks of K in turn and add up at the end:
+// each works alone, with a ring of kStages blocks in LDS (its W, X and X's scales) and no barrier in the loop.
+template <int kM, int kWaves, int kStages>
 __global__ __launch_bounds__(kWaves * 64) void matmul_fp8_rows_kernel(Fp8Matmul a) {
-    __shared__ float sums[kWaves][16 * kM][16 * kN + 4];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, column = lane & 15, quarter = lane >> 4;
-    const int first_o = blockIdx.x * 16 * kN, first_r = blockIdx.y * 16 * kM;
+    constexpr int kRows = 16 * kM, kStage = 2048 + kRows * 128 + 256;  // W, X, a scale a row
+    constexpr int kLoads = 2 + 2 * kM + 1;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, column = lane & 15, quarter = lane >> 4;
+    const int first_o = blockIdx.x * 16, first_r = blockIdx.y * kRows;
     const int blocks = fp8_blocks(a.in_dim);
-    const uint4* w[kN];
-    const uint4* x[kM];
-    const float* x_scale[kM];
-    const float* w_scale[kN];
+    const float* w_scale = a.w_scales + static_cast<size_t>(first_o / kFp8Block) * blocks;
+    char* ring = lds + wave * (kStages * kStage);
+    const uint32_t ring_at = lds_address(ring);
+    const float* x_scale = a.x_scales + static_cast<size_t>(min(first_r + min(lane, kRows - 1), a.rows - 1)) * blocks;
+
+    auto request = [&](int block, int stage) {
+        const uint32_t to = ring_at + stage * kStage;
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
-        w[n] = reinterpret_cast<const uint4*>(a.w + static_cast<size_t>(min(first_o + n * 16 + column, a.out_dim - 1)) * a.in_dim);
-        w_scale[n] = a.w_scales + static_cast<size_t>(min(first_o + n * 16, a.out_dim - 1) / kFp8Block) * blocks;
+        for (int i = 0; i < 2; ++i) request_rows(to + i * 1024, a.w, first_o + i * 8, i * 8, a.out_dim, a.in_dim, block, lane);
+#pragma unroll
+        for (int i = 0; i < 2 * kM; ++i) request_rows(to + 2048 + i * 1024, a.x, first_r + i * 8, i * 8, a.rows, a.in_dim, block, lane);
+        load_dword_to_lds(to + 2048 + kRows * 128, x_scale + block);
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+        if (wave + i * kWaves < blocks) request(wave + i * kWaves, i);
     }
+    f32x4 total[kM];
 #pragma unroll
-    for (int m = 0; m < kM; ++m) {
-        const size_t row = min(first_r + m * 16 + column, a.rows - 1);
-        x[m] = reinterpret_cast<const uint4*>(a.x + row * a.in_dim);
-        x_scale[m] = a.x_scales + row * blocks;
-    }
-    f32x4 total[kN][kM];
+    for (int m = 0; m < kM; ++m) total[m] = f32x4{0, 0, 0, 0};
+    int stage = 0, free_stage = kStages - 1;
+    float ws_ahead = wave < blocks ? load_uniform(w_scale + wave) : 0.0f;
+    for (int b = wave; b < blocks; b += kWaves) {
+        if (b + (kStages - 2) * kWaves < blocks) wait_loads<kLoads * (kStages - 2)>();
+        else wait_loads<0>();
+        if (b + (kStages - 1) * kWaves < blocks) request(b + (kStages - 1) * kWaves, free_stage);
+        const char* w = ring + stage * kStage;
+        const char* x = w + 2048;
+        const float* scales = reinterpret_cast<const float*>(x + kRows * 128);
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+        free_stage = free_stage + 1 == kStages ? 0 : free_stage + 1;
+        const float ws = ws_ahead;
+        if (b + kWaves < blocks) ws_ahead = load_uniform(w_scale + b + kWaves);
+        f32x4 dot[kM];
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
-#pragma unroll
-        for (int m = 0; m < kM; ++m) total[n][m] = f32x4{0, 0, 0, 0};
-    }
-    const int pieces = a.in_dim / 16;
-    const uint4 zero{0, 0, 0, 0};
-    for (int b0 = wave; b0 < blocks; b0 += kWaves * kAhead) {
-        uint4 wv[kAhead][kN][2], xv[kAhead][kM][2];
-        float ws[kAhead][kN], xs[kAhead][kM];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const int b = b0 + i * kWaves;
-            const int p0 = b * 8 + quarter, p1 = p0 + 4;
-            const bool first = b < blocks && p0 < pieces, second = b < blocks && p1 < pieces;
-#pragma unroll
-            for (int n = 0; n < kN; ++n) {
-                wv[i][n][0] = first ? w[n][p0] : zero;
-                wv[i][n][1] = second ? w[n][p1] : zero;
-                ws[i][n] = b < blocks ? w_scale[n][b] : 0.0f;
-            }
+        for (int k = 0; k < 2; ++k) {
+            const uint4 wp = read_piece(w, column, k * 4 + quarter);
+            const f16x8 w0 = widen(wp.x, wp.y), w1 = widen(wp.z, wp.w);
 #pragma unroll
             for (int m = 0; m < kM; ++m) {
-                xv[i][m][0] = first ? x[m][p0] : zero;
-                xv[i][m][1] = second ? x[m][p1] : zero;
-                xs[i][m] = b < blocks ? x_scale[m][b] : 0.0f;
+                const uint4 xp = read_piece(x + m * 2048, column, k * 4 + quarter);
+                dot[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w0, widen(xp.x, xp.y), k == 0 ? f32x4{0, 0, 0, 0} : dot[m], 0, 0, 0);
+                dot[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w1, widen(xp.z, xp.w), dot[m], 0, 0, 0);
             }
         }
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            f32x4 dot[kN][kM];
+        for (int m = 0; m < kM; ++m) {
+            const float scale = scales[m * 16 + column] * ws;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                f16x8 wide_w[kN], wide_x[kM];
-#pragma unroll
-                for (int n = 0; n < kN; ++n) wide_w[n] = k & 1 ? widen(wv[i][n][k / 2].z, wv[i][n][k / 2].w) : widen(wv[i][n][k / 2].x, wv[i][n][k / 2].y);
-#pragma unroll
-                for (int m = 0; m < kM; ++m) wide_x[m] = k & 1 ? widen(xv[i][m][k / 2].z, xv[i][m][k / 2].w) : widen(xv[i][m][k / 2].x, xv[i][m][k / 2].y);
-#pragma unroll
-                for (int n = 0; n < kN; ++n) {
-#pragma unroll
-                    for (int m = 0; m < kM; ++m)
-                        dot[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wide_w[n], wide_x[m], k == 0 ? f32x4{0, 0, 0, 0} : dot[n][m], 0, 0, 0);
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < kN; ++n) {
-#pragma unroll
-                for (int m = 0; m < kM; ++m) {
-                    const float scale = xs[i][m] * ws[i][n];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) total[n][m][j] = __builtin_fmaf(dot[n][m][j], scale, total[n][m][j]);
-                }
-            }
+            for (int j = 0; j < 4; ++j) total[m][j] = __builtin_fmaf(dot[m][j], scale, total[m][j]);
         }
     }
+    constexpr int kPitch = 20;  // floats of a row's 16 columns
+    float* sums = reinterpret_cast<float*>(lds);  // [kWaves][kRows][kPitch]
+    __syncthreads();                              // everyone is done with the ring
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
-#pragma unroll
-        for (int m = 0; m < kM; ++m) *reinterpret_cast<f32x4*>(&sums[wave][m * 16 + column][n * 16 + quarter * 4]) = total[n][m];
-    }
+    for (int m = 0; m < kM; ++m) *reinterpret_cast<f32x4*>(sums + (wave * kRows + m * 16 + column) * kPitch + quarter * 4) = total[m];
     __syncthreads();
-    for (int i = threadIdx.x; i < 256 * kM * kN; i += kWaves * 64) {
-        const int m = i / (16 * kN), n = i % (16 * kN), row = first_r + m, o = first_o + n;
+    for (int i = threadIdx.x; i < kRows * 16; i += kWaves * 64) {
+        const int m = i / 16, n = i % 16, row = first_r + m, o = first_o + n;
         if (row >= a.rows || o >= a.out_dim) continue;
         float v = 0.0f;
 #pragma unroll
-        for (int s = 0; s < kWaves; ++s) v += sums[s][m][n];
+        for (int s = 0; s < kWaves; ++s) v += sums[(s * kRows + m) * kPitch + n];
         const size_t to = static_cast<size_t>(row) * a.out_dim + o;
         a.y[to] = finish_output(a.ep, o, to, v);
     }
 }
 
-// ---- many rows: tiles through LDS
+// ---- few values of X: quantized by every workgroup itself
 //
-// 128 rows of X and 128 columns of W a workgroup, four wavefronts with 64 x 64 results each; a block of K (128 bytes a row)
-// at a time, the next one on its way from memory straight into the other half of LDS.  16-byte piece p of row r lies at
-// place p ^ (r % 8): eight lanes that read the same piece of eight rows fall on other banks.
-__device__ const uint4 kZeroPiece{0, 0, 0, 0};  // what pieces past in_dim are loaded from
+// While the first blocks of W are on their way, a workgroup quantizes all of X (up to 16 rows, kFusedValues values) into LDS: one
+// launch instead of two, and X read by every workgroup from L2.
+constexpr int kFusedWaves = 8, kFusedStages = 4;
+__global__ __launch_bounds__(kFusedWaves * 64) void linear_fp8_rows_kernel(Fp8Matmul a, const float* input) {
+    constexpr int kWaves = kFusedWaves, kStages = kFusedStages, kLoads = 2;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, column = lane & 15, quarter = lane >> 4;
+    const int first_o = blockIdx.x * 16, blocks = fp8_blocks(a.in_dim);
+    const float* w_scale = a.w_scales + static_cast<size_t>(first_o / kFp8Block) * blocks;
+    char* ring = lds + wave * (kStages * 2048);
+    const uint32_t ring_at = lds_address(ring);
+    const int x_pitch = blocks * kFp8Block + 16;  // bytes of a row of codes: rows fall on other banks
+    char* x_codes = lds + kWaves * kStages * 2048;
+    float* x_scales = reinterpret_cast<float*>(x_codes + a.rows * x_pitch);  // [rows][blocks]
 
-__global__ __launch_bounds__(256) void matmul_fp8_tile_kernel(Fp8Matmul a) {
-    __shared__ __attribute__((aligned(16))) char lds[2][2][128 * 128];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int first_o = blockIdx.x * 128, first_r = blockIdx.y * 128;
-    const int blocks = fp8_blocks(a.in_dim), pieces = a.in_dim / 16;
-    const int wave_o = (wave & 1) * 64, wave_r = (wave >> 1) * 64;
-    const float* w_scale = a.w_scales + static_cast<size_t>(blockIdx.x) * blocks;
-    const float* x_scale[2];
+    const int parts = a.rows * blocks, part = threadIdx.x & 7;
+    BlockPart first_part;
+    const int mine = threadIdx.x / 8;
+    if (mine < parts) first_part.load(input + static_cast<size_t>(mine / blocks) * a.in_dim, mine % blocks, part, a.in_dim);
+    auto request = [&](int block, int stage) {
 #pragma unroll
-    for (int m = 0; m < 2; ++m) x_scale[m] = a.x_scales + static_cast<size_t>(min(first_r + wave_r + m * 32 + (lane & 31), a.rows - 1)) * blocks;
-
-    auto request = [&](int b, int half) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int slot = i * 256 + wave * 64 + lane, row = slot >> 3, piece = b * 8 + ((slot & 7) ^ (row & 7));
-            const uint4* w = reinterpret_cast<const uint4*>(a.w + static_cast<size_t>(min(first_o + row, a.out_dim - 1)) * a.in_dim) + piece;
-            const uint4* x = reinterpret_cast<const uint4*>(a.x + static_cast<size_t>(min(first_r + row, a.rows - 1)) * a.in_dim) + piece;
-            if (piece >= pieces) w = x = &kZeroPiece;
-            char* to = lds[half][0] + (i * 256 + wave * 64) * 16;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)w, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)x, (__attribute__((address_space(3))) void*)(to + 128 * 128), 16, 0, 0);
-        }
+        for (int i = 0; i < 2; ++i) request_rows(ring_at + stage * 2048 + i * 1024, a.w, first_o + i * 8, i * 8, a.out_dim, a.in_dim, block, lane);
     };
-    f32x16 total[2][2];
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+        if (wave + i * kWaves < blocks) request(wave + i * kWaves, i);
+    }
+    for (int at = mine; at < parts; at += kWaves * 8) {
+        const int row = at / blocks, block = at % blocks;
+        if (at != mine) first_part.load(input + static_cast<size_t>(row) * a.in_dim, block, part, a.in_dim);
+        int codes[4];
+        const float scale = first_part.quantize(codes);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<int*>(x_codes + row * x_pitch + block * kFp8Block + i * 32 + part * 4) = codes[i];
+        if (part == 0) x_scales[at] = scale;
+    }
+    __syncthreads();
+    const int row = min(column, a.rows - 1);
+    const char* x = x_codes + row * x_pitch;
+    f32x4 total{0, 0, 0, 0};
+    int stage = 0, free_stage = kStages - 1;
+    float ws_ahead = wave < blocks ? load_uniform(w_scale + wave) : 0.0f;
+    for (int b = wave; b < blocks; b += kWaves) {
+        if (b + (kStages - 2) * kWaves < blocks) wait_loads<kLoads * (kStages - 2)>();
+        else wait_loads<0>();
+        if (b + (kStages - 1) * kWaves < blocks) request(b + (kStages - 1) * kWaves, free_stage);
+        const char* w = ring + stage * 2048;
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+        free_stage = free_stage + 1 == kStages ? 0 : free_stage + 1;
+        const float ws = ws_ahead;
+        if (b + kWaves < blocks) ws_ahead = load_uniform(w_scale + b + kWaves);
+        f32x4 dot{0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint4 wp = read_piece(w, column, k * 4 + quarter);
+            const uint4 xp = *reinterpret_cast<const uint4*>(x + b * kFp8Block + (k * 4 + quarter) * 16);
+            dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(wp.x, wp.y), widen(xp.x, xp.y), dot, 0, 0, 0);
+            dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(wp.z, wp.w), widen(xp.z, xp.w), dot, 0, 0, 0);
+        }
+        const float scale = x_scales[row * blocks + b] * ws;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) total[j] = __builtin_fmaf(dot[j], scale, total[j]);
+    }
+    constexpr int kPitch = 20;
+    float* sums = reinterpret_cast<float*>(lds);  // [kWaves][16][kPitch]
+    __syncthreads();
+    *reinterpret_cast<f32x4*>(sums + (wave * 16 + column) * kPitch + quarter * 4) = total;
+    __syncthreads();
+    if (threadIdx.x < static_cast<unsigned>(a.rows) * 16) {
+        const int m = threadIdx.x / 16, n = threadIdx.x % 16, o = first_o + n;
+        if (o >= a.out_dim) return;
+        float v = 0.0f;
+#pragma unroll
+        for (int s = 0; s < kWaves; ++s) v += sums[(s * 16 + m) * kPitch + n];
+        const size_t to = static_cast<size_t>(m) * a.out_dim + o;
+        a.y[to] = finish_output(a.ep, o, to, v);
+    }
+}
+
+// ---- many rows
+//
+// kRowWaves x kColWaves wavefronts with 32 kR rows x 64 columns each, a block of K at a time from a ring of three in LDS that all
+// of them fill and read.  Every wavefront widens its own operands: of a block's instructions about half are conversions, which
+// run beside the other wavefront's products.  `sums`: blocks of K are shared out over gridDim.y workgroups, whose sums go there,
+// [share][rows][out_dim rounded up to 4], for add_shares_kernel.
+template <int kR, int kRowWaves, int kColWaves>
+__global__ __launch_bounds__(kRowWaves * kColWaves * 64, 2) void matmul_fp8_tile_kernel(Fp8Matmul a, int row_tiles, int col_tiles, float* sums) {
+    constexpr int kWaves = kRowWaves * kColWaves, kRows = 32 * kR * kRowWaves, kCols = 64 * kColWaves, kStages = 3;
+    constexpr int kStage = (kRows + kCols) * 128 + kWaves * 256;                 // W, X, X's scales
+    constexpr int kWLoads = kCols / 8 / kWaves, kXLoads = kRows / 8 / kWaves, kLoads = kWLoads + kXLoads + 1;
+    constexpr int kOwn = kRows / kWaves;                                         // rows whose scales a wavefront loads
+    static_assert(kOwn <= 64 && kOwn % 8 == 0 && kWLoads > 0, "");
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, column = lane & 31, half = lane >> 5;
+    // An XCD has neighbouring columns of tiles, row tile by row tile: what its units load at a time fits its L2.
+    const int per_xcd = (col_tiles + 7) / 8, local = blockIdx.x >> 3;
+    const int col_tile = (blockIdx.x & 7) * per_xcd + local / row_tiles, row_tile = local % row_tiles;
+    if (local / row_tiles >= per_xcd || col_tile >= col_tiles) return;
+    const int first_o = col_tile * kCols, first_r = row_tile * kRows;
+    const int wave_o = wave % kColWaves * 64, wave_r = wave / kColWaves * (32 * kR);
+    const int blocks = fp8_blocks(a.in_dim), each = (blocks + gridDim.y - 1) / gridDim.y;
+    const int first_block = blockIdx.y * each, end_block = min(first_block + each, blocks);  // (a last share may be empty: sums of zero)
+    const float* w_scale = a.w_scales + static_cast<size_t>(min(first_o + wave_o, a.out_dim - 1) / kFp8Block) * blocks;
+    const float* x_scale = a.x_scales + static_cast<size_t>(min(first_r + wave * kOwn + lane % kOwn, a.rows - 1)) * blocks;
+    const uint32_t ring_at = lds_address(lds);
+
+    auto request = [&](int block, int stage) {
+        const uint32_t to = ring_at + stage * kStage;
+#pragma unroll
+        for (int i = 0; i < kWLoads; ++i) {
+            const int at = (wave * kWLoads + i) * 8;
+            request_rows(to + at * 128, a.w, first_o + at, at, a.out_dim, a.in_dim, block, lane);
+        }
+#pragma unroll
+        for (int i = 0; i < kXLoads; ++i) {
+            const int at = (wave * kXLoads + i) * 8;
+            request_rows(to + (kCols + at) * 128, a.x, first_r + at, at, a.rows, a.in_dim, block, lane);
+        }
+        load_dword_to_lds(to + (kCols + kRows) * 128 + wave * 256, x_scale + block);
+    };
+    if (first_block < end_block) request(first_block, 0);
+    if (first_block + 1 < end_block) request(first_block + 1, 1);
+    f32x16 total[2][kR];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
-        for (int m = 0; m < 2; ++m) total[n][m] = f32x16{};
+        for (int m = 0; m < kR; ++m) total[n][m] = f32x16{};
     }
-    request(0, 0);
-    for (int b = 0; b < blocks; ++b) {
-        const float xs[2] = {x_scale[0][b], x_scale[1][b]}, ws = w_scale[b];
-        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // the wavefront's own bytes of this block are in LDS (a barrier alone does not wait for them)
-        __syncthreads();                                    // everyone's are, and the other half has been read
-        if (b + 1 < blocks) request(b + 1, (b + 1) & 1);
-        const char* at = lds[b & 1][0];
-        f32x16 dot[2][2];
+    int stage = 0, free_stage = 2;
+    float ws_ahead = first_block < end_block ? load_uniform(w_scale + first_block) : 0.0f;
+    for (int b = first_block; b < end_block; ++b) {
+        if (b + 1 < end_block) wait_loads<kLoads>();
+        else wait_loads<0>();
+        __syncthreads();  // everyone's part of the block is there, and the stage to be filled has been read
+        if (b + 2 < end_block) request(b + 2, free_stage);
+        const char* w = lds + stage * kStage + wave_o * 128;
+        const char* x = lds + stage * kStage + (kCols + wave_r) * 128;
+        const float* scales = reinterpret_cast<const float*>(lds + stage * kStage + (kCols + kRows) * 128);
+        stage = stage == 2 ? 0 : stage + 1;
+        free_stage = free_stage == 2 ? 0 : free_stage + 1;
+        const float ws = ws_ahead;
+        if (b + 1 < end_block) ws_ahead = load_uniform(w_scale + b + 1);
+        float scale[kR];
+#pragma unroll
+        for (int m = 0; m < kR; ++m) {
+            const int row = wave_r + m * 32 + column;
+            scale[m] = scales[row / kOwn * 64 + row % kOwn] * ws;
+        }
+        f32x16 dot[2][kR];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {  // 32 of K: a 16-byte piece a lane, two instructions' worth
-            f16x8 w[2][2], x[2][2];
-            const int piece = k * 2 + (lane >> 5);
+            f16x8 wide_w[2][2], wide_x[kR][2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int wr = wave_o + t * 32 + (lane & 31), xr = wave_r + t * 32 + (lane & 31);
-                const uint4 wp = *reinterpret_cast<const uint4*>(at + wr * 128 + (piece ^ (wr & 7)) * 16);
-                const uint4 xp = *reinterpret_cast<const uint4*>(at + 128 * 128 + xr * 128 + (piece ^ (xr & 7)) * 16);
-                w[t][0] = widen(wp.x, wp.y);
-                w[t][1] = widen(wp.z, wp.w);
-                x[t][0] = widen(xp.x, xp.y);
-                x[t][1] = widen(xp.z, xp.w);
+            for (int n = 0; n < 2; ++n) {
+                const uint4 p = read_piece(w + n * 4096, column, k * 2 + half);
+                wide_w[n][0] = widen(p.x, p.y);
+                wide_w[n][1] = widen(p.z, p.w);
             }
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
+            for (int m = 0; m < kR; ++m) {
+                const uint4 p = read_piece(x + m * 4096, column, k * 2 + half);
+                wide_x[m][0] = widen(p.x, p.y);
+                wide_x[m][1] = widen(p.z, p.w);
+            }
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
 #pragma unroll
-                    for (int m = 0; m < 2; ++m)
-                        dot[n][m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w[n][half], x[m][half], k + half == 0 ? f32x16{} : dot[n][m], 0, 0, 0);
+                    for (int m = 0; m < kR; ++m)
+                        dot[n][m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wide_w[n][part], wide_x[m][part], k + part == 0 ? f32x16{} : dot[n][m], 0, 0, 0);
                 }
             }
         }
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                const float scale = xs[m] * ws;
+            for (int m = 0; m < kR; ++m) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) total[n][m][j] = __builtin_fmaf(dot[n][m][j], scale, total[n][m][j]);
+                for (int j = 0; j < 16; ++j) total[n][m][j] = __builtin_fmaf(dot[n][m][j], scale[m], total[n][m][j]);
             }
         }
     }
+    const size_t pitch = sums != nullptr ? fp8_sums_pitch(a.out_dim) : a.out_dim;
+    float* y = sums != nullptr ? sums + blockIdx.y * pitch * a.rows : a.y;
+    const bool fours = pitch % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        const int row = first_r + wave_r + m * 32 + (lane & 31);
+    for (int m = 0; m < kR; ++m) {
+        const int row = first_r + wave_r + m * 32 + column;
         if (row >= a.rows) continue;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int o = first_o + wave_o + n * 32 + (j >> 2) * 8 + (lane >> 5) * 4 + (j & 3);
-                const size_t to = static_cast<size_t>(row) * a.out_dim + o;
-                if (o < a.out_dim) a.y[to] = finish_output(a.ep, o, to, total[n][m][j]);
+            for (int q = 0; q < 4; ++q) {
+                const int o = first_o + wave_o + n * 32 + q * 8 + half * 4;
+                const size_t to = row * pitch + o;
+                f32x4 v;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[j] = total[n][m][q * 4 + j];
+                    if (sums == nullptr && o + j < a.out_dim) v[j] = finish_output(a.ep, o + j, to + j, v[j]);
+                }
+                if (fours && o < a.out_dim) {
+                    *reinterpret_cast<f32x4*>(y + to) = v;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (o + j < a.out_dim) y[to + j] = v[j];
+                    }
+                }
             }
         }
     }
 }
 
-template <int kM, int kN, int kWaves, int kAhead>
+// The sums of the shares of K, in their order, and what follows them: four columns a thread, 1024 of a row a workgroup.
+__global__ __launch_bounds__(256) void add_shares_kernel(Fp8Matmul a, const float* sums, int shares) {
+    const size_t pitch = fp8_sums_pitch(a.out_dim);
+    const int parts = (a.out_dim + 1023) / 1024, row = blockIdx.x / parts, o = (blockIdx.x % parts * 256 + threadIdx.x) * 4;
+    if (o >= a.out_dim) return;
+    f32x4 v{0, 0, 0, 0};
+#pragma unroll 4
+    for (int s = 0; s < shares; ++s) v += *reinterpret_cast<const f32x4*>(sums + (static_cast<size_t>(s) * a.rows + row) * pitch + o);
+    const size_t to = static_cast<size_t>(row) * a.out_dim + o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (o + j < a.out_dim) a.y[to + j] = finish_output(a.ep, o + j, to + j, v[j]);
+    }
+}
+
+template <int kM, int kWaves, int kStages>
 hipError_t rows_kernel(hipStream_t stream, const Fp8Matmul& a) {
-    const dim3 grid((a.out_dim + 16 * kN - 1) / (16 * kN), (a.rows + 16 * kM - 1) / (16 * kM));
-    matmul_fp8_rows_kernel<kM, kN, kWaves, kAhead><<<grid, kWaves * 64, 0, stream>>>(a);
+    static LdsLimit limit;
+    constexpr size_t ring = static_cast<size_t>(kWaves) * kStages * (2048 + kM * 2048 + 256), sums = static_cast<size_t>(kWaves) * 16 * kM * 20 * 4;
+    constexpr size_t lds = ring > sums ? ring : sums;
+    const auto kernel = matmul_fp8_rows_kernel<kM, kWaves, kStages>;
+    const hipError_t e = allow_lds(kernel, lds, &limit);
+    if (e != hipSuccess) return e;
+    const dim3 grid((a.out_dim + 15) / 16, (a.rows + 16 * kM - 1) / (16 * kM));
+    kernel<<<grid, kWaves * 64, lds, stream>>>(a);
+    return hipGetLastError();
+}
+
+template <int kR, int kRowWaves, int kColWaves>
+hipError_t tile_kernel(hipStream_t stream, const Fp8Matmul& a, int shares, float* sums) {
+    static LdsLimit limit;
+    constexpr int kRows = 32 * kR * kRowWaves, kCols = 64 * kColWaves;
+    constexpr size_t lds = 3 * ((kRows + kCols) * 128 + kRowWaves * kColWaves * 256);
+    const auto kernel = matmul_fp8_tile_kernel<kR, kRowWaves, kColWaves>;
+    hipError_t e = allow_lds(kernel, lds, &limit);
+    if (e != hipSuccess) return e;
+    const int row_tiles = (a.rows + kRows - 1) / kRows, col_tiles = (a.out_dim + kCols - 1) / kCols;
+    const dim3 grid((col_tiles + 7) / 8 * 8 * row_tiles, shares);
+    kernel<<<grid, kRowWaves * kColWaves * 64, lds, stream>>>(a, row_tiles, col_tiles, shares > 1 ? sums : nullptr);
+    e = hipGetLastError();
+    if (e != hipSuccess || shares == 1) return e;
+    add_shares_kernel<<<static_cast<uint32_t>(a.rows) * static_cast<uint32_t>((a.out_dim + 1023) / 1024), 256, 0, stream>>>(a, sums, shares);
     return hipGetLastError();
 }
 
@@ -273,14 +470,55 @@ hipError_t launch_quantize_fp8(hipStream_t stream, uint8_t* q, float* scales, co
     return hipGetLastError();
 }
 
-hipError_t launch_matmul_fp8(hipStream_t stream, const Fp8Matmul& a) {
-    if (a.rows <= 16) return rows_kernel<1, 1, 8, 4>(stream, a);
-    if (a.rows <= 32) return rows_kernel<2, 2, 8, 2>(stream, a);
-    const int64_t tiles = static_cast<int64_t>((a.out_dim + 127) / 128) * ((a.rows + 127) / 128);
-    if (a.rows <= 64 || tiles < gemv_compute_units()) return rows_kernel<4, 2, 4, 2>(stream, a);
-    const dim3 grid((a.out_dim + 127) / 128, (a.rows + 127) / 128);
-    matmul_fp8_tile_kernel<<<grid, 256, 0, stream>>>(a);
+// Up to how many values of X every workgroup quantizes them itself.
+constexpr int64_t kFusedValues = 16384;
+
+bool linear_fp8_is_fused(int rows, int in_dim) { return rows <= 16 && static_cast<int64_t>(rows) * in_dim <= kFusedValues; }
+
+hipError_t launch_linear_fp8_fused(hipStream_t stream, const Fp8Matmul& a, const float* input) {
+    static LdsLimit limit;
+    const size_t blocks = fp8_blocks(a.in_dim);
+    const size_t lds = kFusedWaves * kFusedStages * 2048 + a.rows * (blocks * kFp8Block + 16 + blocks * 4);
+    const hipError_t e = allow_lds(linear_fp8_rows_kernel, lds, &limit);
+    if (e != hipSuccess) return e;
+    linear_fp8_rows_kernel<<<(a.out_dim + 15) / 16, kFusedWaves * 64, lds, stream>>>(a, input);
     return hipGetLastError();
+}
+
+// What the kernels take, in us, as measured (512 to 14336 columns, K = 1024 to 14336, 24 to 2048 rows): few rows pass over W
+// once for each 32 of them, 4 us for 2^24 weights (less on a long K); tiles take rounds of workgroups on the compute units, a time for each block
+// of K (64 rows: two workgroups a unit); sums of shares are written and read at 5 TB/s.  Below them 3 or 4 us of a launch.
+Fp8Plan plan_matmul_fp8(int rows, int in_dim, int out_dim, int compute_units, size_t room) {
+    Fp8Plan best{kFp8Rows16, 1};
+    if (rows <= 16) return best;
+    const double units = compute_units, blocks = fp8_blocks(in_dim), weights = static_cast<double>(in_dim) * out_dim;
+    // 16 rows a workgroup where W stays in every XCD's L2 (4 MiB) over its passes: 333 rows on 2000 x 1111 9 us, 32 rows a workgroup
+    // 10 us; 64 rows on 4096 x 14336 45 us against 34 us.
+    if (weights > (4 << 20)) best.kernel = kFp8Rows32;
+    double least = 3 + (3.0 + fmin(2.2, 4096.0 / in_dim)) * ((rows + 31) / 32) * (weights / (1 << 24));
+    const auto tiles = [&](int of) { return static_cast<double>((out_dim + 127) / 128) * ((rows + of - 1) / of); };
+    for (int shares = 1; shares <= 8; shares *= 2) {
+        const size_t sums = Fp8Plan{kFp8Tile64, shares}.sums_bytes(rows, out_dim);
+        if (shares > 1 && (sums > room || blocks < 4 * shares)) break;
+        const double each = ceil(blocks / shares), rest = 4 + (shares > 1 ? 3 + 2.0 * sums / 5e6 : 0.0);
+        const double t64 = rest + each * (tiles(64) * shares <= units ? 1.06 : 1.4 * ceil(tiles(64) * shares / (2 * units)));
+        const double t128 = rest + each * 1.33 * ceil(tiles(128) * shares / units);
+        const double t256 = rest + each * 1.75 * ceil(tiles(256) * shares / units);
+        if (t64 < least) least = t64, best = Fp8Plan{kFp8Tile64, shares};
+        if (t128 < least) least = t128, best = Fp8Plan{kFp8Tile128, shares};
+        if (t256 < least) least = t256, best = Fp8Plan{kFp8Tile256, shares};
+    }
+    return best;
+}
+
+hipError_t launch_matmul_fp8(hipStream_t stream, const Fp8Matmul& a, const Fp8Plan& plan, float* sums) {
+    switch (plan.kernel) {
+        case kFp8Rows16: return rows_kernel<1, 8, 2>(stream, a);
+        case kFp8Rows32: return rows_kernel<2, 8, 2>(stream, a);
+        case kFp8Tile64: return tile_kernel<1, 2, 2>(stream, a, plan.shares, sums);
+        case kFp8Tile128: return tile_kernel<2, 2, 2>(stream, a, plan.shares, sums);
+        default: return tile_kernel<2, 4, 2>(stream, a, plan.shares, sums);
+    }
 }
 
 }  // namespace afhip

@@ -13,6 +13,9 @@ constexpr int kFp8Block = 128;  // values that share a scale
 
 __host__ __device__ inline int fp8_blocks(int n) { return (n + kFp8Block - 1) / kFp8Block; }
 
+// Floats of a row of the sums of K's shares: whole vectors.
+__host__ __device__ inline size_t fp8_sums_pitch(int out_dim) { return (static_cast<size_t>(out_dim) + 3) / 4 * 4; }
+
 struct Fp8Matmul {
     const uint8_t* x;       // e4m3 [rows][in_dim]
     const float* x_scales;  // [rows][blocks of in_dim]
@@ -24,6 +27,17 @@ struct Fp8Matmul {
 };
 
 hipError_t launch_quantize_fp8(hipStream_t stream, uint8_t* q, float* scales, const float* x, size_t rows, int in_dim);
-hipError_t launch_matmul_fp8(hipStream_t stream, const Fp8Matmul& call);
+// Few values of X: f32, quantized in the product's own launch (a.x and a.x_scales are not read).
+bool linear_fp8_is_fused(int rows, int in_dim);
+hipError_t launch_linear_fp8_fused(hipStream_t stream, const Fp8Matmul& call, const float* input);
+// Which kernel, and over how many workgroups the blocks of K are shared out; `room`: bytes for the shares' sums.
+enum Fp8Kernel { kFp8Rows16, kFp8Rows32, kFp8Tile64, kFp8Tile128, kFp8Tile256 };
+struct Fp8Plan {
+    Fp8Kernel kernel;
+    int shares;
+    size_t sums_bytes(int rows, int out_dim) const { return shares > 1 ? shares * rows * fp8_sums_pitch(out_dim) * sizeof(float) : 0; }
+};
+Fp8Plan plan_matmul_fp8(int rows, int in_dim, int out_dim, int compute_units, size_t room);
+hipError_t launch_matmul_fp8(hipStream_t stream, const Fp8Matmul& call, const Fp8Plan& plan, float* sums);
 
 }  // namespace afhip

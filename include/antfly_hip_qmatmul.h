@@ -364,8 +364,10 @@ afhip_status afhip_launch_decode_fp16(void *stream, afhip_buffer dst_f32, afhip_
  * number stays one, and an infinite one makes its block's values no numbers. */
 afhip_status afhip_launch_quantize_fp8(void *stream, afhip_buffer q, afhip_buffer scales, afhip_buffer input, size_t rows,
                                        size_t in_dim);
-/* Scratch of the two products below, 256-byte aligned.  afhip_launch_matmul_fp8_f32 runs with less or none (then K is not
- * shared out over workgroups: the same sums in another order); afhip_launch_linear_fp8_f32 refuses less. */
+/* Scratch of the two products below, 256-byte aligned: the quantized activations, and the sums of K's shares where a small
+ * grid of tiles has a long K; 0 where few activations are quantized in the product's own launch.  afhip_launch_matmul_fp8_f32
+ * runs with less or none (on fewer shares or one: the same products summed in another order); afhip_launch_linear_fp8_f32
+ * refuses less. */
 size_t afhip_linear_fp8_workspace_bytes(size_t rows, size_t in_dim, size_t out_dim);
 /* Y = act(X W^T + bias) + residual on activations that are codes already (several projections of one input quantize it
  * once).  bias f32 [out_dim] and residual f32 [rows][out_dim] are optional (.ptr == 0); activation: afhip_activation. */
@@ -374,7 +376,7 @@ afhip_status afhip_launch_matmul_fp8_f32(void *stream, afhip_buffer dst, afhip_b
                                          afhip_buffer residual, int activation, size_t rows, size_t in_dim, size_t out_dim,
                                          afhip_buffer workspace);
 /* The same on f32 activations: quantized as by afhip_launch_quantize_fp8, in the product's own launch where the rows are
- * few, into the workspace otherwise. */
+ * few (rows * in_dim <= 16384, rows <= 16), into the workspace otherwise. */
 afhip_status afhip_launch_linear_fp8_f32(void *stream, afhip_buffer dst, afhip_buffer input, afhip_buffer weight,
                                          afhip_buffer weight_scales, afhip_buffer bias, afhip_buffer residual,
                                          int activation, size_t rows, size_t in_dim, size_t out_dim,

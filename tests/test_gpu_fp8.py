@@ -114,6 +114,23 @@ def test_product_many_rows(rows, in_dim, out_dim):
     assert np.isfinite(got).all()
 
 
+@pytest.mark.parametrize("rows,in_dim,out_dim", [(512, 14336, 1024), (300, 8192, 2049), (128, 14336, 2000)])
+def test_shares_of_k(rows, in_dim, out_dim):
+    """A small grid on a long K: its blocks shared out over workgroups with a workspace lent, and not without one."""
+    print(f"case: fp8 shares rows={rows} in={in_dim} out={out_dim}", flush=True)
+    rng = np.random.default_rng(rows)
+    x, (w, w_scales) = activations(rng, rows, in_dim), F.weights(rng, out_dim, in_dim)
+    bias, residual = rng.standard_normal(out_dim).astype(np.float32), rng.standard_normal((rows, out_dim)).astype(np.float32)
+    sample = np.unique(np.r_[0, 31, 64, 127, rows - 1, rng.integers(0, rows, 12)])
+    y, off = F.matmul(*F.quantize(x[sample]), w, w_scales)
+    want = np.where(y + bias < 0, 0.0, y + bias) + residual[sample]
+    off = off + 2.0 ** -22 * (np.abs(y) + np.abs(want))
+    assert kernels.linearFp8WorkspaceBytes(rows, in_dim, out_dim) > rows * in_dim + 2 * rows * out_dim * 4
+    for quantized, lend in ((False, True), (True, True), (True, False)):
+        got = product(x, w, w_scales, bias, residual, 1, quantized=quantized, lend=lend)
+        assert (np.abs(got[sample] - want) <= off).all() and np.isfinite(got).all()
+
+
 @pytest.mark.parametrize("rows,in_dim,out_dim", [(1, 512, 300), (5, 2000, 130), (40, 144, 257), (300, 640, 1111), (1100, 256, 4100)])
 @pytest.mark.parametrize("activation", [0, 1, 2, 3])
 def test_epilogue(rows, in_dim, out_dim, activation):

@@ -49,9 +49,10 @@ def test_fp8_product_refusals():
     for bad in (Buffer(0x1000, 4 * 2 * 2 - 1), Buffer(0x1002, 1 << 40), NONE):
         with pytest.raises(_lib.InvalidHipState):
             fp8(scales=bad)
-    for bad in (Buffer(0x1000, kernels.linearFp8WorkspaceBytes(4, 256, 130) - 1), Buffer(0x1080, 1 << 40), NONE):
+    assert kernels.linearFp8WorkspaceBytes(4, 256, 130) == 0  # few values of X: quantized in the product's launch
+    for bad in (Buffer(0x1000, kernels.linearFp8WorkspaceBytes(100, 256, 130) - 1), Buffer(0x1080, 1 << 40), NONE):
         with pytest.raises(_lib.InvalidHipState):
-            fp8(workspace=bad)
+            fp8(rows=100, workspace=bad)
     for bad in (Buffer(0x1000, 4 * 256 - 1), Buffer(0x1008, 1 << 40), NONE):
         with pytest.raises(_lib.InvalidHipState):
             fp8_codes(q=bad)
@@ -64,6 +65,8 @@ def test_fp8_product_refusals():
     kernels.launchQuantizeFp8(None, BIG, BIG, BIG, 0, 256)
     assert kernels.linearFp8WorkspaceBytes(0, 256, 4) == 0 and kernels.linearFp8WorkspaceBytes(3, 250, 4) == 0
     assert kernels.linearFp8WorkspaceBytes(5, 4096, 4096) >= 5 * 4096 + 5 * 32 * 4
+    # a small grid on a long K: room for the sums of its shares behind the codes and scales
+    assert kernels.linearFp8WorkspaceBytes(512, 14336, 1024) > 512 * 14336 + 512 * 112 * 4 + 2 * 512 * 1024 * 4
 
 
 def a_cache(**change):
