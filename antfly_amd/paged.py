@@ -7,58 +7,77 @@ ABI (include/antfly_hip_qmatmul.h); `stream` is a hipStream_t."""
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 from . import _lib
 from ._lib import Buffer, check
 
 NO_BUFFER = Buffer(0, 0)
 _TYPES = {"torch.float32": _lib.TYPE_F32, "torch.float16": _lib.TYPE_F16, "torch.bfloat16": _lib.TYPE_BF16}
+# A decode step makes these calls for every layer: arguments go into the C structs as one packed string of numbers, which
+# takes a fifth of the time that filling their fields does.
+_CACHE, _PLAN, _REST = struct.Struct("4Qi4x7Q"), struct.Struct("26Q"), struct.Struct("if23Q")  # _REST: TreeAttention behind its cache
+assert _CACHE.size == C.sizeof(_lib.PagedCache) and _PLAN.size == C.sizeof(_lib.BatchPlan)
+assert _CACHE.size + _REST.size == C.sizeof(_lib.TreeAttention)
+
+
+def _bad_shape():
+    return _lib.InvalidShape(_lib.ERR_INVALID_SHAPE)
 
 
 def buffer(array) -> Buffer:
     """The memory that an array spans, from its first element to its last; None: no buffer."""
     if array is None:
         return NO_BUFFER
-    count = array.numel()
-    if count and not array.is_contiguous():
-        count = 1 + sum((n - 1) * s for n, s in zip(array.shape, array.stride()))
-    return Buffer(array.data_ptr(), count * array.element_size())
+    return Buffer(array.data_ptr(), _bytes(array))
+
+
+def _bytes(array) -> int:
+    if array.is_contiguous():
+        return array.nbytes
+    return (1 + sum((n - 1) * s for n, s in zip(array.shape, array.stride()))) * array.element_size() if array.numel() else 0
 
 
 def _type(array) -> int:
     return _TYPES.get(str(array.dtype), -1)
 
 
-def _array(array, kind) -> Buffer:
-    """A contiguous array of whole numbers of the given width."""
+def _i32(array):
+    """(address, bytes) of a contiguous array of int32."""
+    if str(array.dtype) != "torch.int32" or not array.is_contiguous():
+        raise _bad_shape()
+    return array.data_ptr(), array.nbytes
+
+
+def _optional(array, dtypes=("torch.int32",)):
     if array is None:
-        return NO_BUFFER
-    if str(array.dtype) not in kind or not array.is_contiguous():
-        raise _lib.InvalidShape(_lib.ERR_INVALID_SHAPE)
-    return Buffer(array.data_ptr(), array.numel() * array.element_size())
+        return 0, 0
+    if str(array.dtype) not in dtypes or not array.is_contiguous():
+        raise _bad_shape()
+    return array.data_ptr(), array.nbytes
 
 
-_I32, _U64 = ("torch.int32",), ("torch.int64", "torch.uint64")
+_U64 = ("torch.int64", "torch.uint64")
 
 
 def _rows_of_heads(array, rows, heads, dim):
     """(token stride, head stride) of [rows, heads, dim] whose last dimension is contiguous."""
-    if tuple(array.shape) != (rows, heads, dim) or (dim > 1 and array.stride(2) != 1):
-        raise _lib.InvalidShape(_lib.ERR_INVALID_SHAPE)
-    return array.stride(0), array.stride(1)
+    strides = array.stride()
+    if array.shape != (rows, heads, dim) or (dim > 1 and strides[2] != 1):
+        raise _bad_shape()
+    return strides[0], strides[1]
 
 
 def cache(keys, values, heads_outside: bool = False) -> _lib.PagedCache:
     """keys, values [blocks, block size, kv heads, head dim], or with heads_outside [blocks, kv heads, block size, head dim]."""
-    if len(keys.shape) != 4 or keys.shape != values.shape or keys.dtype != values.dtype or keys.stride() != values.stride() or \
-            (keys.shape[3] > 1 and keys.stride(3) != 1):
-        raise _lib.InvalidShape(_lib.ERR_INVALID_SHAPE)
-    blocks, slots, heads, dim = keys.shape
-    strides = keys.stride()
-    slot_stride, head_stride = strides[1], strides[2]
-    if heads_outside:
-        slots, heads, slot_stride, head_stride = heads, slots, head_stride, slot_stride
-    made = _lib.PagedCache(buffer(keys), buffer(values), _type(keys), blocks, slots, heads, dim, strides[0], slot_stride, head_stride)
+    shape, strides = keys.shape, keys.stride()
+    if len(shape) != 4 or values.shape != shape or keys.dtype != values.dtype or values.stride() != strides or \
+            (shape[3] > 1 and strides[3] != 1):
+        raise _bad_shape()
+    slot, head = (2, 1) if heads_outside else (1, 2)
+    made = _lib.PagedCache.from_buffer_copy(_CACHE.pack(
+        keys.data_ptr(), _bytes(keys), values.data_ptr(), _bytes(values), _type(keys), shape[0], shape[slot], shape[head],
+        shape[3], strides[0], strides[slot], strides[head]))
     made.arrays = (keys, values)  # alive as long as the description of them is
     return made
 
@@ -68,59 +87,67 @@ def launchBatchPlan(stream, context_lens, query_lens, block_tables, free_blocks,
     """Writes block_tables (new entries), query_starts, slots, positions, masks and blocks_taken from the requests' lengths;
     `blocks`: how many the cache has (numbers outside name none)."""
     requests, columns = block_tables.shape
-    tokens = slots.shape[0]
-    if positions.shape[0] != tokens or (parents is not None and parents.shape[0] != tokens) or \
-            (masks is not None and (len(masks.shape) != 2 or masks.shape[0] != tokens)):
-        raise _lib.InvalidShape(_lib.ERR_INVALID_SHAPE)
-    check(_lib.lib().afhip_launch_batch_plan(stream, C.byref(_lib.BatchPlan(
-        requests, columns, block_size, blocks, tokens, 0 if masks is None else masks.shape[1],
-        _array(context_lens, _I32), _array(query_lens, _I32), _array(free_blocks, _I32),
-        _array(parents, _I32), _array(block_tables, _I32), _array(query_starts, _I32),
-        _array(slots, _I32), _array(positions, _I32), _array(masks, _U64),
-        _array(blocks_taken, _I32)))))
+    tokens, words = slots.shape[0], 0
+    if masks is not None:
+        if len(masks.shape) != 2 or masks.shape[0] != tokens:
+            raise _bad_shape()
+        words = masks.shape[1]
+    if positions.shape[0] != tokens or (parents is not None and parents.shape[0] != tokens):
+        raise _bad_shape()
+    plan = _lib.BatchPlan.from_buffer_copy(_PLAN.pack(
+        requests, columns, block_size, blocks, tokens, words, *_i32(context_lens), *_i32(query_lens), *_i32(free_blocks),
+        *_optional(parents), *_i32(block_tables), *_i32(query_starts), *_i32(slots), *_i32(positions), *_optional(masks, _U64),
+        *_i32(blocks_taken)))
+    check(_lib.lib().afhip_launch_batch_plan(stream, plan))
 
 
 def launchCacheStore(stream, cache: _lib.PagedCache, keys, values, slots) -> None:
     """keys, values [tokens, kv heads, head dim] (f32, f16 or bf16) into the cache's slots."""
     tokens = slots.shape[0]
-    strides = _rows_of_heads(keys, tokens, cache.kv_heads, cache.head_dim)
-    if _rows_of_heads(values, tokens, cache.kv_heads, cache.head_dim) != strides or keys.dtype != values.dtype:
-        raise _lib.InvalidShape(_lib.ERR_INVALID_SHAPE)
-    check(_lib.lib().afhip_launch_cache_store(stream, C.byref(cache), _type(keys), buffer(keys), buffer(values), strides[0],
-                                              strides[1], _array(slots, _I32), tokens))
+    if values.shape != keys.shape or values.stride() != keys.stride() or values.dtype != keys.dtype:
+        raise _bad_shape()
+    token_stride, head_stride = _rows_of_heads(keys, tokens, cache.kv_heads, cache.head_dim)
+    check(_lib.lib().afhip_launch_cache_store(stream, cache, _type(keys), buffer(keys), buffer(values), token_stride, head_stride,
+                                              Buffer(*_i32(slots)), tokens))
 
 
 def launchCacheMove(stream, cache: _lib.PagedCache, block_tables, context_lens, paths, path_lens) -> None:
     """The accepted path of every request's tree to the places behind its context."""
     requests, columns = block_tables.shape
     if len(paths.shape) != 2 or paths.shape[0] != requests:
-        raise _lib.InvalidShape(_lib.ERR_INVALID_SHAPE)
-    check(_lib.lib().afhip_launch_cache_move(stream, C.byref(cache), _array(block_tables, _I32), columns,
-                                             _array(context_lens, _I32), _array(paths, _I32),
-                                             _array(path_lens, _I32), requests, paths.shape[1]))
+        raise _bad_shape()
+    check(_lib.lib().afhip_launch_cache_move(stream, cache, Buffer(*_i32(block_tables)), columns, Buffer(*_i32(context_lens)),
+                                             Buffer(*_i32(paths)), Buffer(*_i32(path_lens)), requests, paths.shape[1]))
 
 
 def treeAttention(cache: _lib.PagedCache, out, query, query_starts, context_lens, block_tables, max_query_len: int,
                   max_key_len: int, masks=None, scale: float = None) -> _lib.TreeAttention:
-    """The arguments of a call (any number of calls while the arrays stay): query, out [tokens, heads, head dim]; scale: head_dim ** -0.5 unless given."""
+    """The arguments of a call (of any number of calls while the arrays stay): query, out [tokens, heads, head dim]; scale:
+    head_dim ** -0.5 unless given."""
     tokens, heads, dim = query.shape
     requests, columns = block_tables.shape
-    q, o = _rows_of_heads(query, tokens, heads, cache.head_dim), _rows_of_heads(out, tokens, heads, cache.head_dim)
-    if out.dtype != query.dtype or (masks is not None and (len(masks.shape) != 2 or masks.shape[0] != tokens)):
-        raise _lib.InvalidShape(_lib.ERR_INVALID_SHAPE)
-    made = _lib.TreeAttention(cache, _type(query), dim ** -0.5 if scale is None else scale, requests, tokens, heads, max_query_len,
-                              max_key_len, columns, 0 if masks is None else masks.shape[1], q[0], q[1], o[0], o[1], buffer(query),
-                              buffer(out), _array(query_starts, _I32), _array(context_lens, _I32),
-                              _array(block_tables, _I32), _array(masks, _U64))
+    q_token, q_head = _rows_of_heads(query, tokens, heads, cache.head_dim)
+    o_token, o_head = _rows_of_heads(out, tokens, heads, cache.head_dim)
+    words = 0
+    if masks is not None:
+        if len(masks.shape) != 2 or masks.shape[0] != tokens:
+            raise _bad_shape()
+        words = masks.shape[1]
+    if out.dtype != query.dtype:
+        raise _bad_shape()
+    made = _lib.TreeAttention.from_buffer_copy(bytes(cache) + _REST.pack(
+        _type(query), dim ** -0.5 if scale is None else scale, requests, tokens, heads, max_query_len, max_key_len, columns, words,
+        q_token, q_head, o_token, o_head, query.data_ptr(), _bytes(query), out.data_ptr(), _bytes(out), *_i32(query_starts),
+        *_i32(context_lens), *_i32(block_tables), *_optional(masks, _U64)))
     made.arrays = (cache, out, query, query_starts, context_lens, block_tables, masks)
     return made
 
 
 def treeAttentionWorkspaceBytes(attention: _lib.TreeAttention) -> int:
-    return _lib.lib().afhip_tree_attention_workspace_bytes(C.byref(attention))
+    return _lib.lib().afhip_tree_attention_workspace_bytes(attention)
 
 
 def launchTreeAttention(stream, attention: _lib.TreeAttention, workspace: Buffer = NO_BUFFER) -> None:
     """`workspace`: a Buffer, or an array, of at least treeAttentionWorkspaceBytes(attention) bytes."""
-    check(_lib.lib().afhip_launch_tree_attention(stream, C.byref(attention),
+    check(_lib.lib().afhip_launch_tree_attention(stream, attention,
                                                  workspace if isinstance(workspace, Buffer) else buffer(workspace)))
