@@ -14,9 +14,10 @@
 //
 // Keys and values come in tiles of 32 keys from memory straight into a ring of tiles in LDS (no registers in between),
 // requested kStages - 1 tiles ahead.  The wavefronts of a workgroup share its tiles and have 16 kQ rows each: a lone wavefront
-// (no barrier anywhere) up to 32 rows, four of them, and every key read once, for 128.  Long contexts are shared out over
+// (no barrier anywhere) up to 16 rows, four of them, and every key read once, for 128.  Long contexts are shared out over
 // workgroups by the lengths that the device holds, so that ragged requests keep all of them busy to the end, and a second
-// kernel joins the parts.
+// kernel joins the parts.  Short ones stay with one workgroup a key head: it has kKeyGroups such groups of
+// wavefronts that take tiles in turn, and adds them up itself.
 #include "paged_launch.h"
 
 #include <hip/hip_runtime.h>
@@ -155,6 +156,21 @@ __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kLeft) : "memory");
 }
 
+// Four values of a result from their sums; zero where nothing was seen.
+template <bool kBf16, bool kF32>
+__device__ __forceinline__ void store_row(const TreeAttentionArgs& a, size_t token, uint32_t head, int d, f32x4 x, float total) {
+    const size_t to = token * a.out_token_stride + static_cast<size_t>(head) * a.out_head_stride + d;
+    const float by = total == 0.0f ? 0.0f : 1.0f / total;
+    if (kF32) {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to) = x * by;
+    } else {
+        s16x4 y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = narrow<kBf16>(x[j] * by);
+        *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(a.out) + to) = y;
+    }
+}
+
 // What the launch's shape and the lengths on the device say of one request.
 struct Share {
     int begin, tokens, context, keys;   // its first row of query, new tokens, cached tokens, both together
@@ -260,15 +276,15 @@ __device__ __forceinline__ bool find_share(const TreeAttentionArgs& a, const Sha
 }
 
 // kDim: the head's values, rounded up to a size that is here (the rest are zeros).  kF32: query and out are f32.
-template <int kDim, bool kBf16, bool kF32, int kQ, int kWaves, int kStages>
-__global__ __launch_bounds__(kWaves * 64, kF32 || kDim == 256 ? 1 : 2) void tree_attention_kernel(TreeAttentionArgs a, SharePlan plan, float* part_out,
+template <int kDim, bool kBf16, bool kF32, int kQ, int kRowWaves, int kKeyGroups, int kStages>
+__global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 1 : 2) void tree_attention_kernel(TreeAttentionArgs a, SharePlan plan, float* part_out,
                                                                                                  Part* parts) {
     constexpr int kSteps = kDim / 32;                            // products of K Q^T along the head
     constexpr int kTerms = kF32 ? (kBf16 ? 3 : 2) : 1;           // of a query value or a weight: 24 bits of three bf16, 22 of two f16
-    constexpr int kRows = 16 * kQ * kWaves;
+    constexpr int kWaves = kRowWaves * kKeyGroups, kRows = 16 * kQ * kRowWaves, kStep = kTile * kKeyGroups;
     constexpr int kPieces = kDim / 8;                            // 16-byte pieces of a row
     constexpr int kTileBytes = kTile * kDim * 2;                 // of K, and of V behind it
-    constexpr int kLoads = kTile * kPieces / 64 / kWaves;        // of a wavefront, 1 KiB each, for K and for V
+    constexpr int kLoads = kTile * kPieces / 64 / kRowWaves;     // of a wavefront, 1 KiB each, for K and for V
     extern __shared__ __attribute__((aligned(1024))) char lds[];
 
     // workgroups go round the eight XCDs in turn: the row tiles of a part, which share its keys, lie on one and share its L2
@@ -289,13 +305,15 @@ __global__ __launch_bounds__(kWaves * 64, kF32 || kDim == 256 ? 1 : 2) void tree
 
     const int tid = static_cast<int>(threadIdx.x), wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int column = lane & 15, quarter = lane >> 4;
-    const int my_row = first_row + wave * 16 * kQ;  // of this wavefront's first
+    const int row_wave = wave % kRowWaves, key_group = wave / kRowWaves;
+    const int my_row = first_row + row_wave * 16 * kQ;  // of this wavefront's first
     const bool works = my_row < rows;               // otherwise it only helps to load
     if (share.splits > 1 && key_begin >= key_end) {  // none of this part's keys is there for these rows: the part says so
         for (int r = tid; r < kRows; r += kWaves * 64) parts[static_cast<size_t>(slot) * kRows + r] = Part{-__builtin_inff(), 0.0f};
         return;
     }
-    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+    char* const ring = lds + key_group * (kStages * 2 * kTileBytes);
+    const uint32_t ring_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)ring));
     const int pieces = static_cast<int>(a.cache.head_dim / 8);  // that hold something
     const bool whole_heads = pieces == kPieces;
 
@@ -320,10 +338,10 @@ __global__ __launch_bounds__(kWaves * 64, kF32 || kDim == 256 ? 1 : 2) void tree
         const uint32_t at = place(tile);  // lane l % 32 has the place of key l % 32
         // a key without a place is not seen by any row: what is loaded for it may be anything
         const int there = static_cast<int>(at == kNowhere ? 0u : at);
-        const uint32_t to = lds_at + stage * (2 * kTileBytes) + wave * (kLoads * 1024);
+        const uint32_t to = ring_at + stage * (2 * kTileBytes) + row_wave * (kLoads * 1024);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int slot = (wave * kLoads + i) * 64 + lane, row = slot / kPieces;
+            const int slot = (row_wave * kLoads + i) * 64 + lane, row = slot / kPieces;
             const int kp = key_piece<kDim>(row, slot % kPieces) % kPieces, vp = value_piece<kDim>(row, slot % kPieces) % kPieces;
             const uint32_t from = static_cast<uint32_t>(__shfl(there, row));
             const uint4 *k = a.cache.keys + (from + kp), *v = a.cache.values + (from + vp);
@@ -338,7 +356,10 @@ __global__ __launch_bounds__(kWaves * 64, kF32 || kDim == 256 ? 1 : 2) void tree
     };
     uint32_t held_ahead[kStages - 1];  // of the tiles on their way, the next one's first
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) held_ahead[i] = key_begin + i * kTile < key_end ? request_tile(key_begin + i * kTile, i) : 0u;
+    for (int i = 0; i < kStages - 1; ++i) {
+        const int tile = key_begin + key_group * kTile + i * kStep;
+        held_ahead[i] = tile < key_end ? request_tile(tile, i) : 0u;
+    }
 
     // ---- the rows
     s16x8 query[kQ][kSteps][kTerms];
@@ -423,20 +444,21 @@ __global__ __launch_bounds__(kWaves * 64, kF32 || kDim == 256 ? 1 : 2) void tree
 
     // ---- the keys
     int stage = 0, free_stage = kStages - 1;
-    for (int tile = key_begin; tile < key_end; tile += kTile) {
+    for (int first = key_begin; first < key_end; first += kStep) {
+        const int tile = first + key_group * kTile;
         // this wavefront's part of the tile is there: all but what was requested behind it, all of it near the end
-        if (tile + (kStages - 2) * kTile < key_end) wait_loads<2 * kLoads * (kStages - 2)>();
+        if (tile + (kStages - 2) * kStep < key_end) wait_loads<2 * kLoads * (kStages - 2)>();
         else wait_loads<0>();
-        if (kWaves > 1) __syncthreads();           // everyone's is, and the stage to be filled has been read
+        if (kRowWaves > 1) __syncthreads();        // everyone's is, and the stage to be filled has been read
         const uint32_t held = held_ahead[0];
 #pragma unroll
         for (int i = 0; i + 1 < kStages - 1; ++i) held_ahead[i] = held_ahead[i + 1];
-        if (tile + (kStages - 1) * kTile < key_end) held_ahead[kStages - 2] = request_tile(tile + (kStages - 1) * kTile, free_stage);
-        const char* k_lds = lds + stage * (2 * kTileBytes);
+        if (tile + (kStages - 1) * kStep < key_end) held_ahead[kStages - 2] = request_tile(tile + (kStages - 1) * kStep, free_stage);
+        const char* k_lds = ring + stage * (2 * kTileBytes);
         const char* v_lds = k_lds + kTileBytes;
         stage = stage + 1 == kStages ? 0 : stage + 1;
         free_stage = free_stage + 1 == kStages ? 0 : free_stage + 1;
-        if (!works) continue;
+        if (!works || tile >= key_end) continue;
         const bool clean = tile + kTile <= context && held == ~0u;  // every row sees every key
 
         f32x4 score[kQ][2];
@@ -572,32 +594,55 @@ __global__ __launch_bounds__(kWaves * 64, kF32 || kDim == 256 ? 1 : 2) void tree
         }
     }
 
+    // ---- the key groups' sums
+    if constexpr (kKeyGroups > 1) {
+        constexpr int kPitch = kDim + 4;                                                   // floats of a row in LDS
+        float* sums = reinterpret_cast<float*>(lds);                                       // [kKeyGroups][kRows][kPitch]
+        Part* group_parts = reinterpret_cast<Part*>(sums + kKeyGroups * kRows * kPitch);   // [kKeyGroups][kRows]
+        __syncthreads();                                                                   // the tiles are done with
+#pragma unroll
+        for (int qt = 0; qt < kQ; ++qt) {
+            const int r = key_group * kRows + (row_wave * kQ + qt) * 16 + column;
+            const float total = row_sum(sum[qt]);
+            if (quarter == 0) group_parts[r] = Part{shift[qt] == kUnset ? -__builtin_inff() : -shift[qt], total};
+#pragma unroll
+            for (int d = 0; d < kDim / 16; ++d) *reinterpret_cast<f32x4*>(sums + r * kPitch + d * 16 + quarter * 4) = out[qt][d];
+        }
+        __syncthreads();
+        for (int i = tid; i < kRows * (kDim / 4); i += kWaves * 64) {
+            const int r = i / (kDim / 4), d = i % (kDim / 4) * 4, row = first_row + r;
+            if (row >= rows || d >= pieces * 8) continue;
+            float highest = -__builtin_inff(), total = 0.0f;
+#pragma unroll
+            for (int g = 0; g < kKeyGroups; ++g) highest = fmaxf(highest, group_parts[g * kRows + r].most);
+            f32x4 x{0, 0, 0, 0};
+#pragma unroll
+            for (int g = 0; g < kKeyGroups; ++g) {
+                const float by = exp2_between(group_parts[g * kRows + r].most, highest);
+                total = __builtin_fmaf(group_parts[g * kRows + r].sum, by, total);
+                const f32x4 y = *reinterpret_cast<const f32x4*>(sums + (g * kRows + r) * kPitch + d);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(y[j], by, x[j]);
+            }
+            store_row<kBf16, kF32>(a, static_cast<size_t>(begin + row / group), kv_head * a.group + row % group, d, x, total);
+        }
+        return;
+    }
+
     // ---- out: a lane has four consecutive values of its row in each register group
 #pragma unroll
     for (int qt = 0; qt < kQ; ++qt) {
         const float total = row_sum(sum[qt]);
         if (!real[qt]) continue;
         const int row = my_row + qt * 16 + column;
-        const size_t token = static_cast<size_t>(begin + row_token[qt]);
-        const int head = static_cast<int>(kv_head) * group + row % group;
         const size_t part = static_cast<size_t>(slot) * kRows + (row - first_row);
         if (share.splits > 1 && quarter == 0) parts[part] = Part{shift[qt] == kUnset ? -__builtin_inff() : -shift[qt], total};
-        const size_t to = token * a.out_token_stride + static_cast<size_t>(head) * a.out_head_stride;
-        const float by = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
         for (int dt = 0; dt < kDim / 16; ++dt) {
             const int d = dt * 16 + quarter * 4;
             if (d >= pieces * 8) continue;
-            if (share.splits > 1) {
-                *reinterpret_cast<f32x4*>(part_out + part * a.cache.head_dim + d) = out[qt][dt];
-            } else if (kF32) {
-                *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to + d) = out[qt][dt] * by;
-            } else {
-                s16x4 y;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) y[j] = narrow<kBf16>(out[qt][dt][j] * by);
-                *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(a.out) + to + d) = y;
-            }
+            if (share.splits > 1) *reinterpret_cast<f32x4*>(part_out + part * a.cache.head_dim + d) = out[qt][dt];
+            else store_row<kBf16, kF32>(a, static_cast<size_t>(begin + row_token[qt]), kv_head * a.group + row % group, d, out[qt][dt], total);
         }
     }
 }
@@ -651,22 +696,13 @@ __global__ __launch_bounds__(kJoinWaves * 64) void join_parts_kernel(TreeAttenti
             for (int j = 0; j < 4; ++j) x[j] += __shfl_xor(x[j], w);
         }
         if (group != 0 || d >= a.cache.head_dim) continue;
-        const float over = total == 0.0f ? 0.0f : 1.0f / total;
-        const size_t token = static_cast<size_t>(share.begin) + row / a.group;
-        const size_t to = token * a.out_token_stride + static_cast<size_t>(kv_head * a.group + row % a.group) * a.out_head_stride + d;
-        if (kF32) {
-            *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to) = x * over;
-        } else {
-            s16x4 y;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = narrow<kBf16>(x[j] * over);
-            *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(a.out) + to) = y;
-        }
+        store_row<kBf16, kF32>(a, static_cast<size_t>(share.begin) + row / a.group, kv_head * a.group + row % a.group, d, x, total);
     }
 }
 
 struct Shape {
-    int dim, sixteens, waves;  // kDim, kQ, kWaves
+    int dim, sixteens, waves;  // kDim, kQ, kRowWaves
+    bool gathered;             // one workgroup for all keys of a key head
     int compute_units;
     SharePlan plan;
     uint64_t groups, slots;  // most workgroups, and parts of requests that have several
@@ -687,12 +723,16 @@ Shape shape_of(const TreeAttentionArgs& a, int compute_units) {
         s.sixteens = rows <= 64 ? 1 : 2;
         s.waves = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     }
+    // One workgroup for all keys where a second launch would take longer than its tiles, one after the other (8 key heads of 128, bf16):
+    // 1 request of 5 tokens 10.5 us against 13.1 on 300 keys, 15.1 against 12.2 on 700; 16 requests of 1 token 16.9 against 21.6 on 1000,
+    // 27.4 against 26.3 on 1500.
+    s.gathered = rows <= 32 && a.max_key_len <= (static_cast<uint64_t>(a.requests) * a.cache.kv_heads >= 64 ? 1024 : 512);
     const uint64_t tile_rows = s.rows_a_tile(), most_row_tiles = (rows + tile_rows - 1) / tile_rows;
     // row tiles of the whole batch: every request's last one may be part empty
     uint64_t row_tiles = static_cast<uint64_t>(a.tokens) * a.group / tile_rows + a.requests;
     if (row_tiles > a.requests * most_row_tiles) row_tiles = a.requests * most_row_tiles;
     const uint64_t tiles = (static_cast<uint64_t>(a.max_key_len) + kTile - 1) / kTile;
-    s.plan.even = a.requests <= kMostEvened;
+    s.plan.even = !s.gathered && a.requests <= kMostEvened;
     s.plan.row_tiles = static_cast<uint32_t>(most_row_tiles);
     s.plan.least = 2;  // fewer tiles are not worth a workgroup
     const uint64_t heads = a.cache.kv_heads, base = row_tiles * heads;
@@ -721,16 +761,19 @@ size_t part_out_bytes(const TreeAttentionArgs& a, const Shape& s) {
     return (s.slots * s.rows_a_tile() * a.cache.head_dim * sizeof(float) + 255) / 256 * 256;
 }
 
-template <int kDim, bool kBf16, bool kF32, int kQ, int kWaves, int kStages>
+template <int kDim, bool kBf16, bool kF32, int kQ, int kRowWaves, int kKeyGroups, int kStages>
 hipError_t attend(hipStream_t stream, const TreeAttentionArgs& a, const Shape& s, void* workspace) {
     static LdsLimit limit;
-    constexpr size_t lds = static_cast<size_t>(kStages) * 2 * kTile * kDim * 2;
-    const auto kernel = tree_attention_kernel<kDim, kBf16, kF32, kQ, kWaves, kStages>;
+    constexpr size_t ring = static_cast<size_t>(kKeyGroups) * kStages * 2 * kTile * kDim * 2;
+    constexpr size_t sums = kKeyGroups == 1 ? 0 : static_cast<size_t>(kKeyGroups) * 16 * kQ * kRowWaves * ((kDim + 4) * sizeof(float) + sizeof(Part));
+    constexpr size_t lds = ring > sums ? ring : sums;
+    static_assert(lds <= 160 * 1024, "a compute unit's LDS");
+    const auto kernel = tree_attention_kernel<kDim, kBf16, kF32, kQ, kRowWaves, kKeyGroups, kStages>;
     hipError_t e = allow_lds(kernel, lds, &limit);
     if (e != hipSuccess) return e;
     float* part_out = static_cast<float*>(workspace);
     Part* parts = s.slots != 0 ? reinterpret_cast<Part*>(static_cast<char*>(workspace) + part_out_bytes(a, s)) : nullptr;
-    kernel<<<static_cast<uint32_t>(s.groups), kWaves * 64, lds, stream>>>(a, s.plan, part_out, parts);
+    kernel<<<static_cast<uint32_t>(s.groups), kRowWaves * kKeyGroups * 64, lds, stream>>>(a, s.plan, part_out, parts);
     e = hipGetLastError();
     if (e != hipSuccess || s.slots == 0) return e;
     // eight workgroups a compute unit over all requests, or one wavefront a row
@@ -741,20 +784,21 @@ hipError_t attend(hipStream_t stream, const TreeAttentionArgs& a, const Shape& s
     return hipGetLastError();
 }
 
-// The ring's length: as many stages as let two workgroups of four wavefronts, or five of one, on a unit's 160 KiB of LDS.
+// The ring's length: as many stages as let two workgroups of four wavefronts, or five of one, on a unit's 160 KiB of LDS; key
+// groups have two.
 template <int kDim, bool kBf16, bool kF32>
 hipError_t attend_rows(hipStream_t stream, const TreeAttentionArgs& a, const Shape& s, void* workspace) {
-    if constexpr (kDim == 256) {
-        if (s.waves == 1) return attend<kDim, kBf16, kF32, 1, 1, 2>(stream, a, s, workspace);
-        if (s.waves == 2) return attend<kDim, kBf16, kF32, 1, 2, 2>(stream, a, s, workspace);
-        return attend<kDim, kBf16, kF32, 1, 4, 2>(stream, a, s, workspace);
-    } else {
-        constexpr int kAlone = kDim == 64 ? 3 : 2;
-        if (s.waves == 1) return attend<kDim, kBf16, kF32, 1, 1, kAlone>(stream, a, s, workspace);
-        if (s.waves == 2) return attend<kDim, kBf16, kF32, 1, 2, 3>(stream, a, s, workspace);
-        if (s.sixteens == 1) return attend<kDim, kBf16, kF32, 1, 4, 3>(stream, a, s, workspace);
-        return attend<kDim, kBf16, kF32, 2, 4, 4>(stream, a, s, workspace);
+    constexpr int kGroups = kDim == 256 ? 2 : 4;
+    if (s.gathered) {
+        if (s.waves == 1) return attend<kDim, kBf16, kF32, 1, 1, kGroups, 2>(stream, a, s, workspace);
+        return attend<kDim, kBf16, kF32, 1, 2, kGroups, 2>(stream, a, s, workspace);
     }
+    constexpr int kAlone = kDim == 64 ? 3 : 2, kTwo = kDim == 256 ? 2 : 3;
+    if (s.waves == 1) return attend<kDim, kBf16, kF32, 1, 1, 1, kAlone>(stream, a, s, workspace);
+    if (s.waves == 2) return attend<kDim, kBf16, kF32, 1, 2, 1, kTwo>(stream, a, s, workspace);
+    if (s.sixteens == 1) return attend<kDim, kBf16, kF32, 1, 4, 1, kTwo>(stream, a, s, workspace);
+    if constexpr (kDim < 256) return attend<kDim, kBf16, kF32, 2, 4, 1, 4>(stream, a, s, workspace);
+    else return hipErrorInvalidValue;  // (heads of 256 have one sixteen)
 }
 
 template <int kDim>
