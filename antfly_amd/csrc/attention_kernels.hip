@@ -99,29 +99,42 @@ struct Part {
 // exp2(a - b) where both may be minus infinity (nothing seen yet): then 1, of sums that are zero.
 __device__ __forceinline__ float exp2_between(float a, float b) { return a == b ? 1.0f : __builtin_amdgcn_exp2f(a - b); }
 
-// Which of the 32 keys from `first` on a row sees: bit j for key first + j.
-__device__ __forceinline__ uint32_t seen_bits(int first, int context, int token, const unsigned long long* words, int count) {
+// Which of the 32 keys from `first` on a row sees: bit j for key first + j.  `word0`: the row's first mask word; `words` null:
+// no masks.
+__device__ __forceinline__ uint32_t seen_bits(int first, int context, int token, unsigned long long word0, const unsigned long long* words, int count) {
     const int draft = first - context;  // the first key as a new token of the request
     if (words == nullptr) {
         const int left = token + 1 - draft;
         return left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
     }
     if (draft <= -32) return ~0u;
-    if (draft < 0) {
-        const uint32_t tree = count > 0 ? static_cast<uint32_t>(words[0] << -draft) : 0u;
-        return tree | ((1u << -draft) - 1);
-    }
+    if (draft < 0) return static_cast<uint32_t>(word0 << -draft) | ((1u << -draft) - 1);
     const int word = draft >> 6, shift = draft & 63;
-    unsigned long long bits = word < count ? words[word] >> shift : 0ull;
-    if (shift > 32 && word + 1 < count) bits |= words[word + 1] << (64 - shift);
+    unsigned long long low = word0, high = 0;
+    if (count > 1) {  // (otherwise no memory is read here)
+        low = word < count ? words[word] : 0ull;
+        if (shift > 32 && word + 1 < count) high = words[word + 1];
+    } else if (word > 0) {
+        low = 0;
+    }
+    unsigned long long bits = low >> shift;
+    if (shift > 32) bits |= high << (64 - shift);
     return static_cast<uint32_t>(bits);
 }
 
-// Whether one of the two values of a register is no finite number.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+// The larger magnitudes of 16 bytes and two so far, as numbers: a value that is not finite has at least the exponent's bits.
+__device__ __forceinline__ u16x2 magnitudes(u16x2 so_far, uint4 v) {
+    const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) so_far = __builtin_elementwise_max(so_far, __builtin_bit_cast(u16x2, words[i] & 0x7FFF7FFFu));
+    return so_far;
+}
 template <bool kBf16>
-__device__ __forceinline__ bool is_odd(uint32_t w) {
-    constexpr uint32_t kExponent = kBf16 ? 0x7F80u : 0x7C00u;
-    return (w & kExponent) == kExponent || (w >> 16 & kExponent) == kExponent;
+__device__ __forceinline__ bool is_odd(u16x2 most) {
+    constexpr unsigned short kExponent = kBf16 ? 0x7F80 : 0x7C00;
+    return most[0] >= kExponent || most[1] >= kExponent;
 }
 template <bool kBf16>
 __device__ __forceinline__ bool is_odd(short v) {
@@ -365,6 +378,7 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
     s16x8 query[kQ][kSteps][kTerms];
     float unit[kQ];  // what a product of the row is multiplied by: |scale|, log2(e), and for f32 on f16 the row's power of two
     const unsigned long long* words[kQ];
+    unsigned long long word0[kQ];
     int row_token[kQ];
     bool real[kQ];
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale turns the queries round
@@ -376,6 +390,7 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
         const int head = static_cast<int>(kv_head) * group + (real[qt] ? row % group : 0);
         const size_t token = static_cast<size_t>(begin + row_token[qt]);
         words[qt] = a.masks != nullptr ? a.masks + token * a.mask_words : nullptr;
+        word0[qt] = a.masks != nullptr && a.mask_words > 0 ? words[qt][0] : 0ull;
         unit[qt] = fmaxf(__builtin_fabsf(a.scale) * kLog2e, 1e-30f);  // (never 0, which would make minus infinity no number)
         const size_t from = token * a.query_token_stride + static_cast<size_t>(head) * a.query_head_stride;
         if (kF32) {
@@ -481,18 +496,22 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
         if (!clean) {
             // (all rows see the context's keys)
             const int from_row = held != ~0u ? 0 : max(context - tile, 0);
-            for (int at = from_row * kPieces + lane; at < kTile * kPieces; at += 64) {
-                const uint4 v = *reinterpret_cast<const uint4*>(v_lds + at * 16);
-                unsigned long long which = __ballot(is_odd<kBf16>(v.x) || is_odd<kBf16>(v.y) || is_odd<kBf16>(v.z) || is_odd<kBf16>(v.w));
-                while (which != 0) {
-                    const int l = __builtin_ctzll(which);
-                    which &= which - 1;
-                    odd |= 1u << __builtin_amdgcn_readlane(at / kPieces, l);
+            u16x2 most{0, 0};
+            for (int at = from_row * kPieces + lane; at < kTile * kPieces; at += 64)
+                most = magnitudes(most, *reinterpret_cast<const uint4*>(v_lds + at * 16));
+            if (__any(is_odd<kBf16>(most))) {  // which keys
+                for (int at = from_row * kPieces + lane; at < kTile * kPieces; at += 64) {
+                    unsigned long long which = __ballot(is_odd<kBf16>(magnitudes(u16x2{0, 0}, *reinterpret_cast<const uint4*>(v_lds + at * 16))));
+                    while (which != 0) {
+                        const int l = __builtin_ctzll(which);
+                        which &= which - 1;
+                        odd |= 1u << __builtin_amdgcn_readlane(at / kPieces, l);
+                    }
                 }
             }
 #pragma unroll
             for (int qt = 0; qt < kQ; ++qt) {
-                seen[qt] = real[qt] ? seen_bits(tile, context, row_token[qt], words[qt], static_cast<int>(a.mask_words)) & held : 0u;
+                seen[qt] = real[qt] ? seen_bits(tile, context, row_token[qt], word0[qt], words[qt], static_cast<int>(a.mask_words)) & held : 0u;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
 #pragma unroll
@@ -734,7 +753,9 @@ Shape shape_of(const TreeAttentionArgs& a, int compute_units) {
     const uint64_t tiles = (static_cast<uint64_t>(a.max_key_len) + kTile - 1) / kTile;
     s.plan.even = !s.gathered && a.requests <= kMostEvened;
     s.plan.row_tiles = static_cast<uint32_t>(most_row_tiles);
-    s.plan.least = 2;  // fewer tiles are not worth a workgroup
+    // A part's sums are written and read again, 8 head_dim bytes a row, where a tile of keys is 128 head_dim: fewer tiles than that, or
+    // than two, are not worth a workgroup.
+    s.plan.least = static_cast<uint32_t>(tile_rows / 16 > 2 ? tile_rows / 16 : 2);
     const uint64_t heads = a.cache.kv_heads, base = row_tiles * heads;
     // One round of what the compute units hold at once (by LDS and registers), the workgroups that rounding adds among them; a
     // batch that fills more than half of that anyway shares out over half a round more.
