@@ -22,6 +22,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 namespace afhip {
 
 namespace {
@@ -496,16 +498,19 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
         if (!clean) {
             // (all rows see the context's keys)
             const int from_row = held != ~0u ? 0 : max(context - tile, 0);
+            auto pieces_at = [&](int base) {
+                const int at = base + lane;
+                return at < kTile * kPieces ? magnitudes(u16x2{0, 0}, *reinterpret_cast<const uint4*>(v_lds + at * 16)) : u16x2{0, 0};
+            };
             u16x2 most{0, 0};
-            for (int at = from_row * kPieces + lane; at < kTile * kPieces; at += 64)
-                most = magnitudes(most, *reinterpret_cast<const uint4*>(v_lds + at * 16));
+            for (int base = from_row * kPieces; base < kTile * kPieces; base += 64) most = __builtin_elementwise_max(most, pieces_at(base));
             if (__any(is_odd<kBf16>(most))) {  // which keys
-                for (int at = from_row * kPieces + lane; at < kTile * kPieces; at += 64) {
-                    unsigned long long which = __ballot(is_odd<kBf16>(magnitudes(u16x2{0, 0}, *reinterpret_cast<const uint4*>(v_lds + at * 16))));
+                for (int base = from_row * kPieces; base < kTile * kPieces; base += 64) {
+                    unsigned long long which = __ballot(is_odd<kBf16>(pieces_at(base)));
                     while (which != 0) {
                         const int l = __builtin_ctzll(which);
                         which &= which - 1;
-                        odd |= 1u << __builtin_amdgcn_readlane(at / kPieces, l);
+                        odd |= 1u << ((base + l) / kPieces);
                     }
                 }
             }
@@ -667,8 +672,8 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
 }
 
 // The parts of a row, brought to their common maximum: a wavefront takes rows of one request in turn.  kLanes lanes have four
-// values of the row each, 64 / kLanes groups of them every so many-th part; kBatch parts are requested at a time.
-constexpr int kJoinWaves = 4, kBatch = 8;
+// values of the row each, 64 / kLanes groups of them every so many-th part; up to eight are requested at a time.
+constexpr int kJoinWaves = 4;
 template <bool kBf16, bool kF32, int kLanes>
 __global__ __launch_bounds__(kJoinWaves * 64) void join_parts_kernel(TreeAttentionArgs a, SharePlan plan, int rows_a_tile, const float* part_out,
                                                                     const Part* parts) {
@@ -685,34 +690,48 @@ __global__ __launch_bounds__(kJoinWaves * 64) void join_parts_kernel(TreeAttenti
         const size_t slot = share.first_slot + static_cast<size_t>(kv_head) * share.splits * share.row_tiles + row / rows_a_tile;
         const size_t first = slot * rows_a_tile + row % rows_a_tile;
         float most = -__builtin_inff(), total = 0.0f;
-        for (uint32_t s = lane; s < share.splits; s += 64) most = fmaxf(most, parts[first + s * stride].most);
-#pragma unroll
-        for (int w = 1; w < 64; w *= 2) most = fmaxf(most, __shfl_xor(most, w));
         f32x4 x{0, 0, 0, 0};
-        for (uint32_t s0 = group; s0 < share.splits; s0 += kBatch * kGroups) {
+        auto add = [&](auto batch, uint32_t s0) {  // (past the end: the last part again, not counted)
+            constexpr int kBatch = decltype(batch)::value;
             f32x4 y[kBatch];
             Part part[kBatch];
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) {  // (past the end: the last part again, not counted)
-                const size_t from = first + min(s0 + i * kGroups, share.splits - 1) * stride;
+            for (int i = 0; i < kBatch; ++i) {
+                const uint32_t s = s0 + group + i * kGroups;
+                const size_t from = first + min(s, share.splits - 1) * stride;
                 part[i] = parts[from];
+                if (s >= share.splits) part[i] = Part{-__builtin_inff(), 0.0f};
                 y[i] = *reinterpret_cast<const f32x4*>(part_out + from * a.cache.head_dim + (d < a.cache.head_dim ? d : 0));
             }
+            float next = most;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) next = fmaxf(next, part[i].most);
+            const float kept = exp2_between(most, next);
+            total *= kept;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] *= kept;
+            most = next;
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
-                // (a part that saw no key has not been written)
-                const bool counts = s0 + i * kGroups < share.splits && part[i].most != -__builtin_inff();
+                const bool counts = part[i].most != -__builtin_inff();  // (a part that saw no key has not been written)
                 const float by = counts ? exp2_between(part[i].most, most) : 0.0f;
                 total = __builtin_fmaf(part[i].sum, by, total);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(counts ? y[i][j] : 0.0f, by, x[j]);
             }
-        }
+        };
+        uint32_t s0 = 0;
+        for (; s0 + 8 * kGroups <= share.splits; s0 += 8 * kGroups) add(std::integral_constant<int, 8>{}, s0);
+        for (; s0 + kGroups < share.splits; s0 += 4 * kGroups) add(std::integral_constant<int, 4>{}, s0);
+        if (s0 < share.splits) add(std::integral_constant<int, 1>{}, s0);
 #pragma unroll
         for (int w = kLanes; w < 64; w *= 2) {
-            total += __shfl_xor(total, w);
+            const float other = __shfl_xor(most, w), next = fmaxf(most, other);
+            const float mine = exp2_between(most, next), theirs = exp2_between(other, next);
+            most = next;
+            total = total * mine + __shfl_xor(total, w) * theirs;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] += __shfl_xor(x[j], w);
+            for (int j = 0; j < 4; ++j) x[j] = x[j] * mine + __shfl_xor(x[j], w) * theirs;
         }
         if (group != 0 || d >= a.cache.head_dim) continue;
         store_row<kBf16, kF32>(a, static_cast<size_t>(share.begin) + row / a.group, kv_head * a.group + row % a.group, d, x, total);

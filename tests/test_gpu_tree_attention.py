@@ -127,6 +127,19 @@ def test_as_many_parts_as_a_row_can_have(activations, stored, dim):
     Batch(np.random.default_rng(dim), [15900], [2], 2, 1, dim, 16, activations, stored).check()
 
 
+@pytest.mark.parametrize("requests,context,tokens,heads,kv_heads", [(200, (0, 90), (1, 3), 16, 1), (130, (1200, 1500), (1, 2), 2, 1), (1100, (0, 60), (1, 2), 24, 1),
+                                                                    (70, (900, 1030), (1, 1), 2, 2)])
+def test_many_requests(requests, context, tokens, heads, kv_heads):
+    """More requests than a wavefront has lanes, and more than are evened out; ragged, some without new tokens."""
+    print(f"case: {requests} requests context={context} tokens={tokens} heads={heads}", flush=True)
+    rng = np.random.default_rng(requests)
+    lens = rng.integers(tokens[0], tokens[1] + 1, requests)
+    lens[[3, requests // 2]] = 0
+    lens[5] = tokens[1]
+    Batch(rng, rng.integers(context[0], context[1] + 1, requests), lens, heads, kv_heads, 64, 16, "f32", "bf16").check(
+        max_query=tokens[1] + 1, max_keys=context[1] + tokens[1])
+
+
 @pytest.mark.parametrize("activations,stored", KINDS)
 def test_prompt_without_masks(activations, stored):
     """Hundreds of new tokens behind a short context: causal, many row tiles."""
