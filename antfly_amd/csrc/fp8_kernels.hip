@@ -286,9 +286,9 @@ __global__ __launch_bounds__(kFusedWaves * 64) void linear_fp8_rows_kernel(Fp8Ma
 // of them fill and read.  Every wavefront widens its own operands: of a block's instructions about half are conversions, which
 // run beside the other wavefront's products.  `sums`: blocks of K are shared out over gridDim.y workgroups, whose sums go there,
 // [share][rows][out_dim rounded up to 4], for add_shares_kernel.
-template <int kR, int kRowWaves, int kColWaves>
+template <int kR, int kRowWaves, int kColWaves, int kStages>
 __global__ __launch_bounds__(kRowWaves * kColWaves * 64, 2) void matmul_fp8_tile_kernel(Fp8Matmul a, int row_tiles, int col_tiles, float* sums) {
-    constexpr int kWaves = kRowWaves * kColWaves, kRows = 32 * kR * kRowWaves, kCols = 64 * kColWaves, kStages = 3;
+    constexpr int kWaves = kRowWaves * kColWaves, kRows = 32 * kR * kRowWaves, kCols = 64 * kColWaves;
     constexpr int kStage = (kRows + kCols) * 128 + kWaves * 256;                 // W, X, X's scales
     constexpr int kWLoads = kCols / 8 / kWaves, kXLoads = kRows / 8 / kWaves, kLoads = kWLoads + kXLoads + 1;
     constexpr int kOwn = kRows / kWaves;                                         // rows whose scales a wavefront loads
@@ -321,26 +321,28 @@ __global__ __launch_bounds__(kRowWaves * kColWaves * 64, 2) void matmul_fp8_tile
         }
         load_dword_to_lds(to + (kCols + kRows) * 128 + wave * 256, x_scale + block);
     };
-    if (first_block < end_block) request(first_block, 0);
-    if (first_block + 1 < end_block) request(first_block + 1, 1);
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+        if (first_block + i < end_block) request(first_block + i, i);
+    }
     f32x16 total[2][kR];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
         for (int m = 0; m < kR; ++m) total[n][m] = f32x16{};
     }
-    int stage = 0, free_stage = 2;
+    int stage = 0, free_stage = kStages - 1;
     float ws_ahead = first_block < end_block ? load_uniform(w_scale + first_block) : 0.0f;
     for (int b = first_block; b < end_block; ++b) {
-        if (b + 1 < end_block) wait_loads<kLoads>();
+        if (b + kStages - 2 < end_block) wait_loads<kLoads * (kStages - 2)>();
         else wait_loads<0>();
         __syncthreads();  // everyone's part of the block is there, and the stage to be filled has been read
-        if (b + 2 < end_block) request(b + 2, free_stage);
+        if (b + kStages - 1 < end_block) request(b + kStages - 1, free_stage);
         const char* w = lds + stage * kStage + wave_o * 128;
         const char* x = lds + stage * kStage + (kCols + wave_r) * 128;
         const float* scales = reinterpret_cast<const float*>(lds + stage * kStage + (kCols + kRows) * 128);
-        stage = stage == 2 ? 0 : stage + 1;
-        free_stage = free_stage == 2 ? 0 : free_stage + 1;
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+        free_stage = free_stage + 1 == kStages ? 0 : free_stage + 1;
         const float ws = ws_ahead;
         if (b + 1 < end_block) ws_ahead = load_uniform(w_scale + b + 1);
         float scale[kR];
@@ -444,12 +446,12 @@ hipError_t rows_kernel(hipStream_t stream, const Fp8Matmul& a) {
     return hipGetLastError();
 }
 
-template <int kR, int kRowWaves, int kColWaves>
+template <int kR, int kRowWaves, int kColWaves, int kStages>
 hipError_t tile_kernel(hipStream_t stream, const Fp8Matmul& a, int shares, float* sums) {
     static LdsLimit limit;
     constexpr int kRows = 32 * kR * kRowWaves, kCols = 64 * kColWaves;
-    constexpr size_t lds = 3 * ((kRows + kCols) * 128 + kRowWaves * kColWaves * 256);
-    const auto kernel = matmul_fp8_tile_kernel<kR, kRowWaves, kColWaves>;
+    constexpr size_t lds = kStages * ((kRows + kCols) * 128 + kRowWaves * kColWaves * 256);
+    const auto kernel = matmul_fp8_tile_kernel<kR, kRowWaves, kColWaves, kStages>;
     hipError_t e = allow_lds(kernel, lds, &limit);
     if (e != hipSuccess) return e;
     const int row_tiles = (a.rows + kRows - 1) / kRows, col_tiles = (a.out_dim + kCols - 1) / kCols;
@@ -497,16 +499,18 @@ Fp8Plan plan_matmul_fp8(int rows, int in_dim, int out_dim, int compute_units, si
     if (weights > (4 << 20)) best.kernel = kFp8Rows32;
     double least = 3 + (3.0 + fmin(2.2, 4096.0 / in_dim)) * ((rows + 31) / 32) * (weights / (1 << 24));
     const auto tiles = [&](int of) { return static_cast<double>((out_dim + 127) / 128) * ((rows + of - 1) / of); };
+    // Two workgroups a compute unit at a time, `two` a block of K; a last round of one a unit takes `one`.
+    const auto rounds = [&](double n, double one, double two) {
+        const double full = floor(n / (2 * units)), left = n - full * 2 * units;
+        return full * two + (left > units ? two : left > 0 ? one : 0);
+    };
     for (int shares = 1; shares <= 8; shares *= 2) {
         const size_t sums = Fp8Plan{kFp8Tile64, shares}.sums_bytes(rows, out_dim);
         if (shares > 1 && (sums > room || blocks < 4 * shares)) break;
         const double each = ceil(blocks / shares), rest = 4 + (shares > 1 ? 3 + 2.0 * sums / 5e6 : 0.0);
-        const double t64 = rest + each * (tiles(64) * shares <= units ? 1.06 : 1.4 * ceil(tiles(64) * shares / (2 * units)));
-        const double t128 = rest + each * 1.33 * ceil(tiles(128) * shares / units);
-        const double t256 = rest + each * 1.75 * ceil(tiles(256) * shares / units);
+        const double t64 = rest + each * rounds(tiles(64) * shares, 1.04, 1.36), t128 = rest + each * rounds(tiles(128) * shares, 1.22, 1.98);
         if (t64 < least) least = t64, best = Fp8Plan{kFp8Tile64, shares};
         if (t128 < least) least = t128, best = Fp8Plan{kFp8Tile128, shares};
-        if (t256 < least) least = t256, best = Fp8Plan{kFp8Tile256, shares};
     }
     return best;
 }
@@ -515,9 +519,8 @@ hipError_t launch_matmul_fp8(hipStream_t stream, const Fp8Matmul& a, const Fp8Pl
     switch (plan.kernel) {
         case kFp8Rows16: return rows_kernel<1, 8, 2>(stream, a);
         case kFp8Rows32: return rows_kernel<2, 8, 2>(stream, a);
-        case kFp8Tile64: return tile_kernel<1, 2, 2>(stream, a, plan.shares, sums);
-        case kFp8Tile128: return tile_kernel<2, 2, 2>(stream, a, plan.shares, sums);
-        default: return tile_kernel<2, 4, 2>(stream, a, plan.shares, sums);
+        case kFp8Tile64: return tile_kernel<1, 2, 2, 3>(stream, a, plan.shares, sums);
+        default: return tile_kernel<2, 2, 2, 2>(stream, a, plan.shares, sums);
     }
 }
 
