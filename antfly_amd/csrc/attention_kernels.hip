@@ -91,7 +91,7 @@ __device__ __forceinline__ float row_sum(float v) {
     return v + other;
 }
 
-__device__ __forceinline__ uint32_t divide(uint32_t n, const Divisor& d) { return d.multiplier == 0 ? n : __umulhi(n, d.multiplier); }
+__device__ __forceinline__ uint32_t divide(uint32_t n, const Divisor& d) { return __umulhi(n, d.multiplier) + (n & d.whole); }
 
 // What a split of a request's keys holds for one row: the row's maximum (in units of log2) and the sum of its weights.
 struct Part {
@@ -205,13 +205,21 @@ __device__ __forceinline__ Share lengths_of(const TreeAttentionArgs& a, uint32_t
     return s;
 }
 
+// A lane's value of the data-parallel move kControl, zero where the move has none for it or its row of 16 is not in kRows.
+template <int kControl, int kRows, typename T>
+__device__ __forceinline__ T moved(T v) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kControl, kRows, 0xF, false));
+}
+
+// Sum over the wavefront's lanes up to this one: within rows of 16 lanes, then the rows below.
 template <typename T>
-__device__ __forceinline__ T sum_up_to(T v, int lane) {  // over the wavefront's lanes up to this one
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const T other = __shfl_up(v, d);
-        if (lane >= d) v += other;
-    }
+__device__ __forceinline__ T sum_up_to(T v) {
+    v += moved<0x111, 0xF>(v);  // from 1, 2, 4, 8 lanes below
+    v += moved<0x112, 0xF>(v);
+    v += moved<0x114, 0xF>(v);
+    v += moved<0x118, 0xF>(v);
+    v += moved<0x142, 0xA>(v);  // a row's last lane to the next row
+    v += moved<0x143, 0xC>(v);  // lane 31 to the upper half
     return v;
 }
 
@@ -249,8 +257,7 @@ __device__ __forceinline__ bool find_share(const TreeAttentionArgs& a, const Sha
             work += static_cast<float>((mine.keys + kTile - 1) / kTile) * static_cast<float>(mine.row_tiles);
         }
     }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) work += __shfl_xor(work, d);
+    work = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sum_up_to(work)), 63));
     const float each = work * (static_cast<float>(heads) * 1.001f) / static_cast<float>(plan.target);
     const uint32_t tiles = max(static_cast<uint32_t>(fminf(each, 0x1p30f)) + 1, plan.least);
     uint32_t before = 0, slots_before = 0;
@@ -265,7 +272,7 @@ __device__ __forceinline__ bool find_share(const TreeAttentionArgs& a, const Sha
             count = mine.row_tiles * mine.splits * heads;
             slots = mine.splits > 1 ? count : 0;
         }
-        const uint32_t upto = sum_up_to(count, lane), slots_upto = sum_up_to(slots, lane);
+        const uint32_t upto = sum_up_to(count), slots_upto = sum_up_to(slots);
         mine.first = before + upto - count;
         mine.first_slot = slots_before + slots_upto - slots;
         const unsigned long long here = kByRequest ? (of >= r0 && of < r0 + 64 ? 1ull << (of - r0) : 0ull)
@@ -332,33 +339,41 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
     const int pieces = static_cast<int>(a.cache.head_dim / 8);  // that hold something
     const bool whole_heads = pieces == kPieces;
 
-    // where 64 blocks from `window_at` on lie, in 16-byte units, one a lane
+    // where 64 blocks from `window_at` on lie, in 16-byte units, one a lane; which of them there are
     const int* table = a.block_tables + static_cast<size_t>(request) * a.table_columns;
     const uint32_t last_block = key_begin < key_end ? divide(static_cast<uint32_t>(key_end - 1), a.block_size) : 0;
-    uint32_t window = kNowhere, window_at = 0, window_end = 0;  // (keys from window_end on are not in it)
-    auto place = [&](int tile) -> uint32_t {  // of key tile + lane % 32
+    uint32_t window = 0, window_at = 0, window_end = 0;  // (keys from window_end on are not in it)
+    unsigned long long there = 0;
+    // Where this lane's row of load i of a tile lies.  (A key without a place is not seen by any row: what is loaded for it may
+    // be anything.)
+    uint32_t block_at[kLoads], past[kLoads];  // its block's place, and how far into the block
+    auto find_rows = [&](int tile) -> uint32_t {  // the tile's keys that have a place
         if (static_cast<uint32_t>(tile) + kTile > window_end) {
             window_at = divide(static_cast<uint32_t>(tile), a.block_size);
-            const uint32_t column = window_at + lane;
-            const uint32_t block = column <= last_block ? static_cast<uint32_t>(table[column]) : kNowhere;
-            window = block < a.cache.blocks ? block * a.cache.block_stride + kv_head * a.cache.head_stride : kNowhere;
+            const uint32_t block_column = window_at + lane;
+            const uint32_t block = block_column <= last_block ? static_cast<uint32_t>(table[block_column]) : kNowhere;
+            there = __ballot(block < a.cache.blocks);
+            window = block < a.cache.blocks ? block * a.cache.block_stride + kv_head * a.cache.head_stride : 0;
             window_end = (window_at + 64) * a.block_size.by;  // (below 2^32: a bound of the keys times the block size)
         }
-        const uint32_t key = static_cast<uint32_t>(tile) + (lane & 31), block = divide(key, a.block_size);
-        const uint32_t at = static_cast<uint32_t>(__shfl(static_cast<int>(window), static_cast<int>(block - window_at)));
-        return at == kNowhere || static_cast<int>(key) >= key_end ? kNowhere : at + (key - block * a.block_size.by) * a.cache.slot_stride;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t key = static_cast<uint32_t>(tile) + (row_wave * kLoads + i) * (64 / kPieces) + lane / kPieces, block = divide(key, a.block_size);
+            // (a place past the last key's block is block 0's)
+            block_at[i] = static_cast<uint32_t>(__shfl(static_cast<int>(window), static_cast<int>(block - window_at)));
+            past[i] = (key - block * a.block_size.by) * a.cache.slot_stride;
+        }
+        const uint32_t key = static_cast<uint32_t>(tile) + (lane & 31), column_of = divide(key, a.block_size) - window_at;
+        return static_cast<uint32_t>(__ballot((there >> column_of & 1) != 0 && static_cast<int>(key) < key_end));
     };
-    // Requests this wavefront's part of a tile's K and V; which of its keys have a place.
-    auto request_tile = [&](int tile, int stage) -> uint32_t {
-        const uint32_t at = place(tile);  // lane l % 32 has the place of key l % 32
-        // a key without a place is not seen by any row: what is loaded for it may be anything
-        const int there = static_cast<int>(at == kNowhere ? 0u : at);
+    // Requests this wavefront's part of the K and V that find_rows() has found.
+    auto request_tile = [&](int stage) {
         const uint32_t to = ring_at + stage * (2 * kTileBytes) + row_wave * (kLoads * 1024);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int slot = (row_wave * kLoads + i) * 64 + lane, row = slot / kPieces;
             const int kp = key_piece<kDim>(row, slot % kPieces) % kPieces, vp = value_piece<kDim>(row, slot % kPieces) % kPieces;
-            const uint32_t from = static_cast<uint32_t>(__shfl(there, row));
+            const uint32_t from = block_at[i] + past[i];
             const uint4 *k = a.cache.keys + (from + kp), *v = a.cache.values + (from + vp);
             if (!whole_heads) {
                 if (kp >= pieces) k = &kNothing;
@@ -367,13 +382,13 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
             load_to_lds(to + i * 1024, k);
             load_to_lds(to + kTileBytes + i * 1024, v);
         }
-        return static_cast<uint32_t>(__ballot(at != kNowhere));
     };
-    uint32_t held_ahead[kStages - 1];  // of the tiles on their way, the next one's first
+    uint32_t held_ahead[kStages];  // of the tiles on their way, the next one's first, and of the one found
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) {
+    for (int i = 0; i < kStages; ++i) {
         const int tile = key_begin + key_group * kTile + i * kStep;
-        held_ahead[i] = tile < key_end ? request_tile(tile, i) : 0u;
+        held_ahead[i] = tile < key_end ? find_rows(tile) : 0u;
+        if (i < kStages - 1 && tile < key_end) request_tile(i);
     }
 
     // ---- the rows
@@ -469,8 +484,9 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
         if (kRowWaves > 1) __syncthreads();        // everyone's is, and the stage to be filled has been read
         const uint32_t held = held_ahead[0];
 #pragma unroll
-        for (int i = 0; i + 1 < kStages - 1; ++i) held_ahead[i] = held_ahead[i + 1];
-        if (tile + (kStages - 1) * kStep < key_end) held_ahead[kStages - 2] = request_tile(tile + (kStages - 1) * kStep, free_stage);
+        for (int i = 0; i + 1 < kStages; ++i) held_ahead[i] = held_ahead[i + 1];
+        if (tile + (kStages - 1) * kStep < key_end) request_tile(free_stage);
+        if (tile + kStages * kStep < key_end) held_ahead[kStages - 1] = find_rows(tile + kStages * kStep);  // a tile ahead of its request
         const char* k_lds = ring + stage * (2 * kTileBytes);
         const char* v_lds = k_lds + kTileBytes;
         stage = stage + 1 == kStages ? 0 : stage + 1;
@@ -478,21 +494,41 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
         if (!works || tile >= key_end) continue;
         const bool clean = tile + kTile <= context && held == ~0u;  // every row sees every key
 
-        f32x4 score[kQ][2];
+        // the operands of a product first, all of them: none of them waits for LDS by itself
+        s16x8 key[2][kSteps];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                // (rows 16 apart have their pieces in the same order)
-                const s16x8 k = *reinterpret_cast<const s16x8*>(k_lds + key_piece<kDim>(column, s * 4 + quarter) * 16 + half * (16 * kDim * 2));
+            for (int s = 0; s < kSteps; ++s)  // (rows 16 apart have their pieces in the same order)
+                key[half][s] = *reinterpret_cast<const s16x8*>(k_lds + key_piece<kDim>(column, s * 4 + quarter) * 16 + half * (16 * kDim * 2));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4 score[kQ][2];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
 #pragma unroll
                 for (int qt = 0; qt < kQ; ++qt) {
 #pragma unroll
                     for (int term = kTerms - 1; term >= 0; --term)  // the small terms first
-                        score[qt][half] = mfma<kBf16>(k, query[qt][s][term], s == 0 && term == kTerms - 1 ? f32x4{0, 0, 0, 0} : score[qt][half]);
+                        score[qt][half] = mfma<kBf16>(key[half][s], query[qt][s][term], s == 0 && term == kTerms - 1 ? f32x4{0, 0, 0, 0} : score[qt][half]);
                 }
             }
         }
+        s16x8 value[kDim / 16];
+#pragma unroll
+        for (int d = 0; d < kDim / 16; ++d) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int row = quarter * 4 + (column >> 2);
+                const char* from = v_lds + value_piece<kDim>(row, d * 2 + (column >> 1 & 1)) * 16 + (column & 1) * 8 + half * (16 * kDim * 2);
+                const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)from);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) value[d][half * 4 + j] = four[j];
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
         uint32_t odd = 0;  // keys with a value that is no finite number (looked for only where some row may not see them)
         uint32_t seen[kQ];
         if (!clean) {
@@ -569,25 +605,19 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
             }
         }
         odd = __builtin_amdgcn_readfirstlane(odd);
+        if (odd != 0) {
 #pragma unroll
-        for (int d = 0; d < kDim / 16; ++d) {
-            s16x8 v;
+            for (int d = 0; d < kDim / 16; ++d) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int row = quarter * 4 + (column >> 2);
-                const char* from = v_lds + value_piece<kDim>(row, d * 2 + (column >> 1 & 1)) * 16 + (column & 1) * 8 + half * (16 * kDim * 2);
-                const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)from);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[half * 4 + j] = four[j];
+                for (int j = 0; j < 8; ++j) value[d][j] = is_odd<kBf16>(static_cast<short>(value[d][j])) ? static_cast<short>(0) : value[d][j];
             }
-            if (odd != 0) {
+        }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = is_odd<kBf16>(static_cast<short>(v[j])) ? static_cast<short>(0) : v[j];
-            }
+        for (int term = kTerms - 1; term >= 0; --term) {
 #pragma unroll
-            for (int qt = 0; qt < kQ; ++qt) {
+            for (int d = 0; d < kDim / 16; ++d) {
 #pragma unroll
-                for (int term = kTerms - 1; term >= 0; --term) out[qt][d] = mfma<kBf16>(v, weight[qt][term], out[qt][d]);
+                for (int qt = 0; qt < kQ; ++qt) out[qt][d] = mfma<kBf16>(value[d], weight[qt][term], out[qt][d]);
             }
         }
         // A row that does not see a key must not get 0 * inf from it: the products above took such values as zeros, and the

@@ -19,11 +19,11 @@ struct CacheView {
 };
 
 // n / d for a fixed d: n * ceil(2^32 / d) >> 32, exact while n * d < 2^32 (the product's error, n * (d - 1) at most, stays
-// below 2^32); d = 1 has no 32-bit multiplier and is marked by 0.
+// below 2^32).
 struct Divisor {
-    uint32_t by, multiplier;
+    uint32_t by, multiplier, whole;  // whole: all bits where the divisor is 1, whose multiplier 2^32 does not fit
     Divisor() : Divisor(1) {}
-    explicit Divisor(uint32_t d) : by(d), multiplier(d == 1 ? 0 : static_cast<uint32_t>(((uint64_t{1} << 32) + d - 1) / d)) {}
+    explicit Divisor(uint32_t d) : by(d), multiplier(d == 1 ? 0 : static_cast<uint32_t>(((uint64_t{1} << 32) + d - 1) / d)), whole(d == 1 ? ~0u : 0) {}
 };
 
 constexpr int kPlanTokens = 1024;       // token places of one workgroup
