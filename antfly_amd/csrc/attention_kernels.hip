@@ -126,21 +126,10 @@ __device__ __forceinline__ uint32_t seen_bits(int first, int context, int token,
 
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
-// The larger magnitudes of 16 bytes and two so far, as numbers: a value that is not finite has at least the exponent's bits.
-__device__ __forceinline__ u16x2 magnitudes(u16x2 so_far, uint4 v) {
-    const uint32_t words[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) so_far = __builtin_elementwise_max(so_far, __builtin_bit_cast(u16x2, words[i] & 0x7FFF7FFFu));
-    return so_far;
-}
+// No finite number: all bits of the exponent.
 template <bool kBf16>
-__device__ __forceinline__ bool is_odd(u16x2 most) {
+__device__ __forceinline__ bool is_odd(unsigned short v) {
     constexpr unsigned short kExponent = kBf16 ? 0x7F80 : 0x7C00;
-    return most[0] >= kExponent || most[1] >= kExponent;
-}
-template <bool kBf16>
-__device__ __forceinline__ bool is_odd(short v) {
-    constexpr short kExponent = kBf16 ? 0x7F80 : 0x7C00;
     return (v & kExponent) == kExponent;
 }
 
@@ -383,22 +372,14 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
             load_to_lds(to + kTileBytes + i * 1024, v);
         }
     };
-    uint32_t held_ahead[kStages];  // of the tiles on their way, the next one's first, and of the one found
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) {
-        const int tile = key_begin + key_group * kTile + i * kStep;
-        held_ahead[i] = tile < key_end ? find_rows(tile) : 0u;
-        if (i < kStages - 1 && tile < key_end) request_tile(i);
-    }
-
     // ---- the rows
-    s16x8 query[kQ][kSteps][kTerms];
+    // (requested before the tiles: what waits for them does not wait for a tile)
+    uint4 raw[kQ][kSteps][kF32 ? 2 : 1];
     float unit[kQ];  // what a product of the row is multiplied by: |scale|, log2(e), and for f32 on f16 the row's power of two
     const unsigned long long* words[kQ];
     unsigned long long word0[kQ];
     int row_token[kQ];
     bool real[kQ];
-    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale turns the queries round
 #pragma unroll
     for (int qt = 0; qt < kQ; ++qt) {
         const int row = my_row + qt * 16 + column;
@@ -410,19 +391,37 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
         word0[qt] = a.masks != nullptr && a.mask_words > 0 ? words[qt][0] : 0ull;
         unit[qt] = fmaxf(__builtin_fabsf(a.scale) * kLog2e, 1e-30f);  // (never 0, which would make minus infinity no number)
         const size_t from = token * a.query_token_stride + static_cast<size_t>(head) * a.query_head_stride;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int piece = s * 4 + quarter;
+            const char* p = static_cast<const char*>(a.query) + (from + static_cast<size_t>(piece) * 8) * (kF32 ? 4 : 2);
+#pragma unroll
+            for (int i = 0; i < (kF32 ? 2 : 1); ++i) raw[qt][s][i] = real[qt] && piece < pieces ? reinterpret_cast<const uint4*>(p)[i] : uint4{0, 0, 0, 0};
+        }
+    }
+
+    uint32_t held_ahead[kStages];  // of the tiles on their way, the next one's first, and of the one found
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) {
+        const int tile = key_begin + key_group * kTile + i * kStep;
+        held_ahead[i] = tile < key_end ? find_rows(tile) : 0u;
+        if (i < kStages - 1 && tile < key_end) request_tile(i);
+    }
+
+    s16x8 query[kQ][kSteps][kTerms];
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale turns the queries round
+#pragma unroll
+    for (int qt = 0; qt < kQ; ++qt) {
         if (kF32) {
             float v[kSteps][8];
             float most = 0.0f;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
-                const int piece = s * 4 + quarter;
-                const bool held = real[qt] && piece < pieces;
-                const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.query) + from) + 2 * piece;
-                const float4 x = held ? p[0] : float4{0, 0, 0, 0}, y = held ? p[1] : float4{0, 0, 0, 0};
-                v[s][0] = x.x; v[s][1] = x.y; v[s][2] = x.z; v[s][3] = x.w;
-                v[s][4] = y.x; v[s][5] = y.y; v[s][6] = y.z; v[s][7] = y.w;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
+                    const uint4 four = raw[qt][s][j / 4 * kF32];
+                    const uint32_t words[4] = {four.x, four.y, four.z, four.w};
+                    v[s][j] = __builtin_bit_cast(float, words[j % 4]);
                     if (flip != 0) v[s][j] = -v[s][j];
                     most = fmaxf(most, __builtin_fabsf(v[s][j]));
                 }
@@ -453,11 +452,8 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
         } else {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
-                const int piece = s * 4 + quarter;
-                const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.query) + from) + piece;
-                uint4 raw = real[qt] && piece < pieces ? *p : uint4{0, 0, 0, 0};
-                raw = uint4{raw.x ^ flip, raw.y ^ flip, raw.z ^ flip, raw.w ^ flip};
-                query[qt][s][0] = __builtin_bit_cast(s16x8, raw);
+                const uint4 v = raw[qt][s][0];
+                query[qt][s][0] = __builtin_bit_cast(s16x8, uint4{v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip});
             }
         }
     }
@@ -532,21 +528,24 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
         uint32_t odd = 0;  // keys with a value that is no finite number (looked for only where some row may not see them)
         uint32_t seen[kQ];
         if (!clean) {
-            // (all rows see the context's keys)
-            const int from_row = held != ~0u ? 0 : max(context - tile, 0);
-            auto pieces_at = [&](int base) {
-                const int at = base + lane;
-                return at < kTile * kPieces ? magnitudes(u16x2{0, 0}, *reinterpret_cast<const uint4*>(v_lds + at * 16)) : u16x2{0, 0};
-            };
-            u16x2 most{0, 0};
-            for (int base = from_row * kPieces; base < kTile * kPieces; base += 64) most = __builtin_elementwise_max(most, pieces_at(base));
-            if (__any(is_odd<kBf16>(most))) {  // which keys
-                for (int base = from_row * kPieces; base < kTile * kPieces; base += 64) {
-                    unsigned long long which = __ballot(is_odd<kBf16>(pieces_at(base)));
-                    while (which != 0) {
-                        const int l = __builtin_ctzll(which);
-                        which &= which - 1;
-                        odd |= 1u << ((base + l) / kPieces);
+            u16x2 most[4];  // largest magnitudes of this lane's keys: two a register, as in `value`
+#pragma unroll
+            for (int pair = 0; pair < 4; ++pair) {
+                most[pair] = u16x2{0, 0};
+#pragma unroll
+                for (int d = 0; d < kDim / 16; ++d) {
+                    const u16x2 two{static_cast<unsigned short>(value[d][2 * pair]), static_cast<unsigned short>(value[d][2 * pair + 1])};
+                    most[pair] = __builtin_elementwise_max(most[pair], static_cast<u16x2>(two & static_cast<unsigned short>(0x7FFF)));
+                }
+            }
+            u16x2 all = __builtin_elementwise_max(__builtin_elementwise_max(most[0], most[1]), __builtin_elementwise_max(most[2], most[3]));
+            if (__any(is_odd<kBf16>(all[0]) || is_odd<kBf16>(all[1]))) {  // which keys
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const unsigned long long which = __ballot(is_odd<kBf16>(most[j / 2][j % 2]));
+#pragma unroll
+                    for (int holder = 0; holder < 4; ++holder) {
+                        if ((which >> (holder * 16) & 0xFFFF) != 0) odd |= 1u << (j / 4 * 16 + holder * 4 + j % 4);
                     }
                 }
             }
@@ -609,7 +608,7 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
 #pragma unroll
             for (int d = 0; d < kDim / 16; ++d) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) value[d][j] = is_odd<kBf16>(static_cast<short>(value[d][j])) ? static_cast<short>(0) : value[d][j];
+                for (int j = 0; j < 8; ++j) value[d][j] = is_odd<kBf16>(static_cast<unsigned short>(value[d][j])) ? static_cast<short>(0) : value[d][j];
             }
         }
 #pragma unroll
@@ -641,7 +640,7 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
                     const s16x4 four = *reinterpret_cast<const s16x4*>(from);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        if (is_odd<kBf16>(static_cast<short>(four[j]))) out[qt][d][j] = __builtin_fmaf(p, widen<kBf16>(four[j]), out[qt][d][j]);
+                        if (is_odd<kBf16>(static_cast<unsigned short>(four[j]))) out[qt][d][j] = __builtin_fmaf(p, widen<kBf16>(four[j]), out[qt][d][j]);
                     }
                 }
             }
@@ -715,7 +714,10 @@ __global__ __launch_bounds__(kJoinWaves * 64) void join_parts_kernel(TreeAttenti
     const uint32_t group = lane / kLanes, d = lane % kLanes * 4;
     const uint32_t rows = static_cast<uint32_t>(share.tokens) * a.group;  // of one key head
     const size_t stride = static_cast<size_t>(share.row_tiles) * rows_a_tile;
-    for (uint32_t at = blockIdx.x * kJoinWaves + (threadIdx.x >> 6); at < rows * a.cache.kv_heads; at += gridDim.x * kJoinWaves) {
+    const bool alone = share.splits <= 8;
+    const uint32_t rows_a_wave = alone ? kGroups : 1, step = alone ? 1 : kGroups, first_part = alone ? 0 : group;
+    for (uint32_t base = (blockIdx.x * kJoinWaves + (threadIdx.x >> 6)) * rows_a_wave; base < rows * a.cache.kv_heads; base += gridDim.x * kJoinWaves * rows_a_wave) {
+        const uint32_t at = min(base + (alone ? group : 0), rows * a.cache.kv_heads - 1);  // (past the last row: it again, not stored)
         const uint32_t kv_head = at / rows, row = at % rows;
         const size_t slot = share.first_slot + static_cast<size_t>(kv_head) * share.splits * share.row_tiles + row / rows_a_tile;
         const size_t first = slot * rows_a_tile + row % rows_a_tile;
@@ -727,7 +729,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void join_parts_kernel(TreeAttenti
             Part part[kBatch];
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
-                const uint32_t s = s0 + group + i * kGroups;
+                const uint32_t s = s0 + first_part + i * step;
                 const size_t from = first + min(s, share.splits - 1) * stride;
                 part[i] = parts[from];
                 if (s >= share.splits) part[i] = Part{-__builtin_inff(), 0.0f};
@@ -751,11 +753,11 @@ __global__ __launch_bounds__(kJoinWaves * 64) void join_parts_kernel(TreeAttenti
             }
         };
         uint32_t s0 = 0;
-        for (; s0 + 8 * kGroups <= share.splits; s0 += 8 * kGroups) add(std::integral_constant<int, 8>{}, s0);
-        for (; s0 + kGroups < share.splits; s0 += 4 * kGroups) add(std::integral_constant<int, 4>{}, s0);
+        for (; s0 + 8 * step <= share.splits; s0 += 8 * step) add(std::integral_constant<int, 8>{}, s0);
+        for (; s0 + step < share.splits; s0 += 4 * step) add(std::integral_constant<int, 4>{}, s0);
         if (s0 < share.splits) add(std::integral_constant<int, 1>{}, s0);
 #pragma unroll
-        for (int w = kLanes; w < 64; w *= 2) {
+        for (int w = kLanes; w < 64 && !alone; w *= 2) {
             const float other = __shfl_xor(most, w), next = fmaxf(most, other);
             const float mine = exp2_between(most, next), theirs = exp2_between(other, next);
             most = next;
@@ -763,7 +765,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void join_parts_kernel(TreeAttenti
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = x[j] * mine + __shfl_xor(x[j], w) * theirs;
         }
-        if (group != 0 || d >= a.cache.head_dim) continue;
+        if ((alone ? base + group >= rows * a.cache.kv_heads : group != 0) || d >= a.cache.head_dim) continue;
         store_row<kBf16, kF32>(a, static_cast<size_t>(share.begin) + row / a.group, kv_head * a.group + row % a.group, d, x, total);
     }
 }
