@@ -21,6 +21,7 @@
 #include "paged_launch.h"
 
 #include <hip/hip_runtime.h>
+#include <math.h>
 
 #include <type_traits>
 
@@ -212,14 +213,17 @@ __device__ __forceinline__ T sum_up_to(T v) {
     return v;
 }
 
-// How the keys are shared out.  A part has the same number of tiles for all requests (rounded to whole tiles and evened out
-// within a request): all the batch's tiles of keys, counted once for every row tile and key head, over plan.target
-// workgroups, and `least` tiles at least.  Workgroups are numbered by request, key head, part, row tile; parts of requests that
-// have several are numbered the same way.  Every wavefront works this out for itself from the lengths.
+// How the keys are shared out.  A part has the same number of tiles for all requests (evened out within a request), `least`
+// at least: the smallest of a few sizes for which the parts, each request's rounded up, are no more than plan.most
+// workgroups.  The sizes lie between what plan.most would hold if nothing had to be rounded and what it surely holds, when
+// the rounding adds a part to every row tile and key head.  Workgroups are numbered by request, key head, part, row tile;
+// parts of requests that have several are numbered the same way.  Every wavefront works this out for itself from the lengths.
 struct SharePlan {
-    uint32_t target, least;
-    uint32_t row_tiles;  // of the largest request
-    bool even;           // otherwise every request is one part, and has as many workgroups as the largest may need
+    uint32_t target, most, least;  // workgroups without and with the rounding's
+    uint32_t row_tiles;            // of the largest request
+    uint32_t slots;                // parts that there is room for
+    bool one_round;                // all parts at once: as many as plan.most allows
+    bool even;                     // otherwise every request is one part, and has as many workgroups as the largest may need
 };
 
 // `of`: a workgroup's number (by_request false) or a request's.  False: there is no such workgroup.
@@ -247,8 +251,39 @@ __device__ __forceinline__ bool find_share(const TreeAttentionArgs& a, const Sha
         }
     }
     work = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sum_up_to(work)), 63));
-    const float each = work * (static_cast<float>(heads) * 1.001f) / static_cast<float>(plan.target);
-    const uint32_t tiles = max(static_cast<uint32_t>(fminf(each, 0x1p30f)) + 1, plan.least);
+    const auto size = [&](uint32_t workgroups) {
+        const float each = work * (static_cast<float>(heads) * 1.001f) / static_cast<float>(workgroups);
+        return max(static_cast<uint32_t>(fminf(each, 0x1p30f)) + 1, plan.least);
+    };
+    // (a quotient in floats may be off by a part: the same here and below, and a part's tiles follow from it)
+    const auto parts_of = [](uint32_t all, float inverse) { return max(static_cast<uint32_t>(static_cast<float>(all) * inverse + 0.9999f), 1u); };
+    constexpr int kSizes = 4;
+    const uint32_t surely = size(plan.target), hardly = plan.one_round ? min(size(plan.most), surely) : surely;
+    uint32_t tiles = surely;
+    if (hardly < surely) {
+        uint32_t sizes[kSizes], counts[kSizes];
+        float inverse[kSizes];
+#pragma unroll
+        for (int i = 0; i < kSizes; ++i) {
+            sizes[i] = hardly + (surely - hardly) * i / kSizes;
+            inverse[i] = __builtin_amdgcn_rcpf(static_cast<float>(sizes[i]));
+            counts[i] = 0;
+        }
+        for (uint32_t r0 = 0; r0 < a.requests; r0 += 64) {
+            if (r0 + lane < a.requests) {
+                if (a.requests > 64) mine = lengths_of(a, r0 + lane, rows_a_tile);
+                const uint32_t all = (mine.keys + kTile - 1) / kTile;
+#pragma unroll
+                for (int i = 0; i < kSizes; ++i) counts[i] += mine.row_tiles * parts_of(all, inverse[i]);
+            }
+        }
+#pragma unroll
+        for (int i = kSizes - 1; i >= 0; --i) {
+            const uint32_t parts = __builtin_amdgcn_readlane(sum_up_to(counts[i]), 63);
+            if (parts * heads <= plan.most) tiles = sizes[i];
+        }
+    }
+    const float inverse_tiles = __builtin_amdgcn_rcpf(static_cast<float>(tiles));
     uint32_t before = 0, slots_before = 0;
     for (uint32_t r0 = 0; r0 < a.requests; r0 += 64) {
         uint32_t count = 0, slots = 0;
@@ -256,7 +291,7 @@ __device__ __forceinline__ bool find_share(const TreeAttentionArgs& a, const Sha
         if (r0 + lane < a.requests) {
             if (a.requests > 64) mine = lengths_of(a, r0 + lane, rows_a_tile);
             const uint32_t all = (mine.keys + kTile - 1) / kTile;
-            mine.splits = max((all + tiles - 1) / tiles, 1u);
+            mine.splits = parts_of(all, inverse_tiles);
             mine.tiles = (all + mine.splits - 1) / mine.splits;
             count = mine.row_tiles * mine.splits * heads;
             slots = mine.splits > 1 ? count : 0;
@@ -307,7 +342,7 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
     const uint32_t kv_head = inside / share.row_tiles / share.splits, slot = share.first_slot + inside;
     const int begin = share.begin, context = share.context, group = static_cast<int>(a.group), rows = share.tokens * group;
     const int first_row = static_cast<int>(row_tile) * kRows;
-    if (first_row >= rows) return;
+    if (first_row >= rows || (share.splits > 1 && slot >= plan.slots)) return;
     int keys = share.keys;
     const int last_token = min(first_row + kRows - 1, rows - 1) / group;
     if (a.masks == nullptr) keys = static_cast<int>(min(static_cast<unsigned long long>(keys), static_cast<unsigned long long>(context) + last_token + 1));
@@ -710,6 +745,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void join_parts_kernel(TreeAttenti
     uint32_t request;
     Share share;
     if (!find_share<true>(a, plan, rows_a_tile, blockIdx.y, &request, &share) || share.splits == 1) return;
+    if (share.first_slot + share.row_tiles * share.splits * a.cache.kv_heads > plan.slots) return;  // (starts that go back: more rows than tokens)
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const uint32_t group = lane / kLanes, d = lane % kLanes * 4;
     const uint32_t rows = static_cast<uint32_t>(share.tokens) * a.group;  // of one key head
@@ -802,30 +838,38 @@ Shape shape_of(const TreeAttentionArgs& a, int compute_units) {
     uint64_t row_tiles = static_cast<uint64_t>(a.tokens) * a.group / tile_rows + a.requests;
     if (row_tiles > a.requests * most_row_tiles) row_tiles = a.requests * most_row_tiles;
     const uint64_t tiles = (static_cast<uint64_t>(a.max_key_len) + kTile - 1) / kTile;
-    s.plan.even = !s.gathered && a.requests <= kMostEvened;
     s.plan.row_tiles = static_cast<uint32_t>(most_row_tiles);
     // A part's sums are written and read again, 8 head_dim bytes a row, where a tile of keys is 128 head_dim: fewer tiles than that, or
     // than two, are not worth a workgroup.
     s.plan.least = static_cast<uint32_t>(tile_rows / 16 > 2 ? tile_rows / 16 : 2);
     const uint64_t heads = a.cache.kv_heads, base = row_tiles * heads;
     // One round of what the compute units hold at once (by LDS and registers), the workgroups that rounding adds among them; a
-    // batch that fills more than half of that anyway shares out over half a round more.
-    const uint64_t resident = static_cast<uint64_t>(compute_units) * (s.waves == 1 ? 5 : s.waves == 2 ? 3 : 2);
+    // batch that fills much of that anyway shares out over half a round more, three quarters for lone wavefronts.
+    const uint64_t resident = static_cast<uint64_t>(compute_units) * (s.waves == 1 ? 4 : s.waves == 2 ? 3 : 2), fewest = s.waves == 1 ? resident * 3 / 4 : resident / 2;
+    s.plan.one_round = s.sixteens == 2 && base <= resident;
     uint64_t target = resident > base ? resident - base : 0;
-    if (target < resident / 2) target = resident / 2;
+    if (target < fewest && !s.plan.one_round) target = fewest;
     s.plan.target = static_cast<uint32_t>(target);
+    s.plan.most = static_cast<uint32_t>(base + target);
+    s.plan.even = !s.gathered && a.requests <= kMostEvened;
+    if (s.plan.even && s.plan.one_round) {
+        // Parts are worth it where they save more tiles than the second launch takes (3 us) and their sums, in and out at 6 TB/s; a
+        // tile takes 0.75 us, 1.4 times that with two workgroups on a unit.  64 tokens x 32 heads, 8 key heads of 128, bf16: 16
+        // requests on 300 keys 24.7 us in one part and 33 in two, on 4000 keys 129 and 103; 1 request on 300 keys 18 and 16.5.
+        const double parts = fmin(base == 0 ? 1.0 : floor(static_cast<double>(s.plan.most) / base), ceil(static_cast<double>(tiles) / s.plan.least));
+        const double saved = tiles - tiles / parts * (base * parts > compute_units ? 1.4 : 1.0);
+        s.plan.even = parts > 1 && saved > 4 + 0.029 * base * parts;
+    }
     if (!s.plan.even) {
         s.groups = a.requests * most_row_tiles * heads;
-        s.slots = 0;
     } else {
-        // in parts of p tiles a request of t has at most t / p + 1, and fewer than 2 t / p if it has several; the tiles of all over
-        // p are no more than the target
         const uint64_t finest = row_tiles * heads * (tiles <= s.plan.least ? 1 : (tiles + s.plan.least - 1) / s.plan.least);
-        s.groups = row_tiles * heads + s.plan.target;
+        s.groups = s.plan.most;
         if (s.groups > finest) s.groups = finest;
-        s.slots = tiles <= s.plan.least ? 0 : 2 * static_cast<uint64_t>(s.plan.target) < s.groups ? 2 * static_cast<uint64_t>(s.plan.target) : s.groups;
     }
     s.groups = (s.groups + 8 * most_row_tiles - 1) / (8 * most_row_tiles) * (8 * most_row_tiles);
+    s.slots = !s.plan.even || tiles <= s.plan.least ? 0 : s.groups;
+    s.plan.slots = static_cast<uint32_t>(s.slots);
     return s;
 }
 
