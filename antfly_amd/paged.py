@@ -68,10 +68,16 @@ def _rows_of_heads(array, rows, heads, dim):
     return strides[0], strides[1]
 
 
+def _same_strides(a, b) -> bool:
+    """Of arrays of one shape: those of dimensions of one element say nothing."""
+    mine, theirs = a.stride(), b.stride()
+    return mine == theirs or all(n <= 1 or s == t for n, s, t in zip(a.shape, mine, theirs))
+
+
 def cache(keys, values, heads_outside: bool = False) -> _lib.PagedCache:
     """keys, values [blocks, block size, kv heads, head dim], or with heads_outside [blocks, kv heads, block size, head dim]."""
     shape, strides = keys.shape, keys.stride()
-    if len(shape) != 4 or values.shape != shape or keys.dtype != values.dtype or values.stride() != strides or \
+    if len(shape) != 4 or values.shape != shape or keys.dtype != values.dtype or not _same_strides(keys, values) or \
             (shape[3] > 1 and strides[3] != 1):
         raise _bad_shape()
     slot, head = (2, 1) if heads_outside else (1, 2)
@@ -104,7 +110,7 @@ def launchBatchPlan(stream, context_lens, query_lens, block_tables, free_blocks,
 def launchCacheStore(stream, cache: _lib.PagedCache, keys, values, slots) -> None:
     """keys, values [tokens, kv heads, head dim] (f32, f16 or bf16) into the cache's slots."""
     tokens = slots.shape[0]
-    if values.shape != keys.shape or values.stride() != keys.stride() or values.dtype != keys.dtype:
+    if values.shape != keys.shape or values.dtype != keys.dtype or not _same_strides(keys, values):
         raise _bad_shape()
     token_stride, head_stride = _rows_of_heads(keys, tokens, cache.kv_heads, cache.head_dim)
     check(_lib.lib().afhip_launch_cache_store(stream, cache, _type(keys), buffer(keys), buffer(values), token_stride, head_stride,

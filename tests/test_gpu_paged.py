@@ -200,3 +200,16 @@ def test_plan_and_store_in_a_replayed_graph():
         live = want[2] >= 0
         rows[torch.from_numpy(want[2][live]).long()] = new[0].cpu().to(torch.bfloat16)[torch.from_numpy(live)]
         assert np.array_equal(bits(cache[0]), bits(rows.view(80, block, heads, dim)))
+
+
+def test_strides_of_one_token_do_not_count():
+    """One token's keys and values as views with different strides of the token dimension."""
+    wide = torch.arange(6 * 64, dtype=torch.float32, device=G.DEV).view(1, 6, 64)
+    keys, values = wide[:, :2], wide[:, 2:4].clone(memory_format=torch.contiguous_format)
+    assert keys.stride() != values.stride()
+    k, v = (torch.zeros(3, 4, 2, 64, dtype=torch.bfloat16, device=G.DEV) for _ in range(2))
+    paged.launchCacheStore(G.stream(), paged.cache(k, v), keys, values, torch.full((1,), 6, dtype=torch.int32, device=G.DEV))
+    torch.cuda.synchronize()
+    assert torch.equal(k[1, 2], keys[0].bfloat16()) and torch.equal(v[1, 2], values[0].bfloat16())
+    k[1, 2], v[1, 2] = 0, 0
+    assert not k.any() and not v.any()
