@@ -829,10 +829,12 @@ Shape shape_of(const TreeAttentionArgs& a, int compute_units) {
         s.sixteens = rows <= 64 ? 1 : 2;
         s.waves = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     }
-    // One workgroup for all keys where a second launch would take longer than its tiles, one after the other (8 key heads of 128, bf16):
-    // 1 request of 5 tokens 10.5 us against 13.1 on 300 keys, 15.1 against 12.2 on 700; 16 requests of 1 token 16.9 against 21.6 on 1000,
-    // 27.4 against 26.3 on 1500.
-    s.gathered = rows <= 32 && a.max_key_len <= (static_cast<uint64_t>(a.requests) * a.cache.kv_heads >= 64 ? 1024 : 512);
+    // One workgroup for all keys of a key head where a second launch would take longer than its tiles, one after the other: the more
+    // such workgroups, the longer (8 key heads of 128, bf16, uniform lengths; in parts / gathered): 1 request of 1 token on 500 keys
+    // 10.0 / 8.6 us, on 1000 10.4 / 13.2; 8 requests on 700 keys 13.3 / 12.0, on 1500 16.2 / 19.7; 32 requests on 700 keys 22.1 / 18.4,
+    // on 2000 53.6 / 49.8.  Up to 2048 keys: past that ragged requests would keep few units busy.
+    const uint64_t together = 512 + 6 * static_cast<uint64_t>(a.requests) * a.cache.kv_heads;
+    s.gathered = rows <= 32 && a.max_key_len <= (together < 2048 ? together : 2048);
     const uint64_t tile_rows = s.rows_a_tile(), most_row_tiles = (rows + tile_rows - 1) / tile_rows;
     // row tiles of the whole batch: every request's last one may be part empty
     uint64_t row_tiles = static_cast<uint64_t>(a.tokens) * a.group / tile_rows + a.requests;
