@@ -203,9 +203,9 @@ __global__ __launch_bounds__(kWaves * 64) void matmul_fp8_rows_kernel(Fp8Matmul 
 //
 // While the first blocks of W are on their way, a workgroup quantizes all of X (up to 16 rows, kFusedValues values) into LDS: one
 // launch instead of two, and X read by every workgroup from L2.
-constexpr int kFusedWaves = 8, kFusedStages = 4;
-__global__ __launch_bounds__(kFusedWaves * 64) void linear_fp8_rows_kernel(Fp8Matmul a, const float* input) {
-    constexpr int kWaves = kFusedWaves, kStages = kFusedStages, kLoads = 2;
+template <int kWaves, int kStages>
+__global__ __launch_bounds__(kWaves * 64) void linear_fp8_rows_kernel(Fp8Matmul a, const float* input) {
+    constexpr int kLoads = 2;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, column = lane & 15, quarter = lane >> 4;
     const int first_o = blockIdx.x * 16, blocks = fp8_blocks(a.in_dim);
@@ -463,6 +463,21 @@ hipError_t tile_kernel(hipStream_t stream, const Fp8Matmul& a, int shares, float
     return hipGetLastError();
 }
 
+template <int kWaves, int kStages>
+hipError_t fused_kernel(hipStream_t stream, const Fp8Matmul& a, const float* input) {
+    static LdsLimit limit;
+    const size_t blocks = fp8_blocks(a.in_dim);
+    const size_t lds = kWaves * kStages * 2048 + a.rows * (blocks * kFp8Block + 16 + blocks * 4);
+    const auto kernel = linear_fp8_rows_kernel<kWaves, kStages>;
+    const hipError_t e = allow_lds(kernel, lds, &limit);
+    if (e != hipSuccess) return e;
+    kernel<<<(a.out_dim + 15) / 16, kWaves * 64, lds, stream>>>(a, input);
+    return hipGetLastError();
+}
+
+// Workgroups of 16 columns for more than two rounds and a half on the compute units.
+bool is_wide(int out_dim, int compute_units) { return (out_dim + 15) / 16 >= compute_units * 5 / 2; }
+
 }  // namespace
 
 hipError_t launch_quantize_fp8(hipStream_t stream, uint8_t* q, float* scales, const float* x, size_t rows, int in_dim) {
@@ -477,26 +492,32 @@ constexpr int64_t kFusedValues = 16384;
 
 bool linear_fp8_is_fused(int rows, int in_dim) { return rows <= 16 && static_cast<int64_t>(rows) * in_dim <= kFusedValues; }
 
-hipError_t launch_linear_fp8_fused(hipStream_t stream, const Fp8Matmul& a, const float* input) {
-    static LdsLimit limit;
-    const size_t blocks = fp8_blocks(a.in_dim);
-    const size_t lds = kFusedWaves * kFusedStages * 2048 + a.rows * (blocks * kFp8Block + 16 + blocks * 4);
-    const hipError_t e = allow_lds(linear_fp8_rows_kernel, lds, &limit);
-    if (e != hipSuccess) return e;
-    linear_fp8_rows_kernel<<<(a.out_dim + 15) / 16, kFusedWaves * 64, lds, stream>>>(a, input);
-    return hipGetLastError();
+hipError_t launch_linear_fp8_fused(hipStream_t stream, const Fp8Matmul& a, const float* input, int compute_units) {
+    // Two workgroups or more on a unit (by LDS), and as many as leave no unit idle for long in a last round: many columns four
+    // wavefronts a workgroup, few eight.  K = 4096: 1 row on 8192 columns 8.7 us with eight and 10.0 with four, 4 rows 12.8 with a
+    // ring of four (one workgroup a unit) and 11.2 with three; 1 row on 14336 columns 14.5 with eight and 12.3 with four, 4 rows 21.8
+    // and 15.9.
+    if (is_wide(a.out_dim, compute_units)) return fused_kernel<4, 2>(stream, a, input);
+    if (a.rows * a.in_dim > 8192) return fused_kernel<8, 3>(stream, a, input);
+    return fused_kernel<8, 4>(stream, a, input);
 }
 
 // What the kernels take, in us, as measured (512 to 14336 columns, K = 1024 to 14336, 24 to 2048 rows): few rows pass over W
 // once for each 32 of them, 4 us for 2^24 weights (less on a long K); tiles take rounds of workgroups on the compute units, a time for each block
 // of K (64 rows: two workgroups a unit); sums of shares are written and read at 5 TB/s.  Below them 3 or 4 us of a launch.
 Fp8Plan plan_matmul_fp8(int rows, int in_dim, int out_dim, int compute_units, size_t room) {
-    Fp8Plan best{kFp8Rows16, 1};
+    // Workgroups of four wavefronts instead of eight where those of eight would leave units idle in their last rounds: K = 4096, 16
+    // rows on 4096 columns 5.8 us with eight and 6.4 with four, on 14336 15.7 and 12.9; 32 rows (one workgroup of eight a unit) on 4096
+    // columns 6.6 and 7.6, on 14336 20.4 and 18.0, on 57344 59 and 65.
+    const int groups = (out_dim + 15) / 16;
+    const Fp8Kernel rows16 = is_wide(out_dim, compute_units) ? kFp8Rows16Wide : kFp8Rows16;
+    const Fp8Kernel rows32 = groups > compute_units * 5 / 4 && groups < 8 * compute_units ? kFp8Rows32Wide : kFp8Rows32;
+    Fp8Plan best{rows16, 1};
     if (rows <= 16) return best;
     const double units = compute_units, blocks = fp8_blocks(in_dim), weights = static_cast<double>(in_dim) * out_dim;
     // 16 rows a workgroup where W stays in every XCD's L2 (4 MiB) over its passes: 333 rows on 2000 x 1111 9 us, 32 rows a workgroup
     // 10 us; 64 rows on 4096 x 14336 45 us against 34 us.
-    if (weights > (4 << 20)) best.kernel = kFp8Rows32;
+    if (weights > (4 << 20)) best.kernel = rows32;
     double least = 3 + (3.0 + fmin(2.2, 4096.0 / in_dim)) * ((rows + 31) / 32) * (weights / (1 << 24));
     const auto tiles = [&](int of) { return static_cast<double>((out_dim + 127) / 128) * ((rows + of - 1) / of); };
     // Two workgroups a compute unit at a time, `two` a block of K; a last round of one a unit takes `one`.
@@ -518,7 +539,9 @@ Fp8Plan plan_matmul_fp8(int rows, int in_dim, int out_dim, int compute_units, si
 hipError_t launch_matmul_fp8(hipStream_t stream, const Fp8Matmul& a, const Fp8Plan& plan, float* sums) {
     switch (plan.kernel) {
         case kFp8Rows16: return rows_kernel<1, 8, 2>(stream, a);
+        case kFp8Rows16Wide: return rows_kernel<1, 4, 2>(stream, a);
         case kFp8Rows32: return rows_kernel<2, 8, 2>(stream, a);
+        case kFp8Rows32Wide: return rows_kernel<2, 4, 2>(stream, a);
         case kFp8Tile64: return tile_kernel<1, 2, 2, 3>(stream, a, plan.shares, sums);
         default: return tile_kernel<2, 2, 2, 2>(stream, a, plan.shares, sums);
     }

@@ -100,6 +100,13 @@ def test_product(rows, in_dim, out_dim, quantized):
     assert np.linalg.norm(got - want) <= 5e-6 * np.linalg.norm(want)
 
 
+@pytest.mark.parametrize("out_dim", [6001, 10239, 10241, 14336])
+@pytest.mark.parametrize("rows,in_dim", [(1, 272), (3, 2000), (16, 144), (16, 2048), (17, 272), (32, 656)])
+def test_product_many_columns(rows, in_dim, out_dim):
+    """Both sides of where workgroups get smaller."""
+    test_product(rows, in_dim, out_dim, rows % 2 == 0)
+
+
 @pytest.mark.parametrize("rows,in_dim,out_dim", [(2048, 1024, 4000), (1100, 2192, 4096), (8193, 128, 1040)])
 def test_product_many_rows(rows, in_dim, out_dim):
     """A prompt's sizes, with the activations' scales spread: every row of a sample against 64 bits."""
