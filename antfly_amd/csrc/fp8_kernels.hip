@@ -503,22 +503,30 @@ hipError_t launch_linear_fp8_fused(hipStream_t stream, const Fp8Matmul& a, const
 }
 
 // What the kernels take, in us, as measured (512 to 14336 columns, K = 1024 to 14336, 24 to 2048 rows): few rows pass over W
-// once for each 32 of them, 4 us for 2^24 weights (less on a long K); tiles take rounds of workgroups on the compute units, a time for each block
+// once for each 32 or 48 of them, 4 and 5 us for 2^24 weights (less on a long K); tiles take rounds of workgroups on the compute units, a time for each block
 // of K (64 rows: two workgroups a unit); sums of shares are written and read at 5 TB/s.  Below them 3 or 4 us of a launch.
 Fp8Plan plan_matmul_fp8(int rows, int in_dim, int out_dim, int compute_units, size_t room) {
     // Workgroups of four wavefronts instead of eight where those of eight would leave units idle in their last rounds: K = 4096, 16
     // rows on 4096 columns 5.8 us with eight and 6.4 with four, on 14336 15.7 and 12.9; 32 rows (one workgroup of eight a unit) on 4096
-    // columns 6.6 and 7.6, on 14336 20.4 and 18.0, on 57344 59 and 65.
-    const int groups = (out_dim + 15) / 16;
+    // columns 6.6 and 7.6, on 14336 20.4 and 18.0, on 57344 59 and 65; 48 rows on 4096 columns 7.7 and 8.5, on 6144 12.2 and 10.7.
+    const double units = compute_units, blocks = fp8_blocks(in_dim), weights = static_cast<double>(in_dim) * out_dim;
+    const auto groups = [&](int of) { return static_cast<double>((out_dim + 15) / 16) * ((rows + of - 1) / of); };
+    const auto half_filled = [&](int of) { return groups(of) > 1.25 * units && groups(of) < 8 * units; };
     const Fp8Kernel rows16 = is_wide(out_dim, compute_units) ? kFp8Rows16Wide : kFp8Rows16;
-    const Fp8Kernel rows32 = groups > compute_units * 5 / 4 && groups < 8 * compute_units ? kFp8Rows32Wide : kFp8Rows32;
     Fp8Plan best{rows16, 1};
     if (rows <= 16) return best;
-    const double units = compute_units, blocks = fp8_blocks(in_dim), weights = static_cast<double>(in_dim) * out_dim;
+    // 32 or 48 rows a workgroup: a pass over W takes less than its rows' share longer (48 rows on 4096 x 4096: 10.4 us in two passes, 7.7 in one).
+    const double shorter = fmin(2.2, 4096.0 / in_dim);
+    const auto passes = [&](int of, double each, double partly) {  // `each`: 2^24 weights by workgroups that fill the units
+        return each * (units * 16 * in_dim / (1 << 24)) * (half_filled(of) ? partly * groups(of) / units : fmax(groups(of) / units, 0.75));
+    };
+    const double by32 = passes(32, 2.3 + 1.2 * shorter, 1.25), by48 = passes(48, 3.75 + 1.15 * shorter, 1.05);
+    double least = 3 + fmin(by32, by48);
     // 16 rows a workgroup where W stays in every XCD's L2 (4 MiB) over its passes: 333 rows on 2000 x 1111 9 us, 32 rows a workgroup
     // 10 us; 64 rows on 4096 x 14336 45 us against 34 us.
-    if (weights > (4 << 20)) best.kernel = rows32;
-    double least = 3 + (3.0 + fmin(2.2, 4096.0 / in_dim)) * ((rows + 31) / 32) * (weights / (1 << 24));
+    if (weights > (4 << 20)) {
+        best.kernel = by32 <= by48 ? (half_filled(32) ? kFp8Rows32Wide : kFp8Rows32) : (half_filled(48) ? kFp8Rows48Wide : kFp8Rows48);
+    }
     const auto tiles = [&](int of) { return static_cast<double>((out_dim + 127) / 128) * ((rows + of - 1) / of); };
     // Two workgroups a compute unit at a time, `two` a block of K; a last round of one a unit takes `one`.
     const auto rounds = [&](double n, double one, double two) {
@@ -542,6 +550,8 @@ hipError_t launch_matmul_fp8(hipStream_t stream, const Fp8Matmul& a, const Fp8Pl
         case kFp8Rows16Wide: return rows_kernel<1, 4, 2>(stream, a);
         case kFp8Rows32: return rows_kernel<2, 8, 2>(stream, a);
         case kFp8Rows32Wide: return rows_kernel<2, 4, 2>(stream, a);
+        case kFp8Rows48: return rows_kernel<3, 8, 2>(stream, a);
+        case kFp8Rows48Wide: return rows_kernel<3, 4, 2>(stream, a);
         case kFp8Tile64: return tile_kernel<1, 2, 2, 3>(stream, a, plan.shares, sums);
         default: return tile_kernel<2, 2, 2, 2>(stream, a, plan.shares, sums);
     }

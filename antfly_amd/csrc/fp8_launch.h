@@ -31,7 +31,7 @@ hipError_t launch_quantize_fp8(hipStream_t stream, uint8_t* q, float* scales, co
 bool linear_fp8_is_fused(int rows, int in_dim);
 hipError_t launch_linear_fp8_fused(hipStream_t stream, const Fp8Matmul& call, const float* input, int compute_units);
 // Which kernel, and over how many workgroups the blocks of K are shared out; `room`: bytes for the shares' sums.
-enum Fp8Kernel { kFp8Rows16, kFp8Rows16Wide, kFp8Rows32, kFp8Rows32Wide, kFp8Tile64, kFp8Tile128 };
+enum Fp8Kernel { kFp8Rows16, kFp8Rows16Wide, kFp8Rows32, kFp8Rows32Wide, kFp8Rows48, kFp8Rows48Wide, kFp8Tile64, kFp8Tile128 };
 struct Fp8Plan {
     Fp8Kernel kernel;
     int shares;

@@ -107,6 +107,11 @@ def test_product_many_columns(rows, in_dim, out_dim):
     test_product(rows, in_dim, out_dim, rows % 2 == 0)
 
 
+@pytest.mark.parametrize("rows,in_dim,out_dim", [(33, 2048, 4096), (48, 1040, 4097), (48, 4096, 6000), (41, 656, 10241), (96, 2064, 4111), (49, 2048, 4096)])
+def test_product_up_to_three_sixteens_a_workgroup(rows, in_dim, out_dim):
+    test_product(rows, in_dim, out_dim, rows % 2 == 0)
+
+
 @pytest.mark.parametrize("rows,in_dim,out_dim", [(2048, 1024, 4000), (1100, 2192, 4096), (8193, 128, 1040)])
 def test_product_many_rows(rows, in_dim, out_dim):
     """A prompt's sizes, with the activations' scales spread: every row of a sample against 64 bits."""
