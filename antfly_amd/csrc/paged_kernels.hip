@@ -233,6 +233,7 @@ __global__ __launch_bounds__(kThreads) void cache_store_kernel(CacheView cache, 
 // program order.  Step i reads place path[i] >= i and the steps before it wrote places below i: no step reads what an
 // earlier one wrote, and kSteps of them are loaded before the first is stored.
 constexpr int kSteps = 8;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __global__ __launch_bounds__(kThreads) void cache_move_kernel(CacheView cache, const int* block_tables, uint32_t table_columns,
                                                              const int* context_lens, const int* paths, const int* path_lens,
                                                              uint32_t path_columns, uint32_t chunks_a_head, uint32_t chunks) {
@@ -245,30 +246,32 @@ __global__ __launch_bounds__(kThreads) void cache_move_kernel(CacheView cache, c
     const int* table = block_tables + static_cast<size_t>(r) * table_columns;
     const uint32_t count = min(static_cast<uint32_t>(at_least_zero(path_lens[r])), path_columns);
     const uint32_t context = static_cast<uint32_t>(at_least_zero(context_lens[r]));
-    auto place = [&](uint32_t position, size_t* out) {
+    constexpr size_t kNone = ~size_t{0};
+    auto place = [&](uint32_t position) -> size_t {
         const uint32_t column = position / cache.block_size;
-        if (column >= table_columns) return false;
-        const uint32_t block = static_cast<uint32_t>(table[column]);
-        *out = static_cast<size_t>(block) * cache.block_stride + static_cast<size_t>(position % cache.block_size) * cache.slot_stride + inside;
-        return block < cache.blocks;
+        const uint32_t block = column < table_columns ? static_cast<uint32_t>(table[column]) : ~0u;
+        if (block >= cache.blocks) return kNone;
+        return static_cast<size_t>(block) * cache.block_stride + static_cast<size_t>(position % cache.block_size) * cache.slot_stride + inside;
     };
     for (uint32_t i0 = 0; i0 < count; i0 += kSteps) {
-        uint4 held[kSteps];
-        size_t to[kSteps];
-        bool moves[kSteps];
+        int step[kSteps];
+        size_t from[kSteps], to[kSteps];
+        u32x4 held[kSteps];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) step[s] = i0 + s < count ? path[i0 + s] : -1;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            moves[s] = false;
-            const uint32_t i = i0 + s;
-            if (i < count && path[i] >= 0) {
-                size_t from;
-                moves[s] = place(context + static_cast<uint32_t>(path[i]), &from) && place(context + i, &to[s]);
-                if (moves[s]) held[s] = store[from];
-            }
+            from[s] = step[s] >= 0 ? place(context + static_cast<uint32_t>(step[s])) : kNone;
+            to[s] = step[s] >= 0 ? place(context + i0 + s) : kNone;
+            if (to[s] == kNone) from[s] = kNone;
         }
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            if (moves[s]) store[to[s]] = held[s];
+            if (from[s] != kNone) held[s] = *reinterpret_cast<const u32x4*>(store + from[s]);
+        }
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            if (from[s] != kNone) *reinterpret_cast<u32x4*>(store + to[s]) = held[s];
         }
     }
 }
