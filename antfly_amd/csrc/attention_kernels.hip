@@ -9,15 +9,23 @@
 // row of the packed queries to a lane (column = lane % 16) and four consecutive keys in its registers, so maximum, sum and
 // rescaling are a lane's own, but for one exchange between the four lanes of a row.  Its registers are the second operand of
 // V^T P^T as they stand: the order of the 32 keys inside the instruction is free as long as V follows it (lane group g holds
-// keys 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3).  V comes row-major and is needed column-major: it goes through LDS and
-// is read with the transposing ds_read_b64_tr_b16.  K goes from memory into the operand registers, no LDS.
+// keys 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3).  V comes row-major and is needed column-major: it is read from LDS with the
+// transposing ds_read_b64_tr_b16.  F32 queries and the weights beside them are two terms of f16 or three of bf16, each a product
+// of its own: 22 and 24 bits.
 //
 // Keys and values come in tiles of 32 keys from memory straight into a ring of tiles in LDS (no registers in between),
-// requested kStages - 1 tiles ahead.  The wavefronts of a workgroup share its tiles and have 16 kQ rows each: a lone wavefront
-// (no barrier anywhere) up to 16 rows, four of them, and every key read once, for 128.  Long contexts are shared out over
-// workgroups by the lengths that the device holds, so that ragged requests keep all of them busy to the end, and a second
-// kernel joins the parts.  Short ones stay with one workgroup a key head: it has kKeyGroups such groups of
-// wavefronts that take tiles in turn, and adds them up itself.
+// requested kStages - 1 tiles ahead, their places found a tile before that.  The wavefronts of a workgroup share its tiles and
+// have 16 kQ rows each: a lone wavefront (no barrier anywhere) up to 16 rows, four of them, and every key read once, for 128.
+// Long contexts are shared out over workgroups by the lengths that the device holds, so that ragged requests keep all of them
+// busy to the end, and a second kernel joins the parts.  Short ones stay with one workgroup a key head: it has kKeyGroups such
+// groups of wavefronts that take tiles in turn, and adds them up itself.
+//
+// What bounds it, on heads of 128, 32 of them on 8 key heads, 5.15 TB/s being what a copy reaches.  Few rows: the cache's bytes.
+// 64 requests of 1 token on 4000 keys 185 us (5.7 TB/s), on 1000 keys 53 us (4.9); 2 requests of 7 to 13 tokens x 28 heads on 99000
+// to 131000 keys 110 us (4.3 TB/s).  Many rows: the issue of a tile, 32 matrix instructions and 138 others (16 exponentials among
+// them) a wavefront with 32 rows, of which two fit a SIMD: 8 requests of 64 tokens on 8000 keys 103 us, 660 TFLOP/s.  Short
+// contexts: the round trips to memory before the first tile (lengths, block table, keys), and a tile's own latency, 0.85 us: 8
+// requests of 64 tokens on 20 keys (3 tiles) 11.9 us, on 190 keys (8 tiles) 16.3.
 #include "paged_launch.h"
 
 #include <hip/hip_runtime.h>
@@ -255,8 +263,9 @@ __device__ __forceinline__ bool find_share(const TreeAttentionArgs& a, const Sha
         const float each = work * (static_cast<float>(heads) * 1.001f) / static_cast<float>(workgroups);
         return max(static_cast<uint32_t>(fminf(each, 0x1p30f)) + 1, plan.least);
     };
-    // (a quotient in floats may be off by a part: the same here and below, and a part's tiles follow from it)
-    const auto parts_of = [](uint32_t all, float inverse) { return max(static_cast<uint32_t>(static_cast<float>(all) * inverse + 0.9999f), 1u); };
+    // (a quotient in floats, rounded up but for a thousandth of a part, which is more than its error: the same here and below, and
+    // a part's tiles follow from it)
+    const auto parts_of = [](uint32_t all, float inverse) { return max(static_cast<uint32_t>(static_cast<float>(all) * inverse + 0.999f), 1u); };
     constexpr int kSizes = 4;
     const uint32_t surely = size(plan.target), hardly = plan.one_round ? min(size(plan.most), surely) : surely;
     uint32_t tiles = surely;
@@ -736,7 +745,9 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
 }
 
 // The parts of a row, brought to their common maximum: a wavefront takes rows of one request in turn.  kLanes lanes have four
-// values of the row each, 64 / kLanes groups of them every so many-th part; up to eight are requested at a time.
+// values of a row each.  Few parts: every group of kLanes has a row of its own; many: the groups share a row's parts.  Up to
+// eight parts are requested at a time.  Bound by the parts' bytes, which come from beyond the L2 that wrote them: 4 parts of 16384 rows
+// of 128 (33 MB) 10 us, of which a launch and the lengths are 4.
 constexpr int kJoinWaves = 4;
 template <bool kBf16, bool kF32, int kLanes>
 __global__ __launch_bounds__(kJoinWaves * 64) void join_parts_kernel(TreeAttentionArgs a, SharePlan plan, int rows_a_tile, const float* part_out,
@@ -845,9 +856,14 @@ Shape shape_of(const TreeAttentionArgs& a, int compute_units) {
     // than two, are not worth a workgroup.
     s.plan.least = static_cast<uint32_t>(tile_rows / 16 > 2 ? tile_rows / 16 : 2);
     const uint64_t heads = a.cache.kv_heads, base = row_tiles * heads;
-    // One round of what the compute units hold at once (by LDS and registers), the workgroups that rounding adds among them; a
-    // batch that fills much of that anyway shares out over half a round more, three quarters for lone wavefronts.
-    const uint64_t resident = static_cast<uint64_t>(compute_units) * (s.waves == 1 ? 4 : s.waves == 2 ? 3 : 2), fewest = s.waves == 1 ? resident * 3 / 4 : resident / 2;
+    // One round of what the compute units hold at once (by LDS and registers; lone wavefronts four, not the five whose LDS would be
+    // all there is: 16 requests of 1 token on 8000 keys 107 us with four, 120 with five), the workgroups that rounding adds among
+    // them; a batch that fills much of that anyway shares out over half a round more, three quarters for lone wavefronts (64
+    // requests of 1 token on 100 to 4000 keys: 112 us with three quarters, 121 with half).  Workgroups of 128 rows, which the units
+    // are slow on, fill the round exactly: 8 requests of 64 tokens on 8000 keys 103 us, with what surely fits 116.  Fewer rows wait for
+    // memory, and parts cost more than idle units do: 24 requests of 16 tokens on 8000 keys 175 us filled, 172 not.
+    const uint64_t resident = static_cast<uint64_t>(compute_units) * (s.waves == 1 ? 4 : s.waves == 2 ? 3 : 2);
+    const uint64_t fewest = s.waves == 1 ? resident * 3 / 4 : resident / 2;
     s.plan.one_round = s.sixteens == 2 && base <= resident;
     uint64_t target = resident > base ? resident - base : 0;
     if (target < fewest && !s.plan.one_round) target = fewest;
@@ -857,7 +873,7 @@ Shape shape_of(const TreeAttentionArgs& a, int compute_units) {
     if (s.plan.even && s.plan.one_round) {
         // Parts are worth it where they save more tiles than the second launch takes (3 us) and their sums, in and out at 6 TB/s; a
         // tile takes 0.75 us, 1.4 times that with two workgroups on a unit.  64 tokens x 32 heads, 8 key heads of 128, bf16: 16
-        // requests on 300 keys 24.7 us in one part and 33 in two, on 4000 keys 129 and 103; 1 request on 300 keys 18 and 16.5.
+        // requests on 300 keys 20 us in one part and 33 in two, on 4000 keys 129 and 105; 1 request on 300 keys 18 and 16.5.
         const double parts = fmin(base == 0 ? 1.0 : floor(static_cast<double>(s.plan.most) / base), ceil(static_cast<double>(tiles) / s.plan.least));
         const double saved = tiles - tiles / parts * (base * parts > compute_units ? 1.4 : 1.0);
         s.plan.even = parts > 1 && saved > 4 + 0.029 * base * parts;
@@ -902,7 +918,7 @@ hipError_t attend(hipStream_t stream, const TreeAttentionArgs& a, const Shape& s
     return hipGetLastError();
 }
 
-// The ring's length: as many stages as let two workgroups of four wavefronts, or five of one, on a unit's 160 KiB of LDS; key
+// The ring's length: as many stages as let two workgroups of four wavefronts, or four of one, on a unit's 160 KiB of LDS; key
 // groups have two.
 template <int kDim, bool kBf16, bool kF32>
 hipError_t attend_rows(hipStream_t stream, const TreeAttentionArgs& a, const Shape& s, void* workspace) {

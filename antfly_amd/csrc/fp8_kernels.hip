@@ -39,6 +39,9 @@ __device__ __forceinline__ f16x8 widen(uint32_t lo, uint32_t hi) {
 }
 
 // ---- quantizer: eight lanes a block, four values of each 32 to a lane
+//
+// Bound by memory: 5 bytes a value, once.  Whole 128-byte lines in and 32-byte pieces out; the block's maximum takes three moves
+// between neighbouring lanes.  2048 x 4096: 10 us (4.2 TB/s); 333 x 2000: 3 us, a launch's own time.
 struct BlockPart {
     float4 v[4];
     __device__ __forceinline__ void load(const float* row, int block, int part, int in_dim) {
@@ -120,8 +123,11 @@ __device__ __forceinline__ uint4 read_piece(const char* tile, int row, int piece
 
 // ---- few rows
 //
-// A workgroup has 16 columns of W and 16 kM rows of X.  Its wavefronts share out the blocks of K in turn and add up at the end:
-// each works alone, with a ring of kStages blocks in LDS (its W, X and X's scales) and no barrier in the loop.
+// Bound by the weights' bytes, which all rows of a workgroup share.  A workgroup has 16 columns of W and 16 kM rows of X.  Its
+// wavefronts share out the blocks of K in turn and add up at the end: each works alone, with a ring of kStages blocks in LDS (its
+// W, X and X's scales) and no barrier in the loop, so that a few columns are enough to keep a compute unit's memory queue full.
+// K = 4096, 14336 columns (59 MB, 11.4 us at a copy's rate): 1 row 11.9 us (4.9 TB/s), 16 rows 12.6, 32 rows 17.8, 48 rows 20.8;
+// past one sixteen it is X, read by every workgroup from L2 into LDS, that takes the time.
 template <int kM, int kWaves, int kStages>
 __global__ __launch_bounds__(kWaves * 64) void matmul_fp8_rows_kernel(Fp8Matmul a) {
     constexpr int kRows = 16 * kM, kStage = 2048 + kRows * 128 + 256;  // W, X, a scale a row
@@ -202,7 +208,8 @@ __global__ __launch_bounds__(kWaves * 64) void matmul_fp8_rows_kernel(Fp8Matmul 
 // ---- few values of X: quantized by every workgroup itself
 //
 // While the first blocks of W are on their way, a workgroup quantizes all of X (up to 16 rows, kFusedValues values) into LDS: one
-// launch instead of two, and X read by every workgroup from L2.
+// launch instead of two, and X read by every workgroup from L2.  1 row: 4096 x 4096 5.2 us (3.2 TB/s: start, one round
+// trip to memory and the sums are most of it), 4096 x 14336 12.3 us (4.8 TB/s).
 template <int kWaves, int kStages>
 __global__ __launch_bounds__(kWaves * 64) void linear_fp8_rows_kernel(Fp8Matmul a, const float* input) {
     constexpr int kLoads = 2;
@@ -282,10 +289,15 @@ __global__ __launch_bounds__(kWaves * 64) void linear_fp8_rows_kernel(Fp8Matmul 
 
 // ---- many rows
 //
-// kRowWaves x kColWaves wavefronts with 32 kR rows x 64 columns each, a block of K at a time from a ring of three in LDS that all
+// kRowWaves x kColWaves wavefronts with 32 kR rows x 64 columns each, a block of K at a time from a ring of kStages in LDS that all
 // of them fill and read.  Every wavefront widens its own operands: of a block's instructions about half are conversions, which
-// run beside the other wavefront's products.  `sums`: blocks of K are shared out over gridDim.y workgroups, whose sums go there,
-// [share][rows][out_dim rounded up to 4], for add_shares_kernel.
+// run beside another wavefront's products.  128 x 128 with a ring of two is two workgroups a compute unit (64 KiB of LDS and 210
+// registers each), whose barriers, waits and last stores fall into the other's products: 2048 x 4096 x 14336 247 us (970 TFLOP/s), a
+// ring of three and one workgroup 310 us, 256 x 128 and a ring of three 278 us; a library's f16 product of that size takes 212 us.
+// What is left is the matrix instructions' own time at the clock that they are given on dense data and the conversions' issue.
+// 64 x 128 with a ring of three fills the units where there are few rows: 256 x 4096 x 4096 36.8 us, 128 x 128 42.9 (no shares).
+// `sums`: blocks of K are shared out over gridDim.y workgroups, whose sums go there, [share][rows][out_dim rounded up to 4], for
+// add_shares_kernel.
 template <int kR, int kRowWaves, int kColWaves, int kStages>
 __global__ __launch_bounds__(kRowWaves * kColWaves * 64, 2) void matmul_fp8_tile_kernel(Fp8Matmul a, int row_tiles, int col_tiles, float* sums) {
     constexpr int kWaves = kRowWaves * kColWaves, kRows = 32 * kR * kRowWaves, kCols = 64 * kColWaves;
@@ -418,7 +430,8 @@ __global__ __launch_bounds__(kRowWaves * kColWaves * 64, 2) void matmul_fp8_tile
     }
 }
 
-// The sums of the shares of K, in their order, and what follows them: four columns a thread, 1024 of a row a workgroup.
+// The sums of the shares of K, in their order, and what follows them: four columns a thread, 1024 of a row a workgroup.  Bound by
+// their bytes, most of them still in the caches: 8 shares of 48 x 4096 4 us.
 __global__ __launch_bounds__(256) void add_shares_kernel(Fp8Matmul a, const float* sums, int shares) {
     const size_t pitch = fp8_sums_pitch(a.out_dim);
     const int parts = (a.out_dim + 1023) / 1024, row = blockIdx.x / parts, o = (blockIdx.x % parts * 256 + threadIdx.x) * 4;

@@ -22,6 +22,8 @@ __device__ __forceinline__ int at_least_zero(int v) { return v > 0 ? v : 0; }
 // bisection there.  The token that opens a new block writes the table's entry, and no other token reads it.
 // Ancestors: a token follows its parents to the root, in LDS, setting a bit for each (a parent has the smaller index, so the
 // words are finished from high to low and the walk ends).
+// A few bytes a token: bound by the round trips to memory, one after the other (lengths, then table or free list).  8 requests with
+// trees of up to 24 drafts 4 us; 512 requests and 260000 tokens 8 us.
 __global__ __launch_bounds__(kThreads) void batch_plan_kernel(BatchPlanArgs a) {
     extern __shared__ int lds[];
     const int requests = static_cast<int>(a.requests);
@@ -199,7 +201,8 @@ __device__ __forceinline__ uint4 load8(const void* base, size_t element) {
     return pack8<kToBf16>(v);
 }
 
-// A thread moves eight values of a key and of a value: 32 + 32 bytes of f32 in, 16 + 16 out.
+// A thread moves eight values of a key and of a value: 32 + 32 bytes of f32 in, 16 + 16 out.  Bound by those bytes: 7500 tokens of
+// 8 heads of 128 (92 MB) 16.5 us, 5.6 TB/s, what a copy reaches.
 template <int kType, bool kToBf16>
 __global__ __launch_bounds__(kThreads) void cache_store_kernel(CacheView cache, const void* keys, const void* values, size_t token_stride,
                                                               size_t head_stride, const int* slots, uint32_t tokens,
@@ -231,7 +234,8 @@ __global__ __launch_bounds__(kThreads) void cache_store_kernel(CacheView cache, 
 //
 // A thread owns 16 bytes of every token (a part of one head's key or value), so the order of a path's steps is its own
 // program order.  Step i reads place path[i] >= i and the steps before it wrote places below i: no step reads what an
-// earlier one wrote, and kSteps of them are loaded before the first is stored.
+// earlier one wrote, and kSteps of them are loaded before the first is stored.  Bound by three round trips to memory (path,
+// table, token): 8 requests with paths of up to 5 tokens 5.5 us.
 constexpr int kSteps = 8;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __global__ __launch_bounds__(kThreads) void cache_move_kernel(CacheView cache, const int* block_tables, uint32_t table_columns,

@@ -416,7 +416,8 @@ typedef struct afhip_paged_cache {
  *                 the batch's tokens
  *   masks         uint64 [tokens][mask_words], optional: bit p of a token's words says that it sees token p of its
  *                 request: itself and its ancestors (without parents: itself and the tokens before it); 0 past the batch
- *   blocks_taken  int32 [1]: the blocks that the batch needs from the list (more than it holds: the batch does not fit)
+ *   blocks_taken  int32 [1]: the blocks that the batch needs from the list (more than it holds: the batch does not fit, and the
+ *                 entries past the list become -1)
  * parents, int32 [tokens], optional: the index within its request of the draft that a token follows, -1 behind the
  * context; an index that is not smaller than the token's own counts as -1.  At most mask_words * 64 (without masks:
  * 1024) tokens of a request are walked; later ones see nothing of their tree and keep depth 0.
@@ -452,14 +453,15 @@ afhip_status afhip_launch_cache_move(void *stream, const afhip_paged_cache *cach
  *
  * What is not seen does not count, whatever it holds (an infinity or no number included).  query and out: F32, or the
  * cache's own type; [tokens][heads][head_dim] with strides in elements (multiples of 4 for F32, of 8 otherwise; 16-byte
- * aligned).  F32 queries keep their bits (they are multiplied as two or three terms of the cache's type) and so do the
- * softmax's weights (two terms); 16-bit queries take one term of each.  Sums are f32.
+ * aligned).  F32 queries and the softmax's weights beside them are multiplied as three terms of bf16 or two of f16, whichever
+ * the cache holds (24 and 22 bits); with 16-bit queries the weights are rounded to the cache's type.  Sums are f32.
  * max_query_len and max_key_len bound what the batch holds (new tokens; context plus new tokens) and choose the launch's
  * shape; tokens past the first and keys past the second are left out.  A key whose block the table does not name is not
  * seen.  head_dim <= 256, heads a multiple of kv_heads, mask_words <= 16, max_key_len * block_size < 2^32, else
  * AFHIP_ERR_OP_UNSUPPORTED.
  * `workspace` (256-byte aligned, afhip_tree_attention_workspace_bytes) holds the parts of rows whose keys are shared out
- * over workgroups; less than asked for is refused (AFHIP_ERR_INVALID_STATE). */
+ * over workgroups (0 bytes where one workgroup has all of a row's keys); less than asked for is refused
+ * (AFHIP_ERR_INVALID_STATE). */
 typedef struct afhip_tree_attention {
     afhip_paged_cache cache;
     int type; /* of query and out */
