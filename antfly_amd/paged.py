@@ -25,11 +25,21 @@ def _bad_shape():
     return _lib.InvalidShape(_lib.ERR_INVALID_SHAPE)
 
 
+_names = {}  # of the types that have been seen
+
+
+def _name(dtype) -> str:
+    name = _names.get(dtype)
+    if name is None:
+        name = _names[dtype] = str(dtype)
+    return name
+
+
 def buffer(array) -> Buffer:
     """The memory that an array spans, from its first element to its last; None: no buffer."""
     if array is None:
         return NO_BUFFER
-    return Buffer(array.data_ptr(), _bytes(array))
+    return Buffer(array.data_ptr(), array.nbytes if array.is_contiguous() else _bytes(array))
 
 
 def _bytes(array) -> int:
@@ -39,20 +49,26 @@ def _bytes(array) -> int:
 
 
 def _type(array) -> int:
-    return _TYPES.get(str(array.dtype), -1)
+    return _TYPES.get(_name(array.dtype), -1)
 
 
 def _i32(array):
     """(address, bytes) of a contiguous array of int32."""
-    if str(array.dtype) != "torch.int32" or not array.is_contiguous():
+    if _name(array.dtype) != "torch.int32" or not array.is_contiguous():
         raise _bad_shape()
     return array.data_ptr(), array.nbytes
+
+
+def _i32_buffer(array) -> Buffer:
+    if _name(array.dtype) != "torch.int32" or not array.is_contiguous():
+        raise _bad_shape()
+    return Buffer(array.data_ptr(), array.nbytes)
 
 
 def _optional(array, dtypes=("torch.int32",)):
     if array is None:
         return 0, 0
-    if str(array.dtype) not in dtypes or not array.is_contiguous():
+    if _name(array.dtype) not in dtypes or not array.is_contiguous():
         raise _bad_shape()
     return array.data_ptr(), array.nbytes
 
@@ -109,21 +125,22 @@ def launchBatchPlan(stream, context_lens, query_lens, block_tables, free_blocks,
 
 def launchCacheStore(stream, cache: _lib.PagedCache, keys, values, slots) -> None:
     """keys, values [tokens, kv heads, head dim] (f32, f16 or bf16) into the cache's slots."""
-    tokens = slots.shape[0]
-    if values.shape != keys.shape or values.dtype != keys.dtype or not _same_strides(keys, values):
+    shape, strides, dtype = keys.shape, keys.stride(), keys.dtype
+    if values.shape != shape or values.dtype != dtype or (values.stride() != strides and not _same_strides(keys, values)) or \
+            shape != (slots.shape[0], cache.kv_heads, cache.head_dim) or (shape[2] > 1 and strides[2] != 1):
         raise _bad_shape()
-    token_stride, head_stride = _rows_of_heads(keys, tokens, cache.kv_heads, cache.head_dim)
-    check(_lib.lib().afhip_launch_cache_store(stream, cache, _type(keys), buffer(keys), buffer(values), token_stride, head_stride,
-                                              Buffer(*_i32(slots)), tokens))
+    check(_lib.lib().afhip_launch_cache_store(stream, cache, _TYPES.get(_name(dtype), -1), buffer(keys), buffer(values), strides[0],
+                                              strides[1], _i32_buffer(slots), shape[0]))
 
 
 def launchCacheMove(stream, cache: _lib.PagedCache, block_tables, context_lens, paths, path_lens) -> None:
     """The accepted path of every request's tree to the places behind its context."""
     requests, columns = block_tables.shape
-    if len(paths.shape) != 2 or paths.shape[0] != requests:
+    shape = paths.shape
+    if len(shape) != 2 or shape[0] != requests:
         raise _bad_shape()
-    check(_lib.lib().afhip_launch_cache_move(stream, cache, Buffer(*_i32(block_tables)), columns, Buffer(*_i32(context_lens)),
-                                             Buffer(*_i32(paths)), Buffer(*_i32(path_lens)), requests, paths.shape[1]))
+    check(_lib.lib().afhip_launch_cache_move(stream, cache, _i32_buffer(block_tables), columns, _i32_buffer(context_lens),
+                                             _i32_buffer(paths), _i32_buffer(path_lens), requests, shape[1]))
 
 
 def treeAttention(cache: _lib.PagedCache, out, query, query_starts, context_lens, block_tables, max_query_len: int,
