@@ -140,6 +140,20 @@ def test_many_requests(requests, context, tokens, heads, kv_heads):
         max_query=tokens[1] + 1, max_keys=context[1] + tokens[1])
 
 
+@pytest.mark.parametrize("requests,context,tokens,heads,kv_heads,dim", [
+    (100, (0, 1500), (17, 40), 4, 1, 64), (3, (900, 2600), (33, 64), 32, 8, 128), (16, (0, 900), (40, 64), 16, 4, 64), (70, (300, 700), (30, 33), 32, 4, 64),
+    (12, (500, 1000), (1, 1), 32, 8, 128), (40, (0, 1900), (1, 4), 32, 8, 64)])
+def test_ragged_batches_of_many_rows(requests, context, tokens, heads, kv_heads, dim):
+    """Parts that fill one round of workgroups, batches that fill more, and single workgroups on a thousand keys and more."""
+    print(f"case: {requests} requests context={context} tokens={tokens} heads={heads}/{kv_heads}", flush=True)
+    rng = np.random.default_rng(requests + heads)
+    lens = rng.integers(tokens[0], tokens[1] + 1, requests)
+    lens[requests // 2] = 0
+    lens[0] = tokens[1]
+    Batch(rng, rng.integers(context[0], context[1] + 1, requests), lens, heads, kv_heads, dim, 16, "bf16", "bf16").check(
+        max_query=tokens[1], max_keys=context[1] + tokens[1])
+
+
 @pytest.mark.parametrize("activations,stored", KINDS)
 def test_prompt_without_masks(activations, stored):
     """Hundreds of new tokens behind a short context: causal, many row tiles."""
