@@ -400,33 +400,72 @@ __global__ __launch_bounds__(kRowWaves * kColWaves * 64, 2) void matmul_fp8_tile
     }
     const size_t pitch = sums != nullptr ? fp8_sums_pitch(a.out_dim) : a.out_dim;
     float* y = sums != nullptr ? sums + blockIdx.y * pitch * a.rows : a.y;
-    const bool fours = pitch % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+    // Through LDS into whole rows of 64 columns: a lane has four neighbouring columns of every fourth row, whose bias it loads once,
+    // and the residual's loads of 32 rows go out together, ahead of the stores (the residual may be Y itself).  2048 x 4096 x 14336 with
+    // bias, GELU and residual 296 us; from the registers as they stand, 16 bytes of 32 rows at a time, 380 (without them the same).
+    const bool fours = pitch % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0 && reinterpret_cast<uintptr_t>(a.ep.residual) % 16 == 0;
+    const bool finish = sums == nullptr;
+    const int o = first_o + wave_o + lane % 16 * 4;
+    constexpr int kPitch = 68;
+    float* own = reinterpret_cast<float*>(lds) + wave * 32 * kPitch;
+    f32x4 bias{0, 0, 0, 0};
+    if (finish && a.ep.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bias[j] = o + j < a.out_dim ? a.ep.bias[o + j] : 0.0f;
+    }
+    __syncthreads();  // everyone is done with the ring
 #pragma unroll
     for (int m = 0; m < kR; ++m) {
-        const int row = first_r + wave_r + m * 32 + column;
-        if (row >= a.rows) continue;
+        const int row = first_r + wave_r + m * 32 + lane / 16;  // and every fourth from there
+        f32x4 residual[8];
+        if (finish && a.ep.residual != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const size_t at = static_cast<size_t>(min(row + i * 4, a.rows - 1)) * pitch;
+                if (fours) {
+                    residual[i] = *reinterpret_cast<const f32x4*>(a.ep.residual + at + min(o, a.out_dim - 4));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) residual[i][j] = a.ep.residual[at + min(o + j, a.out_dim - 1)];
+                }
+            }
+        }
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int o = first_o + wave_o + n * 32 + q * 8 + half * 4;
-                const size_t to = row * pitch + o;
                 f32x4 v;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    v[j] = total[n][m][q * 4 + j];
-                    if (sums == nullptr && o + j < a.out_dim) v[j] = finish_output(a.ep, o + j, to + j, v[j]);
-                }
-                if (fours && o < a.out_dim) {
-                    *reinterpret_cast<f32x4*>(y + to) = v;
-                } else {
+                for (int j = 0; j < 4; ++j) v[j] = total[n][m][q * 4 + j];
+                *reinterpret_cast<f32x4*>(own + column * kPitch + n * 32 + q * 8 + half * 4) = v;
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (o + j < a.out_dim) y[to + j] = v[j];
-                    }
+        for (int i = 0; i < 8; ++i) {
+            f32x4 v = *reinterpret_cast<const f32x4*>(own + (i * 4 + lane / 16) * kPitch + lane % 16 * 4);
+            if (finish) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (a.ep.bias != nullptr) v[j] += bias[j];
+                    v[j] = activate(a.ep.activation, v[j]);
+                    if (a.ep.residual != nullptr) v[j] += residual[i][j];
+                }
+            }
+            if (row + i * 4 >= a.rows || o >= a.out_dim) continue;
+            float* to = y + static_cast<size_t>(row + i * 4) * pitch + o;
+            if (fours) {
+                *reinterpret_cast<f32x4*>(to) = v;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (o + j < a.out_dim) to[j] = v[j];
                 }
             }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -441,8 +480,12 @@ __global__ __launch_bounds__(256) void add_shares_kernel(Fp8Matmul a, const floa
     for (int s = 0; s < shares; ++s) v += *reinterpret_cast<const f32x4*>(sums + (static_cast<size_t>(s) * a.rows + row) * pitch + o);
     const size_t to = static_cast<size_t>(row) * a.out_dim + o;
 #pragma unroll
+    for (int j = 0; j < 4; ++j) {  // (all loads ahead of the stores)
+        if (o + j < a.out_dim) v[j] = finish_output(a.ep, o + j, to + j, v[j]);
+    }
+#pragma unroll
     for (int j = 0; j < 4; ++j) {
-        if (o + j < a.out_dim) a.y[to + j] = finish_output(a.ep, o + j, to + j, v[j]);
+        if (o + j < a.out_dim) a.y[to + j] = v[j];
     }
 }
 
@@ -464,6 +507,7 @@ hipError_t tile_kernel(hipStream_t stream, const Fp8Matmul& a, int shares, float
     static LdsLimit limit;
     constexpr int kRows = 32 * kR * kRowWaves, kCols = 64 * kColWaves;
     constexpr size_t lds = kStages * ((kRows + kCols) * 128 + kRowWaves * kColWaves * 256);
+    static_assert(lds >= kRowWaves * kColWaves * 32 * 68 * 4, "the results' way through LDS");
     const auto kernel = matmul_fp8_tile_kernel<kR, kRowWaves, kColWaves, kStages>;
     hipError_t e = allow_lds(kernel, lds, &limit);
     if (e != hipSuccess) return e;
@@ -535,10 +579,14 @@ Fp8Plan plan_matmul_fp8(int rows, int in_dim, int out_dim, int compute_units, si
     };
     const double by32 = passes(32, 2.3 + 1.2 * shorter, 1.25), by48 = passes(48, 3.75 + 1.15 * shorter, 1.05);
     double least = 3 + fmin(by32, by48);
-    // 16 rows a workgroup where W stays in every XCD's L2 (4 MiB) over its passes: 333 rows on 2000 x 1111 9 us, 32 rows a workgroup
-    // 10 us; 64 rows on 4096 x 14336 45 us against 34 us.
     if (weights > (4 << 20)) {
         best.kernel = by32 <= by48 ? (half_filled(32) ? kFp8Rows32Wide : kFp8Rows32) : (half_filled(48) ? kFp8Rows48Wide : kFp8Rows48);
+    } else {
+        // W stays in every XCD's L2 (4 MiB) over its passes: 16 rows a workgroup, many workgroups (of four wavefronts where they are
+        // more than two a unit).  Bias, GELU and residual with it: 333 rows on 2000 x 1111 9.4 us, with eight wavefronts 10.7, 32 rows a
+        // workgroup 9.5 and 12.4; 512 rows on 768 x 2304 11.6, 16.6, 11.4, 18.5.
+        if (groups(16) >= 2.5 * units) best.kernel = kFp8Rows16Wide;
+        least = 3 + (0.95 + 1.4 * fmin(2.2, 1024.0 / in_dim)) * ((rows + 15) / 16) * (weights / (1 << 24));
     }
     const auto tiles = [&](int of) { return static_cast<double>((out_dim + 127) / 128) * ((rows + of - 1) / of); };
     // Two workgroups a compute unit at a time, `two` a block of K; a last round of one a unit takes `one`.
