@@ -295,7 +295,8 @@ __global__ __launch_bounds__(kWaves * 64) void linear_fp8_rows_kernel(Fp8Matmul 
 // registers each), whose barriers, waits and last stores fall into the other's products: 2048 x 4096 x 14336 247 us (970 TFLOP/s), a
 // ring of three and one workgroup 310 us, 256 x 128 and a ring of three 278 us; a library's f16 product of that size takes 212 us.
 // What is left is the matrix instructions' own time at the clock that they are given on dense data and the conversions' issue.
-// 64 x 128 with a ring of three fills the units where there are few rows: 256 x 4096 x 4096 36.8 us, 128 x 128 42.9 (no shares).
+// 64 x 128 with a ring of three fills the units where there are few rows, and has the registers for all of a block's pieces at once
+// (one workgroup a unit: 29 us instead of 35): 256 x 4096 x 4096 30 us, 128 x 128 42 (no shares).
 // `sums`: blocks of K are shared out over gridDim.y workgroups, whose sums go there, [share][rows][out_dim rounded up to 4], for
 // add_shares_kernel.
 template <int kR, int kRowWaves, int kColWaves, int kStages>
@@ -364,28 +365,39 @@ __global__ __launch_bounds__(kRowWaves * kColWaves * 64, 2) void matmul_fp8_tile
             scale[m] = scales[row / kOwn * 64 + row % kOwn] * ws;
         }
         f32x16 dot[2][kR];
+        constexpr int kHeld = kR == 1 ? 4 : 1;  // steps whose pieces are requested together, as registers allow
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {  // 32 of K: a 16-byte piece a lane, two instructions' worth
-            f16x8 wide_w[2][2], wide_x[kR][2];
+        for (int k0 = 0; k0 < 4; k0 += kHeld) {  // 32 of K a step: a 16-byte piece a lane, two instructions' worth
+            uint4 w_piece[kHeld][2], x_piece[kHeld][kR];
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const uint4 p = read_piece(w + n * 4096, column, k * 2 + half);
-                wide_w[n][0] = widen(p.x, p.y);
-                wide_w[n][1] = widen(p.z, p.w);
+            for (int i = 0; i < kHeld; ++i) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n) w_piece[i][n] = read_piece(w + n * 4096, column, (k0 + i) * 2 + half);
+#pragma unroll
+                for (int m = 0; m < kR; ++m) x_piece[i][m] = read_piece(x + m * 4096, column, (k0 + i) * 2 + half);
             }
+            if (kHeld > 1) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int m = 0; m < kR; ++m) {
-                const uint4 p = read_piece(x + m * 4096, column, k * 2 + half);
-                wide_x[m][0] = widen(p.x, p.y);
-                wide_x[m][1] = widen(p.z, p.w);
-            }
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {
+            for (int i = 0; i < kHeld; ++i) {
+                f16x8 wide_w[2][2], wide_x[kR][2];
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
+                    wide_w[n][0] = widen(w_piece[i][n].x, w_piece[i][n].y);
+                    wide_w[n][1] = widen(w_piece[i][n].z, w_piece[i][n].w);
+                }
 #pragma unroll
-                    for (int m = 0; m < kR; ++m)
-                        dot[n][m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wide_w[n][part], wide_x[m][part], k + part == 0 ? f32x16{} : dot[n][m], 0, 0, 0);
+                for (int m = 0; m < kR; ++m) {
+                    wide_x[m][0] = widen(x_piece[i][m].x, x_piece[i][m].y);
+                    wide_x[m][1] = widen(x_piece[i][m].z, x_piece[i][m].w);
+                }
+#pragma unroll
+                for (int part = 0; part < 2; ++part) {
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                        for (int m = 0; m < kR; ++m)
+                            dot[n][m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wide_w[n][part], wide_x[m][part], k0 + i + part == 0 ? f32x16{} : dot[n][m], 0, 0, 0);
+                    }
                 }
             }
         }
@@ -598,7 +610,7 @@ Fp8Plan plan_matmul_fp8(int rows, int in_dim, int out_dim, int compute_units, si
         const size_t sums = Fp8Plan{kFp8Tile64, shares}.sums_bytes(rows, out_dim);
         if (shares > 1 && (sums > room || blocks < 4 * shares)) break;
         const double each = ceil(blocks / shares), rest = 4 + (shares > 1 ? 3 + 2.0 * sums / 5e6 : 0.0);
-        const double t64 = rest + each * rounds(tiles(64) * shares, 1.04, 1.36), t128 = rest + each * rounds(tiles(128) * shares, 1.22, 1.98);
+        const double t64 = rest + each * rounds(tiles(64) * shares, 0.80, 1.30), t128 = rest + each * rounds(tiles(128) * shares, 1.22, 1.98);
         if (t64 < least) least = t64, best = Fp8Plan{kFp8Tile64, shares};
         if (t128 < least) least = t128, best = Fp8Plan{kFp8Tile128, shares};
     }
