@@ -23,7 +23,7 @@ __device__ __forceinline__ int at_least_zero(int v) { return v > 0 ? v : 0; }
 // Ancestors: a token follows its parents to the root, in LDS, setting a bit for each (a parent has the smaller index, so the
 // words are finished from high to low and the walk ends).
 // A few bytes a token: bound by the round trips to memory, one after the other (lengths, then table or free list).  8 requests with
-// trees of up to 24 drafts 4 us; 512 requests and 260000 tokens 8 us.
+// trees of up to 24 drafts 4 us; 512 requests and 260000 tokens 6 us.
 __global__ __launch_bounds__(kThreads) void batch_plan_kernel(BatchPlanArgs a) {
     extern __shared__ int lds[];
     const int requests = static_cast<int>(a.requests);
@@ -31,13 +31,13 @@ __global__ __launch_bounds__(kThreads) void batch_plan_kernel(BatchPlanArgs a) {
     int* fresh = start + requests + 1;      // [requests + 1]
     int* context = fresh + requests + 1;    // [requests]
     int* sums = context + requests;         // [2][4]: the wavefronts' totals
-    int* parent = sums + 8;                 // [kPlanWalk + kPlanTokens], with parents
+    int* parent = sums + 8;                 // [kPlanWalk + group_tokens], with parents
 
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
-    const unsigned base = blockIdx.x * static_cast<unsigned>(kPlanTokens);
+    const unsigned base = blockIdx.x * a.group_tokens;
     const unsigned window = base > kPlanWalk ? base - kPlanWalk : 0;
     if (a.parents != nullptr) {
-        for (unsigned i = window + tid; i < base + kPlanTokens && i < a.tokens; i += kThreads) parent[i - window] = a.parents[i];
+        for (unsigned i = window + tid; i < base + a.group_tokens && i < a.tokens; i += kThreads) parent[i - window] = a.parents[i];
     }
     // a run of requests a thread
     const int run = (requests + kThreads - 1) / kThreads, first = tid * run;
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(kThreads) void batch_plan_kernel(BatchPlanArgs a) {
     }
     const int words = static_cast<int>(a.mask_words);
     const int walked = a.masks != nullptr ? words * 64 : kPlanWalk;
-    for (unsigned i = base + tid; i < base + kPlanTokens && i < a.tokens; i += kThreads) {
+    for (unsigned i = base + tid; i < base + a.group_tokens && i < a.tokens; i += kThreads) {
         unsigned long long* mask = a.masks != nullptr ? a.masks + static_cast<size_t>(i) * words : nullptr;
         if (static_cast<int>(i) >= total) {
             a.slots[i] = -1;
@@ -295,12 +295,17 @@ hipError_t store(hipStream_t stream, const CacheView& cache, const void* keys, c
 
 hipError_t launch_batch_plan(hipStream_t stream, const BatchPlanArgs& args) {
     static LdsLimit limit;
+    // A thread has one token, whose round trips follow one another; four where the lengths' sums, made by every workgroup, would take
+    // longer: 512 requests of 512 tokens 6.1 us with one and 7.6 with four, 8192 of one 28 and 32; 2048 of 100 14.5 and 10.5, 8192 of
+    // 16 64 and 33.
+    BatchPlanArgs a = args;
+    a.group_tokens = static_cast<uint64_t>(args.requests) * args.tokens > (1u << 28) ? kPlanTokens : kThreads;
     size_t lds = (3 * static_cast<size_t>(args.requests) + 2 + 8) * sizeof(int);
-    if (args.parents != nullptr) lds += (kPlanWalk + kPlanTokens) * sizeof(int);
+    if (args.parents != nullptr) lds += (kPlanWalk + a.group_tokens) * sizeof(int);
     const hipError_t e = allow_lds(batch_plan_kernel, lds, &limit);
     if (e != hipSuccess) return e;
-    const uint32_t grid = args.tokens == 0 ? 1 : (args.tokens + kPlanTokens - 1) / kPlanTokens;
-    batch_plan_kernel<<<grid, kThreads, lds, stream>>>(args);
+    const uint32_t grid = args.tokens == 0 ? 1 : (args.tokens + a.group_tokens - 1) / a.group_tokens;
+    batch_plan_kernel<<<grid, kThreads, lds, stream>>>(a);
     return hipGetLastError();
 }
 

@@ -26,7 +26,7 @@ struct Divisor {
     explicit Divisor(uint32_t d) : by(d), multiplier(d == 1 ? 0 : static_cast<uint32_t>(((uint64_t{1} << 32) + d - 1) / d)), whole(d == 1 ? ~0u : 0) {}
 };
 
-constexpr int kPlanTokens = 1024;       // token places of one workgroup
+constexpr int kPlanTokens = 1024;       // most token places of one workgroup
 constexpr int kPlanWalk = 1024;         // most tokens of a request that are walked to the tree's root
 constexpr size_t kPlanRequests = 8192;  // their prefix sums are in every workgroup's LDS
 
@@ -36,6 +36,7 @@ struct BatchPlanArgs {
     int *block_tables, *query_starts, *slots, *positions;
     unsigned long long* masks;
     int* blocks_taken;
+    uint32_t group_tokens;  // token places of a workgroup (the launch sets it)
 };
 hipError_t launch_batch_plan(hipStream_t stream, const BatchPlanArgs& args);
 

@@ -213,3 +213,18 @@ def test_strides_of_one_token_do_not_count():
     assert torch.equal(k[1, 2], keys[0].bfloat16()) and torch.equal(v[1, 2], values[0].bfloat16())
     k[1, 2], v[1, 2] = 0, 0
     assert not k.any() and not v.any()
+
+
+@pytest.mark.parametrize("requests,most", [(8000, 9), (8000, 70), (700, 300)])
+def test_plan_of_many_requests(requests, most):
+    """Both sides of where a workgroup takes more tokens."""
+    rng = np.random.default_rng(requests + most)
+    context, lens = rng.integers(0, 300, requests), rng.integers(0, most, requests)
+    columns = 24 + most // 16
+    table, free = a_table(rng, context, lens, 16, columns)
+    tokens = int(lens.sum()) + 77
+    parents = R.parents_of(rng, lens)
+    got = run_plan(context, lens, table, free, 16, tokens, parents)
+    want = R.plan(context, lens, table, free, 16, (1 << 31) - 1, tokens, parents, 0, False)
+    for g, w in zip(got, want):
+        assert g is None or np.array_equal(g, w)
