@@ -39,14 +39,18 @@ __global__ __launch_bounds__(kThreads) void batch_plan_kernel(BatchPlanArgs a) {
     if (a.parents != nullptr) {
         for (unsigned i = window + tid; i < base + a.group_tokens && i < a.tokens; i += kThreads) parent[i - window] = a.parents[i];
     }
-    // a run of requests a thread
-    const int run = (requests + kThreads - 1) / kThreads, first = tid * run;
+    for (int r = tid; r < requests; r += kThreads) {
+        context[r] = at_least_zero(a.context_lens[r]);
+        start[r] = at_least_zero(a.query_lens[r]);
+    }
+    __syncthreads();
+    // a run of requests a thread, an odd number: the threads' runs fall on different banks
+    const int run = ((requests + kThreads - 1) / kThreads) | 1, first = tid * run;
     int queries = 0, blocks = 0;
     for (int r = first; r < first + run && r < requests; ++r) {
-        const int c = at_least_zero(a.context_lens[r]), q = at_least_zero(a.query_lens[r]);
+        const int c = context[r], q = start[r];
         const unsigned owned = (static_cast<unsigned>(c) + a.block_size - 1) / a.block_size;
         const unsigned needed = (static_cast<unsigned>(c) + static_cast<unsigned>(q) + a.block_size - 1) / a.block_size;
-        context[r] = c;
         start[r] = queries;
         fresh[r] = blocks;
         queries += q;
@@ -296,10 +300,10 @@ hipError_t store(hipStream_t stream, const CacheView& cache, const void* keys, c
 hipError_t launch_batch_plan(hipStream_t stream, const BatchPlanArgs& args) {
     static LdsLimit limit;
     // A thread has one token, whose round trips follow one another; four where the lengths' sums, made by every workgroup, would take
-    // longer: 512 requests of 512 tokens 6.1 us with one and 7.6 with four, 8192 of one 28 and 32; 2048 of 100 14.5 and 10.5, 8192 of
-    // 16 64 and 33.
+    // longer: 512 requests of 512 tokens 6.5 us with one and 7.9 with four, 2048 of 100 8.4 and 10.1, 8192 of one 13.8 and 17.4; 8192
+    // of 16 25.8 and 18.0, 4096 of 100 24.4 and 13.9.
     BatchPlanArgs a = args;
-    a.group_tokens = static_cast<uint64_t>(args.requests) * args.tokens > (1u << 28) ? kPlanTokens : kThreads;
+    a.group_tokens = static_cast<uint64_t>(args.requests) * args.tokens > (1u << 29) ? kPlanTokens : kThreads;
     size_t lds = (3 * static_cast<size_t>(args.requests) + 2 + 8) * sizeof(int);
     if (args.parents != nullptr) lds += (kPlanWalk + a.group_tokens) * sizeof(int);
     const hipError_t e = allow_lds(batch_plan_kernel, lds, &limit);
