@@ -11,7 +11,8 @@
 // V^T P^T as they stand: the order of the 32 keys inside the instruction is free as long as V follows it (lane group g holds
 // keys 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3).  V comes row-major and is needed column-major: it is read from LDS with the
 // transposing ds_read_b64_tr_b16.  F32 queries and the weights beside them are two terms of f16 or three of bf16, each a product
-// of its own: 22 and 24 bits.
+// of its own: 22 and 24 bits.  f16 ends at 2^-24: its weights are kept high in the type (kLift), and a weight's second term is 2^12
+// times itself, with sums of its own.
 //
 // Keys and values come in tiles of 32 keys from memory straight into a ring of tiles in LDS (no registers in between),
 // requested kStages - 1 tiles ahead, their places found a tile before that.  The wavefronts of a workgroup share its tiles and
@@ -51,6 +52,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 // scores to see that.
 constexpr float kSlack = 8.0f;
 constexpr float kUnset = 1e38f;
+// Where a row's largest weight is put (a power of two): as high as f16 allows, whose steps below 2^-14 are 2^-24 whatever the
+// weight.  Half a step is 2^-32 of the largest weight then, 2^-44 where there is a second term of 2^12 times the rest.  bf16 has
+// f32's exponents.
+template <bool kBf16>
+constexpr float kLift = kBf16 ? 0.0f : 7.0f;
+constexpr float kRestScale = 4096.0f;  // (the rest of a weight of 2^15 is 2^3 at most)
 
 template <bool kBf16>
 __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
@@ -331,8 +338,11 @@ __device__ __forceinline__ bool find_share(const TreeAttentionArgs& a, const Sha
 }
 
 // kDim: the head's values, rounded up to a size that is here (the rest are zeros).  kF32: query and out are f32.
+// Two wavefronts a SIMD (256 registers) wherever the sums leave room for them: f32 rows of heads of 256, and 32 rows a wavefront of 128, do
+// not (8 requests of 5 tokens on 3000 keys, f32 on f16: 28.9 us, with the 260 to 320 registers that the compiler takes when it may
+// 37.7).
 template <int kDim, bool kBf16, bool kF32, int kQ, int kRowWaves, int kKeyGroups, int kStages>
-__global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 1 : 2) void tree_attention_kernel(TreeAttentionArgs a, SharePlan plan, float* part_out,
+__global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kDim == 256 || (kF32 && kDim * kQ == 256) ? 1 : 2) void tree_attention_kernel(TreeAttentionArgs a, SharePlan plan, float* part_out,
                                                                                                  Part* parts) {
     constexpr int kSteps = kDim / 32;                            // products of K Q^T along the head
     constexpr int kTerms = kF32 ? (kBf16 ? 3 : 2) : 1;           // of a query value or a weight: 24 bits of three bf16, 22 of two f16
@@ -503,15 +513,21 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
     }
 
     f32x4 out[kQ][kDim / 16];
-    // A weight is exp2(product * unit + shift): the shift takes off the row's largest score (up to kSlack more than it), kUnset
-    // until the row has seen a key.  And this lane's part of the weights' sum.
+    constexpr bool kApart = kF32 && !kBf16;  // the second terms' sums, kRestScale times themselves
+    f32x4 low[kApart ? kQ : 1][kApart ? kDim / 16 : 1];
+    // A weight is exp2(product * unit + shift): the shift takes off the row's largest score (up to kSlack more than it) and adds
+    // kLift, kUnset until the row has seen a key.  And this lane's part of the weights' sum.
+    constexpr float kHighest = kLift<kBf16> + kSlack;
     float shift[kQ], sum[kQ];
 #pragma unroll
     for (int qt = 0; qt < kQ; ++qt) {
         shift[qt] = kUnset;
         sum[qt] = 0.0f;
 #pragma unroll
-        for (int d = 0; d < kDim / 16; ++d) out[qt][d] = f32x4{0, 0, 0, 0};
+        for (int d = 0; d < kDim / 16; ++d) {
+            out[qt][d] = f32x4{0, 0, 0, 0};
+            if constexpr (kApart) low[qt][d] = f32x4{0, 0, 0, 0};
+        }
     }
 
     // ---- the keys
@@ -611,7 +627,7 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
         for (int qt = 0; qt < kQ; ++qt) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[qt][j] = __builtin_fmaf(score[qt][j >> 2][j & 3], unit[qt], shift[qt]);
-            passes |= fmaxf(fmaxf(fmaxf(x[qt][0], x[qt][1]), fmaxf(x[qt][2], x[qt][3])), fmaxf(fmaxf(x[qt][4], x[qt][5]), fmaxf(x[qt][6], x[qt][7]))) > kSlack;
+            passes |= fmaxf(fmaxf(fmaxf(x[qt][0], x[qt][1]), fmaxf(x[qt][2], x[qt][3])), fmaxf(fmaxf(x[qt][4], x[qt][5]), fmaxf(x[qt][6], x[qt][7]))) > kHighest;
         }
         if (__any(passes)) {
 #pragma unroll
@@ -619,14 +635,17 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
                 const f32x4 lo = score[qt][0], hi = score[qt][1];
                 const float peak = row_max(fmaxf(fmaxf(fmaxf(lo[0], lo[1]), fmaxf(lo[2], lo[3])), fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3]))));
                 // each row by itself: no other row's keys move its bits
-                const float next = __builtin_fmaf(peak, unit[qt], shift[qt]) > kSlack ? -peak * unit[qt] : shift[qt];
+                const float next = __builtin_fmaf(peak, unit[qt], shift[qt]) > kHighest ? __builtin_fmaf(-peak, unit[qt], kLift<kBf16>) : shift[qt];
                 const float by = next == shift[qt] ? 1.0f : __builtin_amdgcn_exp2f(next - shift[qt]);
                 shift[qt] = next;
                 sum[qt] *= by;
 #pragma unroll
                 for (int d = 0; d < kDim / 16; ++d) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) out[qt][d][j] *= by;
+                    for (int j = 0; j < 4; ++j) {
+                        out[qt][d][j] *= by;
+                        if constexpr (kApart) low[qt][d][j] *= by;
+                    }
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[qt][j] = __builtin_fmaf(score[qt][j >> 2][j & 3], unit[qt], next);
@@ -643,7 +662,7 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
 #pragma unroll
                 for (int term = 0; term < kTerms; ++term) {
                     weight[qt][term][j] = narrow<kBf16>(rest);
-                    if (term + 1 < kTerms) rest -= widen<kBf16>(weight[qt][term][j]);
+                    if (term + 1 < kTerms) rest = (rest - widen<kBf16>(weight[qt][term][j])) * (kApart ? kRestScale : 1.0f);
                 }
             }
         }
@@ -660,7 +679,15 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
 #pragma unroll
             for (int d = 0; d < kDim / 16; ++d) {
 #pragma unroll
-                for (int qt = 0; qt < kQ; ++qt) out[qt][d] = mfma<kBf16>(value[d], weight[qt][term], out[qt][d]);
+                for (int qt = 0; qt < kQ; ++qt) {
+                    if constexpr (kApart) {
+                        if (term > 0) {
+                            low[qt][d] = mfma<kBf16>(value[d], weight[qt][term], low[qt][d]);
+                            continue;
+                        }
+                    }
+                    out[qt][d] = mfma<kBf16>(value[d], weight[qt][term], out[qt][d]);
+                }
             }
         }
         // A row that does not see a key must not get 0 * inf from it: the products above took such values as zeros, and the
@@ -687,6 +714,17 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kF32 || kDim == 256 ? 
                         if (is_odd<kBf16>(static_cast<unsigned short>(four[j]))) out[qt][d][j] = __builtin_fmaf(p, widen<kBf16>(four[j]), out[qt][d][j]);
                     }
                 }
+            }
+        }
+    }
+
+    if constexpr (kApart) {
+#pragma unroll
+        for (int qt = 0; qt < kQ; ++qt) {
+#pragma unroll
+            for (int d = 0; d < kDim / 16; ++d) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) out[qt][d][j] = __builtin_fmaf(low[qt][d][j], 1.0f / kRestScale, out[qt][d][j]);
             }
         }
     }
