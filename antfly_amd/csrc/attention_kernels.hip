@@ -52,6 +52,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // scores to see that.
 constexpr float kSlack = 8.0f;
 constexpr float kUnset = 1e38f;
+constexpr float kLeastUnit = 0x1p-126f;  // of what a product is multiplied by
 // Where a row's largest weight is put (a power of two): as high as f16 allows, whose steps below 2^-14 are 2^-24 whatever the
 // weight.  Half a step is 2^-32 of the largest weight then, 2^-44 where there is a second term of 2^12 times the rest.  bf16 has
 // f32's exponents.
@@ -443,7 +444,7 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kDim == 256 || (kF32 &
         const size_t token = static_cast<size_t>(begin + row_token[qt]);
         words[qt] = a.masks != nullptr ? a.masks + token * a.mask_words : nullptr;
         word0[qt] = a.masks != nullptr && a.mask_words > 0 ? words[qt][0] : 0ull;
-        unit[qt] = fmaxf(__builtin_fabsf(a.scale) * kLog2e, 1e-30f);  // (never 0, which would make minus infinity no number)
+        unit[qt] = __builtin_fabsf(a.scale) * kLog2e;
         const size_t from = token * a.query_token_stride + static_cast<size_t>(head) * a.query_head_stride;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
@@ -510,6 +511,8 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kDim == 256 || (kF32 &
                 query[qt][s][0] = __builtin_bit_cast(s16x8, uint4{v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip});
             }
         }
+        // (never 0, which would make the minus infinity of a key that is not seen no number; a scale that is no number stays one)
+        if (unit[qt] < kLeastUnit) unit[qt] = kLeastUnit;
     }
 
     f32x4 out[kQ][kDim / 16];

@@ -58,8 +58,8 @@ def check(b, **bounds):
     finite = np.isfinite(expected)
     assert np.array_equal(got[~finite], expected[~finite], equal_nan=True)
     assert np.isfinite(got[finite]).all()
-    wrong = np.abs(got - expected)[finite] / off[finite]
-    assert (wrong <= 1).all(), float(wrong.max())
+    wrong, off = np.abs(got - expected)[finite], off[finite]
+    assert (wrong <= off).all(), float((wrong / np.maximum(off, 1e-300)).max())
     return got
 
 
@@ -107,4 +107,26 @@ def test_scores_of_all_sizes_beside_a_large_one(activations, stored, shape):
         b.kv[0][b.table[r, 2 // 16], 2 % 16] = 0
         b.kv[0][b.table[r, 2 // 16], 2 % 16, :, 0] = 16
         b.kv[1][b.table[r, 2 // 16], 2 % 16] = 0
+    check(b)
+
+
+@pytest.mark.parametrize("activations,stored", KINDS)
+@pytest.mark.parametrize("shape", [([0, 40], [9, 40], 4, 2, 64), ([600], [2], 2, 1, 128), ([5000, 70], [3, 6], 4, 2, 128), ([300], [5], 2, 1, 256)])
+def test_scores_that_vanish(activations, stored, shape):
+    """Scales and queries so small that every seen key counts the same; keys that are not seen stay out."""
+    sizes = [(1.0, 0.0), (1.0, -0.0), (1.0, 1e-42)] + ([(2.0 ** -60, 0.0), (2.0 ** -60, 1e-30), (2e-45, 0.125), (1e-38, 1e-38)] if activations != "f16" else [])
+    for size, scale in sizes:
+        print(f"case: vanishing scores {activations}/{stored} {shape} queries {size} scale {scale}", flush=True)
+        b = Batch(np.random.default_rng(1), *shape, 16, activations, stored, spread=size)
+        b.scale = scale
+        b.tables[0][-1] = False
+        check(b)
+
+
+@pytest.mark.parametrize("activations,stored", [("f32", "f16"), ("f32", "bf16"), ("bf16", "bf16")])
+def test_large_queries_under_a_small_scale(activations, stored):
+    """Queries of 10^33 under a scale that brings the scores back."""
+    print(f"case: small scale {activations}/{stored}", flush=True)
+    b = Batch(np.random.default_rng(2), [90, 300], [7, 3], 4, 2, 128, 16, activations, stored, spread=1e33)
+    b.scale = 2e-34
     check(b)
