@@ -481,10 +481,12 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kDim == 256 || (kF32 &
                     most = fmaxf(most, __builtin_fabsf(v[s][j]));
                 }
             }
-            if (!kBf16) {  // f16 has 5 exponent bits: the row's largest value goes to [0.5, 1)
+            if (!kBf16) {
+                // f16 has 5 exponent bits: the row's largest value goes to [2^14, 2^15), and half of the second term's smallest step
+                // is 2^-39 of it
                 most = row_max(most);
                 const bool moves = most > 0.0f && most < __builtin_inff();
-                const int exponent = moves ? __builtin_amdgcn_frexp_expf(most) : 0;
+                const int exponent = moves ? __builtin_amdgcn_frexp_expf(most) - 15 : 0;
 #pragma unroll
                 for (int s = 0; s < kSteps; ++s) {
 #pragma unroll

@@ -455,7 +455,8 @@ afhip_status afhip_launch_cache_move(void *stream, const afhip_paged_cache *cach
  * cache's own type; [tokens][heads][head_dim] with strides in elements (multiples of 4 for F32, of 8 otherwise; 16-byte
  * aligned).  F32 queries and the softmax's weights beside them are multiplied as three terms of bf16 or two of f16, whichever
  * the cache holds (24 and 22 bits); with 16-bit queries the weights are rounded to the cache's type.  On an f16 cache a weight is
- * held to 2^-44 of the row's largest at best, with 16-bit queries to 2^-32.  Sums are f32.
+ * held to 2^-44 of the row's largest at best, with 16-bit queries to 2^-32, and an f32 query value to 2^-39 of its row's largest.
+ * Sums are f32.
  * max_query_len and max_key_len bound what the batch holds (new tokens; context plus new tokens) and choose the launch's
  * shape; tokens past the first and keys past the second are left out.  A key whose block the table does not name is not
  * seen.  head_dim <= 256, heads a multiple of kv_heads, mask_words <= 16, max_key_len * block_size < 2^32, else

@@ -130,3 +130,17 @@ def test_large_queries_under_a_small_scale(activations, stored):
     b = Batch(np.random.default_rng(2), [90, 300], [7, 3], 4, 2, 128, 16, activations, stored, spread=1e33)
     b.scale = 2e-34
     check(b)
+
+
+# ---- queries
+
+@pytest.mark.parametrize("activations,stored", [("f32", "f16"), ("f32", "bf16")])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_queries_of_one_large_value(activations, stored, shape):
+    """One value of a row 2^18 times the others', beside keys that have nothing there: the others keep their bits."""
+    print(f"case: one large query value {activations}/{stored} {SHAPES[shape]}", flush=True)
+    context, lens, heads, kv_heads, dim = SHAPES[shape]
+    b = Batch(np.random.default_rng(shape), context, lens, heads, kv_heads, dim, 16, activations, stored, tree=False, spread=3.0)
+    b.q[..., 5] = 2.0 ** 18
+    b.kv[0][..., 5] = np.where(np.isnan(b.kv[0][..., 5]), np.nan, 0)
+    check(b)
