@@ -51,7 +51,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // stay below 2^kSlack, far inside every type here, most tiles leave the sums as they are, and no lane has to know the others'
 // scores to see that.
 constexpr float kSlack = 8.0f;
-constexpr float kUnset = 1e38f;
+constexpr float kUnset = 3e38f;
+constexpr float kLowest = -3e38f;        // the maximum of a row whose seen scores are all minus infinity, or no numbers
 constexpr float kLeastUnit = 0x1p-126f;  // of what a product is multiplied by
 // Where a row's largest weight is put (a power of two): as high as f16 allows, whose steps below 2^-14 are 2^-24 whatever the
 // weight.  Half a step is 2^-32 of the largest weight then, 2^-44 where there is a second term of 2^12 times the rest.  bf16 has
@@ -110,10 +111,12 @@ __device__ __forceinline__ float row_sum(float v) {
 
 __device__ __forceinline__ uint32_t divide(uint32_t n, const Divisor& d) { return __umulhi(n, d.multiplier) + (n & d.whole); }
 
-// What a split of a request's keys holds for one row: the row's maximum (in units of log2) and the sum of its weights.
+// What a split of a request's keys holds for one row: the row's maximum (in units of log2, minus infinity where it saw no key) and
+// the sum of its weights.
 struct Part {
     float most, sum;
 };
+__device__ __forceinline__ Part part_of(bool saw, float shift, float sum) { return Part{!saw ? -__builtin_inff() : shift == kUnset ? kLowest : -shift, sum}; }
 
 // exp2(a - b) where both may be minus infinity (nothing seen yet): then 1, of sums that are zero.
 __device__ __forceinline__ float exp2_between(float a, float b) { return a == b ? 1.0f : __builtin_amdgcn_exp2f(a - b); }
@@ -177,17 +180,20 @@ __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kLeft) : "memory");
 }
 
-// Four values of a result from their sums; zero where nothing was seen.
+// Four values of a result from their sums; zero where nothing was seen (a sum of zero of what was seen, weights of minus infinity
+// only, makes no numbers).
 template <bool kBf16, bool kF32>
-__device__ __forceinline__ void store_row(const TreeAttentionArgs& a, size_t token, uint32_t head, int d, f32x4 x, float total) {
+__device__ __forceinline__ void store_row(const TreeAttentionArgs& a, size_t token, uint32_t head, int d, f32x4 x, float total, bool saw) {
     const size_t to = token * a.out_token_stride + static_cast<size_t>(head) * a.out_head_stride + d;
-    const float by = total == 0.0f ? 0.0f : 1.0f / total;
+    const float by = 1.0f / total;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = saw ? x[j] * by : 0.0f;
     if (kF32) {
-        *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to) = x * by;
+        *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to) = x;
     } else {
         s16x4 y;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = narrow<kBf16>(x[j] * by);
+        for (int j = 0; j < 4; ++j) y[j] = narrow<kBf16>(x[j]);
         *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(a.out) + to) = y;
     }
 }
@@ -524,10 +530,13 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kDim == 256 || (kF32 &
     // kLift, kUnset until the row has seen a key.  And this lane's part of the weights' sum.
     constexpr float kHighest = kLift<kBf16> + kSlack;
     float shift[kQ], sum[kQ];
+    uint32_t saw[kQ];       // not zero: the row has seen a key of a tile that not every row sees
+    uint32_t all_saw = 0;  // not zero: every row has seen a tile
 #pragma unroll
     for (int qt = 0; qt < kQ; ++qt) {
         shift[qt] = kUnset;
         sum[qt] = 0.0f;
+        saw[qt] = 0;
 #pragma unroll
         for (int d = 0; d < kDim / 16; ++d) {
             out[qt][d] = f32x4{0, 0, 0, 0};
@@ -554,6 +563,7 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kDim == 256 || (kF32 &
         free_stage = free_stage + 1 == kStages ? 0 : free_stage + 1;
         if (!works || tile >= key_end) continue;
         const bool clean = tile + kTile <= context && held == ~0u;  // every row sees every key
+        all_saw |= clean;
 
         // the operands of a product first, all of them: none of them waits for LDS by itself
         s16x8 key[2][kSteps];
@@ -617,6 +627,7 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kDim == 256 || (kF32 &
 #pragma unroll
             for (int qt = 0; qt < kQ; ++qt) {
                 seen[qt] = real[qt] ? seen_bits(tile, context, row_token[qt], word0[qt], words[qt], static_cast<int>(a.mask_words)) & held : 0u;
+                saw[qt] |= seen[qt];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
 #pragma unroll
@@ -744,7 +755,7 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kDim == 256 || (kF32 &
         for (int qt = 0; qt < kQ; ++qt) {
             const int r = key_group * kRows + (row_wave * kQ + qt) * 16 + column;
             const float total = row_sum(sum[qt]);
-            if (quarter == 0) group_parts[r] = Part{shift[qt] == kUnset ? -__builtin_inff() : -shift[qt], total};
+            if (quarter == 0) group_parts[r] = part_of((saw[qt] | all_saw) != 0, shift[qt], total);
 #pragma unroll
             for (int d = 0; d < kDim / 16; ++d) *reinterpret_cast<f32x4*>(sums + r * kPitch + d * 16 + quarter * 4) = out[qt][d];
         }
@@ -764,7 +775,7 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kDim == 256 || (kF32 &
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(y[j], by, x[j]);
             }
-            store_row<kBf16, kF32>(a, static_cast<size_t>(begin + row / group), kv_head * a.group + row % group, d, x, total);
+            store_row<kBf16, kF32>(a, static_cast<size_t>(begin + row / group), kv_head * a.group + row % group, d, x, total, highest != -__builtin_inff());
         }
         return;
     }
@@ -776,13 +787,13 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kDim == 256 || (kF32 &
         if (!real[qt]) continue;
         const int row = my_row + qt * 16 + column;
         const size_t part = static_cast<size_t>(slot) * kRows + (row - first_row);
-        if (share.splits > 1 && quarter == 0) parts[part] = Part{shift[qt] == kUnset ? -__builtin_inff() : -shift[qt], total};
+        if (share.splits > 1 && quarter == 0) parts[part] = part_of((saw[qt] | all_saw) != 0, shift[qt], total);
 #pragma unroll
         for (int dt = 0; dt < kDim / 16; ++dt) {
             const int d = dt * 16 + quarter * 4;
             if (d >= pieces * 8) continue;
             if (share.splits > 1) *reinterpret_cast<f32x4*>(part_out + part * a.cache.head_dim + d) = out[qt][dt];
-            else store_row<kBf16, kF32>(a, static_cast<size_t>(begin + row_token[qt]), kv_head * a.group + row % group, d, out[qt][dt], total);
+            else store_row<kBf16, kF32>(a, static_cast<size_t>(begin + row_token[qt]), kv_head * a.group + row % group, d, out[qt][dt], total, (saw[qt] | all_saw) != 0);
         }
     }
 }
@@ -856,7 +867,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void join_parts_kernel(TreeAttenti
             for (int j = 0; j < 4; ++j) x[j] = x[j] * mine + __shfl_xor(x[j], w) * theirs;
         }
         if ((alone ? base + group >= rows * a.cache.kv_heads : group != 0) || d >= a.cache.head_dim) continue;
-        store_row<kBf16, kF32>(a, static_cast<size_t>(share.begin) + row / a.group, kv_head * a.group + row % a.group, d, x, total);
+        store_row<kBf16, kF32>(a, static_cast<size_t>(share.begin) + row / a.group, kv_head * a.group + row % a.group, d, x, total, most != -__builtin_inff());
     }
 }
 

@@ -43,6 +43,8 @@ def want(b):
                 keys, values, row = kk[seen, h // group], vv[seen, h // group], q[i, h]
                 with np.errstate(all="ignore"):
                     s = b.scale * (keys @ row)
+                    if (s > -np.inf).any() and not np.isnan(s).any():  # weights of zero add no error
+                        keys, values, s = keys[s > -np.inf], values[s > -np.inf], s[s > -np.inf]
                     p = np.exp(s - s.max())
                     w = p / p.sum()
                     out[i, h] = w @ values
@@ -144,3 +146,65 @@ def test_queries_of_one_large_value(activations, stored, shape):
     b.q[..., 5] = 2.0 ** 18
     b.kv[0][..., 5] = np.where(np.isnan(b.kv[0][..., 5]), np.nan, 0)
     check(b)
+
+
+@pytest.mark.parametrize("activations,stored", KINDS)
+@pytest.mark.parametrize("context", [20, 3000])
+def test_a_scale_that_is_no_number(activations, stored, context):
+    print(f"case: scale nan {activations}/{stored} context={context}", flush=True)
+    b = Batch(np.random.default_rng(3), [context, 0], [7, 3], 4, 2, 64, 16, activations, stored)
+    b.tables[1][1] = False
+    b.scale = np.nan
+    got = b.run()
+    assert (got[8] == 0).all() and np.isnan(np.delete(got, 8, 0)).all()
+
+
+# ---- infinities and no numbers that a row sees
+
+PLACES = [([40], [9], 4, 2, 64), ([500, 30], [2, 5], 4, 2, 128), ([5000], [2], 4, 2, 128), ([3000, 200], [33, 64], 4, 2, 64), ([5000], [3], 2, 1, 256)]
+
+
+@pytest.mark.parametrize("activations,stored", [("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("place", range(len(PLACES)))
+@pytest.mark.parametrize("share", [0.3, 1.0])
+def test_scores_of_minus_infinity(activations, stored, place, share):
+    """A score of minus infinity is a weight of zero beside others, and no number where a row has no other."""
+    scores_of_minus_infinity(activations, stored, place, share)
+
+
+def scores_of_minus_infinity(activations, stored, place, share):
+    context, lens, heads, kv_heads, dim = PLACES[place]
+    print(f"case: minus infinity {activations}/{stored} {PLACES[place]} share={share}", flush=True)
+    rng = np.random.default_rng(place)
+    b = Batch(rng, context, lens, heads, kv_heads, dim, 16, activations, stored)
+    b.q[..., 0] = 1 + np.abs(b.q[..., 0])
+    for r, c in enumerate(context):
+        p = np.arange(c + lens[r])
+        p = p[(rng.random(len(p)) < share) | (p < c // 2)]  # all of some parts' keys
+        b.kv[0][b.table[r, p // 16], p % 16, :, 0] = -np.inf
+    b.tables[0][1] = False
+    b.tables[0][1, 1] = True
+    got = check(b)
+    assert np.isnan(got).any() == (share == 1.0)
+
+
+@pytest.mark.parametrize("activations,stored", KINDS)
+@pytest.mark.parametrize("place", range(len(PLACES)))
+def test_queries_and_keys_that_are_no_numbers(activations, stored, place):
+    """A query that is none takes its own row, a key that is none the rows that see it."""
+    context, lens, heads, kv_heads, dim = PLACES[place]
+    print(f"case: no numbers {activations}/{stored} {PLACES[place]}", flush=True)
+    b = Batch(np.random.default_rng(place), context, lens, heads, kv_heads, dim, 16, activations, stored)
+    clean = b.run()
+    b.q[1, heads - 1, 3] = np.nan
+    got = b.run()
+    assert np.isnan(got[1, heads - 1]).all()
+    got[1, heads - 1] = clean[1, heads - 1]
+    assert np.array_equal(got, clean)
+    b.kv[0][b.table[0, 1], 5, 0, 7] = np.nan
+    got = b.run()
+    first, group = slice(0, lens[0]), heads // kv_heads
+    assert np.isnan(got[first, :group]).all()
+    got[first, :group] = clean[first, :group]
+    got[1, heads - 1] = clean[1, heads - 1]
+    assert np.array_equal(got, clean)
