@@ -643,9 +643,42 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kDim == 256 || (kF32 &
         for (int qt = 0; qt < kQ; ++qt) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[qt][j] = __builtin_fmaf(score[qt][j >> 2][j & 3], unit[qt], shift[qt]);
-            passes |= fmaxf(fmaxf(fmaxf(x[qt][0], x[qt][1]), fmaxf(x[qt][2], x[qt][3])), fmaxf(fmaxf(x[qt][4], x[qt][5]), fmaxf(x[qt][6], x[qt][7]))) > kHighest;
+            float most = x[qt][0];  // (no number if one of f32 queries' is none)
+#pragma unroll
+            for (int j = 1; j < 8; ++j) most = kF32 ? __builtin_elementwise_maximum(most, x[qt][j]) : fmaxf(most, x[qt][j]);
+            passes |= !(most <= kHighest);
         }
         if (__any(passes)) {
+            if constexpr (kF32) {
+                // An infinite key: the terms of a query value may be zero or of either sign, and their infinities then make no number of
+                // the score.  The first terms alone give it as the value would.
+                bool none = false;
+#pragma unroll
+                for (int qt = 0; qt < kQ; ++qt) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) none |= __builtin_isnan(x[qt][j]);
+                }
+                if (__any(none)) {
+                    f32x4 first_terms[kQ][2];
+#pragma unroll
+                    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const s16x8 k = *reinterpret_cast<const s16x8*>(k_lds + key_piece<kDim>(column, s * 4 + quarter) * 16 + half * (16 * kDim * 2));
+#pragma unroll
+                            for (int qt = 0; qt < kQ; ++qt) first_terms[qt][half] = mfma<kBf16>(k, query[qt][s][0], s == 0 ? f32x4{0, 0, 0, 0} : first_terms[qt][half]);
+                        }
+                    }
+#pragma unroll
+                    for (int qt = 0; qt < kQ; ++qt) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            if (__builtin_isnan(score[qt][j >> 2][j & 3])) score[qt][j >> 2][j & 3] = first_terms[qt][j >> 2][j & 3];
+                            x[qt][j] = __builtin_fmaf(score[qt][j >> 2][j & 3], unit[qt], shift[qt]);
+                        }
+                    }
+                }
+            }
 #pragma unroll
             for (int qt = 0; qt < kQ; ++qt) {
                 const f32x4 lo = score[qt][0], hi = score[qt][1];

@@ -208,3 +208,17 @@ def test_queries_and_keys_that_are_no_numbers(activations, stored, place):
     got[first, :group] = clean[first, :group]
     got[1, heads - 1] = clean[1, heads - 1]
     assert np.array_equal(got, clean)
+
+
+@pytest.mark.parametrize("stored", ["f16", "bf16"])
+@pytest.mark.parametrize("place", range(len(PLACES)))
+@pytest.mark.parametrize("share", [0.3, 1.0])
+def test_f32_queries_on_scores_of_minus_infinity(stored, place, share):
+    """A query value's terms agree about an infinite key, also where the value is its first term."""
+    scores_of_minus_infinity("f32", stored, place, share)
+    context, lens, heads, kv_heads, dim = PLACES[place]
+    b = Batch(np.random.default_rng(place), context, lens, heads, kv_heads, dim, 16, "f32", stored)
+    b.q[..., 3] = 2.0
+    for r, c in enumerate(context):
+        b.kv[0][b.table[r, 0], 1::3, :, 3] = -np.inf
+    assert np.isfinite(check(b)).all()
