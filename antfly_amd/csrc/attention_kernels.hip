@@ -11,8 +11,8 @@
 // V^T P^T as they stand: the order of the 32 keys inside the instruction is free as long as V follows it (lane group g holds
 // keys 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3).  V comes row-major and is needed column-major: it is read from LDS with the
 // transposing ds_read_b64_tr_b16.  F32 queries and the weights beside them are two terms of f16 or three of bf16, each a product
-// of its own: 22 and 24 bits.  f16 ends at 2^-24: its weights are kept high in the type (kLift), and a weight's second term is 2^12
-// times itself, with sums of its own.
+// of its own: 22 and 24 bits.  A weight's first term has sums of its own.  f16 ends at 2^-24: its weights are kept high in the type
+// (kLift), and the second term is 2^12 times itself.
 //
 // Keys and values come in tiles of 32 keys from memory straight into a ring of tiles in LDS (no registers in between),
 // requested kStages - 1 tiles ahead, their places found a tile before that.  The wavefronts of a workgroup share its tiles and
@@ -524,7 +524,10 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kDim == 256 || (kF32 &
     }
 
     f32x4 out[kQ][kDim / 16];
-    constexpr bool kApart = kF32 && !kBf16;  // the second terms' sums, kRestScale times themselves
+    // The later terms' sums, with f16 kRestScale times themselves.  An infinite value makes infinities of either sign or no numbers of
+    // them; those of the first terms are what the weights would make of it.
+    constexpr bool kApart = kF32;
+    constexpr float kRestIs = kBf16 ? 1.0f : kRestScale;
     f32x4 low[kApart ? kQ : 1][kApart ? kDim / 16 : 1];
     // A weight is exp2(product * unit + shift): the shift takes off the row's largest score (up to kSlack more than it) and adds
     // kLift, kUnset until the row has seen a key.  And this lane's part of the weights' sum.
@@ -711,7 +714,7 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kDim == 256 || (kF32 &
 #pragma unroll
                 for (int term = 0; term < kTerms; ++term) {
                     weight[qt][term][j] = narrow<kBf16>(rest);
-                    if (term + 1 < kTerms) rest = (rest - widen<kBf16>(weight[qt][term][j])) * (kApart ? kRestScale : 1.0f);
+                    if (term + 1 < kTerms) rest = (rest - widen<kBf16>(weight[qt][term][j])) * kRestIs;
                 }
             }
         }
@@ -773,7 +776,9 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kDim == 256 || (kF32 &
 #pragma unroll
             for (int d = 0; d < kDim / 16; ++d) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) out[qt][d][j] = __builtin_fmaf(low[qt][d][j], 1.0f / kRestScale, out[qt][d][j]);
+                for (int j = 0; j < 4; ++j) {
+                    if (__builtin_isfinite(out[qt][d][j])) out[qt][d][j] = __builtin_fmaf(low[qt][d][j], 1.0f / kRestIs, out[qt][d][j]);
+                }
             }
         }
     }

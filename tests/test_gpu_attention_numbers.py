@@ -222,3 +222,18 @@ def test_f32_queries_on_scores_of_minus_infinity(stored, place, share):
     for r, c in enumerate(context):
         b.kv[0][b.table[r, 0], 1::3, :, 3] = -np.inf
     assert np.isfinite(check(b)).all()
+
+
+@pytest.mark.parametrize("activations,stored", KINDS)
+@pytest.mark.parametrize("place", range(len(PLACES)))
+def test_infinite_values_of_the_context(activations, stored, place):
+    """Values that every row sees: an infinity reaches its own dimensions with its sign, two signs make no number."""
+    context, lens, heads, kv_heads, dim = PLACES[place]
+    print(f"case: infinite values {activations}/{stored} {PLACES[place]}", flush=True)
+    b = Batch(np.random.default_rng(place), context, lens, heads, kv_heads, dim, 16, activations, stored)
+    for r in range(len(lens)):
+        b.kv[1][b.table[r, 0], 3, :, 5] = np.inf
+        b.kv[1][b.table[r, 1], 2, 0, 9:12] = -np.inf
+        b.kv[1][b.table[r, 0], 7, :, 11] = np.inf
+    got = check(b)
+    assert np.isposinf(got[0, :, 5]).all() and np.isneginf(got[0, 0, 9:11]).all() and np.isnan(got[0, 0, 11])
