@@ -100,9 +100,9 @@ afhip_status afhip_launch_linear_fp8_f32(void* stream, afhip_buffer dst, afhip_b
     if (rows == 0 || out_dim == 0) return AFHIP_OK;
     if (linear_fp8_is_fused(call.rows, call.in_dim))
         return status_of(launch_linear_fp8_fused(static_cast<hipStream_t>(stream), call, reinterpret_cast<const float*>(input.ptr), gemv_compute_units()));
-    const Fp8Plan plan = plan_matmul_fp8(call.rows, call.in_dim, call.out_dim, gemv_compute_units(), SIZE_MAX);
     const size_t quantized = codes_bytes(rows, in_dim) + scales_bytes(rows, in_dim);
-    if (!holds(workspace, quantized + plan.sums_bytes(call.rows, call.out_dim), 1, 256)) return AFHIP_ERR_INVALID_STATE;
+    if (!holds(workspace, quantized, 1, 256)) return AFHIP_ERR_INVALID_STATE;
+    const Fp8Plan plan = plan_matmul_fp8(call.rows, call.in_dim, call.out_dim, gemv_compute_units(), workspace.len - quantized);
     uint8_t* codes = reinterpret_cast<uint8_t*>(workspace.ptr);
     float* scales = reinterpret_cast<float*>(workspace.ptr + codes_bytes(rows, in_dim));
     const hipError_t e = launch_quantize_fp8(static_cast<hipStream_t>(stream), codes, scales, reinterpret_cast<const float*>(input.ptr), rows,

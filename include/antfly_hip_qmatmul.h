@@ -365,9 +365,10 @@ afhip_status afhip_launch_decode_fp16(void *stream, afhip_buffer dst_f32, afhip_
 afhip_status afhip_launch_quantize_fp8(void *stream, afhip_buffer q, afhip_buffer scales, afhip_buffer input, size_t rows,
                                        size_t in_dim);
 /* Scratch of the two products below, 256-byte aligned: the quantized activations, and the sums of K's shares where a small
- * grid of tiles has a long K; 0 where few activations are quantized in the product's own launch.  afhip_launch_matmul_fp8_f32
- * runs with less or none (on fewer shares or one: the same products summed in another order); afhip_launch_linear_fp8_f32
- * refuses less. */
+ * grid of tiles has a long K; 0 where few activations are quantized in the product's own launch.  Both run with less (on fewer
+ * shares or one: the same products summed in another order), afhip_launch_matmul_fp8_f32 with none, afhip_launch_linear_fp8_f32
+ * with the codes and scales at least: in_dim and 4 ceil(in_dim / 128) bytes a row, each of the two rounded up to 256.  So what was
+ * asked for some rows does for any fewer of the same weight, though the sums of fewer rows may ask for more. */
 size_t afhip_linear_fp8_workspace_bytes(size_t rows, size_t in_dim, size_t out_dim);
 /* Y = act(X W^T + bias) + residual on activations that are codes already (several projections of one input quantize it
  * once).  bias f32 [out_dim] and residual f32 [rows][out_dim] are optional (.ptr == 0); activation: afhip_activation. */

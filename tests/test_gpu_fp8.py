@@ -217,3 +217,26 @@ def test_other_stream_and_replayed_graph(rows):
         graph.replay()
         torch.cuda.synchronize()
         assert np.array_equal(y.cpu().numpy(), eager[i])
+
+
+@pytest.mark.parametrize("most,fewer,in_dim,out_dim", [(258, (257, 200, 40, 3), 4096, 4096), (85, (84, 65), 8192, 4096)])
+def test_a_workspace_of_more_rows_does_for_fewer(most, fewer, in_dim, out_dim):
+    """The shares' sums of fewer rows may take more room than all that more rows ask for: then there are fewer shares."""
+    size = kernels.linearFp8WorkspaceBytes(most, in_dim, out_dim)
+    assert any(kernels.linearFp8WorkspaceBytes(rows, in_dim, out_dim) > size for rows in fewer)
+    rng = np.random.default_rng(most)
+    w, w_scales = F.weights(rng, out_dim, in_dim)
+    wd, sd = G.to_dev(w), G.to_dev(w_scales)
+    ws = torch.full((size + 256,), 0xFF, dtype=torch.uint8, device=G.DEV)
+    for rows in fewer:
+        print(f"case: fp8 workspace of {most} rows, {rows} rows in={in_dim} out={out_dim}", flush=True)
+        x = activations(rng, rows, in_dim)
+        whole, y = guarded(rows, out_dim)
+        xd = G.to_dev(x)
+        kernels.launchLinearFp8F32(G.stream(), G.buf(y), G.buf(xd), G.buf(wd), G.buf(sd), rows, in_dim, out_dim, workspace=G.buf(ws[:size]))
+        torch.cuda.synchronize()
+        assert guards_hold(whole) and bool((ws[size:] == 0xFF).all())
+        sample = np.unique(np.r_[0, rows - 1, rng.integers(0, rows, 10)])
+        want, off = F.matmul(*F.quantize(x[sample]), w, w_scales)
+        got = y.cpu().numpy()
+        assert (np.abs(got[sample] - want) <= off).all() and np.isfinite(got).all()
