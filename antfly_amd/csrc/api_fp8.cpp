@@ -64,6 +64,7 @@ afhip_status afhip_launch_quantize_fp8(void* stream, afhip_buffer q, afhip_buffe
     if (!holds(input, rows * in_dim, 4, 16) || !holds(q, rows * in_dim, 1, 16) || !holds(scales, rows * ((in_dim + 127) / 128), 4, 4))
         return AFHIP_ERR_INVALID_STATE;
     if (rows == 0) return AFHIP_OK;
+    if (!quantize_fp8_fits_a_launch(rows, static_cast<int>(in_dim))) return AFHIP_ERR_OP_UNSUPPORTED;
     return status_of(launch_quantize_fp8(static_cast<hipStream_t>(stream), reinterpret_cast<uint8_t*>(q.ptr), reinterpret_cast<float*>(scales.ptr),
                                          reinterpret_cast<const float*>(input.ptr), rows, static_cast<int>(in_dim)));
 }
@@ -87,6 +88,7 @@ afhip_status afhip_launch_matmul_fp8_f32(void* stream, afhip_buffer dst, afhip_b
     call.x_scales = reinterpret_cast<const float*>(q_scales.ptr);
     const bool lent = workspace.ptr != 0 && workspace.ptr % 256 == 0;
     const Fp8Plan plan = plan_matmul_fp8(call.rows, call.in_dim, call.out_dim, gemv_compute_units(), lent ? workspace.len : 0);
+    if (!matmul_fp8_fits_a_launch(call.rows, call.out_dim, plan)) return AFHIP_ERR_OP_UNSUPPORTED;
     return status_of(launch_matmul_fp8(static_cast<hipStream_t>(stream), call, plan, reinterpret_cast<float*>(workspace.ptr)));
 }
 
@@ -98,11 +100,14 @@ afhip_status afhip_launch_linear_fp8_f32(void* stream, afhip_buffer dst, afhip_b
     if (s != AFHIP_OK) return s;
     if (!holds(input, rows * in_dim, 4, 16)) return AFHIP_ERR_INVALID_STATE;
     if (rows == 0 || out_dim == 0) return AFHIP_OK;
-    if (linear_fp8_is_fused(call.rows, call.in_dim))
+    if (linear_fp8_is_fused(call.rows, call.in_dim)) {
+        if (!linear_fp8_fused_fits_a_launch(call.out_dim)) return AFHIP_ERR_OP_UNSUPPORTED;
         return status_of(launch_linear_fp8_fused(static_cast<hipStream_t>(stream), call, reinterpret_cast<const float*>(input.ptr), gemv_compute_units()));
+    }
     const size_t quantized = codes_bytes(rows, in_dim) + scales_bytes(rows, in_dim);
     if (!holds(workspace, quantized, 1, 256)) return AFHIP_ERR_INVALID_STATE;
     const Fp8Plan plan = plan_matmul_fp8(call.rows, call.in_dim, call.out_dim, gemv_compute_units(), workspace.len - quantized);
+    if (!quantize_fp8_fits_a_launch(rows, call.in_dim) || !matmul_fp8_fits_a_launch(call.rows, call.out_dim, plan)) return AFHIP_ERR_OP_UNSUPPORTED;
     uint8_t* codes = reinterpret_cast<uint8_t*>(workspace.ptr);
     float* scales = reinterpret_cast<float*>(workspace.ptr + codes_bytes(rows, in_dim));
     const hipError_t e = launch_quantize_fp8(static_cast<hipStream_t>(stream), codes, scales, reinterpret_cast<const float*>(input.ptr), rows,

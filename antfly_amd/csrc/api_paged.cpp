@@ -162,13 +162,13 @@ afhip_status afhip_launch_cache_store(void* stream, const afhip_paged_cache* cac
     if (type != AFHIP_TYPE_F32 && type != AFHIP_TYPE_F16 && type != AFHIP_TYPE_BF16) return AFHIP_ERR_UNSUPPORTED_TENSOR_TYPE;
     if (tokens == 0) return AFHIP_OK;
     const size_t unit = type == AFHIP_TYPE_F32 ? 4 : 8, size = type == AFHIP_TYPE_F32 ? 4 : 2;
-    size_t elements, bytes, work;
+    size_t elements, bytes, chunks;
     if (tokens > kInt32Max || token_stride % unit != 0 || head_stride % unit != 0 ||
         !span(tokens, token_stride, cache->kv_heads, head_stride, cache->head_dim, &elements) || !checked_mul(elements, size, &bytes) ||
         bytes > keys.len || bytes > values.len || !aligned(keys, 16) || !aligned(values, 16) || !holds(slots, tokens, 4))
         return AFHIP_ERR_INVALID_STATE;
-    // a workgroup takes at most 256 parts of eight values of one token, and a launch 2^31 - 1 workgroups
-    if (!checked_mul(cache->kv_heads, cache->head_dim / 8, &work) || !checked_mul((work + 255) / 256, tokens, &work) || work > kInt32Max)
+    if (!checked_mul(cache->kv_heads, cache->head_dim / 8, &chunks) || chunks > kInt32Max ||
+        !fits_a_launch(StoreGrid(static_cast<uint32_t>(chunks)).groups(static_cast<uint32_t>(tokens)), kCacheThreads))
         return AFHIP_ERR_OP_UNSUPPORTED;
     return status_of(launch_cache_store(static_cast<hipStream_t>(stream), view, cache->type == AFHIP_TYPE_BF16, type,
                                         reinterpret_cast<const void*>(keys.ptr), reinterpret_cast<const void*>(values.ptr), token_stride,
@@ -188,7 +188,8 @@ afhip_status afhip_launch_cache_move(void* stream, const afhip_paged_cache* cach
         !checked_mul(requests, path_columns, &steps) || !holds(block_tables, entries, 4) || !holds(context_lens, requests, 4) ||
         !holds(paths, steps, 4) || !holds(path_lens, requests, 4))
         return AFHIP_ERR_INVALID_STATE;
-    if (!checked_mul(cache->kv_heads, cache->head_dim / 8, &chunks) || chunks > 65535 * 128) return AFHIP_ERR_OP_UNSUPPORTED;
+    if (!checked_mul(cache->kv_heads, cache->head_dim / 8, &chunks) || chunks > 65535 * 128 || !fits_a_launch(requests, kCacheThreads))
+        return AFHIP_ERR_OP_UNSUPPORTED;
     return status_of(launch_cache_move(static_cast<hipStream_t>(stream), view, reinterpret_cast<const int*>(block_tables.ptr),
                                        static_cast<uint32_t>(table_columns), reinterpret_cast<const int*>(context_lens.ptr),
                                        reinterpret_cast<const int*>(paths.ptr), reinterpret_cast<const int*>(path_lens.ptr),

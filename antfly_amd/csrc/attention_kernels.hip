@@ -1010,11 +1010,14 @@ hipError_t attend(hipStream_t stream, const TreeAttentionArgs& a, const Shape& s
     return hipGetLastError();
 }
 
+// Groups of wavefronts that a workgroup with all of a head's keys has (by LDS).
+constexpr int key_groups(int dim) { return dim == 256 ? 2 : 4; }
+
 // The ring's length: as many stages as let two workgroups of four wavefronts, or four of one, on a unit's 160 KiB of LDS; key
 // groups have two.
 template <int kDim, bool kBf16, bool kF32>
 hipError_t attend_rows(hipStream_t stream, const TreeAttentionArgs& a, const Shape& s, void* workspace) {
-    constexpr int kGroups = kDim == 256 ? 2 : 4;
+    constexpr int kGroups = key_groups(kDim);
     if (s.gathered) {
         if (s.waves == 1) return attend<kDim, kBf16, kF32, 1, 1, kGroups, 2>(stream, a, s, workspace);
         return attend<kDim, kBf16, kF32, 1, 2, kGroups, 2>(stream, a, s, workspace);
@@ -1040,7 +1043,10 @@ size_t tree_attention_workspace_bytes(const TreeAttentionArgs& args, int compute
     return s.slots == 0 ? 0 : part_out_bytes(args, s) + s.slots * s.rows_a_tile() * sizeof(Part);
 }
 
-bool tree_attention_fits_a_launch(const TreeAttentionArgs& args, int compute_units) { return shape_of(args, compute_units).groups <= 0x7fffffff; }
+bool tree_attention_fits_a_launch(const TreeAttentionArgs& args, int compute_units) {
+    const Shape s = shape_of(args, compute_units);
+    return fits_a_launch(s.groups, static_cast<uint64_t>(s.waves) * (s.gathered ? key_groups(s.dim) : 1) * 64);
+}
 
 hipError_t launch_tree_attention(hipStream_t stream, const TreeAttentionArgs& args, void* workspace, int compute_units) {
     const Shape s = shape_of(args, compute_units);

@@ -556,6 +556,18 @@ hipError_t launch_quantize_fp8(hipStream_t stream, uint8_t* q, float* scales, co
     return hipGetLastError();
 }
 
+bool quantize_fp8_fits_a_launch(size_t rows, int in_dim) { return fits_a_launch((rows * fp8_blocks(in_dim) + 31) / 32, 256); }
+
+// (512 threads: the most that a workgroup of 16 columns has)
+bool linear_fp8_fused_fits_a_launch(int out_dim) { return fits_a_launch((static_cast<uint64_t>(out_dim) + 15) / 16, 512); }
+
+bool matmul_fp8_fits_a_launch(int rows, int out_dim, const Fp8Plan& plan) {
+    if (plan.kernel != kFp8Tile64 && plan.kernel != kFp8Tile128) return linear_fp8_fused_fits_a_launch(out_dim);
+    const uint64_t tile = plan.kernel == kFp8Tile64 ? 64 : 128;
+    return fits_a_launch((static_cast<uint64_t>(out_dim) + 1023) / 1024 * 8 * ((rows + tile - 1) / tile), 256) &&
+           (plan.shares == 1 || fits_a_launch(static_cast<uint64_t>(rows) * ((static_cast<uint64_t>(out_dim) + 1023) / 1024), 256));
+}
+
 // Up to how many values of X every workgroup quantizes them itself.
 constexpr int64_t kFusedValues = 16384;
 

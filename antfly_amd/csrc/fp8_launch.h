@@ -39,5 +39,9 @@ struct Fp8Plan {
 };
 Fp8Plan plan_matmul_fp8(int rows, int in_dim, int out_dim, int compute_units, size_t room);
 hipError_t launch_matmul_fp8(hipStream_t stream, const Fp8Matmul& call, const Fp8Plan& plan, float* sums);
+// Whether their grids are within what a launch may have.
+bool quantize_fp8_fits_a_launch(size_t rows, int in_dim);
+bool linear_fp8_fused_fits_a_launch(int out_dim);
+bool matmul_fp8_fits_a_launch(int rows, int out_dim, const Fp8Plan& plan);
 
 }  // namespace afhip

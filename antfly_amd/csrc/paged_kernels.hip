@@ -8,7 +8,7 @@ namespace afhip {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = kCacheThreads;
 
 __device__ __forceinline__ int at_least_zero(int v) { return v > 0 ? v : 0; }
 
@@ -288,10 +288,9 @@ template <int kType, bool kToBf16>
 hipError_t store(hipStream_t stream, const CacheView& cache, const void* keys, const void* values, size_t token_stride,
                  size_t head_stride, const int* slots, uint32_t tokens) {
     const uint32_t chunks_a_head = cache.head_dim / 8, chunks = cache.kv_heads * chunks_a_head;
-    const uint32_t tokens_a_group = chunks < kThreads ? kThreads / chunks : 1, groups_a_token = (chunks + kThreads - 1) / kThreads;
-    const uint32_t grid = groups_a_token > 1 ? tokens * groups_a_token : (tokens + tokens_a_group - 1) / tokens_a_group;
-    cache_store_kernel<kType, kToBf16><<<grid, kThreads, 0, stream>>>(cache, keys, values, token_stride, head_stride, slots, tokens,
-                                                                     chunks_a_head, chunks, tokens_a_group, groups_a_token);
+    const StoreGrid grid(chunks);
+    cache_store_kernel<kType, kToBf16><<<static_cast<uint32_t>(grid.groups(tokens)), kThreads, 0, stream>>>(
+        cache, keys, values, token_stride, head_stride, slots, tokens, chunks_a_head, chunks, grid.tokens_a_group, grid.groups_a_token);
     return hipGetLastError();
 }
 

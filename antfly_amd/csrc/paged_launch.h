@@ -40,6 +40,16 @@ struct BatchPlanArgs {
 };
 hipError_t launch_batch_plan(hipStream_t stream, const BatchPlanArgs& args);
 
+constexpr uint32_t kCacheThreads = 256;  // of a workgroup of the store and the move
+// A workgroup of the store takes eight values a thread: whole tokens while they fit it, a part of one token otherwise.
+struct StoreGrid {
+    uint32_t tokens_a_group, groups_a_token;
+    StoreGrid(uint32_t chunks) : tokens_a_group(chunks < kCacheThreads ? kCacheThreads / chunks : 1), groups_a_token((chunks - 1) / kCacheThreads + 1) {}
+    uint64_t groups(uint32_t tokens) const {
+        return groups_a_token > 1 ? static_cast<uint64_t>(tokens) * groups_a_token : (static_cast<uint64_t>(tokens) + tokens_a_group - 1) / tokens_a_group;
+    }
+};
+
 // type: 0 f32, 1 f16, 30 bf16 (the source's); to_bf16: the cache's.  Strides in elements.
 hipError_t launch_cache_store(hipStream_t stream, const CacheView& cache, bool to_bf16, int type, const void* keys,
                               const void* values, size_t token_stride, size_t head_stride, const int* slots, uint32_t tokens);

@@ -15,6 +15,9 @@ hipError_t allow_lds(Kernel kernel, size_t lds, LdsLimit* limit) {
                         [&] { return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024); });
 }
 
+// Threads along one dimension of a launch: HIP refuses 2^32 and more.
+inline bool fits_a_launch(uint64_t workgroups, uint64_t threads) { return workgroups * threads <= 0xffffffffull; }
+
 // What the kernel that writes Y does to each total before storing it: + bias[o], then the
 // activation, then + residual[r][o] -- the engine's linear / linearRelu / linearQuickGelu /
 // linearGelu / linearAdd (ops/ops.zig:1728, :2164-2230), in the order of the CUDA backend's

@@ -354,7 +354,8 @@ afhip_status afhip_launch_decode_fp16(void *stream, afhip_buffer dst_f32, afhip_
  *   Y[r][o] = sum over blocks b of  x_scale[r][b] * weight_scale[o / 128][b] * (sum over k in b of  x[r][k] * w[o][k])
  *
  * with every sum in f32.  in_dim is a non-zero multiple of 16 (the last block may be shorter than 128), out_dim and rows
- * are any numbers (rows up to 2^20 - 16, else AFHIP_ERR_OP_UNSUPPORTED); everything is contiguous; codes and f32 activations are 16-byte aligned, the other
+ * are any numbers (rows up to 2^20 - 16, out_dim up to 2^27 - 16, and grids of fewer than 2^32 threads, which some 2^34 results and
+ * 2^36 activations to quantize reach; else AFHIP_ERR_OP_UNSUPPORTED); everything is contiguous; codes and f32 activations are 16-byte aligned, the other
  * buffers 4-byte (else AFHIP_ERR_INVALID_STATE).  rows * out_dim == 0 is a successful no-op.  Results must not overlap
  * what is read, except that the residual may be Y itself.
  * ---------------------------------------------------------------------- */
@@ -434,14 +435,15 @@ afhip_status afhip_launch_batch_plan(void *stream, const afhip_batch_plan *plan)
 
 /* Keys and values of `tokens` new tokens into their slots: type F32, F16 or BF16 (converted to the cache's type, to
  * nearest, ties to even), [tokens][kv_heads][head_dim] with the given strides (elements; multiples of 4 for F32 and of 8
- * otherwise, 16-byte aligned).  A slot outside the cache writes nothing; two tokens of one slot race. */
+ * otherwise, 16-byte aligned).  A slot outside the cache writes nothing; two tokens of one slot race.  2^24 tokens of more than
+ * 128 x 8 values and more than that of smaller ones (a grid of 2^32 threads): AFHIP_ERR_OP_UNSUPPORTED. */
 afhip_status afhip_launch_cache_store(void *stream, const afhip_paged_cache *cache, int type, afhip_buffer keys,
                                       afhip_buffer values, size_t token_stride, size_t head_stride, afhip_buffer slots,
                                       size_t tokens);
 /* After a verification: for i = 0 .. path_lens[r] - 1 in this order, the cache's token at position
  * context_lens[r] + paths[r][i] becomes the one at context_lens[r] + i.  paths int32 [requests][path_columns] with
  * paths[r][i] >= i, ascending (a tree's path from its root).  Steps whose index is negative, or whose slots the table does
- * not name, move nothing. */
+ * not name, move nothing.  2^24 requests, or tokens of 2^26 values: AFHIP_ERR_OP_UNSUPPORTED. */
 afhip_status afhip_launch_cache_move(void *stream, const afhip_paged_cache *cache, afhip_buffer block_tables,
                                      size_t table_columns, afhip_buffer context_lens, afhip_buffer paths,
                                      afhip_buffer path_lens, size_t requests, size_t path_columns);
@@ -460,8 +462,9 @@ afhip_status afhip_launch_cache_move(void *stream, const afhip_paged_cache *cach
  * Sums are f32.
  * max_query_len and max_key_len bound what the batch holds (new tokens; context plus new tokens) and choose the launch's
  * shape; tokens past the first and keys past the second are left out.  A key whose block the table does not name is not
- * seen.  head_dim <= 256, heads a multiple of kv_heads, mask_words <= 16, max_key_len * block_size < 2^32, else
- * AFHIP_ERR_OP_UNSUPPORTED.
+ * seen.  heads is a multiple of kv_heads (else AFHIP_ERR_INVALID_STATE); head_dim <= 256, mask_words <= 16, requests <= 65535,
+ * max_key_len * block_size < 2^32, max_query_len * heads < 2^31 and a grid of fewer than 2^32 threads (one of 64 to 512 for every 16 to
+ * 128 of a request's max_query_len * heads / kv_heads rows and every key head, or as many as the units hold), else AFHIP_ERR_OP_UNSUPPORTED.
  * `workspace` (256-byte aligned, afhip_tree_attention_workspace_bytes) holds the parts of rows whose keys are shared out
  * over workgroups (0 bytes where one workgroup has all of a row's keys); less than asked for is refused
  * (AFHIP_ERR_INVALID_STATE). */
