@@ -73,3 +73,25 @@ def in_64_bits(example, model, tokens):
         up = fp8_ref.activate(up, example.GELU)
         x = x + linear(layer["down"], up)
     return linear(model.head, norm(x))
+
+
+@pytest.mark.parametrize("drafts", [6, 15])
+def test_accepted_paths_move(example, drafts, monkeypatch):
+    """Drafts are accepted, some of them not where their path's place is: the cache's tokens move, and the tokens stay the model's."""
+    moved = []
+    launch = example.paged.launchCacheMove
+
+    def recorded(stream, cache, table, context, paths, lens):
+        for path, n in zip(paths.tolist(), lens.tolist()):
+            moved.extend(p - i for i, p in enumerate(path[:n]))
+        launch(stream, cache, table, context, paths, lens)
+
+    monkeypatch.setattr(example.paged, "launchCacheMove", recorded)
+    model = example.Model()
+    prompts = prompts_of(model, (3, 40, 17))
+    plain, steps = example.generate(model, prompts, 48, 0)
+    assert moved and not any(moved)  # one token a step: it lies where it belongs
+    moved.clear()
+    drafted, fewer = example.generate(model, prompts, 48, drafts)
+    assert drafted == plain
+    assert fewer < steps and any(moved) and min(moved) == 0
