@@ -646,10 +646,9 @@ __global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kDim == 256 || (kF32 &
         for (int qt = 0; qt < kQ; ++qt) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[qt][j] = __builtin_fmaf(score[qt][j >> 2][j & 3], unit[qt], shift[qt]);
-            float most = x[qt][0];  // (no number if one of f32 queries' is none)
-#pragma unroll
-            for (int j = 1; j < 8; ++j) most = kF32 ? __builtin_elementwise_maximum(most, x[qt][j]) : fmaxf(most, x[qt][j]);
-            passes |= !(most <= kHighest);
+            const auto larger = [](float a, float b) { return kF32 ? __builtin_elementwise_maximum(a, b) : fmaxf(a, b); };  // (f32 queries: no number if one is none)
+            const float most = larger(larger(larger(x[qt][0], x[qt][1]), larger(x[qt][2], x[qt][3])), larger(larger(x[qt][4], x[qt][5]), larger(x[qt][6], x[qt][7])));
+            passes |= kF32 ? !(most <= kHighest) : most > kHighest;
         }
         if (__any(passes)) {
             if constexpr (kF32) {
