@@ -343,11 +343,10 @@ __device__ __forceinline__ bool find_share(const TreeAttentionArgs& a, const Sha
 }
 
 // kDim: the head's values, rounded up to a size that is here (the rest are zeros).  kF32: query and out are f32.
-// Two wavefronts a SIMD (256 registers) wherever the sums leave room for them: f32 rows of heads of 256, and 32 rows a wavefront of 128, do
-// not (8 requests of 5 tokens on 3000 keys, f32 on f16: 28.9 us, with the 260 to 320 registers that the compiler takes when it may
-// 37.7).
+// Two wavefronts a SIMD (256 registers) wherever the sums leave room for them, all but heads of 256 (8 requests of 5 tokens on 3000
+// keys, f32 on f16: 28.9 us, with the 260 to 320 registers that the compiler takes when it may 37.7).
 template <int kDim, bool kBf16, bool kF32, int kQ, int kRowWaves, int kKeyGroups, int kStages>
-__global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kDim == 256 || (kF32 && kDim * kQ == 256) ? 1 : 2) void tree_attention_kernel(TreeAttentionArgs a, SharePlan plan, float* part_out,
+__global__ __launch_bounds__(kRowWaves * kKeyGroups * 64, kDim == 256 ? 1 : 2) void tree_attention_kernel(TreeAttentionArgs a, SharePlan plan, float* part_out,
                                                                                                  Part* parts) {
     constexpr int kSteps = kDim / 32;                            // products of K Q^T along the head
     constexpr int kTerms = kF32 ? (kBf16 ? 3 : 2) : 1;           // of a query value or a weight: 24 bits of three bf16, 22 of two f16
@@ -944,6 +943,11 @@ struct Shape {
     int rows_a_tile() const { return 16 * sixteens * waves; }
 };
 
+// Sixteens of rows that a wavefront has where there are many: two where its registers leave room for another wavefront on the SIMD.
+// Heads of 128, f32 on f16, one and two: 8 requests of 64 tokens on 300 keys 19.3 and 28.9 us, on 4000 keys 99 and 126, 512 tokens
+// on 2000 keys 72 and 100; on bf16 20.6 and 32.5, 114 and 142, 81 and 111.
+constexpr int most_sixteens(int dim, bool f32) { return dim == 256 || (dim == 128 && f32) ? 1 : 2; }
+
 constexpr uint32_t kMostEvened = 1024;  // requests: every wavefront reads their lengths, 64 at a time
 
 Shape shape_of(const TreeAttentionArgs& a, int compute_units) {
@@ -951,13 +955,8 @@ Shape shape_of(const TreeAttentionArgs& a, int compute_units) {
     s.compute_units = compute_units;
     s.dim = a.cache.head_dim <= 64 ? 64 : a.cache.head_dim <= 128 ? 128 : 256;
     const uint64_t rows = static_cast<uint64_t>(a.max_query_len) * a.group;
-    if (s.dim == 256) {  // (two sixteens of rows would not fit the registers)
-        s.sixteens = 1;
-        s.waves = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    } else {
-        s.sixteens = rows <= 64 ? 1 : 2;
-        s.waves = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    }
+    s.sixteens = rows <= 64 ? 1 : most_sixteens(s.dim, a.f32);
+    s.waves = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     // One workgroup for all keys of a key head where a second launch would take longer than its tiles, one after the other: the more
     // such workgroups, the longer (8 key heads of 128, bf16, uniform lengths; in parts / gathered): 1 request of 1 token on 500 keys
     // 10.0 / 8.6 us, on 1000 10.4 / 13.2; 8 requests on 700 keys 13.3 / 12.0, on 1500 16.2 / 19.7; 32 requests on 700 keys 22.1 / 18.4,
@@ -977,12 +976,13 @@ Shape shape_of(const TreeAttentionArgs& a, int compute_units) {
     // One round of what the compute units hold at once (by LDS and registers; lone wavefronts four, not the five whose LDS would be
     // all there is: 16 requests of 1 token on 8000 keys 107 us with four, 120 with five), the workgroups that rounding adds among
     // them; a batch that fills much of that anyway shares out over half a round more, three quarters for lone wavefronts (64
-    // requests of 1 token on 100 to 4000 keys: 112 us with three quarters, 121 with half).  Workgroups of 128 rows, which the units
-    // are slow on, fill the round exactly: 8 requests of 64 tokens on 8000 keys 103 us, with what surely fits 116.  Fewer rows wait for
-    // memory, and parts cost more than idle units do: 24 requests of 16 tokens on 8000 keys 175 us filled, 172 not.
+    // requests of 1 token on 100 to 4000 keys: 112 us with three quarters, 121 with half).  Workgroups of 128 rows, and of 64 f32
+    // rows of heads of 128 where there are more, which the units are slow on, fill the round exactly: 8 requests of 64 tokens on 8000 keys
+    // 103 us, with what surely fits 116 (f32 on f16 174 and 237).  Fewer rows wait for memory, and parts cost more than idle units
+    // do: 24 requests of 16 tokens on 8000 keys 175 us filled, 172 not.
     const uint64_t resident = static_cast<uint64_t>(compute_units) * (s.waves == 1 ? 4 : s.waves == 2 ? 3 : 2);
     const uint64_t fewest = s.waves == 1 ? resident * 3 / 4 : resident / 2;
-    s.plan.one_round = s.sixteens == 2 && base <= resident;
+    s.plan.one_round = (s.sixteens == 2 || (a.f32 && s.dim == 128 && rows > 64)) && base <= resident;
     uint64_t target = resident > base ? resident - base : 0;
     if (target < fewest && !s.plan.one_round) target = fewest;
     s.plan.target = static_cast<uint32_t>(target);
@@ -1052,8 +1052,8 @@ hipError_t attend_rows(hipStream_t stream, const TreeAttentionArgs& a, const Sha
     if (s.waves == 1) return attend<kDim, kBf16, kF32, 1, 1, 1, kAlone>(stream, a, s, workspace);
     if (s.waves == 2) return attend<kDim, kBf16, kF32, 1, 2, 1, kTwo>(stream, a, s, workspace);
     if (s.sixteens == 1) return attend<kDim, kBf16, kF32, 1, 4, 1, kTwo>(stream, a, s, workspace);
-    if constexpr (kDim < 256) return attend<kDim, kBf16, kF32, 2, 4, 1, 4>(stream, a, s, workspace);
-    else return hipErrorInvalidValue;  // (heads of 256 have one sixteen)
+    if constexpr (most_sixteens(kDim, kF32) == 2) return attend<kDim, kBf16, kF32, 2, 4, 1, 4>(stream, a, s, workspace);
+    else return hipErrorInvalidValue;  // (one sixteen always)
 }
 
 template <int kDim>
