@@ -23,8 +23,8 @@
 //
 // What bounds it, on heads of 128, 32 of them on 8 key heads, 5.15 TB/s being what a copy reaches.  Few rows: the cache's bytes.
 // 64 requests of 1 token on 4000 keys 185 us (5.7 TB/s), on 1000 keys 53 us (4.9); 2 requests of 7 to 13 tokens x 28 heads on 107000
-// and 119000 keys 110 us (4.2 TB/s).  Many rows: the issue of a tile, 32 matrix instructions and 138 others (16 exponentials among
-// them) a wavefront with 32 rows, of which two fit a SIMD: 8 requests of 64 tokens on 8000 keys 103 us, 660 TFLOP/s.  Short
+// and 119000 keys 110 us (4.2 TB/s).  Many rows: the issue of a tile, 32 matrix instructions and 142 others (16 exponentials among
+// them) a wavefront with 32 rows, of which two fit a SIMD: 8 requests of 64 tokens on 8000 keys 107 us, 630 TFLOP/s.  Short
 // contexts: the round trips to memory before the first tile (lengths, block table, keys), and a tile's own latency, 0.85 us: 8
 // requests of 64 tokens on 20 keys (3 tiles) 11.9 us, on 190 keys (8 tiles) 16.3.
 #include "paged_launch.h"

@@ -292,7 +292,7 @@ __global__ __launch_bounds__(kWaves * 64) void linear_fp8_rows_kernel(Fp8Matmul 
 // kRowWaves x kColWaves wavefronts with 32 kR rows x 64 columns each, a block of K at a time from a ring of kStages in LDS that all
 // of them fill and read.  Every wavefront widens its own operands: of a block's instructions about half are conversions, which
 // run beside another wavefront's products.  128 x 128 with a ring of two is two workgroups a compute unit (66 KiB of LDS and 210
-// registers each), whose barriers, waits and last stores fall into the other's products: 2048 x 4096 x 14336 247 us (970 TFLOP/s), a
+// registers each), whose barriers, waits and last stores fall into the other's products: 2048 x 4096 x 14336 248 us (970 TFLOP/s), a
 // ring of three and one workgroup 310 us, 256 x 128 and a ring of three 278 us; a library's f16 product of that size takes 212 us.
 // What is left is the matrix instructions' own time at the clock that they are given on dense data and the conversions' issue.
 // 64 x 128 with a ring of three fills the units where there are few rows, and has the registers for all of a block's pieces at once
