@@ -153,7 +153,7 @@ def treeAttention(cache: _lib.PagedCache, out, query, query_starts, context_lens
     o_token, o_head = _rows_of_heads(out, tokens, heads, cache.head_dim)
     words = 0
     if masks is not None:
-        if len(masks.shape) != 2 or masks.shape[0] != tokens:
+        if len(masks.shape) != 2 or masks.shape[0] != tokens or masks.shape[1] == 0:  # (no words have no address, as no masks have)
             raise _bad_shape()
         words = masks.shape[1]
     if out.dtype != query.dtype:

@@ -1,7 +1,7 @@
 """Calls whose grids a launch cannot have (2^32 threads and more) are refused as such, before any launch (CPU only)."""
 import pytest
 
-from antfly_amd import _lib, kernels
+from antfly_amd import _lib, kernels, paged
 from antfly_amd._lib import Buffer
 from tests.test_operator_checks import BIG, a_cache, attention, fp8, fp8_codes
 
@@ -38,3 +38,17 @@ def test_fp8_products():
             call(rows=(1 << 20) - 16, in_dim=16, out_dim=1 << 18)
     with pytest.raises(_lib.HipOpUnsupported):  # the quantizer's
         fp8(rows=(1 << 20) - 16, in_dim=(1 << 16) + 16, out_dim=16, x=Buffer(0x1000, 1 << 44), workspace=Buffer(0x1000, 1 << 44))
+
+
+def some_arrays():
+    torch = pytest.importorskip("torch")
+    k, q = torch.zeros(4, 16, 2, 64, dtype=torch.float16), torch.zeros(5, 4, 64)
+    lens, table = torch.zeros(3, dtype=torch.int32), torch.zeros(2, 3, dtype=torch.int32)
+    return torch, k, q, lens, table
+
+
+def test_masks_of_no_words():
+    """They have no address: the call would have read none as the causal mask."""
+    torch, k, q, lens, table = some_arrays()
+    with pytest.raises(_lib.InvalidShape):
+        paged.treeAttention(paged.cache(k, k), q, q, lens, lens[:2], table, 4, 40, masks=torch.zeros(5, 0, dtype=torch.int64))
