@@ -25,6 +25,11 @@ def _bad_shape():
     return _lib.InvalidShape(_lib.ERR_INVALID_SHAPE)
 
 
+def _bad_number():
+    """Of a number below zero, or none that is whole: what the C ABI answers to one that is too large."""
+    return _lib.InvalidHipState(_lib.ERR_INVALID_STATE)
+
+
 _names = {}  # of the types that have been seen
 
 
@@ -116,10 +121,13 @@ def launchBatchPlan(stream, context_lens, query_lens, block_tables, free_blocks,
         words = masks.shape[1]
     if positions.shape[0] != tokens or (parents is not None and parents.shape[0] != tokens):
         raise _bad_shape()
-    plan = _lib.BatchPlan.from_buffer_copy(_PLAN.pack(
-        requests, columns, block_size, blocks, tokens, words, *_i32(context_lens), *_i32(query_lens), *_i32(free_blocks),
-        *_optional(parents), *_i32(block_tables), *_i32(query_starts), *_i32(slots), *_i32(positions), *_optional(masks, _U64),
-        *_i32(blocks_taken)))
+    try:
+        plan = _lib.BatchPlan.from_buffer_copy(_PLAN.pack(
+            requests, columns, block_size, blocks, tokens, words, *_i32(context_lens), *_i32(query_lens), *_i32(free_blocks),
+            *_optional(parents), *_i32(block_tables), *_i32(query_starts), *_i32(slots), *_i32(positions), *_optional(masks, _U64),
+            *_i32(blocks_taken)))
+    except struct.error:
+        raise _bad_number() from None
     check(_lib.lib().afhip_launch_batch_plan(stream, plan))
 
 
@@ -158,10 +166,13 @@ def treeAttention(cache: _lib.PagedCache, out, query, query_starts, context_lens
         words = masks.shape[1]
     if out.dtype != query.dtype:
         raise _bad_shape()
-    made = _lib.TreeAttention.from_buffer_copy(bytes(cache) + _REST.pack(
-        _type(query), dim ** -0.5 if scale is None else scale, requests, tokens, heads, max_query_len, max_key_len, columns, words,
-        q_token, q_head, o_token, o_head, query.data_ptr(), _bytes(query), out.data_ptr(), _bytes(out), *_i32(query_starts),
-        *_i32(context_lens), *_i32(block_tables), *_optional(masks, _U64)))
+    try:
+        made = _lib.TreeAttention.from_buffer_copy(bytes(cache) + _REST.pack(
+            _type(query), dim ** -0.5 if scale is None else scale, requests, tokens, heads, max_query_len, max_key_len, columns, words,
+            q_token, q_head, o_token, o_head, query.data_ptr(), _bytes(query), out.data_ptr(), _bytes(out), *_i32(query_starts),
+            *_i32(context_lens), *_i32(block_tables), *_optional(masks, _U64)))
+    except struct.error:
+        raise _bad_number() from None
     made.arrays = (cache, out, query, query_starts, context_lens, block_tables, masks)
     return made
 

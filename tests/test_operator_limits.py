@@ -52,3 +52,15 @@ def test_masks_of_no_words():
     torch, k, q, lens, table = some_arrays()
     with pytest.raises(_lib.InvalidShape):
         paged.treeAttention(paged.cache(k, k), q, q, lens, lens[:2], table, 4, 40, masks=torch.zeros(5, 0, dtype=torch.int64))
+
+
+def test_numbers_below_zero():
+    """Refused as they are by the launchers that pass them on."""
+    torch, k, q, lens, table = some_arrays()
+    for most in ((-1, 40), (4, -40), (4, 40.5)):
+        with pytest.raises(_lib.InvalidHipState):
+            paged.treeAttention(paged.cache(k, k), q, q, lens, lens[:2], table, *most)
+    for change in ({"block_size": -16}, {"blocks": -1}):
+        with pytest.raises(_lib.InvalidHipState):
+            paged.launchBatchPlan(None, lens[:2], lens[:2], table, lens, query_starts=lens, slots=lens, positions=lens, blocks_taken=lens[:1],
+                                  **dict({"block_size": 16}, **change))
