@@ -454,7 +454,8 @@ afhip_status afhip_launch_cache_move(void *stream, const afhip_paged_cache *cach
  *
  *   out[t][h] = sum over seen j of  softmax_j(scale * q[t][h] . k[j]) v[j],   zero where nothing is seen
  *
- * What is not seen does not count, whatever it holds (an infinity or no number included).  query and out: F32, or the
+ * What is not seen does not count, whatever it holds (an infinity or no number included).  A seen score of minus infinity is a weight
+ * of zero, a row that has no other no number.  query and out: F32, or the
  * cache's own type; [tokens][heads][head_dim] with strides in elements (multiples of 4 for F32, of 8 otherwise; 16-byte
  * aligned).  F32 queries and the softmax's weights beside them are multiplied as three terms of bf16 or two of f16, whichever
  * the cache holds (24 and 22 bits); with 16-bit queries the weights are rounded to the cache's type.  On an f16 cache a weight is
