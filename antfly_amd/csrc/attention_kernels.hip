@@ -16,7 +16,7 @@
 //
 // Keys and values come in tiles of 32 keys from memory straight into a ring of tiles in LDS (no registers in between),
 // requested kStages - 1 tiles ahead, their places found a tile before that.  The wavefronts of a workgroup share its tiles and
-// have 16 kQ rows each: a lone wavefront (no barrier anywhere) up to 16 rows, four of them, and every key read once, for 128.
+// have 16 kQ rows each: a lone wavefront (no barrier anywhere) up to 16 rows, four of them, and every key read once, for 64 or 128.
 // Long contexts are shared out over workgroups by the lengths that the device holds, so that ragged requests keep all of them
 // busy to the end, and a second kernel joins the parts.  Short ones stay with one workgroup a key head: it has kKeyGroups such
 // groups of wavefronts that take tiles in turn, and adds them up itself.
