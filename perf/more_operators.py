@@ -6,7 +6,7 @@ A case is a dict of plain values:
                     and the values go straight into an e4m3 or 16-bit paged cache, otherwise both come back as arrays
   kind "cache"      new keys and values quantized into the slots of their tokens, then `read` tokens of the request read back
   kind "attention"  every request's new tokens over its quantized cache: scores capped by a tanh, biased by distance, in a window
-  kind "sample"     a token of every row of logits by temperature, top-k, top-p and min-p from a given random number
+  kind "sample"     a token of every row of logits by temperature, top-k, top-p and min-p from a given random number, likely ones first
 
 The lengths of a case's requests follow from the case alone, so that its work is known; everything else is made from the seed.
 """
@@ -487,11 +487,10 @@ def _plain_sample(state):
     kept = (before < state["p"].double()[:, None] * total) | (state["p"] >= 1.0)[:, None]
     kept = kept & (weights >= state["m"].double()[:, None]) | (rank == 0)
     weights = torch.where(kept, weights, 0.0)
-    placed = torch.zeros_like(weights).scatter_(1, order, weights)
-    sums = torch.cumsum(placed, -1)
-    target = state["u"].double()[:, None] * sums[:, -1:]
-    token = torch.searchsorted(sums, target, right=True).clamp_max(vocab - 1)
-    return [token[:, 0].int(), (placed.gather(1, token) / sums[:, -1:])[:, 0].float()]
+    sums = torch.cumsum(weights, -1)
+    total = sums[:, -1:].contiguous()
+    place = torch.searchsorted(sums, state["u"].double()[:, None] * total, right=True).clamp_max(vocab - 1)
+    return [order.gather(1, place)[:, 0].int(), (weights.gather(1, place) / total)[:, 0].float()]
 
 
 # ---- from the definitions, in 64 bits ----------------------------------------------------------------------------------
@@ -616,8 +615,6 @@ def _exact_sample(state):
             sums = np.cumsum(weights)
             count = 1 + int(np.sum(sums[:-1] < np.float64(p[r]) * sums[-1]))
         count = max(1, min(count, int(np.sum(weights >= np.float64(m[r])))))
-        order, weights = order[:count], weights[:count]
-        by_index = np.argsort(order)
-        sums = np.cumsum(weights[by_index])
-        made.append(weights[by_index][min(count - 1, np.searchsorted(sums, np.float64(u[r]) * sums[-1], side="right"))] / sums[-1])
+        sums = np.cumsum(weights[:count])
+        made.append(weights[min(count - 1, np.searchsorted(sums, np.float64(u[r]) * sums[-1], side="right"))] / sums[-1])
     return [None, torch.tensor(made, dtype=torch.float64)]
