@@ -33,6 +33,7 @@ ERR_IO = -18
 
 TYPE_F32, TYPE_Q4_0, TYPE_Q8_0, TYPE_Q4_K = 0, 2, 8, 12
 TYPE_F16, TYPE_BF16 = 1, 30  # of a paged cache and what is attended with it
+TYPE_I8, TYPE_E4M3 = 24, 256  # of a quantized cache
 ACTIVATION_NONE, ACTIVATION_RELU, ACTIVATION_QUICK_GELU, ACTIVATION_GELU = 0, 1, 2, 3
 LAYOUT_RAW, LAYOUT_PREPARED = 0, 1
 # a launcher's `dispatch` besides a kind (0 .. 3): choose by rows; ... and keep Q4_K on f32 activations everywhere
@@ -94,6 +95,35 @@ class TreeAttention(C.Structure):
                                            "mask_words", "query_token_stride", "query_head_stride", "out_token_stride",
                                            "out_head_stride")] +
                 [(n, Buffer) for n in ("query", "out", "query_starts", "context_lens", "block_tables", "masks")])
+
+
+class QuantizedCache(C.Structure):
+    """afhip_quantized_cache: blocks of slots of 8-bit keys and values with an f32 scale a head (strides in elements)."""
+
+    _fields_ = ([(n, Buffer) for n in ("keys", "values", "key_scales", "value_scales")] + [("type", C.c_int)] +
+                [(n, C.c_size_t) for n in ("blocks", "block_size", "kv_heads", "head_dim", "block_stride", "slot_stride", "head_stride",
+                                           "scale_block_stride", "scale_slot_stride", "scale_head_stride")])
+
+
+class HeadRotation(C.Structure):
+    _fields_ = ([("type", C.c_int), ("out_type", C.c_int), ("interleaved", C.c_int), ("epsilon", C.c_float)] +
+                [(n, C.c_size_t) for n in ("tokens", "heads", "kv_heads", "head_dim", "rotary_dim", "axes", "query_token_stride",
+                                           "query_head_stride", "key_token_stride", "key_head_stride", "out_query_token_stride",
+                                           "out_query_head_stride", "out_key_token_stride", "out_key_head_stride")] +
+                [(n, Buffer) for n in ("query", "key", "out_query", "out_key", "positions", "frequencies", "query_weight", "key_weight")] +
+                [("pair_axes", C.c_ubyte * 128)])
+
+
+class QuantizedAttention(C.Structure):
+    _fields_ = ([("cache", QuantizedCache), ("type", C.c_int), ("scale", C.c_float), ("softcap", C.c_float)] +
+                [(n, C.c_size_t) for n in ("window", "requests", "tokens", "heads", "max_query_len", "max_key_len", "table_columns",
+                                           "query_token_stride", "query_head_stride", "out_token_stride", "out_head_stride")] +
+                [(n, Buffer) for n in ("query", "out", "query_starts", "context_lens", "block_tables", "slopes")])
+
+
+class Sample(C.Structure):
+    _fields_ = ([("type", C.c_int)] + [(n, C.c_size_t) for n in ("rows", "vocab", "row_stride")] +
+                [(n, Buffer) for n in ("logits", "temperatures", "top_k", "top_p", "min_p", "uniforms", "tokens", "probabilities")])
 
 
 class DebugStats(C.Structure):
@@ -178,6 +208,14 @@ SIGNATURES = {
     "afhip_launch_cache_move": (_st, [_vp, C.POINTER(PagedCache), Buffer, _sz, Buffer, Buffer, Buffer, _sz, _sz]),
     "afhip_tree_attention_workspace_bytes": (_sz, [C.POINTER(TreeAttention)]),
     "afhip_launch_tree_attention": (_st, [_vp, C.POINTER(TreeAttention), Buffer]),
+    "afhip_launch_quantized_store": (_st, [_vp, C.POINTER(QuantizedCache), _i, Buffer, Buffer, _sz, _sz, Buffer, _sz]),
+    "afhip_launch_quantized_load": (_st, [_vp, C.POINTER(QuantizedCache), _i, Buffer, Buffer, _sz, _sz, Buffer, _sz]),
+    "afhip_launch_head_rotation": (_st, [_vp, C.POINTER(HeadRotation)]),
+    "afhip_launch_rotated_store": (_st, [_vp, C.POINTER(HeadRotation), C.POINTER(PagedCache), C.POINTER(QuantizedCache), Buffer, _sz, _sz, Buffer]),
+    "afhip_quantized_attention_workspace_bytes": (_sz, [C.POINTER(QuantizedAttention)]),
+    "afhip_launch_quantized_attention": (_st, [_vp, C.POINTER(QuantizedAttention), Buffer]),
+    "afhip_sample_workspace_bytes": (_sz, [C.POINTER(Sample)]),
+    "afhip_launch_sample": (_st, [_vp, C.POINTER(Sample), Buffer]),
     "afhip_compute_create": (_st, [C.POINTER(_vp)]),
     "afhip_compute_destroy": (None, [_vp]),
     "afhip_compute_backend_kind": (_i, [_vp]),

@@ -1,5 +1,6 @@
 """A paged key / value cache and what a speculative decode step does with it: plan the batch, store the drafted tokens' keys
-and values, attend over context and draft tree, move the accepted path behind the context.
+and values, attend over context and draft tree, move the accepted path behind the context.  And the same cache in 8 bits: heads of
+a projection normed, rotated and stored, stored as they are, read back, attended.
 
 The functions take device arrays: anything with torch's `data_ptr()`, `shape`, `stride()`, `dtype`, `numel()` and
 `element_size()` (this package does not import torch).  Layouts, and what each launch reads and writes, are those of the C
@@ -17,8 +18,12 @@ _TYPES = {"torch.float32": _lib.TYPE_F32, "torch.float16": _lib.TYPE_F16, "torch
 # A decode step makes these calls for every layer: arguments go into the C structs as one packed string of numbers, which
 # takes a fifth of the time that filling their fields does.
 _CACHE, _PLAN, _REST = struct.Struct("4Qi4x7Q"), struct.Struct("26Q"), struct.Struct("if23Q")  # _REST: TreeAttention behind its cache
+_CODES, _ROTATION, _QUANTIZED_REST = struct.Struct("8Qi4x10Q"), struct.Struct("3if30Q128s"), struct.Struct("i2f4x23Q")
 assert _CACHE.size == C.sizeof(_lib.PagedCache) and _PLAN.size == C.sizeof(_lib.BatchPlan)
 assert _CACHE.size + _REST.size == C.sizeof(_lib.TreeAttention)
+assert _CODES.size == C.sizeof(_lib.QuantizedCache) and _ROTATION.size == C.sizeof(_lib.HeadRotation)
+assert _CODES.size + _QUANTIZED_REST.size == C.sizeof(_lib.QuantizedAttention)
+_CODE_TYPES = {"torch.int8": _lib.TYPE_I8, "torch.float8_e4m3fn": _lib.TYPE_E4M3}
 
 
 def _bad_shape():
@@ -185,3 +190,144 @@ def launchTreeAttention(stream, attention: _lib.TreeAttention, workspace: Buffer
     """`workspace`: a Buffer, or an array, of at least treeAttentionWorkspaceBytes(attention) bytes."""
     check(_lib.lib().afhip_launch_tree_attention(stream, attention,
                                                  workspace if isinstance(workspace, Buffer) else buffer(workspace)))
+
+
+# ---- 8-bit caches -----------------------------------------------------------------------------------------------------
+
+def quantizedCache(keys, values, key_scales, value_scales, heads_outside: bool = False) -> _lib.QuantizedCache:
+    """keys, values int8 or float8_e4m3fn [blocks, block size, kv heads, head dim] and their scales f32 [blocks, block size, kv
+    heads]; with heads_outside [blocks, kv heads, block size(, head dim)]."""
+    shape, strides, scale_strides = keys.shape, keys.stride(), key_scales.stride()
+    if len(shape) != 4 or values.shape != shape or keys.dtype != values.dtype or (values.stride() != strides and not _same_strides(keys, values)) or \
+            (shape[3] > 1 and strides[3] != 1) or key_scales.shape != shape[:3] or value_scales.shape != shape[:3] or \
+            (value_scales.stride() != scale_strides and not _same_strides(key_scales, value_scales)) or \
+            _name(key_scales.dtype) != "torch.float32" or _name(value_scales.dtype) != "torch.float32":
+        raise _bad_shape()
+    slot, head = (2, 1) if heads_outside else (1, 2)
+    made = _lib.QuantizedCache.from_buffer_copy(_CODES.pack(
+        keys.data_ptr(), _bytes(keys), values.data_ptr(), _bytes(values), key_scales.data_ptr(), _bytes(key_scales), value_scales.data_ptr(),
+        _bytes(value_scales), _CODE_TYPES.get(_name(keys.dtype), -1), shape[0], shape[slot], shape[head], shape[3], strides[0], strides[slot],
+        strides[head], scale_strides[0], scale_strides[slot], scale_strides[head]))
+    made.arrays = (keys, values, key_scales, value_scales)  # alive as long as the description of them is
+    return made
+
+
+def _token_rows(cache, keys, values, slots):
+    """What a store or a load of tokens [tokens, kv heads, head dim] passes on behind the cache."""
+    shape, strides, dtype = keys.shape, keys.stride(), keys.dtype
+    if values.shape != shape or values.dtype != dtype or (values.stride() != strides and not _same_strides(keys, values)) or \
+            shape != (slots.shape[0], cache.kv_heads, cache.head_dim) or (shape[2] > 1 and strides[2] != 1):
+        raise _bad_shape()
+    return _TYPES.get(_name(dtype), -1), buffer(keys), buffer(values), strides[0], strides[1], _i32_buffer(slots), shape[0]
+
+
+def launchQuantizedStore(stream, cache: _lib.QuantizedCache, keys, values, slots) -> None:
+    """keys, values [tokens, kv heads, head dim] (f32, f16 or bf16) quantized into the cache's slots."""
+    check(_lib.lib().afhip_launch_quantized_store(stream, cache, *_token_rows(cache, keys, values, slots)))
+
+
+def launchQuantizedLoad(stream, cache: _lib.QuantizedCache, keys, values, slots) -> None:
+    """The slots' keys and values read back into keys, values [tokens, kv heads, head dim] (f32, f16 or bf16)."""
+    check(_lib.lib().afhip_launch_quantized_load(stream, cache, *_token_rows(cache, keys, values, slots)))
+
+
+_ONE_AXIS = bytes(128)
+
+
+def _weight(array, dim):
+    """(address, bytes) of a head's weights, f32 [dim]; None: no norm."""
+    if array is None:
+        return 0, 0
+    if _name(array.dtype) != "torch.float32" or array.shape != (dim,) or not array.is_contiguous():
+        raise _bad_shape()
+    return array.data_ptr(), array.nbytes
+
+
+def headRotation(query, key, out_query, out_key, positions, frequencies, query_weight=None, key_weight=None, epsilon: float = 1e-6,
+                 interleaved: bool = False, pair_axes=None) -> _lib.HeadRotation:
+    """The norm and rotation of query [tokens, heads, head dim] (or None) and key [tokens, kv heads, head dim] into out_query and
+    out_key (None for launchRotatedStore), which may be query and key themselves.  positions int32 [tokens] or [axes, tokens],
+    frequencies f32 [pairs]: twice as many dimensions turn.  pair_axes: the axis of every pair (all 0 unless given)."""
+    tokens, kv_heads, dim = key.shape
+    heads = 0 if query is None else query.shape[1]
+    k = _rows_of_heads(key, tokens, kv_heads, dim)
+    q = o = ok = (0, 0)
+    if query is not None:
+        q, o = _rows_of_heads(query, tokens, heads, dim), _rows_of_heads(out_query, tokens, heads, dim)
+        if query.dtype != key.dtype or (out_key is not None and out_key.dtype != out_query.dtype):
+            raise _bad_shape()
+    if out_key is not None:
+        ok = _rows_of_heads(out_key, tokens, kv_heads, dim)
+    out_type = _type(out_query if query is not None else key if out_key is None else out_key)
+    pairs, place = frequencies.shape[0], positions.shape
+    if len(frequencies.shape) != 1 or _name(frequencies.dtype) != "torch.float32" or not frequencies.is_contiguous() or pairs > 128 or \
+            place[-1] != tokens or len(place) > 2:
+        raise _bad_shape()
+    axes = place[0] if len(place) == 2 else 1
+    if pair_axes is None:
+        packed = _ONE_AXIS
+    else:
+        try:
+            packed = bytes(pair_axes)
+        except (TypeError, ValueError):
+            raise _bad_number() from None
+        if len(packed) != pairs:
+            raise _bad_shape()
+    try:
+        made = _lib.HeadRotation.from_buffer_copy(_ROTATION.pack(
+            _type(key), out_type, 1 if interleaved else 0, epsilon, tokens, heads, kv_heads, dim, 2 * pairs, axes, *q, *k, *o, *ok,
+            *((query.data_ptr(), _bytes(query)) if query is not None else (0, 0)), key.data_ptr(), _bytes(key),
+            *((out_query.data_ptr(), _bytes(out_query)) if query is not None else (0, 0)),
+            *((out_key.data_ptr(), _bytes(out_key)) if out_key is not None else (0, 0)), *_i32(positions), frequencies.data_ptr(),
+            frequencies.nbytes, *_weight(query_weight, dim), *_weight(key_weight, dim), packed))
+    except struct.error:
+        raise _bad_number() from None
+    made.arrays = (query, key, out_query, out_key, positions, frequencies, query_weight, key_weight)
+    return made
+
+
+def launchHeadRotation(stream, rotation: _lib.HeadRotation) -> None:
+    check(_lib.lib().afhip_launch_head_rotation(stream, rotation))
+
+
+def launchRotatedStore(stream, rotation: _lib.HeadRotation, cache, values, slots) -> None:
+    """The rotation's queries into out_query, its keys and `values` [tokens, kv heads, head dim] into the slots of `cache` (a
+    PagedCache or a QuantizedCache)."""
+    tokens, kv_heads, dim = values.shape
+    if _type(values) != rotation.type or slots.shape[0] != tokens or (tokens, kv_heads, dim) != (rotation.tokens, rotation.kv_heads, rotation.head_dim):
+        raise _bad_shape()
+    v_token, v_head = _rows_of_heads(values, tokens, kv_heads, dim)
+    quantized = isinstance(cache, _lib.QuantizedCache)
+    check(_lib.lib().afhip_launch_rotated_store(stream, rotation, None if quantized else cache, cache if quantized else None, buffer(values),
+                                                v_token, v_head, _i32_buffer(slots)))
+
+
+def quantizedAttention(cache: _lib.QuantizedCache, out, query, query_starts, context_lens, block_tables, max_query_len: int, max_key_len: int,
+                       scale: float = None, softcap: float = 0.0, window: int = 0, slopes=None) -> _lib.QuantizedAttention:
+    """The arguments of a call (of any number of calls while the arrays stay): query, out [tokens, heads, head dim]; scale:
+    head_dim ** -0.5 unless given; softcap 0: scores as they are; window 0: all earlier keys; slopes f32 [heads]."""
+    tokens, heads, dim = query.shape
+    requests, columns = block_tables.shape
+    q_token, q_head = _rows_of_heads(query, tokens, heads, cache.head_dim)
+    o_token, o_head = _rows_of_heads(out, tokens, heads, cache.head_dim)
+    if out.dtype != query.dtype:
+        raise _bad_shape()
+    try:
+        made = _lib.QuantizedAttention.from_buffer_copy(bytes(cache) + _QUANTIZED_REST.pack(
+            _type(query), dim ** -0.5 if scale is None else scale, softcap, window, requests, tokens, heads, max_query_len, max_key_len,
+            columns, q_token, q_head, o_token, o_head, query.data_ptr(), _bytes(query), out.data_ptr(), _bytes(out), *_i32(query_starts),
+            *_i32(context_lens), *_i32(block_tables), *_weight(slopes, heads)))
+    except struct.error:
+        raise _bad_number() from None
+    made.arrays = (cache, out, query, query_starts, context_lens, block_tables, slopes)
+    return made
+
+
+def quantizedAttentionWorkspaceBytes(attention: _lib.QuantizedAttention) -> int:
+    return _lib.lib().afhip_quantized_attention_workspace_bytes(attention)
+
+
+def launchQuantizedAttention(stream, attention: _lib.QuantizedAttention, workspace: Buffer = NO_BUFFER) -> None:
+    """`workspace`: a Buffer, or an array, of at least quantizedAttentionWorkspaceBytes(attention) bytes."""
+    check(_lib.lib().afhip_launch_quantized_attention(stream, attention,
+                                                      workspace if isinstance(workspace, Buffer) else buffer(workspace)))

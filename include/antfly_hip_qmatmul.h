@@ -61,6 +61,8 @@ const char *afhip_status_string(afhip_status status);
 enum afhip_tensor_type { AFHIP_TYPE_F32 = 0, AFHIP_TYPE_Q4_0 = 2, AFHIP_TYPE_Q8_0 = 8, AFHIP_TYPE_Q4_K = 12 };
 /* Two more ids of the same table, for the paged key / value cache and what is attended with it; no linear op takes them. */
 enum afhip_half_type { AFHIP_TYPE_F16 = 1, AFHIP_TYPE_BF16 = 30 };
+/* The 8-bit types of a quantized cache: whole numbers, and floating point of 4 exponent and 3 mantissa bits (no id of the table). */
+enum afhip_code_type { AFHIP_TYPE_I8 = 24, AFHIP_TYPE_E4M3 = 256 };
 /* Q4_K (144-byte super-blocks of 256 weights) is computed on f32 activations against the
  * dequantized weights, as the engine does on the CPU (ops/native_compute.zig:31075-31144)
  * and in its CUDA backend (ops/cuda/cuda_compute.zig:708) -- except on the CPU engine's gated
@@ -479,6 +481,125 @@ typedef struct afhip_tree_attention {
 } afhip_tree_attention;
 size_t afhip_tree_attention_workspace_bytes(const afhip_tree_attention *attention);
 afhip_status afhip_launch_tree_attention(void *stream, const afhip_tree_attention *attention, afhip_buffer workspace);
+
+/* ------------------------------------------------------------------------
+ * A sampled serving step on an 8-bit paged cache: queries and keys of a projection normed and rotated, keys and values quantized
+ * into the cache, attention over it, and a token drawn from the logits.  Like the calls above these take device buffers, never
+ * wait and allocate nothing.  No counterpart in the reference's backend interface.
+ *
+ * The quantized cache has the blocks, slots and block tables of afhip_paged_cache.  A key (value) of one head is head_dim codes of
+ * one byte and one f32 scale: value d is code d times the scale.  Codes lie at [b * block_stride + s * slot_stride +
+ * h * head_stride + d], scales at [b * scale_block_stride + s * scale_slot_stride + h * scale_head_stride] (strides in elements).
+ * type: AFHIP_TYPE_I8 or AFHIP_TYPE_E4M3 (else AFHIP_ERR_UNSUPPORTED_TENSOR_TYPE).  head_dim and the code strides are multiples of 16,
+ * codes 16-byte and scales 4-byte aligned; blocks * block_size < 2^31, codes span less than 64 GiB and scales fewer than 2^32
+ * elements (else AFHIP_ERR_INVALID_STATE); head_dim <= 256 (else AFHIP_ERR_OP_UNSUPPORTED).
+ * ---------------------------------------------------------------------- */
+typedef struct afhip_quantized_cache {
+    afhip_buffer keys, values, key_scales, value_scales;
+    int type;
+    size_t blocks, block_size, kv_heads, head_dim;
+    size_t block_stride, slot_stride, head_stride;
+    size_t scale_block_stride, scale_slot_stride, scale_head_stride;
+} afhip_quantized_cache;
+
+/* Keys and values of `tokens` new tokens into their slots, as afhip_launch_cache_store takes them.  With m the largest |x| of a
+ * head's vector, at least 2^-100, and L = 127 (I8) or 448 (E4M3): scale = m / L and code = x * (L / m) to nearest, ties to even, in
+ * f32 operations.  A vector that holds an infinity or no number gets a scale that is no number and codes of zero: all of it
+ * reads back as no numbers.  Grids of 2^32 threads and more (2^24 tokens of 32 heads of 128 in all, keys and values, or more of
+ * fewer): AFHIP_ERR_OP_UNSUPPORTED. */
+afhip_status afhip_launch_quantized_store(void *stream, const afhip_quantized_cache *cache, int type, afhip_buffer keys,
+                                          afhip_buffer values, size_t token_stride, size_t head_stride, afhip_buffer slots,
+                                          size_t tokens);
+/* The other way: the slots' keys and values as F32, F16 or BF16 [tokens][kv_heads][head_dim] (code * scale in f32, rounded once).
+ * A token whose slot is outside the cache is left as it was.  Any slot may be named any number of times.  Grids of 2^32 threads and
+ * more (8, 16 or 32 for a head of up to 64, 128 or 256, of a token's keys and its values): AFHIP_ERR_OP_UNSUPPORTED. */
+afhip_status afhip_launch_quantized_load(void *stream, const afhip_quantized_cache *cache, int type, afhip_buffer keys,
+                                         afhip_buffer values, size_t token_stride, size_t head_stride, afhip_buffer slots,
+                                         size_t tokens);
+
+/* Queries [tokens][heads][head_dim] and keys [tokens][kv_heads][head_dim] of one projection, normed head by head and rotated:
+ *
+ *   y = x / sqrt(mean of x^2 over the head + epsilon) * weight         (query_weight and key_weight, f32 [head_dim]; .ptr == 0: y = x)
+ *   pair p < rotary_dim / 2 of y:  (a, b) -> (a cos t - b sin t, a sin t + b cos t),  t = position * frequencies[p]
+ *
+ * A pair is (y[p], y[p + rotary_dim / 2]), or with `interleaved` (y[2 p], y[2 p + 1]); dimensions from rotary_dim on stay.
+ * position is positions[pair_axes[p]][token], int32 [axes][tokens] (time, height and width of an image's tokens, or one axis: all
+ * pair_axes zero); the angle is formed and reduced in 64 bits, so that far positions keep f32's accuracy.
+ * type: of query and key; out_type: of the arrays that are written (F32, F16 or BF16 each; sums and products in f32, one
+ * rounding at the end).  head_dim a multiple of 8 up to 256, rotary_dim a multiple of 8 up to head_dim, 1 <= axes <= 16; strides
+ * in elements, multiples of 4, base addresses 16-byte (f32) or 8-byte aligned (else AFHIP_ERR_INVALID_STATE; head_dim > 256:
+ * AFHIP_ERR_OP_UNSUPPORTED, as are 2^24 tokens and 2^19 heads).  heads == 0: no queries.  out_query and out_key may be query and key themselves (the same buffer,
+ * strides and type); otherwise nothing that is written overlaps what is read. */
+typedef struct afhip_head_rotation {
+    int type, out_type, interleaved;
+    float epsilon;
+    size_t tokens, heads, kv_heads, head_dim, rotary_dim, axes;
+    size_t query_token_stride, query_head_stride, key_token_stride, key_head_stride;
+    size_t out_query_token_stride, out_query_head_stride, out_key_token_stride, out_key_head_stride;
+    afhip_buffer query, key, out_query, out_key, positions, frequencies, query_weight, key_weight;
+    unsigned char pair_axes[128];
+} afhip_head_rotation;
+afhip_status afhip_launch_head_rotation(void *stream, const afhip_head_rotation *rotation);
+/* The same with the keys, and the tokens' values beside them (of the rotation's type), straight into a cache's slots, in one
+ * launch; out_key is not written.  Exactly one of `cache` (keys and values rounded to its type) and `quantized` is given (else
+ * AFHIP_ERR_INVALID_ARGUMENT), of the rotation's kv_heads and head_dim (else AFHIP_ERR_INVALID_STATE).  A slot outside the cache writes nothing. */
+afhip_status afhip_launch_rotated_store(void *stream, const afhip_head_rotation *rotation, const afhip_paged_cache *cache,
+                                        const afhip_quantized_cache *quantized, afhip_buffer values, size_t token_stride,
+                                        size_t head_stride, afhip_buffer slots);
+
+/* Attention of every request's new tokens over a quantized cache that holds them already.  Token t of request r (row
+ * query_starts[r] + t of query, position i = context_lens[r] + t) sees the keys at positions j <= i, with `window` != 0 those of
+ * them with i - j < window.  Head h reads key head h / (heads / kv_heads).
+ *
+ *   s_j = scale * q[t][h] . k[j];   softcap > 0: s_j = softcap * tanh(s_j / softcap);   slopes: s_j = s_j - slopes[h] * (i - j)
+ *   out[t][h] = sum over seen j of  softmax_j(s_j) v[j],   zero where nothing is seen
+ *
+ * What is not seen does not count, whatever its codes and scales hold.  A key whose block the table does not name is not seen.  A
+ * row whose seen scores are all minus infinity, or whose query holds an infinity or no number, is no numbers.
+ * query and out: F32, F16 or BF16, both of `type`, [tokens][heads][head_dim], strides in elements (multiples of 4 for F32, of 8
+ * otherwise; 16-byte aligned).  Codes are multiplied as bf16, which holds each of them; queries, and the weights beside the values,
+ * as three terms of bf16 for F32 (24 bits), two for F16 (16 bits) and one for BF16.  Sums are f32.
+ * max_query_len and max_key_len bound what the batch holds (new tokens; context plus new tokens) and choose the launch's
+ * shape; tokens past the first and keys past the second are left out.  slopes f32 [heads], optional (.ptr == 0).  heads is a multiple of
+ * kv_heads (else AFHIP_ERR_INVALID_STATE); requests <= 65535, max_key_len * block_size < 2^32, max_query_len * heads < 2^31 and a grid
+ * of fewer than 2^32 threads (256 or 512 for every 16 of a request's max_query_len * heads / kv_heads rows and every key head, or as
+ * many as the units hold), else AFHIP_ERR_OP_UNSUPPORTED.
+ * `workspace` (256-byte aligned, afhip_quantized_attention_workspace_bytes) holds the parts of rows whose keys are shared out over
+ * workgroups; less than asked for is refused (AFHIP_ERR_INVALID_STATE). */
+typedef struct afhip_quantized_attention {
+    afhip_quantized_cache cache;
+    int type;
+    float scale, softcap;
+    size_t window, requests, tokens, heads, max_query_len, max_key_len, table_columns;
+    size_t query_token_stride, query_head_stride, out_token_stride, out_head_stride;
+    afhip_buffer query, out, query_starts, context_lens, block_tables, slopes;
+} afhip_quantized_attention;
+size_t afhip_quantized_attention_workspace_bytes(const afhip_quantized_attention *attention);
+afhip_status afhip_launch_quantized_attention(void *stream, const afhip_quantized_attention *attention, afhip_buffer workspace);
+
+/* A token of every row of logits [rows][vocab] (F32, F16 or BF16, row_stride elements apart), from the row's random number.
+ * A row's tokens are ordered by falling logit, equal ones by rising index, and weigh w = exp((logit - largest) / temperature).
+ * Kept are, one filter after the other,
+ *   the first top_k of them                                          (top_k <= 0: all)
+ *   of these as long as the weights before a token are below top_p of their sum  (top_p >= 1 or no number: all; the first always)
+ *   and of these the tokens with w >= min_p                          (min_p <= 0 or no number: all; the first always)
+ * and the token is the first whose weight and those before it exceed uniform * their sum; probability: its share of that sum.
+ * temperature <= 0 or no number: the first token, probability 1.  A logit that is no number counts as minus infinity, which
+ * weighs nothing; where the largest is infinite, the infinite ones weigh 1 and others nothing; where no logit is above minus
+ * infinity, the token is -1 and the probability 0.  A uniform below 0 or no number counts as 0, one of 1 or more as the last kept token.
+ * Weights are formed in 64 bits and summed as whole numbers (multiples of 2^-50 for up to 4096 tokens, 2^-45 for 131072), so neither the sums nor the token hang
+ * on an order of additions.
+ * temperatures, top_p, min_p, uniforms f32 [rows], top_k int32 [rows]; all but uniforms optional (.ptr == 0: 1, none, none, none).
+ * tokens int32 [rows], probabilities f32 [rows] (optional).  vocab from 1 to 2^24, rows < 2^22 (else AFHIP_ERR_OP_UNSUPPORTED; vocab 0:
+ * AFHIP_ERR_INVALID_STATE); logits aligned to their element; other types: AFHIP_ERR_UNSUPPORTED_TENSOR_TYPE.
+ * `workspace`: 256-byte aligned, afhip_sample_workspace_bytes; less is refused (AFHIP_ERR_INVALID_STATE). */
+typedef struct afhip_sample {
+    int type;
+    size_t rows, vocab, row_stride;
+    afhip_buffer logits, temperatures, top_k, top_p, min_p, uniforms, tokens, probabilities;
+} afhip_sample;
+size_t afhip_sample_workspace_bytes(const afhip_sample *sample);
+afhip_status afhip_launch_sample(void *stream, const afhip_sample *sample, afhip_buffer workspace);
 
 /* ------------------------------------------------------------------------
  * Backend object: ops/cuda/cuda_compute.zig (CudaCompute + the ComputeBackend
