@@ -3,19 +3,22 @@
 //   out[t][h] = sum_j p_j u_j v_j / sum_j p_j,   p_j = exp(s_j - m),   s_j from scale * k_scale_j * (q . k_j),   u_j the value's scale
 //
 // One pass over the keys with a running reference m and sum of the softmax.  The rows of one key head are its query heads' tokens
-// packed together (row = token * group + head in group), sixteen to a wavefront, so a key is read once for all of them.
+// packed together (row = token * group + head in group), sixteen or 32 to a wavefront, so a key is read once for all of them.
 //
 // The products are on the 16 x 16 x 32 bf16 matrix instructions with the keys as the first operand: K Q^T has one row of the packed
-// queries to a lane (column = lane % 16) and four consecutive keys in its registers, and these are, after the softmax, the second
-// operand of V^T P^T as they stand.  Codes go from memory into registers and to bf16 there, which holds every one of them exactly: 16
-// bytes a lane of a key, and of a value one, two or four dwords of eight keys, whose bytes are put side by side key by key before
-// the conversion (the order of the head's values over lanes and products is free: value kVec * column + t is in product t).  So
-// nothing is staged in LDS but a tile's places and scales, which lie one key a lane as they arrive and are needed four a lane.
-// F32 queries and the weights beside them are three terms of bf16, f16 two, each a product of its own.
+// queries to a lane (column = lane % 16) and four keys in its registers, and these are, after the softmax, the second operand of
+// V^T P^T as they stand.  Which key is which row of an instruction, and which of the head's values which row of which product, is
+// free: row 4 q + i of half h of a tile is key 16 h + 4 i + q, so that the four quarters of a wavefront read four neighbouring keys,
+// and value kVec * column + t is in product t, so that a lane's share of a key is one run of bytes.
 //
-// A wavefront steps over tiles of 32 keys, the next one's codes requested before it works on one, the block table a tile before
-// that.  Wavefronts of a workgroup take tiles in turn and add up in LDS; long contexts are shared out over workgroups by the
-// lengths that the device holds, and a second kernel joins the parts.
+// Codes come from memory straight into a ring of tiles in LDS that each wavefront has for itself (no barrier anywhere), and go to
+// bf16, which holds every one of them exactly, as they are read from there; of values the bytes of two keys are put side by side
+// before.  A tile's stage is requested anew as soon as its codes are in registers, so two tiles are on their way while a third is
+// worked on.  F32 queries and the weights beside them are three terms of bf16, f16 two, each a product of its own.  On whole
+// numbers the queries are three digits to the base 256, and K Q^T is on the i8 instructions: the codes as they are, sums exact.
+//
+// Wavefronts of a workgroup have parts of its keys and add up in LDS; long contexts are shared out over workgroups by the lengths
+// that the device holds, and a second kernel joins the parts.
 #include "quantized_launch.h"
 
 #include <hip/hip_runtime.h>
@@ -28,6 +31,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 32;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -58,6 +62,10 @@ __device__ __forceinline__ float row_max(float v) {
     swap_rows(&v, &other);
     return fmaxf(v, other);
 }
+__device__ __forceinline__ uint32_t row_max_bits(uint32_t v) {
+    v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 32)));
+    return max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 16)));
+}
 __device__ __forceinline__ float row_sum(float v) {
     float other;
     swap_halves(&v, &other);
@@ -78,12 +86,8 @@ __device__ __forceinline__ uint32_t two_e4m3(uint32_t codes) {
 __device__ __forceinline__ float one_i8(uint32_t codes, int byte) { return static_cast<float>(static_cast<int8_t>(codes >> (8 * byte))); }
 
 // Eight codes of a key as one operand's registers.
-template <bool kE4m3>
 __device__ __forceinline__ bf16x8 operand_of(uint32_t low, uint32_t high) {
-    u32x4 r;
-    if (kE4m3) r = u32x4{two_e4m3<false>(low), two_e4m3<true>(low), two_e4m3<false>(high), two_e4m3<true>(high)};
-    else r = u32x4{pack(one_i8(low, 0), one_i8(low, 1)), pack(one_i8(low, 2), one_i8(low, 3)), pack(one_i8(high, 0), one_i8(high, 1)), pack(one_i8(high, 2), one_i8(high, 3))};
-    return __builtin_bit_cast(bf16x8, r);
+    return __builtin_bit_cast(bf16x8, u32x4{two_e4m3<false>(low), two_e4m3<true>(low), two_e4m3<false>(high), two_e4m3<true>(high)});
 }
 
 __device__ __forceinline__ f32x4 product(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -117,7 +121,7 @@ struct Plan {
     uint32_t slots;      // parts that there is room for
 };
 
-__device__ __forceinline__ Share lengths_of(const QuantizedAttentionArgs& a, uint32_t request) {
+__device__ __forceinline__ Share lengths_of(const QuantizedAttentionArgs& a, uint32_t request, int rows_a_tile) {
     Share s{};
     s.begin = min(max(a.query_starts[request], 0), static_cast<int>(a.tokens));
     const int end = min(max(a.query_starts[request + 1], s.begin), static_cast<int>(a.tokens));
@@ -128,7 +132,7 @@ __device__ __forceinline__ Share lengths_of(const QuantizedAttentionArgs& a, uin
     const int first = a.window != 0 && s.context >= static_cast<int>(a.window) ? s.context - static_cast<int>(a.window) + 1 : 0;
     s.first_tile = first / kTile;
     s.tiles = s.tokens > 0 && keys > first ? (keys - 1) / kTile - s.first_tile + 1 : 0;
-    s.row_tiles = (static_cast<uint32_t>(s.tokens) * a.group + 15) / 16;
+    s.row_tiles = (static_cast<uint32_t>(s.tokens) * a.group + rows_a_tile - 1) / rows_a_tile;
     return s;
 }
 
@@ -146,13 +150,13 @@ __device__ __forceinline__ T sum_up_to(T v) {
 // The request of workgroup `of` (or of request number `of`), and its share.  A part has the same number of tiles for all requests,
 // evened out within a request.  Every wavefront works this out for itself, 64 requests at a time.
 template <bool kByRequest>
-__device__ __forceinline__ bool find_share(const QuantizedAttentionArgs& a, const Plan& plan, uint32_t of, uint32_t* request, Share* out) {
+__device__ __forceinline__ bool find_share(const QuantizedAttentionArgs& a, const Plan& plan, int rows_a_tile, uint32_t of, uint32_t* request, Share* out) {
     const uint32_t heads = a.cache.kv_heads;
     if (plan.target == 0) {
         const uint32_t r = kByRequest ? of : of / (heads * plan.row_tiles);
         if (r >= a.requests) return false;
         *request = r;
-        *out = lengths_of(a, r);
+        *out = lengths_of(a, r, rows_a_tile);
         out->splits = 1;
         out->each = static_cast<uint32_t>(out->tiles);
         out->first = r * heads * plan.row_tiles;
@@ -164,7 +168,7 @@ __device__ __forceinline__ bool find_share(const QuantizedAttentionArgs& a, cons
     float work = 0.0f;
     for (uint32_t r0 = 0; r0 < a.requests; r0 += 64) {
         if (r0 + lane < a.requests) {
-            mine = lengths_of(a, r0 + lane);
+            mine = lengths_of(a, r0 + lane, rows_a_tile);
             work += static_cast<float>(mine.tiles) * static_cast<float>(mine.row_tiles);
         }
     }
@@ -178,7 +182,7 @@ __device__ __forceinline__ bool find_share(const QuantizedAttentionArgs& a, cons
         uint32_t count = 0, slots = 0;
         mine.splits = 0;
         if (r0 + lane < a.requests) {
-            if (a.requests > 64) mine = lengths_of(a, r0 + lane);
+            if (a.requests > 64) mine = lengths_of(a, r0 + lane, rows_a_tile);
             mine.splits = mine.tiles > 0 ? (static_cast<uint32_t>(mine.tiles) + tiles - 1) / tiles : 1;
             mine.each = (static_cast<uint32_t>(mine.tiles) + mine.splits - 1) / mine.splits;
             count = mine.row_tiles * mine.splits * heads;
@@ -236,352 +240,473 @@ struct Bytes<8> { typedef uint32_t type __attribute__((ext_vector_type(2))); };
 template <>
 struct Bytes<16> { typedef uint32_t type __attribute__((ext_vector_type(4))); };
 
-// A tile on its way: its codes, and what one lane holds of its keys (lanes 0 to 31 keys' scales, 32 to 63 values').
+__device__ const uint4 kNothing{0, 0, 0, 0};  // what values past a head's end are loaded from
+
+// 16 (4) bytes a lane from memory to 1 KiB (256 bytes) of LDS from `to` on (a uniform address).
+__device__ __forceinline__ void load_to_lds(uint32_t to, const uint4* from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ void load_to_lds(uint32_t to, const float* from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(to), "v"(from) : "memory", "m0");
+}
+// The same of 16 bytes from a uniform address on, `past` bytes behind it for a lane (kNoPiece: zeros; `all`: no lane has that).
+constexpr uint32_t kNoPiece = ~0u;
+__device__ __forceinline__ void load_to_lds(uint32_t to, const uint4* from, uint32_t past, bool all) {
+    if (all) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(past), "s"(from) : "memory", "m0");
+    else load_to_lds(to, past == kNoPiece ? &kNothing : reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(from) + past));
+}
+// s_waitcnt for "at most kLeft vector memory operations outstanding" (nothing else waited for).
+template <int kLeft>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kLeft) : "memory");
+}
+
+// Where 16-byte piece `piece` of row `row` of a tile lies in LDS, in pieces.  The pieces of a row are in an order of its own, so that
+// one piece of 16 rows falls on all banks (256 bytes of them).
 template <int kDim>
-struct Tile {
-    typedef typename Bytes<kDim / 16>::type Value;
-    u32x4 key[2][kDim / 64];
-    Value value[8];
-    float scale;
-    uint32_t held;  // its keys that have a place
-};
+__device__ __forceinline__ int piece_at(int row, int piece) {
+    constexpr int kPieces = kDim / 16, kRowsOfBanks = 16 / kPieces;
+    return row * kPieces + (piece ^ (row / kRowsOfBanks & (kPieces - 1)));
+}
 
 constexpr int kMostWaves = 8;
-constexpr int kWaveLds = 3 * kTile * 4;  // of a wavefront: its tile's places and scales
-constexpr int waves_of(int dim) { return dim == 256 ? 4 : kMostWaves; }
+constexpr int stages_of(int dim) { return dim == 64 ? 4 : 2; }
+constexpr int most_waves(int dim) { return dim == 256 ? 4 : kMostWaves; }
+constexpr int sums_stride(int dim) { return dim + 4; }
+constexpr int tile_bytes(int dim) { return kTile * dim * 2 + 2 * kTile * 4; }
+// Of a wavefront: the ring of keys, values and their scales, and in its place, in the end, its sums.
+constexpr int wave_lds(int dim, int rows) {
+    const int ring = stages_of(dim) * tile_bytes(dim), sums = rows * (sums_stride(dim) * 4 + static_cast<int>(sizeof(Part)));
+    return ((ring > sums ? ring : sums) + 1023) / 1024 * 1024;
+}
 
-// kDim: the head's values, rounded up to a size that is here (the rest are zeros).  kTerms: 1 bf16, 2 f16, 3 f32 queries.
-template <int kDim, bool kE4m3, int kTerms>
-__global__ __launch_bounds__(64 * waves_of(kDim)) void quantized_attention_kernel(QuantizedAttentionArgs a, Plan plan, float* part_out, Part* parts) {
-    constexpr int kSteps = kDim / 32, kVec = kDim / 16, kWords = kVec / 4;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    uint32_t(*const place_of)[kTile] = reinterpret_cast<uint32_t(*)[kTile]>(lds);  // [wave][key]
-    float(*const scale_of)[2 * kTile] = reinterpret_cast<float(*)[2 * kTile]>(lds + (blockDim.x >> 6) * (kTile * 4));
+// kDim: the head's values, rounded up to a size that is here (the rest are zeros).  kTerms: 1 bf16, 2 f16, 3 f32 queries.  kQ:
+// sixteens of rows.
+template <int kDim, bool kE4m3, int kTerms, int kQ>
+__global__ __launch_bounds__(64 * most_waves(kDim)) void quantized_attention_kernel(QuantizedAttentionArgs a, Plan plan, float* part_out, Part* parts) {
+    constexpr int kSteps = kDim / 32, kVec = kDim / 16, kWords = kVec / 4, kPieces = kDim / 16, kRows = 16 * kQ;
+    constexpr int kLoads = kTile * kPieces / 64, kRowsALoad = 64 / kPieces;  // of keys, and of values: 1 KiB each
+    typedef typename Bytes<kVec>::type Value;
+    constexpr int kStages = stages_of(kDim), kWaveLds = wave_lds(kDim, kRows);
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
 
-    const uint32_t number = ((blockIdx.x >> 3) / plan.row_tiles * 8 + (blockIdx.x & 7)) * plan.row_tiles + (blockIdx.x >> 3) % plan.row_tiles;
+    // workgroups go round the eight XCDs in turn: the row tiles of a part, which share its keys, and the key heads beside them, whose
+    // scales share its lines of memory, lie on one and share its L2
+    const uint32_t together = plan.row_tiles * a.cache.kv_heads, turn = blockIdx.x >> 3;
+    const uint32_t number = (turn / together * 8 + (blockIdx.x & 7)) * together + turn % together;
     uint32_t request;
     Share share;
-    if (!find_share<false>(a, plan, number, &request, &share)) return;
-    const uint32_t inside = number - share.first, row_tile = inside % share.row_tiles, split = inside / share.row_tiles % share.splits;
-    const uint32_t kv_head = inside / share.row_tiles / share.splits, slot = share.first_slot + inside;
-    const int group = static_cast<int>(a.group), rows = share.tokens * group, first_row = static_cast<int>(row_tile) * 16;
+    if (!find_share<false>(a, plan, kRows, number, &request, &share)) return;
+    const uint32_t inside = number - share.first, row_tile = inside % share.row_tiles, kv_head = inside / share.row_tiles % a.cache.kv_heads;
+    const uint32_t split = inside / share.row_tiles / a.cache.kv_heads, slot = share.first_slot + inside;
+    const int group = static_cast<int>(a.group), rows = share.tokens * group, first_row = static_cast<int>(row_tile) * kRows;
     if (first_row >= rows || (share.splits > 1 && slot >= plan.slots)) return;
-    const int here = min(16, rows - first_row);  // rows of this workgroup
+    const int here = min(kRows, rows - first_row);  // rows of this workgroup
     const int tid = static_cast<int>(threadIdx.x), wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, waves = static_cast<int>(blockDim.x) >> 6;
-    const int column = lane & 15, quarter = lane >> 4;
+    const int column = lane & 15, quarter = lane >> 4, head_dim = static_cast<int>(a.cache.head_dim);
+    const bool whole_heads = head_dim == kDim;
 
     // ---- the rows: their queries, requested first
-    const bool real = column < here;
-    const int row = first_row + (real ? column : 0), token = row / group, head = static_cast<int>(kv_head) * group + row % group;
-    const int position = real ? share.context + token : -1;  // (a row that is none sees nothing)
-    u32x4 raw[kSteps / 2][kTerms == 3 ? 4 : 2];
-    {
+    u32x4 raw[kQ][kSteps / 2][kTerms == 3 ? 4 : 2];
+    int position[kQ];
+    float slope[kQ];
+#pragma unroll
+    for (int qt = 0; qt < kQ; ++qt) {
+        const bool real = qt * 16 + column < here;
+        const int row = first_row + (real ? qt * 16 + column : 0), token = row / group, head = static_cast<int>(kv_head) * group + row % group;
+        position[qt] = real ? share.context + token : -1;  // (a row that is none sees nothing)
+        slope[qt] = a.slopes != nullptr ? a.slopes[head] * kLog2e : 0.0f;
         const size_t from = static_cast<size_t>(share.begin + token) * a.query_token_stride + static_cast<size_t>(head) * a.query_head_stride;
 #pragma unroll
         for (int b = 0; b < kSteps / 2; ++b) {
             const int d = 64 * b + 16 * quarter;
             const char* p = static_cast<const char*>(a.query) + (from + d) * (kTerms == 3 ? 4 : 2);
 #pragma unroll
-            for (int i = 0; i < (kTerms == 3 ? 4 : 2); ++i) raw[b][i] = real && d < static_cast<int>(a.cache.head_dim) ? reinterpret_cast<const u32x4*>(p)[i] : u32x4{0, 0, 0, 0};
+            for (int i = 0; i < (kTerms == 3 ? 4 : 2); ++i) raw[qt][b][i] = real && d < head_dim ? reinterpret_cast<const u32x4*>(p)[i] : u32x4{0, 0, 0, 0};
         }
     }
-    const float slope = a.slopes != nullptr ? a.slopes[head] * kLog2e : 0.0f;
 
-    // ---- the keys of this part that any of these rows sees
+    // ---- the keys of this part that any of these rows sees, and this wavefront's of them
     const int first_position = share.context + first_row / group, last_position = share.context + (first_row + here - 1) / group;
     const unsigned long long most = min(static_cast<unsigned long long>(a.table_columns) * a.block_size.by, static_cast<unsigned long long>(a.max_key_len));
     const int keys = static_cast<int>(min(static_cast<unsigned long long>(last_position) + 1, most));  // seen by none from here on
     const uint32_t limit = a.window != 0 ? a.window : 0x80000000u;                                      // a key is seen where position - key is below
     int tile = share.first_tile + static_cast<int>(split * share.each);
-    const int end = min(min(tile + static_cast<int>(share.each), share.first_tile + share.tiles), (keys + kTile - 1) / kTile);
+    int end = min(min(tile + static_cast<int>(share.each), share.first_tile + share.tiles), (keys + kTile - 1) / kTile);
     if (a.window != 0 && first_position >= static_cast<int>(a.window)) tile = max(tile, (first_position - static_cast<int>(a.window) + 1) / kTile);
-    tile += wave;
+    if (end > tile) {
+        const int each = (end - tile + waves - 1) / waves;
+        tile += wave * each;
+        end = min(tile + each, end);
+    }
 
+    char* const ring = lds + wave * kWaveLds;
+    const uint32_t ring_at = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)ring)));
+    // 64 entries of the block table from `window_at` on, one a lane, and which of them name a block
     const int* table = a.block_tables + static_cast<size_t>(request) * a.table_columns;
-    const uint32_t mine = lane & 31;
-    uint32_t entry = ~0u;  // the block of this lane's key, of the next tile to be requested
-    auto find = [&](int t) {
-        const uint32_t key = static_cast<uint32_t>(t) * kTile + mine;
-        entry = static_cast<int>(key) < keys ? static_cast<uint32_t>(table[divide(key, a.block_size)]) : ~0u;
+    const uint32_t last_block = keys > 0 ? divide(static_cast<uint32_t>(keys - 1), a.block_size) : 0;
+    uint32_t window = 0, window_at = 0, window_end = 0;  // (keys from window_end on are not in it)
+    unsigned long long named = 0;
+    // Where a lane's bytes of load i lie behind its first row's, where the rows of a load are in one block.
+    const bool in_one = a.block_size.by % kRowsALoad == 0 && a.cache.slot_stride < (1u << 20);
+    uint32_t lane_at[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int row = i * kRowsALoad + lane / kPieces, piece = piece_at<kDim>(row, lane % kPieces) % kPieces;
+        lane_at[i] = (static_cast<uint32_t>(lane / kPieces) * a.cache.slot_stride + piece) * 16;
+        if (piece * 16 >= head_dim) lane_at[i] = kNoPiece;
+    }
+    // Requests tile t into a stage; its keys that have a place are returned, in the order of the products' rows.  (A key without one
+    // is not seen by any row: what is loaded for it, the first block's, may be anything.)
+    auto request_tile = [&](int t, int stage) -> uint32_t {
+        const uint32_t first_key = static_cast<uint32_t>(t) * kTile;
+        if (first_key + kTile > window_end) {
+            window_at = divide(first_key, a.block_size);
+            const uint32_t block = window_at + lane <= last_block ? static_cast<uint32_t>(table[window_at + lane]) : ~0u;
+            named = __ballot(block < a.cache.blocks);
+            window = block < a.cache.blocks ? block : 0;
+            window_end = (window_at + 64) * a.block_size.by;  // (below 2^32: a bound of the keys times the block size)
+        }
+        const uint32_t to = ring_at + stage * tile_bytes(kDim);
+        const uint32_t head_at = kv_head * a.cache.head_stride;
+        if (in_one) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const uint32_t key = first_key + i * kRowsALoad, column_of = divide(key, a.block_size);
+                const uint32_t block = __builtin_amdgcn_readlane(window, column_of - window_at);
+                const uint32_t place = block * a.cache.block_stride + (key - column_of * a.block_size.by) * a.cache.slot_stride + head_at;
+                load_to_lds(to + i * 1024, a.cache.keys + place, lane_at[i], whole_heads);
+                load_to_lds(to + kTile * kDim + i * 1024, a.cache.values + place, lane_at[i], whole_heads);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int row = i * kRowsALoad + lane / kPieces, piece = piece_at<kDim>(row, lane % kPieces) % kPieces;
+                const uint32_t key = first_key + row, column_of = divide(key, a.block_size);
+                const uint32_t block = static_cast<uint32_t>(__shfl(static_cast<int>(window), static_cast<int>(column_of - window_at)));
+                const uint32_t place = block * a.cache.block_stride + (key - column_of * a.block_size.by) * a.cache.slot_stride + head_at + piece;
+                const uint4 *k = a.cache.keys + place, *v = a.cache.values + place;
+                if (piece * 16 >= head_dim) k = v = &kNothing;
+                load_to_lds(to + i * 1024, k);
+                load_to_lds(to + kTile * kDim + i * 1024, v);
+            }
+        }
+        // the scales, keys' and then values'
+        const uint32_t key = first_key + (lane & 16) + 4 * (lane & 3) + (lane >> 2 & 3), column_of = divide(key, a.block_size);
+        const uint32_t block = static_cast<uint32_t>(__shfl(static_cast<int>(window), static_cast<int>(column_of - window_at)));
+        const uint32_t place = block * a.cache.scale_block_stride + (key - column_of * a.block_size.by) * a.cache.scale_slot_stride + kv_head * a.cache.scale_head_stride;
+        load_to_lds(to + 2 * kTile * kDim, (lane < 32 ? a.cache.key_scales : a.cache.value_scales) + place);
+        return static_cast<uint32_t>(__ballot((named >> (column_of - window_at) & 1) != 0 && static_cast<int>(key) < keys));
     };
-    auto request_tile = [&](int t, Tile<kDim>& to) {
-        const uint32_t key = static_cast<uint32_t>(t) * kTile + mine;
-        const uint32_t past = key - divide(key, a.block_size) * a.block_size.by;
-        const bool there = entry < a.cache.blocks;
-        to.held = static_cast<uint32_t>(__ballot(there));
-        // (a key without a place is not seen by any row: what is loaded for it, the cache's first, may be anything)
-        const uint32_t block = there ? entry : 0, within = there ? past : 0;
-        const uint32_t place = block * a.cache.block_stride + within * a.cache.slot_stride + kv_head * a.cache.head_stride;
-        const uint32_t scale_at = block * a.cache.scale_block_stride + within * a.cache.scale_slot_stride + kv_head * a.cache.scale_head_stride;
-        to.scale = (lane < 32 ? a.cache.key_scales : a.cache.value_scales)[scale_at];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (lane < 32) place_of[wave][mine] = place;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+    uint32_t held[kStages] = {};
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const uint4* from = a.cache.keys + place_of[wave][half * 16 + column];
-#pragma unroll
-            for (int b = 0; b < kDim / 64; ++b) {
-                if (64 * b + 16 * quarter < static_cast<int>(a.cache.head_dim)) to.key[half][b] = *reinterpret_cast<const u32x4*>(from + 4 * b + quarter);
-            }
-        }
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const u32x4 places = *reinterpret_cast<const u32x4*>(&place_of[wave][half * 16 + quarter * 4]);
-            if (kVec * column < static_cast<int>(a.cache.head_dim)) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    to.value[half * 4 + j] = *reinterpret_cast<const typename Tile<kDim>::Value*>(reinterpret_cast<const char*>(a.cache.values + places[j]) + kVec * column);
-            }
-        }
-    };
-
-    Tile<kDim> ping, pong;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-#pragma unroll
-        for (int b = 0; b < kDim / 64; ++b) ping.key[half][b] = pong.key[half][b] = u32x4{0, 0, 0, 0};
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ping.value[j] = pong.value[j] = typename Tile<kDim>::Value(0u);
-    if (tile < end) {
-        find(tile);
-        request_tile(tile, ping);
-        if (tile + waves < end) find(tile + waves);
+    for (int i = 0; i < kStages; ++i) {
+        if (tile + i < end) held[i] = request_tile(tile + i, i);
     }
 
-    bf16x8 query[kSteps][kTerms];
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (kTerms == 3) {
-                const uint32_t bits = raw[s / 2][(s % 2) * 2 + j / 4][j % 4];  // (a bit_cast of the element itself reads the first)
-                float rest = __builtin_bit_cast(float, bits);
-#pragma unroll
-                for (int term = 0; term < kTerms; ++term) {
-                    query[s][term][j] = static_cast<__bf16>(rest);
-                    rest -= static_cast<float>(query[s][term][j]);
-                }
-            } else {
-                const uint16_t bits = static_cast<uint16_t>(raw[s / 2][s % 2][j / 2] >> (16 * (j % 2)));
-                if (kTerms == 1) {
-                    query[s][0][j] = __builtin_bit_cast(__bf16, bits);
-                } else {
-                    const float v = static_cast<float>(__builtin_bit_cast(_Float16, bits));
-                    query[s][0][j] = static_cast<__bf16>(v);
-                    query[s][kTerms - 1][j] = static_cast<__bf16>(v - static_cast<float>(query[s][0][j]));
-                }
-            }
-        }
-    }
-
+    // What the products of a row are multiplied by, beside the keys' scales.
     const bool caps = a.softcap > 0.0f;
     const float unit = caps ? a.scale / a.softcap : a.scale * kLog2e, cap = a.softcap * kLog2e;
-    f32x4 out[kVec];
+    float row_unit[kQ];
+    bf16x8 query[kE4m3 ? kQ : 1][kE4m3 ? kSteps : 1][kTerms];
+    i32x4 digits[kE4m3 ? 1 : kQ][kE4m3 ? 1 : kDim / 64][3];
 #pragma unroll
-    for (int t = 0; t < kVec; ++t) out[t] = f32x4{0, 0, 0, 0};
-    float reference = -__builtin_inff(), sum = 0.0f;
-    bool saw = false;
-
-    auto work = [&](int t, Tile<kDim>& at) {
-        const int first_key = t * kTile;
-        // every row sees every key
-        const bool clean = at.held == ~0u && first_key + kTile - 1 <= first_position && static_cast<uint32_t>(last_position - first_key) < limit;
-        scale_of[wave][lane] = at.scale;
-        f32x4 score[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+    for (int qt = 0; qt < kQ; ++qt) {
+        row_unit[qt] = unit;
+        float v[kE4m3 ? 1 : kDim / 4];
+        uint32_t most_bits = 0;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const u32x4 codes = at.key[half][s / 2];
-                const bf16x8 key = operand_of<kE4m3>(codes[(s % 2) * 2], codes[(s % 2) * 2 + 1]);
+            for (int j = 0; j < 8; ++j) {
+                float value;
+                if (kTerms == 3) {
+                    const uint32_t bits = raw[qt][s / 2][(s % 2) * 2 + j / 4][j % 4];  // (a bit_cast of the element itself reads the first)
+                    value = __builtin_bit_cast(float, bits);
+                } else {
+                    const uint16_t bits = static_cast<uint16_t>(raw[qt][s / 2][s % 2][j / 2] >> (16 * (j % 2)));
+                    value = kTerms == 1 ? static_cast<float>(__builtin_bit_cast(__bf16, bits)) : static_cast<float>(__builtin_bit_cast(_Float16, bits));
+                }
+                if constexpr (kE4m3) {
 #pragma unroll
-                for (int term = kTerms - 1; term >= 0; --term) score[half] = product(key, query[s][term], score[half]);
+                    for (int term = 0; term < kTerms; ++term) {
+                        query[qt][s][term][j] = static_cast<__bf16>(value);
+                        value -= static_cast<float>(query[qt][s][term][j]);
+                    }
+                } else {
+                    v[8 * s + j] = value;
+                    most_bits = max(most_bits, __builtin_bit_cast(uint32_t, value) & 0x7FFFFFFFu);
+                }
             }
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        float x[8], value_scale[8];
-        uint32_t seen = 0xFF;
+        if constexpr (!kE4m3) {
+            // The row's largest value goes to [2^21, 2^22): whole numbers of three digits to the base 256, each an i8.
+            most_bits = row_max_bits(most_bits);
+            const int exponent = most_bits == 0 ? 0 : __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, most_bits)) - 22;
+            row_unit[qt] = most_bits >= 0x7F800000u ? __builtin_nanf("") : unit * __builtin_amdgcn_ldexpf(1.0f, exponent);
+#pragma unroll
+            for (int b = 0; b < kDim / 64; ++b) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t words[3] = {0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int whole = static_cast<int>(__builtin_rintf(__builtin_amdgcn_ldexpf(v[16 * b + 4 * w + j], -exponent)));
+                        const int high = (whole + 0x8080) >> 16, rest = whole - high * 65536, middle = (rest + 0x80) >> 8, low = rest - middle * 256;
+                        words[0] |= (static_cast<uint32_t>(high) & 0xFF) << (8 * j);
+                        words[1] |= (static_cast<uint32_t>(middle) & 0xFF) << (8 * j);
+                        words[2] |= (static_cast<uint32_t>(low) & 0xFF) << (8 * j);
+                    }
+#pragma unroll
+                    for (int digit = 0; digit < 3; ++digit) digits[qt][b][digit][w] = static_cast<int>(words[digit]);
+                }
+            }
+        }
+    }
+
+    f32x4 out[kQ][kVec];
+    float reference[kQ], sum[kQ];
+    uint32_t saw[kQ];
+#pragma unroll
+    for (int qt = 0; qt < kQ; ++qt) {
+        reference[qt] = -__builtin_inff();
+        sum[qt] = 0.0f;
+        saw[qt] = 0;
+#pragma unroll
+        for (int t = 0; t < kVec; ++t) out[qt][t] = f32x4{0, 0, 0, 0};
+    }
+
+    int stage = 0;
+    for (; tile < end; ++tile) {
+        if (tile + kStages - 1 < end) wait_loads<(kStages - 1) * (2 * kLoads + 1)>();
+        else wait_loads<0>();
+        const char* const at = ring + stage * tile_bytes(kDim);
+        const uint32_t there = held[0];
+        // everything of the tile into registers
+        u32x4 key[2][kDim / 64];
+        Value value[8];
+        f32x4 key_scale[2], value_scale[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const f32x4 k = *reinterpret_cast<const f32x4*>(&scale_of[wave][half * 16 + quarter * 4]);
-            const f32x4 v = *reinterpret_cast<const f32x4*>(&scale_of[wave][32 + half * 16 + quarter * 4]);
+            const int key_row = half * 16 + 4 * (column & 3) + (column >> 2);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[half * 4 + j] = score[half][j] * (k[j] * unit);
-                value_scale[half * 4 + j] = v[j];
-            }
+            for (int b = 0; b < kDim / 64; ++b) key[half][b] = *reinterpret_cast<const u32x4*>(at + piece_at<kDim>(key_row, 4 * b + quarter) * 16);
+            key_scale[half] = *reinterpret_cast<const f32x4*>(at + 2 * kTile * kDim + (half * 16 + quarter * 4) * 4);
+            value_scale[half] = *reinterpret_cast<const f32x4*>(at + 2 * kTile * kDim + (32 + half * 16 + quarter * 4) * 4);
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        if (caps) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = cap * hyperbolic(x[j]);
-        }
-        const int my_key = first_key + quarter * 4;
-        if (a.slopes != nullptr) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = __builtin_fmaf(-slope, static_cast<float>(position - my_key - (j / 4 * 16 + j % 4)), x[j]);
-        }
-        if (!clean) {
-            seen = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int key = j / 4 * 16 + j % 4;
-                const bool sees = static_cast<uint32_t>(position - my_key - key) < limit && (at.held >> (quarter * 4 + key) & 1) != 0;
-                seen |= static_cast<uint32_t>(sees) << j;
-                if (!sees) x[j] = -__builtin_inff();
-            }
-        }
-        saw |= seen != 0;
-        const float peak = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-        if (__any(peak > reference + kSlack)) {
-            const float highest = row_max(peak);
-            if (highest > reference + kSlack) {  // each row by itself: no other row's keys move its bits
-                const float by = reference == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(reference - highest);
-                reference = highest;
-                sum *= by;
-#pragma unroll
-                for (int t = 0; t < kVec; ++t) out[t] *= by;
-            }
-        }
-        const float shift = reference == -__builtin_inff() ? 0.0f : reference;
-        bf16x8 weight[kTerms];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float p = __builtin_amdgcn_exp2f(x[j] - shift);
-            sum += p;
-            float rest = p * value_scale[j];
-            if (!clean && (seen >> j & 1) == 0) rest = 0.0f;
+            const int row = j / 4 * 16 + j % 4 * 4 + quarter;
+            value[j] = *reinterpret_cast<const Value*>(at + kTile * kDim + piece_at<kDim>(row, kVec * column / 16) * 16 + kVec * column % 16);
+        }
 #pragma unroll
-            for (int term = 0; term < kTerms; ++term) {
-                weight[term][j] = static_cast<__bf16>(rest);
-                rest -= static_cast<float>(weight[term][j]);
+        for (int i = 0; i + 1 < kStages; ++i) held[i] = held[i + 1];
+        if (tile + kStages < end) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage has been read
+            held[kStages - 1] = request_tile(tile + kStages, stage);
+        }
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+
+        const int first_key = tile * kTile;
+        // every row sees every key
+        const bool clean = there == ~0u && first_key + kTile - 1 <= first_position && static_cast<uint32_t>(last_position - first_key) < limit;
+        f32x4 score[kQ][2];
+        if constexpr (kE4m3) {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const u32x4 codes = key[half][s / 2];
+                    const bf16x8 k = operand_of(codes[(s % 2) * 2], codes[(s % 2) * 2 + 1]);
+#pragma unroll
+                    for (int term = kTerms - 1; term >= 0; --term) {  // the small terms first
+#pragma unroll
+                        for (int qt = 0; qt < kQ; ++qt)
+                            score[qt][half] = product(k, query[qt][s][term], s == 0 && term == kTerms - 1 ? f32x4{0, 0, 0, 0} : score[qt][half]);
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int qt = 0; qt < kQ; ++qt) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    i32x4 whole[3];
+#pragma unroll
+                    for (int b = 0; b < kDim / 64; ++b) {
+#pragma unroll
+                        for (int digit = 0; digit < 3; ++digit)
+                            whole[digit] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, key[half][b]), digits[qt][b][digit], b == 0 ? i32x4{0, 0, 0, 0} : whole[digit], 0, 0, 0);
+                    }
+                    // (a digit's sum is below 2^22: two of them fit 32 bits)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        score[qt][half][j] = __builtin_fmaf(static_cast<float>(whole[0][j]), 65536.0f, static_cast<float>(whole[1][j] * 256 + whole[2][j]));
+                }
             }
         }
-        // A row that does not see a value must not get 0 times no number from it: such codes are taken as zeros in tiles where some
-        // row may not see them, and the rows that do are made no numbers afterwards.
-        uint32_t none[kE4m3 ? kWords : 1] = {};  // of each of the lane's values: whether a key's code is no number, bit 8 * byte + j ... by word
-        bool any_none = false;
+        uint32_t seen[kQ];
+        bf16x8 weight[kQ][kTerms];
+#pragma unroll
+        for (int qt = 0; qt < kQ; ++qt) {
+            float x[8], by[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = score[qt][j / 4][j % 4] * (key_scale[j / 4][j % 4] * row_unit[qt]);
+                by[j] = value_scale[j / 4][j % 4];
+            }
+            if (caps) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = cap * hyperbolic(x[j]);
+            }
+            const int distance = position[qt] - first_key - quarter;  // to this lane's first key
+            if (a.slopes != nullptr) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = __builtin_fmaf(-slope[qt], static_cast<float>(distance - (j / 4 * 16 + j % 4 * 4)), x[j]);
+            }
+            seen[qt] = 0xFF;
+            if (!clean) {
+                seen[qt] = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int past = j / 4 * 16 + j % 4 * 4;
+                    const bool sees = static_cast<uint32_t>(distance - past) < limit && (there >> (j / 4 * 16 + quarter * 4 + j % 4) & 1) != 0;
+                    seen[qt] |= static_cast<uint32_t>(sees) << j;
+                    if (!sees) {
+                        x[j] = -__builtin_inff();
+                        by[j] = 0.0f;
+                    }
+                }
+            }
+            saw[qt] |= seen[qt];
+            const float peak = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+            if (__any(peak > reference[qt] + kSlack)) {
+                const float highest = row_max(peak);
+                if (highest > reference[qt] + kSlack) {  // each row by itself: no other row's keys move its bits
+                    const float kept = reference[qt] == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(reference[qt] - highest);
+                    reference[qt] = highest;
+                    sum[qt] *= kept;
+#pragma unroll
+                    for (int t = 0; t < kVec; ++t) out[qt][t] *= kept;
+                }
+            }
+            const float shift = reference[qt] == -__builtin_inff() ? 0.0f : reference[qt];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float p = __builtin_amdgcn_exp2f(x[j] - shift);
+                sum[qt] += p;
+                float rest = p * by[j];
+#pragma unroll
+                for (int term = 0; term < kTerms; ++term) {
+                    weight[qt][term][j] = static_cast<__bf16>(rest);
+                    rest -= static_cast<float>(weight[qt][term][j]);
+                }
+            }
+        }
+        // A row that does not see a value must not get 0 times no number from it: in tiles where some row may not see such codes they
+        // are taken as zeros, and the rows that see them are made no numbers here.
         if (kE4m3 && !clean) {
+            uint32_t any = 0;
 #pragma unroll
             for (int w = 0; w < kWords; ++w) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t odd = ((at.value[j][w] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;  // a byte's top bit: its code is no number
-                    any_none |= odd != 0;
+                for (int j = 0; j < 8; ++j) any |= ((value[j][w] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;  // a byte's top bit: its code is no number
+            }
+            if (__any(any != 0)) {
+#pragma unroll
+                for (int w = 0; w < kWords; ++w) {
+                    uint32_t bad[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        bad[j] = (((value[j][w] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;  // 1 in such a byte
+                        value[j][w] &= ~(bad[j] * 0xFFu);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        bf16x8 is;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) is[j] = static_cast<__bf16>(static_cast<float>(bad[j] >> (8 * i) & 1));
+#pragma unroll
+                        for (int qt = 0; qt < kQ; ++qt) {
+                            bf16x8 sees;
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) sees[j] = static_cast<__bf16>(static_cast<float>(seen[qt] >> j & 1));
+                            const f32x4 count = product(is, sees, f32x4{0, 0, 0, 0});
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) out[qt][4 * w + i][j] += count[j] > 0.0f ? __builtin_nanf("") : 0.0f;
+                        }
+                    }
                 }
             }
-            any_none = __any(any_none);
         }
 #pragma unroll
         for (int w = 0; w < kWords; ++w) {
-            uint32_t codes[8], bad[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) codes[j] = at.value[j][w];
-            if (kE4m3 && any_none) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    bad[j] = (((codes[j] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;  // 1 in such a byte
-                    codes[j] &= ~(bad[j] * 0xFFu);
-                }
-            }
             uint32_t operand[4][4];  // [value of the word][pair of keys]
 #pragma unroll
             for (int pair = 0; pair < 4; ++pair) {
+                const uint32_t one = value[2 * pair][w], other = value[2 * pair + 1][w];
                 if (kE4m3) {
-                    const uint32_t low = __builtin_amdgcn_perm(codes[2 * pair + 1], codes[2 * pair], 0x05010400u);
-                    const uint32_t high = __builtin_amdgcn_perm(codes[2 * pair + 1], codes[2 * pair], 0x07030602u);
+                    const uint32_t low = __builtin_amdgcn_perm(other, one, 0x05010400u), high = __builtin_amdgcn_perm(other, one, 0x07030602u);
                     operand[0][pair] = two_e4m3<false>(low);
                     operand[1][pair] = two_e4m3<true>(low);
                     operand[2][pair] = two_e4m3<false>(high);
                     operand[3][pair] = two_e4m3<true>(high);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) operand[i][pair] = pack(one_i8(codes[2 * pair], i), one_i8(codes[2 * pair + 1], i));
+                    for (int i = 0; i < 4; ++i) operand[i][pair] = pack(one_i8(one, i), one_i8(other, i));
                 }
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bf16x8 value = __builtin_bit_cast(bf16x8, u32x4{operand[i][0], operand[i][1], operand[i][2], operand[i][3]});
+                const bf16x8 v = __builtin_bit_cast(bf16x8, u32x4{operand[i][0], operand[i][1], operand[i][2], operand[i][3]});
 #pragma unroll
-                for (int term = kTerms - 1; term >= 0; --term) out[4 * w + i] = product(value, weight[term], out[4 * w + i]);
-            }
-            if (kE4m3 && any_none) {
-                bf16x8 sees;
+                for (int term = kTerms - 1; term >= 0; --term) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) sees[j] = static_cast<__bf16>(static_cast<float>(seen >> j & 1));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    bf16x8 is;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) is[j] = static_cast<__bf16>(static_cast<float>(bad[j] >> (8 * i) & 1));
-                    const f32x4 count = product(is, sees, f32x4{0, 0, 0, 0});
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (count[j] > 0.0f) out[4 * w + i][j] = __builtin_nanf("");
-                    }
+                    for (int qt = 0; qt < kQ; ++qt) out[qt][4 * w + i] = product(v, weight[qt][term], out[qt][4 * w + i]);
                 }
             }
         }
-        (void)none;
-    };
-
-    while (tile < end) {
-        if (tile + waves < end) {
-            request_tile(tile + waves, pong);
-            if (tile + 2 * waves < end) find(tile + 2 * waves);
-        }
-        work(tile, ping);
-        tile += waves;
-        if (tile >= end) break;
-        if (tile + waves < end) {
-            request_tile(tile + waves, ping);
-            if (tile + 2 * waves < end) find(tile + 2 * waves);
-        }
-        work(tile, pong);
-        tile += waves;
     }
 
-    // ---- the wavefronts' sums together
-    float* const sums = reinterpret_cast<float*>(lds + waves * kWaveLds);  // [wave][row][kDim + 4]
-    constexpr int kStride = kDim + 4;
-    Part* const wave_parts = reinterpret_cast<Part*>(sums + waves * here * kStride);  // [wave][row]
-    const float total = row_sum(sum);
-    const bool row_saw = row_max(saw ? 1.0f : 0.0f) > 0.0f;
-    if (real) {
-        float* to = sums + (wave * here + column) * kStride;
+    // ---- the wavefronts' sums together, each in its ring's place: [row][values], and [row] behind them
+    constexpr int kStride = sums_stride(kDim);
+    const auto sums_of = [&](int w) { return reinterpret_cast<float*>(lds + w * kWaveLds); };
+    const auto parts_of = [&](int w) { return reinterpret_cast<Part*>(lds + w * kWaveLds + kRows * kStride * 4); };
+#pragma unroll
+    for (int qt = 0; qt < kQ; ++qt) {
+        const float total = row_sum(sum[qt]);
+        const bool row_saw = row_max(saw[qt] != 0 ? 1.0f : 0.0f) > 0.0f;
+        const int r = qt * 16 + column;
+        if (r >= here) continue;
+        float* to = sums_of(wave) + r * kStride;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
             for (int w = 0; w < kWords; ++w)
-                *reinterpret_cast<f32x4*>(to + kVec * (4 * quarter + i) + 4 * w) = f32x4{out[4 * w][i], out[4 * w + 1][i], out[4 * w + 2][i], out[4 * w + 3][i]};
+                *reinterpret_cast<f32x4*>(to + kVec * (4 * quarter + i) + 4 * w) = f32x4{out[qt][4 * w][i], out[qt][4 * w + 1][i], out[qt][4 * w + 2][i], out[qt][4 * w + 3][i]};
         }
-        if (quarter == 0) wave_parts[wave * here + column] = Part{!row_saw ? -__builtin_inff() : reference == -__builtin_inff() ? kLowest : reference, total};
+        if (quarter == 0) parts_of(wave)[r] = Part{!row_saw ? -__builtin_inff() : reference[qt] == -__builtin_inff() ? kLowest : reference[qt], total};
     }
     __syncthreads();
     for (int item = tid; item < here * (kDim / 4); item += static_cast<int>(blockDim.x)) {
         const int r = item / (kDim / 4), d = item % (kDim / 4) * 4;
-        if (d >= static_cast<int>(a.cache.head_dim)) continue;
+        if (d >= head_dim) continue;
         float highest = -__builtin_inff();
-        for (int w = 0; w < waves; ++w) highest = fmaxf(highest, wave_parts[w * here + r].most);
+        for (int w = 0; w < waves; ++w) highest = fmaxf(highest, parts_of(w)[r].most);
         f32x4 x{0, 0, 0, 0};
         float all = 0.0f;
         for (int w = 0; w < waves; ++w) {
-            const Part part = wave_parts[w * here + r];
+            const Part part = parts_of(w)[r];
             if (part.most == -__builtin_inff()) continue;
             const float by = exp2_between(part.most, highest);
             all = __builtin_fmaf(part.sum, by, all);
-            const f32x4 y = *reinterpret_cast<const f32x4*>(sums + (w * here + r) * kStride + d);
+            const f32x4 y = *reinterpret_cast<const f32x4*>(sums_of(w) + r * kStride + d);
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(y[j], by, x[j]);
         }
         if (share.splits > 1) {
-            *reinterpret_cast<f32x4*>(part_out + (static_cast<size_t>(slot) * 16 + r) * a.cache.head_dim + d) = x;
-            if (d == 0) parts[static_cast<size_t>(slot) * 16 + r] = Part{highest, all};
+            *reinterpret_cast<f32x4*>(part_out + (static_cast<size_t>(slot) * kRows + r) * a.cache.head_dim + d) = x;
+            if (d == 0) parts[static_cast<size_t>(slot) * kRows + r] = Part{highest, all};
         } else {
             const int whole = first_row + r;
             store4(a, static_cast<size_t>(share.begin + whole / group), kv_head * a.group + static_cast<uint32_t>(whole % group), d, x, all, highest != -__builtin_inff());
@@ -589,41 +714,65 @@ __global__ __launch_bounds__(64 * waves_of(kDim)) void quantized_attention_kerne
     }
 }
 
-// A workgroup has sixteen rows of a request and a key head: a thread four values of a row, over all parts.
-__global__ __launch_bounds__(256) void join_quantized_parts_kernel(QuantizedAttentionArgs a, Plan plan, const float* part_out, const Part* parts) {
+// A workgroup has a row, all its parts: their weights first, then every group of lanes has parts in turn, a lane four values.
+constexpr uint32_t kMostParts = 1100;  // of a request: plan.target is 1024 at most
+__global__ __launch_bounds__(256) void join_quantized_parts_kernel(QuantizedAttentionArgs a, Plan plan, int rows_a_tile, const float* part_out, const Part* parts) {
+    __shared__ float by[kMostParts];
+    __shared__ float numbers[8];
+    __shared__ f32x4 sums[256];
     uint32_t request;
     Share share;
-    if (!find_share<true>(a, plan, blockIdx.y, &request, &share) || share.splits <= 1) return;
-    const uint32_t heads = a.cache.kv_heads, fours = a.cache.head_dim / 4;
-    for (uint32_t number = blockIdx.x; number < share.row_tiles * heads; number += gridDim.x) {
-        const uint32_t kv_head = number / share.row_tiles, row_tile = number % share.row_tiles;
-        const uint32_t rows = min(16u, static_cast<uint32_t>(share.tokens) * a.group - row_tile * 16);
-        const size_t first_slot = share.first_slot + static_cast<size_t>(kv_head) * share.splits * share.row_tiles + row_tile;
-        for (uint32_t item = threadIdx.x; item < rows * fours; item += 256) {
-            const uint32_t r = item / fours, d = item % fours * 4;
-            float highest = -__builtin_inff(), all = 0.0f;
-            f32x4 x{0, 0, 0, 0};
-            for (uint32_t s = 0; s < share.splits; ++s) highest = fmaxf(highest, parts[(first_slot + static_cast<size_t>(s) * share.row_tiles) * 16 + r].most);
-            for (uint32_t s = 0; s < share.splits; ++s) {
-                const size_t at = (first_slot + static_cast<size_t>(s) * share.row_tiles) * 16 + r;
-                const Part part = parts[at];
-                if (part.most == -__builtin_inff()) continue;
-                const float by = exp2_between(part.most, highest);
-                all = __builtin_fmaf(part.sum, by, all);
-                const f32x4 y = *reinterpret_cast<const f32x4*>(part_out + at * a.cache.head_dim + d);
+    if (!find_share<true>(a, plan, rows_a_tile, blockIdx.y, &request, &share) || share.splits <= 1) return;
+    const uint32_t heads = a.cache.kv_heads, fours = a.cache.head_dim / 4, lanes = fours <= 16 ? 16 : fours <= 32 ? 32 : 64, groups = 256 / lanes;
+    const uint32_t tid = threadIdx.x, rows = static_cast<uint32_t>(share.tokens) * a.group, splits = min(share.splits, kMostParts);
+    for (uint32_t number = blockIdx.x; number < rows * heads; number += gridDim.x) {
+        const uint32_t kv_head = number / rows, row = number % rows, row_tile = row / rows_a_tile, r = row % rows_a_tile;
+        const size_t first_slot = share.first_slot + static_cast<size_t>(kv_head) * share.row_tiles + row_tile;
+        const auto part_at = [&](uint32_t s) { return (first_slot + static_cast<size_t>(s) * heads * share.row_tiles) * rows_a_tile + r; };
+        float highest = -__builtin_inff(), all = 0.0f;
+        for (uint32_t s = tid; s < splits; s += 256) highest = fmaxf(highest, parts[part_at(s)].most);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(y[j], by, x[j]);
-            }
-            const uint32_t whole = row_tile * 16 + r;
-            store4(a, static_cast<size_t>(share.begin) + whole / a.group, kv_head * a.group + whole % a.group, static_cast<int>(d), x, all, highest != -__builtin_inff());
+        for (int d = 1; d < 64; d *= 2) highest = fmaxf(highest, __shfl_xor(highest, d));
+        if ((tid & 63) == 0) numbers[tid >> 6] = highest;
+        __syncthreads();
+        highest = fmaxf(fmaxf(numbers[0], numbers[1]), fmaxf(numbers[2], numbers[3]));
+        for (uint32_t s = tid; s < splits; s += 256) {
+            const Part part = parts[part_at(s)];
+            const float w = part.most == -__builtin_inff() ? 0.0f : exp2_between(part.most, highest);
+            by[s] = w;
+            all = __builtin_fmaf(part.sum, w, all);  // (a part that saw nothing has a sum of zero)
         }
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
+        if ((tid & 63) == 0) numbers[4 + (tid >> 6)] = all;
+        __syncthreads();
+        all = (numbers[4] + numbers[5]) + (numbers[6] + numbers[7]);
+        const uint32_t lane = tid % lanes, first = tid / lanes;
+        f32x4 x{0, 0, 0, 0};
+        if (lane < fours) {
+#pragma unroll 4
+            for (uint32_t s = first; s < splits; s += groups) {
+                const f32x4 y = *reinterpret_cast<const f32x4*>(part_out + part_at(s) * a.cache.head_dim + 4 * lane);
+                const float w = by[s];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(w == 0.0f ? 0.0f : y[j], w, x[j]);
+            }
+        }
+        sums[tid] = x;
+        __syncthreads();
+        if (tid < fours) {
+            for (uint32_t g = 1; g < groups; ++g) x += sums[g * lanes + tid];
+            store4(a, static_cast<size_t>(share.begin) + row / a.group, kv_head * a.group + row % a.group, static_cast<int>(4 * tid), x, all, highest != -__builtin_inff());
+        }
+        __syncthreads();
     }
 }
 
 struct Shape {
-    int dim, waves;
+    int dim, sixteens, waves;
     Plan plan;
     uint64_t groups, join_groups;
+    int rows_a_tile() const { return 16 * sixteens; }
 };
 
 constexpr uint32_t kMostShared = 1024;  // requests: every wavefront reads their lengths, 64 at a time
@@ -632,8 +781,10 @@ Shape shape_of(const QuantizedAttentionArgs& a, int compute_units) {
     Shape s;
     s.dim = a.cache.head_dim <= 64 ? 64 : a.cache.head_dim <= 128 ? 128 : 256;
     s.waves = 4;
-    const uint64_t rows = static_cast<uint64_t>(a.max_query_len) * a.group, most_row_tiles = (rows + 15) / 16;
-    uint64_t row_tiles = static_cast<uint64_t>(a.tokens) * a.group / 16 + a.requests;  // of the batch: a request's last may be part empty
+    const uint64_t rows = static_cast<uint64_t>(a.max_query_len) * a.group;
+    s.sixteens = rows <= 16 || s.dim == 256 ? 1 : 2;
+    const uint64_t tile_rows = s.rows_a_tile(), most_row_tiles = (rows + tile_rows - 1) / tile_rows;
+    uint64_t row_tiles = static_cast<uint64_t>(a.tokens) * a.group / tile_rows + a.requests;  // of the batch: a request's last may be part empty
     if (row_tiles > a.requests * most_row_tiles) row_tiles = a.requests * most_row_tiles;
     const uint64_t base = row_tiles * a.cache.kv_heads;
     uint64_t keys = a.max_key_len;
@@ -642,25 +793,28 @@ Shape shape_of(const QuantizedAttentionArgs& a, int compute_units) {
     s.plan.row_tiles = static_cast<uint32_t>(most_row_tiles);
     s.plan.least = 8;
     s.plan.target = 0;
-    const uint64_t resident = 4 * static_cast<uint64_t>(compute_units);
-    if (a.requests <= kMostShared && base < 2 * resident && tiles > 16) s.plan.target = static_cast<uint32_t>(resident);
+    const uint64_t resident = 2 * static_cast<uint64_t>(compute_units < 512 ? compute_units : 512);
+    if (a.requests <= kMostShared && (base < resident || tiles > 160) && tiles > 32) s.plan.target = static_cast<uint32_t>(resident);
+    else if (base < static_cast<uint64_t>(compute_units)) s.waves = most_waves(s.dim);
     s.groups = s.plan.target == 0 ? a.requests * most_row_tiles * a.cache.kv_heads : base + s.plan.target;
     s.plan.slots = s.plan.target == 0 ? 0 : static_cast<uint32_t>(s.groups);
-    s.groups = (s.groups + 8 * most_row_tiles - 1) / (8 * most_row_tiles) * (8 * most_row_tiles);
-    s.join_groups = most_row_tiles * a.cache.kv_heads;
+    const uint64_t together = 8 * most_row_tiles * a.cache.kv_heads;
+    s.groups = (s.groups + together - 1) / together * together;
+    s.join_groups = rows * a.cache.kv_heads;
     if (s.join_groups > 4096) s.join_groups = 4096;
     return s;
 }
 
-size_t part_out_bytes(const QuantizedAttentionArgs& a, const Shape& s) { return (static_cast<size_t>(s.plan.slots) * 16 * a.cache.head_dim * sizeof(float) + 255) / 256 * 256; }
+size_t part_out_bytes(const QuantizedAttentionArgs& a, const Shape& s) {
+    return (static_cast<size_t>(s.plan.slots) * s.rows_a_tile() * a.cache.head_dim * sizeof(float) + 255) / 256 * 256;
+}
 
-template <int kDim, bool kE4m3, int kTerms>
+template <int kDim, bool kE4m3, int kTerms, int kQ>
 hipError_t attend(hipStream_t stream, const QuantizedAttentionArgs& a, const Shape& s, void* workspace) {
     static LdsLimit limit;
-    const uint64_t rows = static_cast<uint64_t>(a.max_query_len) * a.group, here = rows < 16 ? rows : 16;
-    const size_t lds = static_cast<size_t>(s.waves) * (kWaveLds + here * ((kDim + 4) * sizeof(float) + sizeof(Part)));
-    const auto kernel = quantized_attention_kernel<kDim, kE4m3, kTerms>;
-    static_assert(waves_of(kDim) * (kWaveLds + 16 * ((kDim + 4) * sizeof(float) + sizeof(Part))) <= 160 * 1024, "a compute unit's LDS");
+    static_assert(most_waves(kDim) * wave_lds(kDim, 16 * kQ) <= 160 * 1024, "a compute unit's LDS");
+    const size_t lds = static_cast<size_t>(s.waves) * wave_lds(kDim, 16 * kQ);
+    const auto kernel = quantized_attention_kernel<kDim, kE4m3, kTerms, kQ>;
     hipError_t e = allow_lds(kernel, lds, &limit);
     if (e != hipSuccess) return e;
     float* part_out = static_cast<float*>(workspace);
@@ -668,22 +822,30 @@ hipError_t attend(hipStream_t stream, const QuantizedAttentionArgs& a, const Sha
     kernel<<<static_cast<uint32_t>(s.groups), 64 * s.waves, lds, stream>>>(a, s.plan, part_out, parts);
     e = hipGetLastError();
     if (e != hipSuccess || s.plan.slots == 0) return e;
-    join_quantized_parts_kernel<<<dim3(static_cast<uint32_t>(s.join_groups), a.requests), 256, 0, stream>>>(a, s.plan, part_out, parts);
+    join_quantized_parts_kernel<<<dim3(static_cast<uint32_t>(s.join_groups), a.requests), 256, 0, stream>>>(a, s.plan, s.rows_a_tile(), part_out, parts);
     return hipGetLastError();
+}
+
+template <int kDim, bool kE4m3, int kTerms>
+hipError_t attend_rows(hipStream_t stream, const QuantizedAttentionArgs& a, const Shape& s, void* workspace) {
+    if constexpr (kDim != 256) {
+        if (s.sixteens == 2) return attend<kDim, kE4m3, kTerms, 2>(stream, a, s, workspace);
+    }
+    return attend<kDim, kE4m3, kTerms, 1>(stream, a, s, workspace);
 }
 
 template <int kDim, bool kE4m3>
 hipError_t attend_types(hipStream_t stream, const QuantizedAttentionArgs& a, const Shape& s, void* workspace) {
-    if (a.type == 0) return attend<kDim, kE4m3, 3>(stream, a, s, workspace);
-    if (a.type == 1) return attend<kDim, kE4m3, 2>(stream, a, s, workspace);
-    return attend<kDim, kE4m3, 1>(stream, a, s, workspace);
+    if (a.type == 0) return attend_rows<kDim, kE4m3, 3>(stream, a, s, workspace);
+    if (a.type == 1) return attend_rows<kDim, kE4m3, 2>(stream, a, s, workspace);
+    return attend_rows<kDim, kE4m3, 1>(stream, a, s, workspace);
 }
 
 }  // namespace
 
 size_t quantized_attention_workspace_bytes(const QuantizedAttentionArgs& args, int compute_units) {
     const Shape s = shape_of(args, compute_units);
-    return s.plan.slots == 0 ? 0 : part_out_bytes(args, s) + static_cast<size_t>(s.plan.slots) * 16 * sizeof(Part);
+    return s.plan.slots == 0 ? 0 : part_out_bytes(args, s) + static_cast<size_t>(s.plan.slots) * s.rows_a_tile() * sizeof(Part);
 }
 
 bool quantized_attention_fits_a_launch(const QuantizedAttentionArgs& args, int compute_units) {

@@ -194,31 +194,72 @@ def launchTreeAttention(stream, attention: _lib.TreeAttention, workspace: Buffer
 
 # ---- 8-bit caches -----------------------------------------------------------------------------------------------------
 
+_kinds = {}  # of the types that have been seen: (type, bytes of an element)
+_SIZES = {_lib.TYPE_F32: 4, _lib.TYPE_F16: 2, _lib.TYPE_BF16: 2, _lib.TYPE_I8: 1, _lib.TYPE_E4M3: 1, -1: 1}
+_I32, _F32 = ("torch.int32", 4), ("torch.float32", 4)
+
+
+def _kind(dtype):
+    kind = _kinds.get(dtype)
+    if kind is None:
+        name = str(dtype)
+        type = _TYPES.get(name, _CODE_TYPES.get(name, -1))
+        kind = _kinds[dtype] = type, _SIZES[type]
+    return kind
+
+
+def _heads_of(array, size, rows, heads, dim):
+    """(token stride, head stride, address, bytes) of [rows, heads, dim] whose last dimension is contiguous."""
+    strides = array.stride()
+    if array.shape != (rows, heads, dim) or (dim > 1 and strides[2] != 1):
+        raise _bad_shape()
+    token, head = strides[0], strides[1]
+    return token, head, array.data_ptr(), ((rows - 1) * token + (heads - 1) * head + dim) * size if rows and heads else 0
+
+
+def _line(array, dtype, count):
+    """(address, bytes) of a contiguous array [count] of numbers of `dtype`, (name, bytes); None: none."""
+    if array is None:
+        return 0, 0
+    if _name(array.dtype) != dtype[0] or array.shape != (count,) or not array.is_contiguous():
+        raise _bad_shape()
+    return array.data_ptr(), count * dtype[1]
+
+
 def quantizedCache(keys, values, key_scales, value_scales, heads_outside: bool = False) -> _lib.QuantizedCache:
     """keys, values int8 or float8_e4m3fn [blocks, block size, kv heads, head dim] and their scales f32 [blocks, block size, kv
     heads]; with heads_outside [blocks, kv heads, block size(, head dim)]."""
-    shape, strides, scale_strides = keys.shape, keys.stride(), key_scales.stride()
-    if len(shape) != 4 or values.shape != shape or keys.dtype != values.dtype or (values.stride() != strides and not _same_strides(keys, values)) or \
+    shape, strides, scale_strides, dtype = keys.shape, keys.stride(), key_scales.stride(), keys.dtype
+    if len(shape) != 4 or values.shape != shape or values.dtype != dtype or (values.stride() != strides and not _same_strides(keys, values)) or \
             (shape[3] > 1 and strides[3] != 1) or key_scales.shape != shape[:3] or value_scales.shape != shape[:3] or \
             (value_scales.stride() != scale_strides and not _same_strides(key_scales, value_scales)) or \
             _name(key_scales.dtype) != "torch.float32" or _name(value_scales.dtype) != "torch.float32":
         raise _bad_shape()
-    slot, head = (2, 1) if heads_outside else (1, 2)
+    blocks, n1, n2, dim = shape
+    s0, s1, s2, _ = strides
+    t0, t1, t2 = scale_strides
+    held = blocks and n1 and n2 and dim
+    codes = (blocks - 1) * s0 + (n1 - 1) * s1 + (n2 - 1) * s2 + dim if held else 0
+    scales = ((blocks - 1) * t0 + (n1 - 1) * t1 + (n2 - 1) * t2 + 1) * 4 if held else 0
+    if heads_outside:
+        n1, n2, s1, s2, t1, t2 = n2, n1, s2, s1, t2, t1
+    type = _kind(dtype)[0]
     made = _lib.QuantizedCache.from_buffer_copy(_CODES.pack(
-        keys.data_ptr(), _bytes(keys), values.data_ptr(), _bytes(values), key_scales.data_ptr(), _bytes(key_scales), value_scales.data_ptr(),
-        _bytes(value_scales), _CODE_TYPES.get(_name(keys.dtype), -1), shape[0], shape[slot], shape[head], shape[3], strides[0], strides[slot],
-        strides[head], scale_strides[0], scale_strides[slot], scale_strides[head]))
+        keys.data_ptr(), codes, values.data_ptr(), codes, key_scales.data_ptr(), scales, value_scales.data_ptr(), scales, type, blocks, n1,
+        n2, dim, s0, s1, s2, t0, t1, t2))
     made.arrays = (keys, values, key_scales, value_scales)  # alive as long as the description of them is
     return made
 
 
 def _token_rows(cache, keys, values, slots):
     """What a store or a load of tokens [tokens, kv heads, head dim] passes on behind the cache."""
-    shape, strides, dtype = keys.shape, keys.stride(), keys.dtype
-    if values.shape != shape or values.dtype != dtype or (values.stride() != strides and not _same_strides(keys, values)) or \
-            shape != (slots.shape[0], cache.kv_heads, cache.head_dim) or (shape[2] > 1 and strides[2] != 1):
+    tokens, heads, dim = keys.shape
+    dtype = keys.dtype
+    type, size = _kind(dtype)
+    token, head, key_at, held = _heads_of(keys, size, tokens, cache.kv_heads, cache.head_dim)
+    if values.dtype != dtype or values.shape != (tokens, heads, dim) or (values.stride() != keys.stride() and not _same_strides(keys, values)):
         raise _bad_shape()
-    return _TYPES.get(_name(dtype), -1), buffer(keys), buffer(values), strides[0], strides[1], _i32_buffer(slots), shape[0]
+    return type, Buffer(key_at, held), Buffer(values.data_ptr(), held), token, head, Buffer(*_line(slots, _I32, tokens)), tokens
 
 
 def launchQuantizedStore(stream, cache: _lib.QuantizedCache, keys, values, slots) -> None:
@@ -232,15 +273,7 @@ def launchQuantizedLoad(stream, cache: _lib.QuantizedCache, keys, values, slots)
 
 
 _ONE_AXIS = bytes(128)
-
-
-def _weight(array, dim):
-    """(address, bytes) of a head's weights, f32 [dim]; None: no norm."""
-    if array is None:
-        return 0, 0
-    if _name(array.dtype) != "torch.float32" or array.shape != (dim,) or not array.is_contiguous():
-        raise _bad_shape()
-    return array.data_ptr(), array.nbytes
+_NO_HEADS = (0, 0, 0, 0)
 
 
 def headRotation(query, key, out_query, out_key, positions, frequencies, query_weight=None, key_weight=None, epsilon: float = 1e-6,
@@ -249,21 +282,25 @@ def headRotation(query, key, out_query, out_key, positions, frequencies, query_w
     out_key (None for launchRotatedStore), which may be query and key themselves.  positions int32 [tokens] or [axes, tokens],
     frequencies f32 [pairs]: twice as many dimensions turn.  pair_axes: the axis of every pair (all 0 unless given)."""
     tokens, kv_heads, dim = key.shape
-    heads = 0 if query is None else query.shape[1]
-    k = _rows_of_heads(key, tokens, kv_heads, dim)
-    q = o = ok = (0, 0)
+    dtype = key.dtype
+    type, size = _kind(dtype)
+    k_token, k_head, k_at, k_held = _heads_of(key, size, tokens, kv_heads, dim)
+    heads, out_type = 0, type
+    q_token, q_head, q_at, q_held = o_token, o_head, o_at, o_held = ok_token, ok_head, ok_at, ok_held = _NO_HEADS
     if query is not None:
-        q, o = _rows_of_heads(query, tokens, heads, dim), _rows_of_heads(out_query, tokens, heads, dim)
-        if query.dtype != key.dtype or (out_key is not None and out_key.dtype != out_query.dtype):
+        heads, out_dtype = query.shape[1], out_query.dtype
+        out_type, out_size = _kind(out_dtype)
+        if query.dtype != dtype or (out_key is not None and out_key.dtype != out_dtype):
             raise _bad_shape()
+        q_token, q_head, q_at, q_held = _heads_of(query, size, tokens, heads, dim)
+        o_token, o_head, o_at, o_held = _heads_of(out_query, out_size, tokens, heads, dim)
     if out_key is not None:
-        ok = _rows_of_heads(out_key, tokens, kv_heads, dim)
-    out_type = _type(out_query if query is not None else key if out_key is None else out_key)
+        out_type, out_size = _kind(out_key.dtype)
+        ok_token, ok_head, ok_at, ok_held = _heads_of(out_key, out_size, tokens, kv_heads, dim)
     pairs, place = frequencies.shape[0], positions.shape
-    if len(frequencies.shape) != 1 or _name(frequencies.dtype) != "torch.float32" or not frequencies.is_contiguous() or pairs > 128 or \
-            place[-1] != tokens or len(place) > 2:
-        raise _bad_shape()
     axes = place[0] if len(place) == 2 else 1
+    if pairs > 128 or place[-1] != tokens or len(place) > 2 or _name(positions.dtype) != "torch.int32" or not positions.is_contiguous():
+        raise _bad_shape()
     if pair_axes is None:
         packed = _ONE_AXIS
     else:
@@ -273,13 +310,14 @@ def headRotation(query, key, out_query, out_key, positions, frequencies, query_w
             raise _bad_number() from None
         if len(packed) != pairs:
             raise _bad_shape()
+    f_at, f_held = _line(frequencies, _F32, pairs)
+    w_at, w_held = _line(query_weight, _F32, dim)
+    kw_at, kw_held = _line(key_weight, _F32, dim)
     try:
         made = _lib.HeadRotation.from_buffer_copy(_ROTATION.pack(
-            _type(key), out_type, 1 if interleaved else 0, epsilon, tokens, heads, kv_heads, dim, 2 * pairs, axes, *q, *k, *o, *ok,
-            *((query.data_ptr(), _bytes(query)) if query is not None else (0, 0)), key.data_ptr(), _bytes(key),
-            *((out_query.data_ptr(), _bytes(out_query)) if query is not None else (0, 0)),
-            *((out_key.data_ptr(), _bytes(out_key)) if out_key is not None else (0, 0)), *_i32(positions), frequencies.data_ptr(),
-            frequencies.nbytes, *_weight(query_weight, dim), *_weight(key_weight, dim), packed))
+            type, out_type, 1 if interleaved else 0, epsilon, tokens, heads, kv_heads, dim, 2 * pairs, axes, q_token, q_head, k_token, k_head,
+            o_token, o_head, ok_token, ok_head, q_at, q_held, k_at, k_held, o_at, o_held, ok_at, ok_held, positions.data_ptr(),
+            axes * tokens * 4, f_at, f_held, w_at, w_held, kw_at, kw_held, packed))
     except struct.error:
         raise _bad_number() from None
     made.arrays = (query, key, out_query, out_key, positions, frequencies, query_weight, key_weight)
@@ -293,13 +331,14 @@ def launchHeadRotation(stream, rotation: _lib.HeadRotation) -> None:
 def launchRotatedStore(stream, rotation: _lib.HeadRotation, cache, values, slots) -> None:
     """The rotation's queries into out_query, its keys and `values` [tokens, kv heads, head dim] into the slots of `cache` (a
     PagedCache or a QuantizedCache)."""
-    tokens, kv_heads, dim = values.shape
-    if _type(values) != rotation.type or slots.shape[0] != tokens or (tokens, kv_heads, dim) != (rotation.tokens, rotation.kv_heads, rotation.head_dim):
+    tokens = rotation.tokens
+    type, size = _kind(values.dtype)
+    token, head, at, held = _heads_of(values, size, tokens, rotation.kv_heads, rotation.head_dim)
+    if type != rotation.type:
         raise _bad_shape()
-    v_token, v_head = _rows_of_heads(values, tokens, kv_heads, dim)
     quantized = isinstance(cache, _lib.QuantizedCache)
-    check(_lib.lib().afhip_launch_rotated_store(stream, rotation, None if quantized else cache, cache if quantized else None, buffer(values),
-                                                v_token, v_head, _i32_buffer(slots)))
+    check(_lib.lib().afhip_launch_rotated_store(stream, rotation, None if quantized else cache, cache if quantized else None, Buffer(at, held),
+                                                token, head, Buffer(*_line(slots, _I32, tokens))))
 
 
 def quantizedAttention(cache: _lib.QuantizedCache, out, query, query_starts, context_lens, block_tables, max_query_len: int, max_key_len: int,
@@ -308,15 +347,18 @@ def quantizedAttention(cache: _lib.QuantizedCache, out, query, query_starts, con
     head_dim ** -0.5 unless given; softcap 0: scores as they are; window 0: all earlier keys; slopes f32 [heads]."""
     tokens, heads, dim = query.shape
     requests, columns = block_tables.shape
-    q_token, q_head = _rows_of_heads(query, tokens, heads, cache.head_dim)
-    o_token, o_head = _rows_of_heads(out, tokens, heads, cache.head_dim)
-    if out.dtype != query.dtype:
+    dtype = query.dtype
+    type, size = _kind(dtype)
+    if out.dtype != dtype or dim != cache.head_dim:
         raise _bad_shape()
+    q_token, q_head, q_at, q_held = _heads_of(query, size, tokens, heads, dim)
+    o_token, o_head, o_at, o_held = _heads_of(out, size, tokens, heads, dim)
+    s_at, s_held = _line(slopes, _F32, heads)
     try:
         made = _lib.QuantizedAttention.from_buffer_copy(bytes(cache) + _QUANTIZED_REST.pack(
-            _type(query), dim ** -0.5 if scale is None else scale, softcap, window, requests, tokens, heads, max_query_len, max_key_len,
-            columns, q_token, q_head, o_token, o_head, query.data_ptr(), _bytes(query), out.data_ptr(), _bytes(out), *_i32(query_starts),
-            *_i32(context_lens), *_i32(block_tables), *_weight(slopes, heads)))
+            type, dim ** -0.5 if scale is None else scale, softcap, window, requests, tokens, heads, max_query_len, max_key_len, columns,
+            q_token, q_head, o_token, o_head, q_at, q_held, o_at, o_held, *_i32(query_starts), *_i32(context_lens), *_i32(block_tables),
+            s_at, s_held))
     except struct.error:
         raise _bad_number() from None
     made.arrays = (cache, out, query, query_starts, context_lens, block_tables, slopes)

@@ -9,19 +9,10 @@ import struct
 
 from . import _lib
 from ._lib import Buffer, check
-from .paged import NO_BUFFER, _bad_number, _bad_shape, _bytes, _name, _type, buffer
+from .paged import _F32, _I32, NO_BUFFER, _bad_number, _bad_shape, _kind, _line, buffer
 
 _SAMPLE = struct.Struct("i4x19Q")
 assert _SAMPLE.size == C.sizeof(_lib.Sample)
-
-
-def _a_row(array, rows, dtype="torch.float32"):
-    """(address, bytes) of one number a row; None: none."""
-    if array is None:
-        return 0, 0
-    if _name(array.dtype) != dtype or array.shape != (rows,) or not array.is_contiguous():
-        raise _bad_shape()
-    return array.data_ptr(), array.nbytes
 
 
 def sample(logits, tokens, uniforms, temperatures=None, top_k=None, top_p=None, min_p=None, probabilities=None) -> _lib.Sample:
@@ -29,13 +20,15 @@ def sample(logits, tokens, uniforms, temperatures=None, top_k=None, top_p=None, 
     [rows] and probabilities f32 [rows].  uniforms, temperatures, top_p, min_p f32 [rows], top_k int32 [rows]; what is None filters
     nothing, temperatures then are 1."""
     rows, vocab = logits.shape
-    if (vocab > 1 and logits.stride(1) != 1) or tokens is None or uniforms is None:
+    stride, step = logits.stride()
+    if (vocab > 1 and step != 1) or tokens is None or uniforms is None:
         raise _bad_shape()
+    type, size = _kind(logits.dtype)
     try:
         made = _lib.Sample.from_buffer_copy(_SAMPLE.pack(
-            _type(logits), rows, vocab, logits.stride(0), logits.data_ptr(), _bytes(logits), *_a_row(temperatures, rows),
-            *_a_row(top_k, rows, "torch.int32"), *_a_row(top_p, rows), *_a_row(min_p, rows), *_a_row(uniforms, rows),
-            *_a_row(tokens, rows, "torch.int32"), *_a_row(probabilities, rows)))
+            type, rows, vocab, stride, logits.data_ptr(), ((rows - 1) * stride + vocab) * size if rows else 0, *_line(temperatures, _F32, rows),
+            *_line(top_k, _I32, rows), *_line(top_p, _F32, rows), *_line(min_p, _F32, rows), *_line(uniforms, _F32, rows),
+            *_line(tokens, _I32, rows), *_line(probabilities, _F32, rows)))
     except struct.error:
         raise _bad_number() from None
     made.arrays = (logits, tokens, uniforms, temperatures, top_k, top_p, min_p, probabilities)

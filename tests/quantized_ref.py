@@ -54,10 +54,11 @@ def rotation_error(x, weight, y, out, interleaved, pairs):
 
 
 def attend(q, keys, values, key_scales, value_scales, scale, starts, context, table, block, blocks, most_query, most_keys, kind, cap=0.0,
-           window=0, slopes=None):
+           window=0, slopes=None, digits=False):
     """(out, the largest error that the kernel's arithmetic may have), f64 [tokens, heads, dim].  keys, values: code numbers
     [blocks, block, kv heads, dim], scales beside them; kind: of query and out.
 
+    `digits`: queries are whole numbers of 22 bits beside their row's largest value, at least 2^21: half a unit is 2^-22 of that.
     A score is off by its f32 sums (dim additions of exact products, 2^-23 each of the absolute ones), three roundings, and with a cap or
     slopes by tanh's 2^-20 of the cap and one rounding of the bias; a weight by exp's argument, exp2 (2^-22) and by its terms: half a
     step of 8, 16 or 24 bits; the sum over keys by one rounding of 2^-23 a tile of 32 keys, 32 inside it and two a join; the
@@ -86,6 +87,8 @@ def attend(q, keys, values, key_scales, value_scales, scale, starts, context, ta
                 with np.errstate(all="ignore"):
                     s = scale * (kk @ row)
                     wrong = abs(scale) * dim * 2.0 ** -23 * (np.abs(kk) @ np.abs(row)) + 2.0 ** -21 * np.abs(s)
+                    if digits:
+                        wrong = wrong + abs(scale) * 2.0 ** -22 * np.abs(row).max() * np.abs(kk).sum(1)
                     if cap:
                         s = cap * np.tanh(s / cap)
                         wrong = wrong + 2.0 ** -20 * cap

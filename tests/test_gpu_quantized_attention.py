@@ -63,7 +63,8 @@ def check(b, most=None, scale=None, cap=0.0, window=0, slopes=None):
     got = to64(attend(b, most, scale=scale, softcap=cap, window=window, slopes=slopes))
     keys, values, ks, vs = (by_slot(t, b["outside"]) for t in b["tensors"])
     want, off = R.attend(to64(b["q"]), keys, values, ks, vs, b["q"].shape[2] ** -0.5 if scale is None else scale, b["starts"], b["context"], b["table"], b["block"],
-                         b["blocks"], *(most or b["most"]), b["kind"], cap, window, None if slopes is None else slopes.astype(np.float64))
+                         b["blocks"], *(most or b["most"]), b["kind"], cap, window, None if slopes is None else slopes.astype(np.float64),
+                         b["tensors"][0].dtype == torch.int8)
     left = np.isnan(want) & (got == -7)  # tokens past max_query_len are left as they were
     assert np.array_equal(np.isnan(got), np.isnan(want) & ~left)
     wrong = np.where(np.isnan(want), 0, np.abs(got - want)) > off
