@@ -175,7 +175,7 @@ afhip_status sample_args(const afhip_sample* t, SampleArgs* out, bool* empty) {
     if (t == nullptr) return AFHIP_ERR_INVALID_ARGUMENT;
     if (!array_type(t->type)) return AFHIP_ERR_UNSUPPORTED_TENSOR_TYPE;
     if (t->vocab == 0) return AFHIP_ERR_INVALID_STATE;
-    if (t->vocab > (size_t{1} << 24) || !fits_a_launch(t->rows, 1024)) return AFHIP_ERR_OP_UNSUPPORTED;
+    if (t->vocab > (size_t{1} << 24) || t->rows > 65535) return AFHIP_ERR_OP_UNSUPPORTED;
     *empty = t->rows == 0;
     if (!*empty) {
         size_t elements, bytes;

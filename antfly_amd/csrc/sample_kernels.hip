@@ -9,10 +9,15 @@
 // Weights are formed in 64 bits (f64 multiply-adds run at the rate of f32 ones) and summed as whole multiples of 2^-bits: sums are
 // exact, whatever their order, and hang on no atomics' order.
 //
-// A workgroup has a row.  It reads the row once for its largest logit, and once more for the candidates, where a cut is known that
-// leaves few: every thread's own largest logit is at hand after the first pass, and the k-th largest of these is below the k-th
-// largest of all; min-p's cut follows from the largest.  Otherwise the second pass makes a histogram of counts and sums over the
-// logits' range, a third (a fourth) reads the tokens of the bin that a target falls into.
+// A row is shared out over workgroups, and a call is three launches:
+//   most     every part's largest logit, and the largest of every few threads' tokens
+//   spread   with the row's largest known: where a cut is known that leaves few tokens, these into a list (the k-th largest of the
+//            largest logits above is below the k-th largest of all; min-p's cut follows from the largest).  Otherwise a histogram of
+//            counts and sums over the logits' range.  The last workgroup of a row draws from the list, or finds the bins that the
+//            targets can fall into
+//   settle   the tokens of these bins into a list, from which the row's last workgroup draws
+// A list that would not hold what it has to (thousands of equal logits, mostly) leaves the row to one workgroup, which narrows the
+// bins down and counts equal ones.
 #include "quantized_launch.h"
 
 #include <hip/hip_runtime.h>
@@ -21,8 +26,9 @@ namespace afhip {
 
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr uint32_t kBins = 2048, kListed = 4096;
+constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr uint32_t kBins = 1024, kListed = 4096;
+constexpr uint32_t kMostParts = 32, kGroups = kThreads / 4;  // parts of a row, and groups of threads of a part with a largest logit of their own
 constexpr double kLog2e = 1.4426950408889634;
 typedef unsigned long long u64;
 
@@ -83,9 +89,6 @@ struct Shared {
     uint32_t found_count, found_bin, listed, key_low, key_high;
 };
 
-template <typename T>
-__device__ __forceinline__ T shuffled_up(T v, int d) { return __shfl_up(v, d); }
-
 // Sum over all threads, in all of them.
 __device__ __forceinline__ u64 block_sum(u64 v, Shared& s) {
 #pragma unroll
@@ -140,12 +143,12 @@ struct Target {
     }
 };
 
-// Every logit of the row by f(v, i), a thread's own in rising order; no numbers are minus infinity.
+// Tokens [begin, end) of a row (begin a multiple of eight) by f(v, i), a thread's own in rising order; no numbers are minus infinity.
 template <int kType, typename F>
-__device__ __forceinline__ void each_logit(const void* row, uint32_t vocab, F f) {
+__device__ __forceinline__ void each_logit(const void* row, uint32_t begin, uint32_t end, F f) {
     constexpr int kPer = kType == 0 ? 4 : 8;
     struct __attribute__((packed, aligned(kType == 0 ? 4 : 2))) Run { uint32_t words[4]; };  // (rows start at any element)
-    const uint32_t runs = vocab / kPer;
+    const uint32_t runs = end / kPer;
     const auto value = [](uint32_t word, int part) {
         float v;
         if (kType == 0) v = __builtin_bit_cast(float, word);
@@ -159,7 +162,7 @@ __device__ __forceinline__ void each_logit(const void* row, uint32_t vocab, F f)
     };
     const Run* from = static_cast<const Run*>(row);
     constexpr uint32_t kAhead = 4;
-    uint32_t run = threadIdx.x;
+    uint32_t run = begin / kPer + threadIdx.x;
     for (; run + (kAhead - 1) * kThreads < runs; run += kAhead * kThreads) {
         Run held[kAhead];
 #pragma unroll
@@ -168,7 +171,7 @@ __device__ __forceinline__ void each_logit(const void* row, uint32_t vocab, F f)
         for (uint32_t j = 0; j < kAhead; ++j) visit(held[j], run + j * kThreads);
     }
     for (; run < runs; run += kThreads) visit(from[run], run);
-    for (uint32_t i = runs * kPer + threadIdx.x; i < vocab; i += kThreads) {
+    for (uint32_t i = max(runs * kPer, begin) + threadIdx.x; i < end; i += kThreads) {
         const uint32_t word = kType == 0 ? static_cast<const uint32_t*>(row)[i] : static_cast<const uint16_t*>(row)[i];
         f(value(word, 0), i);
     }
@@ -176,10 +179,10 @@ __device__ __forceinline__ void each_logit(const void* row, uint32_t vocab, F f)
 
 // The tokens that `wanted` says, into the list as far as it has room; how many there are.
 template <int kType, typename Wanted>
-__device__ __forceinline__ uint32_t gather(const void* row, uint32_t vocab, Shared& s, Wanted wanted) {
+__device__ __forceinline__ uint32_t gather(const void* row, uint32_t begin, uint32_t end, Shared& s, Wanted wanted) {
     if (threadIdx.x == 0) s.listed = 0;
     __syncthreads();
-    each_logit<kType>(row, vocab, [&](float v, uint32_t i) {
+    each_logit<kType>(row, begin, end, [&](float v, uint32_t i) {
         if (wanted(v)) {
             const uint32_t at = atomicAdd(&s.listed, 1u);
             if (at < kListed) s.list[at] = rank_of(v, i);
@@ -189,59 +192,111 @@ __device__ __forceinline__ uint32_t gather(const void* row, uint32_t vocab, Shar
     return s.listed;
 }
 
-// The list's first n entries in rising order.
-__device__ __forceinline__ void sort_list(uint32_t n, Shared& s) {
-    uint32_t size = 2;
-    while (size < n) size *= 2;
-    for (uint32_t i = n + threadIdx.x; i < size; i += kThreads) s.list[i] = ~0ull;
+// The list's first n entries in rising order: a bitonic sort with kOwn entries a thread, entry r * kThreads + thread in register r.
+// Pairs lie in one thread, in one wavefront or, for three distances of the twelve, go through LDS.
+template <uint32_t kOwn>
+__device__ __forceinline__ void sort_registers(uint32_t n, uint32_t size, Shared& s) {
+    const uint32_t tid = threadIdx.x;
+    u64 own[kOwn];
+#pragma unroll
+    for (uint32_t r = 0; r < kOwn; ++r) own[r] = r * kThreads + tid < n ? s.list[r * kThreads + tid] : ~0ull;
     for (uint32_t k = 2; k <= size; k *= 2) {
         for (uint32_t j = k / 2; j > 0; j /= 2) {
-            __syncthreads();
-            for (uint32_t at = threadIdx.x; at < size / 2; at += kThreads) {
-                const uint32_t i = 2 * at - (at & (j - 1)), other = i + j;
-                const u64 a = s.list[i], b = s.list[other];
-                if ((a > b) == ((i & k) == 0)) {
-                    s.list[i] = b;
-                    s.list[other] = a;
+            if (j >= static_cast<uint32_t>(kThreads)) {
+#pragma unroll
+                for (uint32_t d = 1; d < kOwn; d *= 2) {
+                    if (j != d * kThreads) continue;
+#pragma unroll
+                    for (uint32_t r = 0; r < kOwn; ++r) {
+                        if ((r & d) != 0) continue;
+                        const u64 a = own[r], b = own[r | d];
+                        const bool swaps = (a > b) == (((r * kThreads + tid) & k) == 0);
+                        own[r] = swaps ? b : a;
+                        own[r | d] = swaps ? a : b;
+                    }
                 }
+                continue;
+            }
+            u64 others[kOwn];
+            if (j >= 64) {
+                __syncthreads();
+#pragma unroll
+                for (uint32_t r = 0; r < kOwn; ++r) s.list[r * kThreads + tid] = own[r];
+                __syncthreads();
+#pragma unroll
+                for (uint32_t r = 0; r < kOwn; ++r) others[r] = s.list[r * kThreads + (tid ^ j)];
+            } else {
+#pragma unroll
+                for (uint32_t r = 0; r < kOwn; ++r) others[r] = __shfl_xor(own[r], static_cast<int>(j));
+            }
+#pragma unroll
+            for (uint32_t r = 0; r < kOwn; ++r) {
+                const bool smaller = ((tid & j) == 0) == (((r * kThreads + tid) & k) == 0);  // this place keeps the smaller
+                own[r] = (others[r] < own[r]) == smaller ? others[r] : own[r];
             }
         }
     }
     __syncthreads();
+#pragma unroll
+    for (uint32_t r = 0; r < kOwn; ++r) s.list[r * kThreads + tid] = own[r];
+    __syncthreads();
 }
 
-// The first of the sorted list's n tokens at which the target is passed, counts and sums before the list being given: into
-// found_rank, found_sum (with it), found_before and found_count (with it).  False: none.
-__device__ __forceinline__ bool find_listed(uint32_t n, uint32_t count0, u64 sum0, const Target& target, const Weights& weights, Shared& s) {
-    constexpr uint32_t kEach = kListed / kThreads;
-    const uint32_t first = threadIdx.x * kEach;
-    u64 own[kEach], sum = 0;
-#pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) {
-        own[j] = first + j < n ? weights.of(value_at(s.list[first + j])) : 0;
-        sum += own[j];
-    }
-    uint32_t count;
-    u64 before;
-    block_before(0, sum, s, &count, &before);
-    if (threadIdx.x == 0) s.found_count = 0;
+__device__ __forceinline__ void sort_list(uint32_t n, Shared& s) {
     __syncthreads();
-    before += sum0;
-#pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) {
-        const uint32_t c = count0 + first + j;
-        // (the one at which it passes: not before it, but with it)
-        if (first + j < n && target.passed(c + 1, before + own[j]) && (first + j == 0 || !target.passed(c, before))) {
-            s.found_rank = s.list[first + j];
-            s.found_before = before;
-            s.found_sum = before + own[j];
-            s.found_count = c + 1;
-        }
-        before += own[j];
-    }
-    __syncthreads();
-    return s.found_count != 0;
+    uint32_t size = 2;
+    while (size < n) size *= 2;
+    if (size <= static_cast<uint32_t>(kThreads)) sort_registers<1>(n, size, s);
+    else if (size <= 2u * kThreads) sort_registers<2>(n, size, s);
+    else sort_registers<kListed / kThreads>(n, size, s);
 }
+
+// The weights of the sorted list's n tokens, a run of `each` a thread, and their sum before the thread's.
+struct Listed {
+    static constexpr uint32_t kMost = kListed / kThreads;
+    u64 own[kMost], before, all;
+    uint32_t n, each, first;
+    __device__ __forceinline__ Listed(uint32_t count, const Weights& weights, Shared& s) : n(count), each((count + kThreads - 1) / kThreads), first(threadIdx.x * each) {
+        u64 sum = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kMost; ++j) {
+            own[j] = j < each && first + j < n ? weights.of(value_at(s.list[first + j])) : 0;
+            sum += own[j];
+        }
+        uint32_t unused;
+        block_before(0, sum, s, &unused, &before);
+        all = block_sum(sum, s);
+    }
+    // The first of the tokens [from, until) at which the target is passed, counts and sums before them being given: into found_rank,
+    // found_sum (with it), found_before and found_count (with it).  False: none.
+    __device__ __forceinline__ bool find(uint32_t from, uint32_t until, uint32_t count0, u64 sum0, const Target& target, Shared& s) const {
+        if (threadIdx.x == 0) s.found_count = 0;
+        u64 upto = before;
+#pragma unroll
+        for (uint32_t j = 0; j < kMost; ++j) {
+            if (j < each && first + j == from) s.found_before = upto;  // (of the list's)
+            upto += own[j];
+        }
+        __syncthreads();
+        const u64 base = sum0 - s.found_before;
+        __syncthreads();
+        upto = before;
+#pragma unroll
+        for (uint32_t j = 0; j < kMost; ++j) {
+            const uint32_t at = first + j, c = count0 + at - from;
+            // (the one at which it passes: not before it, but with it)
+            if (j < each && at >= from && at < until && target.passed(c + 1, base + upto + own[j]) && (at == from || !target.passed(c, base + upto))) {
+                s.found_rank = s.list[at];
+                s.found_before = base + upto;
+                s.found_sum = base + upto + own[j];
+                s.found_count = c + 1;
+            }
+            upto += own[j];
+        }
+        __syncthreads();
+        return s.found_count != 0;
+    }
+};
 
 // The j-th (from 1) of the row's tokens with this very logit, by rising index: into found_rank.
 template <int kType>
@@ -316,7 +371,8 @@ __device__ __forceinline__ uint32_t find_bin(const Target& target, uint32_t coun
     for (uint32_t b = threadIdx.x; b < kBins; b += kThreads) {
         const uint32_t c = s.counts[b], next_c = b + 1 < kBins ? s.counts[b + 1] : all_count;
         const u64 m = s.sums[b], next_m = b + 1 < kBins ? s.sums[b + 1] : all_sum;
-        if (next_c > c && target.passed(count0 + next_c, sum0 + next_m) && (c == 0 || !target.passed(count0 + c, sum0 + m))) s.found_bin = b;
+        const bool holds = target.count != 0 ? next_c > c : next_m > m, is_first = target.count != 0 ? c == 0 : m == 0;  // (counts may be left out)
+        if (holds && target.passed(count0 + next_c, sum0 + next_m) && (is_first || !target.passed(count0 + c, sum0 + m))) s.found_bin = b;
     }
     __syncthreads();
     return s.found_bin;
@@ -331,10 +387,10 @@ __device__ bool locate(const void* row, uint32_t vocab, const Histogram& histogr
     if (bin == kBins) return false;
     uint32_t count0 = s.counts[bin];
     u64 sum0 = s.sums[bin];
-    uint32_t n = gather<kType>(row, vocab, s, [&](float v) { return histogram.holds(v) && histogram.bin(v) == bin; });
+    uint32_t n = gather<kType>(row, 0, vocab, s, [&](float v) { return histogram.holds(v) && histogram.bin(v) == bin; });
     if (n <= kListed) {
         sort_list(n, s);
-        return find_listed(n, count0, sum0, target, weights, s);
+        return Listed(n, weights, s).find(0, n, count0, sum0, target, s);
     }
     *fresh = false;
     // the bin's range of keys, halved by as many bins as there are until it holds few tokens, or one logit
@@ -344,7 +400,7 @@ __device__ bool locate(const void* row, uint32_t vocab, const Histogram& histogr
     }
     __syncthreads();
     uint32_t low = ~0u, high = 0;
-    each_logit<kType>(row, vocab, [&](float v, uint32_t) {
+    each_logit<kType>(row, 0, vocab, [&](float v, uint32_t) {
         if (histogram.holds(v) && histogram.bin(v) == bin) {
             low = min(low, key_of(v));
             high = max(high, key_of(v));
@@ -375,10 +431,10 @@ __device__ bool locate(const void* row, uint32_t vocab, const Histogram& histogr
             __syncthreads();
             return true;
         }
-        const int shift = max(0, 32 - __builtin_clz(high - low) - 11);
+        const int shift = max(0, 32 - __builtin_clz(high - low) - 10);  // 2^10 bins
         __syncthreads();
         clear_bins(s);
-        each_logit<kType>(row, vocab, [&](float v, uint32_t) {
+        each_logit<kType>(row, 0, vocab, [&](float v, uint32_t) {
             const uint32_t key = key_of(v);
             if (key >= low && key <= high && v > -__builtin_inff()) {
                 const uint32_t b = (high - key) >> shift;
@@ -395,62 +451,198 @@ __device__ bool locate(const void* row, uint32_t vocab, const Histogram& histogr
         count0 += s.counts[b];
         sum0 += s.sums[b];
         const uint32_t from = high - (b << shift);
-        low = max(low, from - ((1u << shift) - 1));
+        low = max(low, from - ((1u << shift) - 1));  // (the bin's lowest key)
         high = from;
-        n = gather<kType>(row, vocab, s, [&](float v) { const uint32_t key = key_of(v); return key >= low && key <= high && v > -__builtin_inff(); });
+        n = gather<kType>(row, 0, vocab, s, [&](float v) { const uint32_t key = key_of(v); return key >= low && key <= high && v > -__builtin_inff(); });
         if (n <= kListed) {
             sort_list(n, s);
-            return find_listed(n, count0, sum0, target, weights, s);
+            return Listed(n, weights, s).find(0, n, count0, sum0, target, s);
         }
     }
 }
 
-template <int kType>
-__global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
-    __shared__ Shared s;
-    const uint32_t r = blockIdx.x, tid = threadIdx.x;
-    const void* row = static_cast<const char*>(a.logits) + r * a.row_stride * (kType == 0 ? 4 : 2);
-    const float temperature = a.temperatures != nullptr ? a.temperatures[r] : 1.0f, p = a.top_p != nullptr ? a.top_p[r] : 1.0f;
-    const float least = a.min_p != nullptr ? a.min_p[r] : 0.0f;
-    float u = a.uniforms[r];
-    uint32_t k = a.top_k != nullptr && a.top_k[r] > 0 ? static_cast<uint32_t>(a.top_k[r]) : 0u;
-    if (k >= a.vocab) k = 0;
-    const bool has_p = p < 1.0f, has_least = least > 0.0f;
-    if (!(u > 0.0f)) u = 0.0f;
+// What a call's launches pass on of a row.
+enum : uint32_t { kDone, kWide, kNarrow };  // drawn; for one workgroup; tokens of some bins are wanted
+struct Wanted {                             // bins that a target can fall into, and what is before them
+    uint32_t first, last, count;
+    u64 sum;
+};
+struct Row {
+    uint32_t spread_arrived, settle_arrived, listed, state;
+    float top, cut;
+    Wanted of_k, of_p, of_u;
+    u64 all, weighty;
+    uint32_t all_count;
+};
+struct Scratch {
+    Row* rows;
+    u64* best;         // [rows][parts]: ranks
+    float* groups;     // [rows][parts][kGroups]
+    u64* lists;        // [rows][kListed], as the next two only where a row has several parts
+    u64* sums;         // [rows][parts][kBins + 1]: the last the sum of what weighs enough for min-p
+    uint32_t* counts;  // [rows][parts][kBins]
+    uint32_t parts, part_len;
+};
 
-    // ---- the largest
+// What a row's filters ask for.
+struct Wishes {
+    float temperature, p, least, u;
+    uint32_t k;
+    bool has_p, has_least;
+    __device__ __forceinline__ Wishes(const SampleArgs& a, uint32_t r) {
+        temperature = a.temperatures != nullptr ? a.temperatures[r] : 1.0f;
+        p = a.top_p != nullptr ? a.top_p[r] : 1.0f;
+        least = a.min_p != nullptr ? a.min_p[r] : 0.0f;
+        u = a.uniforms[r];
+        k = a.top_k != nullptr && a.top_k[r] > 0 ? static_cast<uint32_t>(a.top_k[r]) : 0u;
+        if (k >= a.vocab) k = 0;
+        has_p = p < 1.0f;
+        has_least = least > 0.0f;
+        if (!(u > 0.0f)) u = 0.0f;
+    }
+    // The target of the drawn token among tokens of this sum.
+    __device__ __forceinline__ Target draw(u64 kept) const {
+        return u >= 1.0f ? Target{0, static_cast<double>(kept), false} : Target{0, static_cast<double>(u) * static_cast<double>(kept), true};
+    }
+    __device__ __forceinline__ Target nucleus(u64 kept) const { return Target{0, static_cast<double>(p) * static_cast<double>(kept), false}; }
+};
+
+__device__ __forceinline__ Weights weights_of(float top, float temperature, uint32_t vocab) {
+    Weights w;
+    w.largest = static_cast<double>(top);
+    w.per_logit = kLog2e / static_cast<double>(temperature);
+    w.top = top;
+    w.bits = min(50, 62 - (32 - __builtin_clz(vocab - 1 | 1)));  // (the sum of all stays below 2^62)
+    return w;
+}
+
+__device__ __forceinline__ Histogram histogram_of(float top, float cut) {
+    Histogram h{top, cut, 0.0f};
+    h.scale = top > cut && top < __builtin_inff() ? static_cast<float>(kBins - 1) / (top - cut) : 0.0f;
+    return h;
+}
+
+__device__ __forceinline__ const void* row_of(const SampleArgs& a, uint32_t r, int size) { return static_cast<const char*>(a.logits) + r * a.row_stride * size; }
+
+__device__ __forceinline__ void put(const SampleArgs& a, uint32_t r, int token, float probability) {
+    a.tokens[r] = token;
+    if (a.probabilities != nullptr) a.probabilities[r] = probability;
+}
+__device__ __forceinline__ void put_drawn(const SampleArgs& a, uint32_t r, u64 rank, const Weights& w, u64 kept) {
+    put(a, r, static_cast<int>(static_cast<uint32_t>(rank)), static_cast<float>(w.fraction(value_at(rank)) * static_cast<double>(1ull << w.bits) / static_cast<double>(kept)));
+}
+
+// What a row's workgroups tell one another within a launch goes past the caches that they do not share (relaxed atomics of the
+// device's scope): a fence for all else that they wrote would write back and drop an XCD's whole L2, some 20 us of every workgroup.
+template <typename T>
+__device__ __forceinline__ void tell(T* to, T v) { __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename T>
+__device__ __forceinline__ T told(const T* from) { return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// Whether this is the last of the row's workgroups to come here; all that the others told is there then.
+__device__ __forceinline__ bool last_of(uint32_t* arrived, uint32_t parts, Shared& s) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what this thread told has arrived
+    __syncthreads();
+    if (threadIdx.x == 0) s.found_bin = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    const bool last = s.found_bin == parts - 1;
+    __syncthreads();
+    return last;
+}
+
+// The row's tokens that `wants` says into the list in LDS, by its parts: true for the last of them, which has them all (as far as
+// there is room; *n: how many there are).
+template <int kType, typename Wants>
+__device__ __forceinline__ bool list_row(const SampleArgs& a, const Scratch& scratch, uint32_t r, uint32_t part, uint32_t* arrived, Shared& s, Wants wants, uint32_t* n) {
+    const void* row = row_of(a, r, kType == 0 ? 4 : 2);
+    const uint32_t begin = part * scratch.part_len, end = min(begin + scratch.part_len, a.vocab);
+    *n = gather<kType>(row, begin, end, s, wants);
+    if (scratch.parts == 1) return true;
+    // behind the other parts' (one addition a part: thousands to one place of memory would follow one another)
+    Row* const state = scratch.rows + r;
+    u64* const list = scratch.lists + static_cast<size_t>(r) * kListed;
+    if (threadIdx.x == 0) s.found_count = __hip_atomic_fetch_add(&state->listed, *n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    const uint32_t at = s.found_count;
+    for (uint32_t i = threadIdx.x; i < min(*n, kListed) && at + i < kListed; i += kThreads) tell(list + at + i, s.list[i]);
+    if (!last_of(arrived, scratch.parts, s)) return false;
+    *n = told(&state->listed);
+    for (uint32_t i = threadIdx.x; i < min(*n, kListed); i += kThreads) s.list[i] = told(list + i);
+    __syncthreads();
+    return true;
+}
+
+template <int kType>
+__global__ __launch_bounds__(kThreads) void most_kernel(SampleArgs a, Scratch scratch) {
+    __shared__ u64 ranks[kWaves];
+    const uint32_t r = blockIdx.y, part = blockIdx.x, begin = part * scratch.part_len, end = min(begin + scratch.part_len, a.vocab);
     float most = -__builtin_inff();
     uint32_t most_at = 0xFFFFFFFFu;
-    each_logit<kType>(row, a.vocab, [&](float v, uint32_t i) {
+    each_logit<kType>(row_of(a, r, kType == 0 ? 4 : 2), begin, end, [&](float v, uint32_t i) {
         if (v > most) {
             most = v;
             most_at = i;
         }
     });
+    float four = fmaxf(most, __shfl_xor(most, 1));
+    four = fmaxf(four, __shfl_xor(four, 2));
+    if ((threadIdx.x & 3) == 0) scratch.groups[(static_cast<size_t>(r) * scratch.parts + part) * kGroups + threadIdx.x / 4] = four;
     u64 best = rank_of(most, most_at);
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
         const u64 other = __shfl_xor(best, d);
         best = other < best ? other : best;
     }
-    if ((tid & 63) == 0) s.wave_ranks[tid >> 6] = best;
+    if ((threadIdx.x & 63) == 0) ranks[threadIdx.x >> 6] = best;
     __syncthreads();
+    if (threadIdx.x == 0) {
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) best = s.wave_ranks[w] < best ? s.wave_ranks[w] : best;
-    const float top = value_at(best);
-    if (top == -__builtin_inff() || !(temperature > 0.0f)) {
-        if (tid == 0) {
-            a.tokens[r] = top == -__builtin_inff() ? -1 : static_cast<int>(static_cast<uint32_t>(best));
-            if (a.probabilities != nullptr) a.probabilities[r] = top == -__builtin_inff() ? 0.0f : 1.0f;
+        for (int w = 0; w < kWaves; ++w) best = ranks[w] < best ? ranks[w] : best;
+        scratch.best[static_cast<size_t>(r) * scratch.parts + part] = best;
+        if (part == 0) {
+            Row* state = scratch.rows + r;
+            state->spread_arrived = state->settle_arrived = state->listed = 0;
+            state->state = kDone;
         }
+    }
+}
+
+// Draws from a row's first tokens, all that its filters can keep, in the sorted list.
+__device__ __forceinline__ void draw_listed(const SampleArgs& a, uint32_t r, const Wishes& wishes, const Weights& weights, uint32_t n, u64 best, Shared& s) {
+    const u64 one = 1ull << weights.bits;
+    const double least_sum = static_cast<double>(wishes.least) * static_cast<double>(one);
+    const uint32_t ranked = wishes.k != 0 && wishes.k < n ? wishes.k : n;
+    const Listed listed(ranked, weights, s);
+    u64 kept = listed.all;
+    if (wishes.has_p) {
+        if (listed.find(0, ranked, 0, 0, wishes.nucleus(kept), s)) kept = s.found_sum;
+        __syncthreads();
+    }
+    if (wishes.has_least) {
+        u64 over = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < Listed::kMost; ++j) over += static_cast<double>(listed.own[j]) >= least_sum ? listed.own[j] : 0;
+        kept = min(kept, block_sum(over, s));
+    }
+    kept = max(kept, one);
+    const bool found = listed.find(0, ranked, 0, 0, wishes.draw(kept), s);
+    if (threadIdx.x == 0) put_drawn(a, r, found ? s.found_rank : best, weights, kept);
+}
+
+template <int kType>
+__global__ __launch_bounds__(kThreads) void spread_kernel(SampleArgs a, Scratch scratch) {
+    __shared__ Shared s;
+    const uint32_t r = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, parts = scratch.parts;
+    const uint32_t begin = part * scratch.part_len, end = min(begin + scratch.part_len, a.vocab);
+    const Wishes wishes(a, r);
+    u64 best = ~0ull;
+    for (uint32_t i = 0; i < parts; ++i) best = min(best, scratch.best[static_cast<size_t>(r) * parts + i]);
+    const float top = value_at(best);
+    if (top == -__builtin_inff() || !(wishes.temperature > 0.0f)) {
+        if (part == 0 && tid == 0) put(a, r, top == -__builtin_inff() ? -1 : static_cast<int>(static_cast<uint32_t>(best)), top == -__builtin_inff() ? 0.0f : 1.0f);
         return;
     }
-
-    Weights weights;
-    weights.largest = static_cast<double>(top);
-    weights.per_logit = kLog2e / static_cast<double>(temperature);
-    weights.top = top;
-    weights.bits = min(50, 62 - (32 - __builtin_clz(a.vocab - 1 | 1)));  // (the sum of all stays below 2^62)
+    const Weights weights = weights_of(top, wishes.temperature, a.vocab);
     const u64 one = 1ull << weights.bits;
 
     // ---- below which logit no token can be kept, or count in a sum: the logits' own roundings and the division's leave a margin
@@ -460,71 +652,173 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     };
     float cut = top == __builtin_inff() ? top : cut_at(-1.5 - weights.bits);
     bool few = false;  // whether the cut is likely to leave a list
-    constexpr uint32_t kMostRanked = kThreads;
-    if (k != 0 && k <= kMostRanked) {
-        // the k-th largest of the threads' largest, bit by bit
-        const uint32_t mine = key_of(most);
+    const uint32_t groups = parts * kGroups;
+    if (wishes.k != 0 && wishes.k <= groups) {
+        // the k-th largest of the groups' largest, bit by bit: with the lowest 14 of them left zero it is a bound as well
+        constexpr uint32_t kOwn = kMostParts * kGroups / kThreads;
+        uint32_t keys[kOwn];
+#pragma unroll
+        for (uint32_t j = 0; j < kOwn; ++j) keys[j] = tid + j * kThreads < groups ? key_of(scratch.groups[static_cast<size_t>(r) * groups + tid + j * kThreads]) : 0u;
         uint32_t found = 0;
-        for (int bit = 31; bit >= 0; --bit) {
+        for (int bit = 31; bit >= 14; --bit) {
             const uint32_t with = found | 1u << bit;
-            if (static_cast<uint32_t>(__syncthreads_count(mine >= with)) >= k) found = with;
+            uint32_t own = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < kOwn; ++j) own += __popcll(__ballot(keys[j] >= with));
+            uint32_t* counts = s.counts + (bit & 1) * kWaves;  // (two in turn: one barrier a bit)
+            if ((tid & 63) == 0) counts[tid >> 6] = own;
+            __syncthreads();
+            uint32_t all = 0;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) all += counts[w];
+            if (all >= wishes.k) found = with;
         }
         const float kth = value_of(found);
         if (kth > cut) cut = kth;
         few = true;
     }
-    if (has_least && !has_p && top < __builtin_inff()) {
-        const float at = cut_at(least >= 1.0f ? 0.0 : static_cast<double>(__builtin_log2f(least)) - 1e-4);
+    if (wishes.has_least && !wishes.has_p && top < __builtin_inff()) {
+        const float at = cut_at(wishes.least >= 1.0f ? 0.0 : static_cast<double>(__builtin_log2f(wishes.least)) - 1e-4);
         if (at > cut) cut = at;
         few = true;
     }
     cut = fminf(fmaxf(cut, -3.402823466e38f), top);  // (minus infinity counts for nothing)
-    const double least_sum = static_cast<double>(least) * static_cast<double>(one);
+    Row* const state = scratch.rows + r;
 
-    u64 kept = 0;
-    bool found = false;
     if (few) {
-        const uint32_t n = gather<kType>(row, a.vocab, s, [&](float v) { return v >= cut; });
-        if (n <= kListed) {
-            sort_list(n, s);
-            constexpr uint32_t kEach = kListed / kThreads;
-            const uint32_t ranked = k != 0 && k < n ? k : n;
-            u64 upto = 0, over = 0;
-#pragma unroll
-            for (uint32_t j = 0; j < kEach; ++j) {
-                const uint32_t i = tid * kEach + j;
-                if (i < ranked) {
-                    const u64 w = weights.of(value_at(s.list[i]));
-                    upto += w;
-                    if (!has_least || static_cast<double>(w) >= least_sum) over += w;
-                }
+        uint32_t n;
+        if (!list_row<kType>(a, scratch, r, part, &state->spread_arrived, s, [&](float v) { return v >= cut; }, &n)) return;
+        if (n > kListed) {
+            if (tid == 0) {
+                state->state = kWide;
+                state->top = top;
+                state->cut = cut;
             }
-            kept = block_sum(upto, s);
-            if (has_p) {
-                find_listed(ranked, 0, 0, Target{0, static_cast<double>(p) * static_cast<double>(kept), false}, weights, s);
-                kept = s.found_sum;
-                __syncthreads();
-            }
-            const u64 weighty = block_sum(over, s);
-            kept = min(kept, weighty);
-            kept = max(kept, one);
-            const double target = static_cast<double>(u) * static_cast<double>(kept);
-            const bool last = u >= 1.0f;
-            found = find_listed(ranked, 0, 0, Target{0, last ? static_cast<double>(kept) : target, !last}, weights, s);
+            return;
         }
+        sort_list(n, s);
+        draw_listed(a, r, wishes, weights, n, best, s);
+        return;
     }
-    if (!found) {
-        Histogram histogram{top, cut, 0.0f};
-        histogram.scale = top > cut && top < __builtin_inff() ? static_cast<float>(kBins - 1) / (top - cut) : 0.0f;
-        uint32_t all_count = 0;
-        u64 all = 0, weighty = 0;
-        bool fresh = false;
-        const auto fill = [&] {
-            if (fresh) return;
+
+    // Lanes take turns among four copies of the sums, in the list's place: neighbouring tokens' bins are often the same, and additions
+    // to one place of LDS follow one another.  Counts are made where top-k asks for them.
+    const Histogram histogram = histogram_of(top, cut);
+    const double least_sum = static_cast<double>(wishes.least) * static_cast<double>(one);
+    const bool counted = wishes.k != 0;
+    constexpr uint32_t kCopies = kListed / kBins;
+    __syncthreads();
+    clear_bins(s);
+    for (uint32_t b = tid; b < kListed; b += kThreads) s.list[b] = 0;
+    __syncthreads();
+    u64 over = 0;
+    each_logit<kType>(row_of(a, r, kType == 0 ? 4 : 2), begin, end, [&](float v, uint32_t) {
+        if (histogram.holds(v)) {
+            const uint32_t b = histogram.bin(v);
+            const u64 w = weights.of(v);
+            if (counted) atomicAdd(&s.counts[b], 1u);
+            atomicAdd(&s.list[b * kCopies + (tid & (kCopies - 1))], w);
+            if (static_cast<double>(w) >= least_sum) over += w;
+        }
+    });
+    __syncthreads();
+    for (uint32_t b = tid; b < kBins; b += kThreads) {
+        u64 sum = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kCopies; ++i) sum += s.list[b * kCopies + i];
+        s.sums[b] = sum;
+    }
+    __syncthreads();
+    over = block_sum(over, s);
+    u64* const sums = scratch.sums + static_cast<size_t>(r) * parts * (kBins + 1);
+    uint32_t* const counts = scratch.counts + static_cast<size_t>(r) * parts * kBins;
+    if (parts > 1) {
+        for (uint32_t b = tid; b < kBins; b += kThreads) {
+            tell(sums + part * (kBins + 1) + b, s.sums[b]);
+            if (counted) tell(counts + part * kBins + b, s.counts[b]);
+        }
+        if (tid == 0) tell(sums + part * (kBins + 1) + kBins, over);
+        if (!last_of(&state->spread_arrived, parts, s)) return;
+        for (uint32_t b = tid; b < kBins; b += kThreads) {
+            u64 sum = 0;
+            uint32_t count = 0;
+            for (uint32_t i = 0; i < parts; ++i) {
+                sum += told(sums + i * (kBins + 1) + b);
+                if (counted) count += told(counts + i * kBins + b);
+            }
+            s.sums[b] = sum;
+            s.counts[b] = count;
+        }
+        over = 0;
+        for (uint32_t i = 0; i < parts; ++i) over += told(sums + i * (kBins + 1) + kBins);
+        __syncthreads();
+    }
+
+    // ---- the bins that the filters' and the draw's targets can fall into: what the earlier ones leave is known to a bin
+    uint32_t all_count;
+    u64 all;
+    scan_bins(s, &all_count, &all);
+    const auto before = [&](uint32_t bin) { return bin < kBins ? s.sums[bin] : all; };
+    const auto bin_of = [&](const Target& target) { return min(find_bin(target, 0, 0, all_count, all, s), kBins - 1); };
+    const auto wanted = [&](uint32_t first, uint32_t last) { return Wanted{first, last, s.counts[first], s.sums[first]}; };
+    const Wanted none{1, 0, 0, 0};
+    Wanted of_k = none, of_p = none;
+    u64 low = all, high = all;  // between which the sum of what is kept so far lies
+    if (wishes.k != 0 && wishes.k < all_count) {
+        const uint32_t b = bin_of(Target{wishes.k, 0.0, false});
+        of_k = wanted(b, b);
+        low = before(b);
+        high = before(b + 1);
+    }
+    if (wishes.has_p) {
+        const uint32_t first = bin_of(wishes.nucleus(low));
+        __syncthreads();
+        const uint32_t last = low == high ? first : bin_of(wishes.nucleus(high));
+        of_p = wanted(first, last);
+        low = before(first);
+        high = before(last + 1);
+    }
+    if (wishes.has_least) {
+        low = min(low, over);
+        high = min(high, over);
+    }
+    low = max(low, one);
+    high = max(high, one);
+    __syncthreads();
+    const uint32_t first = bin_of(wishes.draw(low));
+    __syncthreads();
+    const uint32_t last = low == high ? first : bin_of(wishes.draw(high));
+    if (tid == 0) {
+        state->of_k = of_k;
+        state->of_p = of_p;
+        state->of_u = wanted(first, max(first, last));
+        state->all = all;
+        state->weighty = over;
+        state->all_count = all_count;
+        state->top = top;
+        state->cut = cut;
+        state->state = kNarrow;
+    }
+}
+
+// A row by one workgroup, whatever it holds.
+template <int kType>
+__device__ __forceinline__ void draw_wide(const SampleArgs& a, uint32_t r, float top, float cut, u64 best, Shared& s) {
+    const Wishes wishes(a, r);
+    const void* row = row_of(a, r, kType == 0 ? 4 : 2);
+    const Weights weights = weights_of(top, wishes.temperature, a.vocab);
+    const Histogram histogram = histogram_of(top, cut);
+    const u64 one = 1ull << weights.bits;
+    const double least_sum = static_cast<double>(wishes.least) * static_cast<double>(one);
+    uint32_t all_count = 0;
+    u64 all = 0, weighty = 0, kept = 0;
+    bool fresh = false, found = false;
+    for (int step = 0; step < 3; ++step) {  // the first k, the nucleus, the draw
+        if (!fresh) {
             __syncthreads();
             clear_bins(s);
             u64 over = 0;
-            each_logit<kType>(row, a.vocab, [&](float v, uint32_t) {
+            each_logit<kType>(row, 0, a.vocab, [&](float v, uint32_t) {
                 if (histogram.holds(v)) {
                     const uint32_t b = histogram.bin(v);
                     const u64 w = weights.of(v);
@@ -537,40 +831,125 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
             weighty = block_sum(over, s);
             scan_bins(s, &all_count, &all);
             fresh = true;
-        };
-        fill();
-        kept = all;
-        if (k != 0 && k < all_count) {
-            if (locate<kType>(row, a.vocab, histogram, all_count, all, Target{k, 0.0, false}, weights, s, &fresh)) kept = s.found_sum;
-            __syncthreads();
         }
-        if (has_p) {
-            fill();
-            if (locate<kType>(row, a.vocab, histogram, all_count, all, Target{0, static_cast<double>(p) * static_cast<double>(kept), false}, weights, s, &fresh)) kept = s.found_sum;
-            __syncthreads();
+        if (step == 0) kept = all;
+        if (step == 2) kept = max(wishes.has_least ? min(kept, weighty) : kept, one);
+        if ((step == 0 && (wishes.k == 0 || wishes.k >= all_count)) || (step == 1 && !wishes.has_p)) continue;
+        const Target target = step == 0 ? Target{wishes.k, 0.0, false} : step == 1 ? wishes.nucleus(kept) : wishes.draw(kept);
+        found = locate<kType>(row, a.vocab, histogram, all_count, all, target, weights, s, &fresh);
+        if (found && step < 2) kept = s.found_sum;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) put_drawn(a, r, found ? s.found_rank : best, weights, kept);
+}
+
+template <int kType>
+__global__ __launch_bounds__(kThreads, 4) void settle_kernel(SampleArgs a, Scratch scratch) {
+    __shared__ Shared s;
+    const uint32_t r = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, parts = scratch.parts;
+    Row* const state = scratch.rows + r;
+    const uint32_t todo = state->state;
+    if (todo == kDone || (todo == kWide && part != 0)) return;
+    const float top = state->top, cut = state->cut;
+    u64 best = ~0ull;
+    for (uint32_t i = 0; i < parts; ++i) best = min(best, scratch.best[static_cast<size_t>(r) * parts + i]);
+    bool wide = todo == kWide;
+    const Wishes wishes(a, r);
+    const Weights weights = weights_of(top, wishes.temperature, a.vocab);
+    const Histogram histogram = histogram_of(top, cut);
+    const Wanted of_k = state->of_k, of_p = state->of_p, of_u = state->of_u;
+    const auto in = [](const Wanted& w, uint32_t b) { return b >= w.first && b <= w.last; };
+    const auto wants = [&](float v) {
+        const uint32_t b = histogram.bin(v);
+        return histogram.holds(v) && (in(of_u, b) || in(of_p, b) || in(of_k, b));
+    };
+    uint32_t n = 0;
+    if (!wide) {
+        if (!list_row<kType>(a, scratch, r, part, &state->settle_arrived, s, wants, &n)) return;
+        wide = n > kListed;
+    }
+    if (wide) {
+        draw_wide<kType>(a, r, top, cut, best, s);
+        return;
+    }
+    sort_list(n, s);
+    const Listed listed(n, weights, s);
+    // the run of the list that is of these bins
+    const auto find = [&](const Wanted& w, const Target& target) {
+        uint32_t mine = 0, within = 0;
+        for (uint32_t i = tid; i < n; i += kThreads) {
+            const uint32_t b = histogram.bin(value_at(s.list[i]));
+            mine += b < w.first;
+            within += in(w, b);
         }
-        if (has_least) kept = min(kept, weighty);
-        kept = max(kept, one);
-        fill();
-        const bool last = u >= 1.0f;
-        found = locate<kType>(row, a.vocab, histogram, all_count, all, Target{0, last ? static_cast<double>(kept) : static_cast<double>(u) * static_cast<double>(kept), !last}, weights, s, &fresh);
+        const u64 both = block_sum(static_cast<u64>(mine) << 32 | within, s);
+        const uint32_t from = static_cast<uint32_t>(both >> 32);
+        return listed.find(from, from + static_cast<uint32_t>(both), w.count, w.sum, target, s);
+    };
+    u64 kept = state->all;
+    if (of_k.first <= of_k.last) {
+        if (find(of_k, Target{wishes.k, 0.0, false})) kept = s.found_sum;
+        __syncthreads();
     }
-    if (tid == 0) {
-        const u64 rank = found ? s.found_rank : best;
-        a.tokens[r] = static_cast<int>(static_cast<uint32_t>(rank));
-        if (a.probabilities != nullptr) a.probabilities[r] = static_cast<float>(weights.fraction(value_at(rank)) * static_cast<double>(one) / static_cast<double>(kept));
+    if (wishes.has_p) {
+        if (find(of_p, wishes.nucleus(kept))) kept = s.found_sum;
+        __syncthreads();
     }
+    if (wishes.has_least) kept = min(kept, state->weighty);
+    kept = max(kept, 1ull << weights.bits);
+    const bool found = find(of_u, wishes.draw(kept));
+    if (tid == 0) put_drawn(a, r, found ? s.found_rank : best, weights, kept);
+}
+
+struct Layout {
+    uint32_t parts, part_len;
+    size_t best, groups, lists, sums, counts, bytes;  // where they begin, behind the rows' states
+};
+
+// A row's parts: as many as give the units a few workgroups each, of 4096 tokens at least.
+Layout layout_of(const SampleArgs& a, int compute_units) {
+    Layout l{};
+    const uint64_t wanted = (8 * static_cast<uint64_t>(compute_units) + a.rows - 1) / a.rows, most = (a.vocab + 4095) / 4096;
+    l.parts = static_cast<uint32_t>(wanted < most ? wanted : most);
+    if (l.parts > kMostParts) l.parts = kMostParts;
+    l.part_len = ((a.vocab + l.parts - 1) / l.parts + 7) / 8 * 8;
+    l.parts = (a.vocab + l.part_len - 1) / l.part_len;
+    const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    const size_t rows = a.rows, all = rows * l.parts;
+    l.best = up(rows * sizeof(Row));
+    l.groups = l.best + up(all * sizeof(u64));
+    l.lists = l.groups + up(all * kGroups * sizeof(float));
+    l.sums = l.lists + (l.parts > 1 ? rows * kListed * sizeof(u64) : 0);
+    l.counts = l.sums + (l.parts > 1 ? up(all * (kBins + 1) * sizeof(u64)) : 0);
+    l.bytes = l.counts + (l.parts > 1 ? up(all * kBins * sizeof(uint32_t)) : 0);
+    return l;
+}
+
+template <int kType>
+hipError_t sample(hipStream_t stream, const SampleArgs& a, void* workspace, const Layout& l) {
+    char* const at = static_cast<char*>(workspace);
+    const Scratch scratch{reinterpret_cast<Row*>(at), reinterpret_cast<u64*>(at + l.best), reinterpret_cast<float*>(at + l.groups), reinterpret_cast<u64*>(at + l.lists),
+                          reinterpret_cast<u64*>(at + l.sums), reinterpret_cast<uint32_t*>(at + l.counts), l.parts, l.part_len};
+    const dim3 grid(l.parts, a.rows);
+    most_kernel<kType><<<grid, kThreads, 0, stream>>>(a, scratch);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    spread_kernel<kType><<<grid, kThreads, 0, stream>>>(a, scratch);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    settle_kernel<kType><<<grid, kThreads, 0, stream>>>(a, scratch);
+    return hipGetLastError();
 }
 
 }  // namespace
 
-size_t sample_workspace_bytes(const SampleArgs&, int) { return 0; }
+size_t sample_workspace_bytes(const SampleArgs& args, int compute_units) { return layout_of(args, compute_units).bytes; }
 
-hipError_t launch_sample(hipStream_t stream, const SampleArgs& a, void*, int) {
-    if (a.type == 0) sample_kernel<0><<<a.rows, kThreads, 0, stream>>>(a);
-    else if (a.type == 1) sample_kernel<1><<<a.rows, kThreads, 0, stream>>>(a);
-    else sample_kernel<30><<<a.rows, kThreads, 0, stream>>>(a);
-    return hipGetLastError();
+hipError_t launch_sample(hipStream_t stream, const SampleArgs& a, void* workspace, int compute_units) {
+    const Layout l = layout_of(a, compute_units);
+    if (a.type == 0) return sample<0>(stream, a, workspace, l);
+    if (a.type == 1) return sample<1>(stream, a, workspace, l);
+    return sample<30>(stream, a, workspace, l);
 }
 
 }  // namespace afhip

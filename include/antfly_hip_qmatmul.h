@@ -590,7 +590,7 @@ afhip_status afhip_launch_quantized_attention(void *stream, const afhip_quantize
  * Weights are formed in 64 bits and summed as whole numbers (multiples of 2^-50 for up to 4096 tokens, 2^-45 for 131072), so neither the sums nor the token hang
  * on an order of additions.
  * temperatures, top_p, min_p, uniforms f32 [rows], top_k int32 [rows]; all but uniforms optional (.ptr == 0: 1, none, none, none).
- * tokens int32 [rows], probabilities f32 [rows] (optional).  vocab from 1 to 2^24, rows < 2^22 (else AFHIP_ERR_OP_UNSUPPORTED; vocab 0:
+ * tokens int32 [rows], probabilities f32 [rows] (optional).  vocab from 1 to 2^24, rows up to 65535 (else AFHIP_ERR_OP_UNSUPPORTED; vocab 0:
  * AFHIP_ERR_INVALID_STATE); logits aligned to their element; other types: AFHIP_ERR_UNSUPPORTED_TENSOR_TYPE.
  * `workspace`: 256-byte aligned, afhip_sample_workspace_bytes; less is refused (AFHIP_ERR_INVALID_STATE). */
 typedef struct afhip_sample {
