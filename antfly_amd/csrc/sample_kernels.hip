@@ -153,10 +153,13 @@ struct Target {
     }
 };
 
-// Tokens [begin, end) of a row (begin a multiple of eight) by f(v, i), a thread's own in rising order; no numbers are minus infinity.
+// Tokens [begin, end) of a row (begin a multiple of eight) by f(values, first), runs of four or eight, a thread's own in rising
+// order; no numbers are minus infinity, and so is what fills up the last run.
+template <int kType>
+constexpr int kRun = kType == 0 ? 4 : 8;
 template <int kType, typename F>
-__device__ __forceinline__ void each_logit(const void* row, uint32_t begin, uint32_t end, F f) {
-    constexpr int kPer = kType == 0 ? 4 : 8;
+__device__ __forceinline__ void each_run(const void* row, uint32_t begin, uint32_t end, F f) {
+    constexpr int kPer = kRun<kType>;
     struct __attribute__((packed, aligned(kType == 0 ? 4 : 2))) Run { uint32_t words[4]; };  // (rows start at any element)
     const uint32_t runs = end / kPer;
     const auto value = [](uint32_t word, int part) {
@@ -167,8 +170,10 @@ __device__ __forceinline__ void each_logit(const void* row, uint32_t begin, uint
         return v == v ? v : -__builtin_inff();
     };
     const auto visit = [&](const Run& r, uint32_t run) {
+        float values[kPer];
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) f(value(r.words[kType == 0 ? j : j / 2], kType == 0 ? 0 : j % 2), run * kPer + j);
+        for (int j = 0; j < kPer; ++j) values[j] = value(r.words[kType == 0 ? j : j / 2], kType == 0 ? 0 : j % 2);
+        f(values, run * kPer);
     };
     const Run* from = static_cast<const Run*>(row);
     constexpr uint32_t kAhead = 4;
@@ -181,21 +186,40 @@ __device__ __forceinline__ void each_logit(const void* row, uint32_t begin, uint
         for (uint32_t j = 0; j < kAhead; ++j) visit(held[j], run + j * kThreads);
     }
     for (; run < runs; run += kThreads) visit(from[run], run);
-    for (uint32_t i = max(runs * kPer, begin) + threadIdx.x; i < end; i += kThreads) {
-        const uint32_t word = kType == 0 ? static_cast<const uint32_t*>(row)[i] : static_cast<const uint16_t*>(row)[i];
-        f(value(word, 0), i);
+    const uint32_t rest = max(runs * kPer, begin) + threadIdx.x;  // (fewer than a run: no more than one a thread)
+    if (rest < end) {
+        const uint32_t word = kType == 0 ? static_cast<const uint32_t*>(row)[rest] : static_cast<const uint16_t*>(row)[rest];
+        float values[kPer];
+        values[0] = value(word, 0);
+#pragma unroll
+        for (int j = 1; j < kPer; ++j) values[j] = -__builtin_inff();
+        f(values, rest);
     }
 }
+template <int kType, typename F>
+__device__ __forceinline__ void each_logit(const void* row, uint32_t begin, uint32_t end, F f) {
+    each_run<kType>(row, begin, end, [&](const float (&values)[kRun<kType>], uint32_t first) {
+#pragma unroll
+        for (int j = 0; j < kRun<kType>; ++j) f(values[j], first + j);
+    });
+}
 
-// The tokens that `wanted` says, into the list as far as it has room; how many there are.
+// The tokens that `wanted` says, none of them below `low`, into the list as far as it has room; how many there are.
 template <int kType, typename Wanted>
-__device__ __forceinline__ uint32_t gather(const void* row, uint32_t begin, uint32_t end, Shared& s, Wanted wanted) {
+__device__ __forceinline__ uint32_t gather(const void* row, uint32_t begin, uint32_t end, Shared& s, float low, Wanted wanted) {
     if (threadIdx.x == 0) s.listed = 0;
     __syncthreads();
-    each_logit<kType>(row, begin, end, [&](float v, uint32_t i) {
-        if (wanted(v)) {
-            const uint32_t at = atomicAdd(&s.listed, 1u);
-            if (at < kListed) s.list[at] = rank_of(v, i);
+    each_run<kType>(row, begin, end, [&](const float (&values)[kRun<kType>], uint32_t first) {
+        float most = values[0];
+#pragma unroll
+        for (int j = 1; j < kRun<kType>; ++j) most = fmaxf(most, values[j]);
+        if (!(most >= low)) return;  // (most runs have none)
+#pragma unroll
+        for (int j = 0; j < kRun<kType>; ++j) {
+            if (values[j] >= low && wanted(values[j])) {
+                const uint32_t at = atomicAdd(&s.listed, 1u);
+                if (at < kListed) s.list[at] = rank_of(values[j], first + j);
+            }
         }
     });
     __syncthreads();
@@ -360,6 +384,10 @@ __device__ __forceinline__ void find_equal(const void* row, uint32_t vocab, floa
 struct Histogram {
     float top, low, scale;
     __device__ __forceinline__ bool holds(float v) const { return v >= low; }
+    // Below all logits of the bins up to this one (a bin's number is off by far less than half a bin's width).
+    __device__ __forceinline__ float below(uint32_t last) const {
+        return scale > 0.0f && last < kBins - 1 ? fmaxf(top - (static_cast<float>(last) + 1.5f) / scale, low) : low;
+    }
     __device__ __forceinline__ uint32_t bin(float v) const { return v == top ? 0u : min(static_cast<uint32_t>((top - v) * scale), kBins - 1); }
 };
 
@@ -417,7 +445,7 @@ __device__ bool locate(const void* row, uint32_t vocab, const Histogram& histogr
     if (bin == kBins) return false;
     uint32_t count0 = s.counts[bin];
     u64 sum0 = s.sums[bin];
-    uint32_t n = gather<kType>(row, 0, vocab, s, [&](float v) { return histogram.holds(v) && histogram.bin(v) == bin; });
+    uint32_t n = gather<kType>(row, 0, vocab, s, histogram.below(bin), [&](float v) { return histogram.bin(v) == bin; });
     if (n <= kListed) {
         sort_list(n, s);
         return Listed(n, weights, s).find(0, n, count0, sum0, target, s);
@@ -483,7 +511,7 @@ __device__ bool locate(const void* row, uint32_t vocab, const Histogram& histogr
         const uint32_t from = high - (b << shift);
         low = max(low, from - ((1u << shift) - 1));  // (the bin's lowest key)
         high = from;
-        n = gather<kType>(row, 0, vocab, s, [&](float v) { const uint32_t key = key_of(v); return key >= low && key <= high && v > -__builtin_inff(); });
+        n = gather<kType>(row, 0, vocab, s, value_of(low), [&](float v) { return key_of(v) <= high && v > -__builtin_inff(); });
         if (n <= kListed) {
             sort_list(n, s);
             return Listed(n, weights, s).find(0, n, count0, sum0, target, s);
@@ -594,13 +622,13 @@ __device__ __forceinline__ bool last_of(uint32_t* arrived, uint32_t parts, Share
     return last;
 }
 
-// The row's tokens that `wants` says into the list in LDS, by its parts: true for the last of them, which has them all (as far as
+// The row's tokens that `wants` says, none of them below `low`, into the list in LDS, by its parts: true for the last of them, which has them all (as far as
 // there is room; *n: how many there are).
 template <int kType, typename Wants>
-__device__ __forceinline__ bool list_row(const SampleArgs& a, const Scratch& scratch, uint32_t r, uint32_t part, uint32_t* arrived, Shared& s, Wants wants, uint32_t* n) {
+__device__ __forceinline__ bool list_row(const SampleArgs& a, const Scratch& scratch, uint32_t r, uint32_t part, uint32_t* arrived, Shared& s, float low, Wants wants, uint32_t* n) {
     const void* row = row_of(a, r, kType == 0 ? 4 : 2);
     const uint32_t begin = part * scratch.part_len, end = min(begin + scratch.part_len, a.vocab);
-    *n = gather<kType>(row, begin, end, s, wants);
+    *n = gather<kType>(row, begin, end, s, low, wants);
     if (scratch.parts == 1) return true;
     // behind the other parts' (one addition a part: thousands to one place of memory would follow one another)
     Row* const state = scratch.rows + r;
@@ -708,6 +736,7 @@ __global__ __launch_bounds__(kThreads) void spread_kernel(SampleArgs a, Scratch 
             uint32_t own[3] = {0, 0, 0};
 #pragma unroll
             for (uint32_t j = 0; j < kOwn; ++j) {
+                if (j * kThreads >= groups) break;
 #pragma unroll
                 for (int i = 0; i < 3; ++i) own[i] += __popcll(__ballot(keys[j] >= with[i]));
             }
@@ -749,7 +778,7 @@ __global__ __launch_bounds__(kThreads) void spread_kernel(SampleArgs a, Scratch 
 
     if (few) {
         uint32_t n;
-        if (!list_row<kType>(a, scratch, r, part, &state->spread_arrived, s, [&](float v) { return v >= cut; }, &n)) return;
+        if (!list_row<kType>(a, scratch, r, part, &state->spread_arrived, s, cut, [](float) { return true; }, &n)) return;
         if (n > kListed) {
             if (tid == 0) {
                 state->state = kWide;
@@ -931,11 +960,12 @@ __global__ __launch_bounds__(kThreads, 4) void settle_kernel(SampleArgs a, Scrat
     const auto in = [](const Wanted& w, uint32_t b) { return b >= w.first && b <= w.last; };
     const auto wants = [&](float v) {
         const uint32_t b = histogram.bin(v);
-        return histogram.holds(v) && (in(of_u, b) || in(of_p, b) || in(of_k, b));
+        return in(of_u, b) || in(of_p, b) || in(of_k, b);
     };
+    const float low = histogram.below(max(of_u.last, max(of_p.last, of_k.last)));
     uint32_t n = 0;
     if (!wide) {
-        if (!list_row<kType>(a, scratch, r, part, &state->settle_arrived, s, wants, &n)) return;
+        if (!list_row<kType>(a, scratch, r, part, &state->settle_arrived, s, low, wants, &n)) return;
         wide = n > kListed;
     }
     if (wide) {
