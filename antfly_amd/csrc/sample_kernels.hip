@@ -204,19 +204,19 @@ __device__ __forceinline__ void each_logit(const void* row, uint32_t begin, uint
     });
 }
 
-// The tokens that `wanted` says, none of them below `low`, into the list as far as it has room; how many there are.
+// The tokens that `wanted` says, none of them below `low` or above `high`, into the list as far as it has room; how many there are.
 template <int kType, typename Wanted>
-__device__ __forceinline__ uint32_t gather(const void* row, uint32_t begin, uint32_t end, Shared& s, float low, Wanted wanted) {
+__device__ __forceinline__ uint32_t gather(const void* row, uint32_t begin, uint32_t end, Shared& s, float low, float high, Wanted wanted) {
     if (threadIdx.x == 0) s.listed = 0;
     __syncthreads();
     each_run<kType>(row, begin, end, [&](const float (&values)[kRun<kType>], uint32_t first) {
-        float most = values[0];
+        bool any = false;
 #pragma unroll
-        for (int j = 1; j < kRun<kType>; ++j) most = fmaxf(most, values[j]);
-        if (!(most >= low)) return;  // (most runs have none)
+        for (int j = 0; j < kRun<kType>; ++j) any |= values[j] >= low && values[j] <= high;
+        if (!any) return;  // (as most runs)
 #pragma unroll
         for (int j = 0; j < kRun<kType>; ++j) {
-            if (values[j] >= low && wanted(values[j])) {
+            if (values[j] >= low && values[j] <= high && wanted(values[j])) {
                 const uint32_t at = atomicAdd(&s.listed, 1u);
                 if (at < kListed) s.list[at] = rank_of(values[j], first + j);
             }
@@ -384,10 +384,11 @@ __device__ __forceinline__ void find_equal(const void* row, uint32_t vocab, floa
 struct Histogram {
     float top, low, scale;
     __device__ __forceinline__ bool holds(float v) const { return v >= low; }
-    // Below all logits of the bins up to this one (a bin's number is off by far less than half a bin's width).
+    // Below all logits of the bins up to this one, and above all of those from this one on (a bin's number is off by far less than half a bin's width).
     __device__ __forceinline__ float below(uint32_t last) const {
         return scale > 0.0f && last < kBins - 1 ? fmaxf(top - (static_cast<float>(last) + 1.5f) / scale, low) : low;
     }
+    __device__ __forceinline__ float above(uint32_t first) const { return scale > 0.0f && first > 0 ? top - (static_cast<float>(first) - 0.5f) / scale : top; }
     __device__ __forceinline__ uint32_t bin(float v) const { return v == top ? 0u : min(static_cast<uint32_t>((top - v) * scale), kBins - 1); }
 };
 
@@ -445,7 +446,7 @@ __device__ bool locate(const void* row, uint32_t vocab, const Histogram& histogr
     if (bin == kBins) return false;
     uint32_t count0 = s.counts[bin];
     u64 sum0 = s.sums[bin];
-    uint32_t n = gather<kType>(row, 0, vocab, s, histogram.below(bin), [&](float v) { return histogram.bin(v) == bin; });
+    uint32_t n = gather<kType>(row, 0, vocab, s, histogram.below(bin), histogram.above(bin), [&](float v) { return histogram.bin(v) == bin; });
     if (n <= kListed) {
         sort_list(n, s);
         return Listed(n, weights, s).find(0, n, count0, sum0, target, s);
@@ -511,7 +512,7 @@ __device__ bool locate(const void* row, uint32_t vocab, const Histogram& histogr
         const uint32_t from = high - (b << shift);
         low = max(low, from - ((1u << shift) - 1));  // (the bin's lowest key)
         high = from;
-        n = gather<kType>(row, 0, vocab, s, value_of(low), [&](float v) { return key_of(v) <= high && v > -__builtin_inff(); });
+        n = gather<kType>(row, 0, vocab, s, value_of(low), value_of(high), [](float v) { return v > -__builtin_inff(); });
         if (n <= kListed) {
             sort_list(n, s);
             return Listed(n, weights, s).find(0, n, count0, sum0, target, s);
@@ -622,13 +623,13 @@ __device__ __forceinline__ bool last_of(uint32_t* arrived, uint32_t parts, Share
     return last;
 }
 
-// The row's tokens that `wants` says, none of them below `low`, into the list in LDS, by its parts: true for the last of them, which has them all (as far as
+// The row's tokens that `wants` says, none of them below `low` or above `high`, into the list in LDS, by its parts: true for the last of them, which has them all (as far as
 // there is room; *n: how many there are).
 template <int kType, typename Wants>
-__device__ __forceinline__ bool list_row(const SampleArgs& a, const Scratch& scratch, uint32_t r, uint32_t part, uint32_t* arrived, Shared& s, float low, Wants wants, uint32_t* n) {
+__device__ __forceinline__ bool list_row(const SampleArgs& a, const Scratch& scratch, uint32_t r, uint32_t part, uint32_t* arrived, Shared& s, float low, float high, Wants wants, uint32_t* n) {
     const void* row = row_of(a, r, kType == 0 ? 4 : 2);
     const uint32_t begin = part * scratch.part_len, end = min(begin + scratch.part_len, a.vocab);
-    *n = gather<kType>(row, begin, end, s, low, wants);
+    *n = gather<kType>(row, begin, end, s, low, high, wants);
     if (scratch.parts == 1) return true;
     // behind the other parts' (one addition a part: thousands to one place of memory would follow one another)
     Row* const state = scratch.rows + r;
@@ -778,7 +779,7 @@ __global__ __launch_bounds__(kThreads) void spread_kernel(SampleArgs a, Scratch 
 
     if (few) {
         uint32_t n;
-        if (!list_row<kType>(a, scratch, r, part, &state->spread_arrived, s, cut, [](float) { return true; }, &n)) return;
+        if (!list_row<kType>(a, scratch, r, part, &state->spread_arrived, s, cut, top, [](float) { return true; }, &n)) return;
         if (n > kListed) {
             if (tid == 0) {
                 state->state = kWide;
@@ -962,10 +963,12 @@ __global__ __launch_bounds__(kThreads, 4) void settle_kernel(SampleArgs a, Scrat
         const uint32_t b = histogram.bin(v);
         return in(of_u, b) || in(of_p, b) || in(of_k, b);
     };
+    // (a target that is not there has bins 1 to 0)
     const float low = histogram.below(max(of_u.last, max(of_p.last, of_k.last)));
+    const float high = histogram.above(min(of_u.first, min(of_p.first <= of_p.last ? of_p.first : of_u.first, of_k.first <= of_k.last ? of_k.first : of_u.first)));
     uint32_t n = 0;
     if (!wide) {
-        if (!list_row<kType>(a, scratch, r, part, &state->settle_arrived, s, low, wants, &n)) return;
+        if (!list_row<kType>(a, scratch, r, part, &state->settle_arrived, s, low, high, wants, &n)) return;
         wide = n > kListed;
     }
     if (wide) {
