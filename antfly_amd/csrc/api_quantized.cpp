@@ -110,7 +110,11 @@ afhip_status rotation_args(const afhip_head_rotation* r, bool writes_keys, Heads
     out->rotary_dim = static_cast<uint32_t>(r->rotary_dim);
     out->epsilon = r->epsilon;
     out->interleaved = r->interleaved != 0;
-    for (size_t p = 0; p < 128; ++p) out->pair_axes[p] = p < r->rotary_dim / 2 ? r->pair_axes[p] : 0;
+    out->one_axis = true;
+    for (size_t p = 0; p < 128; ++p) {
+        out->pair_axes[p] = p < r->rotary_dim / 2 ? r->pair_axes[p] : 0;
+        out->one_axis = out->one_axis && out->pair_axes[p] == 0;
+    }
     return AFHIP_OK;
 }
 
@@ -233,7 +237,7 @@ afhip_status afhip_launch_quantized_load(void* stream, const afhip_quantized_cac
     const size_t lanes = view.head_dim <= 64 ? 8 : view.head_dim <= 128 ? 16 : 32, each = 256 / lanes;
     if (!checked_mul(tokens, 2 * cache->kv_heads, &groups) || groups > 0xffffffffu || !fits_a_launch((groups + each - 1) / each, 256)) return AFHIP_ERR_OP_UNSUPPORTED;
     return status_of(launch_quantized_load(static_cast<hipStream_t>(stream), view, type, rows_of(keys, token_stride, head_stride),
-                                           rows_of(values, token_stride, head_stride), reinterpret_cast<const int*>(slots.ptr), static_cast<uint32_t>(tokens)));
+                                           rows_of(values, token_stride, head_stride), reinterpret_cast<const int*>(slots.ptr), static_cast<uint32_t>(tokens), gemv_compute_units()));
 }
 
 afhip_status afhip_launch_head_rotation(void* stream, const afhip_head_rotation* rotation) {

@@ -38,7 +38,7 @@ struct HeadsArgs {
     int out_type;       // of the arrays
     uint32_t tokens, heads, kv_heads, value_heads, head_dim, rotary_dim;  // value_heads: 0 or kv_heads
     float epsilon;
-    bool interleaved;
+    bool interleaved, one_axis;  // one_axis: all pairs turn with the first positions
     uint32_t groups_a_token, tokens_a_group, chunk;  // the launch sets these
     uint8_t pair_axes[128];
 };
@@ -47,7 +47,7 @@ bool heads_fit_a_launch(uint32_t tokens, uint32_t heads, uint32_t head_dim);
 hipError_t launch_heads(hipStream_t stream, int type, const HeadsArgs& args, int compute_units);
 
 hipError_t launch_quantized_load(hipStream_t stream, const QuantizedView& cache, int type, const HeadRows& keys, const HeadRows& values,
-                                 const int* slots, uint32_t tokens);
+                                 const int* slots, uint32_t tokens, int compute_units);
 
 struct QuantizedAttentionArgs {
     QuantizedView cache;
