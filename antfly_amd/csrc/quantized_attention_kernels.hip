@@ -136,14 +136,20 @@ __device__ __forceinline__ Share lengths_of(const QuantizedAttentionArgs& a, uin
     return s;
 }
 
+// A lane's value of the data-parallel move kControl, zero where the move has none for it or its row of 16 is not in kRows.
+template <int kControl, int kRows, typename T>
+__device__ __forceinline__ T moved(T v) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kControl, kRows, 0xF, false));
+}
+// Sum over the wavefront's lanes up to this one: within rows of 16 lanes, then the rows below.
 template <typename T>
 __device__ __forceinline__ T sum_up_to(T v) {
-    const int lane = static_cast<int>(threadIdx.x) & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const T below = __shfl_up(v, d);
-        if (lane >= d) v += below;
-    }
+    v += moved<0x111, 0xF>(v);  // from 1, 2, 4, 8 lanes below
+    v += moved<0x112, 0xF>(v);
+    v += moved<0x114, 0xF>(v);
+    v += moved<0x118, 0xF>(v);
+    v += moved<0x142, 0xA>(v);  // a row's last lane to the next row
+    v += moved<0x143, 0xC>(v);  // lane 31 to the upper half
     return v;
 }
 
@@ -172,8 +178,7 @@ __device__ __forceinline__ bool find_share(const QuantizedAttentionArgs& a, cons
             work += static_cast<float>(mine.tiles) * static_cast<float>(mine.row_tiles);
         }
     }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) work += __shfl_xor(work, d);
+    work = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sum_up_to(work)), 63));
     // (a thousandth more than the quotient, for the floats' error: the parts are no more than plan.target and one a request)
     const float quotient = work * static_cast<float>(heads) * 1.001f / static_cast<float>(plan.target);
     const uint32_t tiles = max(static_cast<uint32_t>(fminf(quotient, 0x1p30f)) + 1, plan.least);
@@ -240,20 +245,17 @@ struct Bytes<8> { typedef uint32_t type __attribute__((ext_vector_type(2))); };
 template <>
 struct Bytes<16> { typedef uint32_t type __attribute__((ext_vector_type(4))); };
 
-__device__ const uint4 kNothing{0, 0, 0, 0};  // what values past a head's end are loaded from
-
-// 16 (4) bytes a lane from memory to 1 KiB (256 bytes) of LDS from `to` on (a uniform address).
+// 16 (4) bytes a lane from memory to 1 KiB (256 bytes) of LDS from `to` on (a uniform address), lane after lane; lanes that are off
+// leave their bytes as they are.
 __device__ __forceinline__ void load_to_lds(uint32_t to, const uint4* from) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "memory", "m0");
 }
 __device__ __forceinline__ void load_to_lds(uint32_t to, const float* from) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(to), "v"(from) : "memory", "m0");
 }
-// The same of 16 bytes from a uniform address on, `past` bytes behind it for a lane (kNoPiece: zeros; `all`: no lane has that).
-constexpr uint32_t kNoPiece = ~0u;
-__device__ __forceinline__ void load_to_lds(uint32_t to, const uint4* from, uint32_t past, bool all) {
-    if (all) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(past), "s"(from) : "memory", "m0");
-    else load_to_lds(to, past == kNoPiece ? &kNothing : reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(from) + past));
+// The same of 16 bytes `past` bytes behind a uniform address.
+__device__ __forceinline__ void load_to_lds(uint32_t to, const uint4* from, uint32_t past) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(past), "s"(from) : "memory", "m0");
 }
 // s_waitcnt for "at most kLeft vector memory operations outstanding" (nothing else waited for).
 template <int kLeft>
@@ -304,9 +306,39 @@ __global__ __launch_bounds__(64 * most_waves(kDim)) void quantized_attention_ker
     const int here = min(kRows, rows - first_row);  // rows of this workgroup
     const int tid = static_cast<int>(threadIdx.x), wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, waves = static_cast<int>(blockDim.x) >> 6;
     const int column = lane & 15, quarter = lane >> 4, head_dim = static_cast<int>(a.cache.head_dim);
-    const bool whole_heads = head_dim == kDim;
 
-    // ---- the rows: their queries, requested first
+    // ---- the keys of this part that any of these rows sees, and this wavefront's of them
+    const int first_position = share.context + first_row / group, last_position = share.context + (first_row + here - 1) / group;
+    const unsigned long long most = min(static_cast<unsigned long long>(a.table_columns) * a.block_size.by, static_cast<unsigned long long>(a.max_key_len));
+    const int keys = static_cast<int>(min(static_cast<unsigned long long>(last_position) + 1, most));  // seen by none from here on
+    const uint32_t limit = a.window != 0 ? a.window : 0x80000000u;                                      // a key is seen where position - key is below
+    int tile = share.first_tile + static_cast<int>(split * share.each);
+    int end = min(min(tile + static_cast<int>(share.each), share.first_tile + share.tiles), (keys + kTile - 1) / kTile);
+    if (a.window != 0 && first_position >= static_cast<int>(a.window)) tile = max(tile, (first_position - static_cast<int>(a.window) + 1) / kTile);
+    if (end > tile) {
+        const int each = (end - tile + waves - 1) / waves;
+        tile += wave * each;
+        end = min(tile + each, end);
+    }
+
+    // 64 entries of the block table from `window_at` on, one a lane, and which of them name a block; the first are asked for before
+    // the queries, whose way from memory nothing here waits for
+    const int* table = a.block_tables + static_cast<size_t>(request) * a.table_columns;
+    const uint32_t last_block = keys > 0 ? divide(static_cast<uint32_t>(keys - 1), a.block_size) : 0;
+    uint32_t window = 0, window_at = 0, window_end = 0;  // (keys from window_end on are not in it)
+    unsigned long long named = 0;
+    const auto entries_from = [&](uint32_t first_key) {
+        window_at = divide(first_key, a.block_size);
+        window_end = (window_at + 64) * a.block_size.by;  // (below 2^32: a bound of the keys times the block size)
+        return window_at + lane <= last_block ? static_cast<uint32_t>(table[window_at + lane]) : ~0u;
+    };
+    const auto keep = [&](uint32_t block) {
+        named = __ballot(block < a.cache.blocks);
+        window = block < a.cache.blocks ? block : 0;
+    };
+    const uint32_t first_entries = tile < end ? entries_from(static_cast<uint32_t>(tile) * kTile) : ~0u;
+
+    // ---- the rows: their queries
     u32x4 raw[kQ][kSteps / 2][kTerms == 3 ? 4 : 2];
     int position[kQ];
     float slope[kQ];
@@ -326,46 +358,29 @@ __global__ __launch_bounds__(64 * most_waves(kDim)) void quantized_attention_ker
         }
     }
 
-    // ---- the keys of this part that any of these rows sees, and this wavefront's of them
-    const int first_position = share.context + first_row / group, last_position = share.context + (first_row + here - 1) / group;
-    const unsigned long long most = min(static_cast<unsigned long long>(a.table_columns) * a.block_size.by, static_cast<unsigned long long>(a.max_key_len));
-    const int keys = static_cast<int>(min(static_cast<unsigned long long>(last_position) + 1, most));  // seen by none from here on
-    const uint32_t limit = a.window != 0 ? a.window : 0x80000000u;                                      // a key is seen where position - key is below
-    int tile = share.first_tile + static_cast<int>(split * share.each);
-    int end = min(min(tile + static_cast<int>(share.each), share.first_tile + share.tiles), (keys + kTile - 1) / kTile);
-    if (a.window != 0 && first_position >= static_cast<int>(a.window)) tile = max(tile, (first_position - static_cast<int>(a.window) + 1) / kTile);
-    if (end > tile) {
-        const int each = (end - tile + waves - 1) / waves;
-        tile += wave * each;
-        end = min(tile + each, end);
-    }
-
     char* const ring = lds + wave * kWaveLds;
     const uint32_t ring_at = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)ring)));
-    // 64 entries of the block table from `window_at` on, one a lane, and which of them name a block
-    const int* table = a.block_tables + static_cast<size_t>(request) * a.table_columns;
-    const uint32_t last_block = keys > 0 ? divide(static_cast<uint32_t>(keys - 1), a.block_size) : 0;
-    uint32_t window = 0, window_at = 0, window_end = 0;  // (keys from window_end on are not in it)
-    unsigned long long named = 0;
-    // Where a lane's bytes of load i lie behind its first row's, where the rows of a load are in one block.
+    // Where a lane's bytes of load i lie behind its first row's, where the rows of a load are in one block; whether there are any (the
+    // ring holds zeros for what is past a head's end).
     const bool in_one = a.block_size.by % kRowsALoad == 0 && a.cache.slot_stride < (1u << 20);
     uint32_t lane_at[kLoads];
+    bool has[kLoads];
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
         const int row = i * kRowsALoad + lane / kPieces, piece = piece_at<kDim>(row, lane % kPieces) % kPieces;
         lane_at[i] = (static_cast<uint32_t>(lane / kPieces) * a.cache.slot_stride + piece) * 16;
-        if (piece * 16 >= head_dim) lane_at[i] = kNoPiece;
+        has[i] = piece * 16 < head_dim;
+    }
+    if (head_dim < kDim) {
+        for (int i = lane; i < kWaveLds / 16; i += 64) reinterpret_cast<u32x4*>(ring)[i] = u32x4{0, 0, 0, 0};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     // Requests tile t into a stage; its keys that have a place are returned, in the order of the products' rows.  (A key without one
     // is not seen by any row: what is loaded for it, the first block's, may be anything.)
     auto request_tile = [&](int t, int stage) -> uint32_t {
         const uint32_t first_key = static_cast<uint32_t>(t) * kTile;
         if (first_key + kTile > window_end) {
-            window_at = divide(first_key, a.block_size);
-            const uint32_t block = window_at + lane <= last_block ? static_cast<uint32_t>(table[window_at + lane]) : ~0u;
-            named = __ballot(block < a.cache.blocks);
-            window = block < a.cache.blocks ? block : 0;
-            window_end = (window_at + 64) * a.block_size.by;  // (below 2^32: a bound of the keys times the block size)
+            keep(entries_from(first_key));
         }
         const uint32_t to = ring_at + stage * tile_bytes(kDim);
         const uint32_t head_at = kv_head * a.cache.head_stride;
@@ -375,8 +390,10 @@ __global__ __launch_bounds__(64 * most_waves(kDim)) void quantized_attention_ker
                 const uint32_t key = first_key + i * kRowsALoad, column_of = divide(key, a.block_size);
                 const uint32_t block = __builtin_amdgcn_readlane(window, column_of - window_at);
                 const uint32_t place = block * a.cache.block_stride + (key - column_of * a.block_size.by) * a.cache.slot_stride + head_at;
-                load_to_lds(to + i * 1024, a.cache.keys + place, lane_at[i], whole_heads);
-                load_to_lds(to + kTile * kDim + i * 1024, a.cache.values + place, lane_at[i], whole_heads);
+                if (has[i]) {
+                    load_to_lds(to + i * 1024, a.cache.keys + place, lane_at[i]);
+                    load_to_lds(to + kTile * kDim + i * 1024, a.cache.values + place, lane_at[i]);
+                }
             }
         } else {
 #pragma unroll
@@ -385,10 +402,10 @@ __global__ __launch_bounds__(64 * most_waves(kDim)) void quantized_attention_ker
                 const uint32_t key = first_key + row, column_of = divide(key, a.block_size);
                 const uint32_t block = static_cast<uint32_t>(__shfl(static_cast<int>(window), static_cast<int>(column_of - window_at)));
                 const uint32_t place = block * a.cache.block_stride + (key - column_of * a.block_size.by) * a.cache.slot_stride + head_at + piece;
-                const uint4 *k = a.cache.keys + place, *v = a.cache.values + place;
-                if (piece * 16 >= head_dim) k = v = &kNothing;
-                load_to_lds(to + i * 1024, k);
-                load_to_lds(to + kTile * kDim + i * 1024, v);
+                if (has[i]) {
+                    load_to_lds(to + i * 1024, a.cache.keys + place);
+                    load_to_lds(to + kTile * kDim + i * 1024, a.cache.values + place);
+                }
             }
         }
         // the scales, keys' and then values'
@@ -398,10 +415,13 @@ __global__ __launch_bounds__(64 * most_waves(kDim)) void quantized_attention_ker
         load_to_lds(to + 2 * kTile * kDim, (lane < 32 ? a.cache.key_scales : a.cache.value_scales) + place);
         return static_cast<uint32_t>(__ballot((named >> (column_of - window_at) & 1) != 0 && static_cast<int>(key) < keys));
     };
-    uint32_t held[kStages] = {};
-#pragma unroll
+    keep(first_entries);
+    uint32_t held[kStages] = {};  // of the tiles on their way, the next one's first
+#pragma unroll 1
     for (int i = 0; i < kStages; ++i) {
-        if (tile + i < end) held[i] = request_tile(tile + i, i);
+        const uint32_t got = tile + i < end ? request_tile(tile + i, i) : 0;
+#pragma unroll
+        for (int j = 0; j < kStages; ++j) held[j] = j == i ? got : held[j];
     }
 
     // What the products of a row are multiplied by, beside the keys' scales.
@@ -729,18 +749,23 @@ __global__ __launch_bounds__(256) void join_quantized_parts_kernel(QuantizedAtte
         const uint32_t kv_head = number / rows, row = number % rows, row_tile = row / rows_a_tile, r = row % rows_a_tile;
         const size_t first_slot = share.first_slot + static_cast<size_t>(kv_head) * share.row_tiles + row_tile;
         const auto part_at = [&](uint32_t s) { return (first_slot + static_cast<size_t>(s) * heads * share.row_tiles) * rows_a_tile + r; };
+        constexpr uint32_t kOwn = (kMostParts + 255) / 256;
+        Part own[kOwn];
         float highest = -__builtin_inff(), all = 0.0f;
-        for (uint32_t s = tid; s < splits; s += 256) highest = fmaxf(highest, parts[part_at(s)].most);
+#pragma unroll
+        for (uint32_t i = 0; i < kOwn; ++i) own[i] = tid + i * 256 < splits ? parts[part_at(tid + i * 256)] : Part{-__builtin_inff(), 0.0f};
+#pragma unroll
+        for (uint32_t i = 0; i < kOwn; ++i) highest = fmaxf(highest, own[i].most);
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) highest = fmaxf(highest, __shfl_xor(highest, d));
         if ((tid & 63) == 0) numbers[tid >> 6] = highest;
         __syncthreads();
         highest = fmaxf(fmaxf(numbers[0], numbers[1]), fmaxf(numbers[2], numbers[3]));
-        for (uint32_t s = tid; s < splits; s += 256) {
-            const Part part = parts[part_at(s)];
-            const float w = part.most == -__builtin_inff() ? 0.0f : exp2_between(part.most, highest);
-            by[s] = w;
-            all = __builtin_fmaf(part.sum, w, all);  // (a part that saw nothing has a sum of zero)
+#pragma unroll
+        for (uint32_t i = 0; i < kOwn; ++i) {
+            const float w = own[i].most == -__builtin_inff() ? 0.0f : exp2_between(own[i].most, highest);
+            if (tid + i * 256 < splits) by[tid + i * 256] = w;
+            all = __builtin_fmaf(own[i].sum, w, all);  // (a part that saw nothing has a sum of zero)
         }
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
