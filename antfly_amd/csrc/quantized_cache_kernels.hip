@@ -7,7 +7,8 @@
 // A head is a group of 8, 16 or 32 lanes with eight values each: its sum of squares and its maximum are three to five exchanges of
 // registers.  A lane's eight values are four pairs of the rotation (two runs of four values), so a pair never leaves its lane.  The
 // angles of a lane's four pairs are the same for all heads of a token: it makes them once and takes several heads.
-// Bound by the bytes.
+// Bound by the bytes: 7500 tokens of 32 and 8 heads of 128, f32 in, bf16 queries out, keys and values to e4m3, 64 us, 4.1 TB/s; 4000
+// tokens of 8 heads of 128 stored and 30001 loaded, 58 us, 3.9 TB/s.  A few tokens cost a launch (one: 4.0 us).
 #include "quantized_launch.h"
 
 #include <hip/hip_runtime.h>
@@ -356,8 +357,8 @@ hipError_t launch_heads(hipStream_t stream, int type, const HeadsArgs& args, int
 
 hipError_t launch_quantized_load(hipStream_t stream, const QuantizedView& cache, int type, const HeadRows& keys, const HeadRows& values,
                                  const int* slots, uint32_t tokens, int compute_units) {
-    // Eight heads a group of lanes where that still gives every unit eight workgroups: 30001 tokens of 8 heads of 128 40 us instead of 55,
-    // 64 tokens 8.0 instead of 3.4.
+    // Eight heads a group of lanes where that still gives every unit eight workgroups: 30001 tokens of 8 heads of 128 39 us instead of 55;
+    // a step that stores and loads 64 tokens takes 10.6 us that way instead of 5.7.
     const uint64_t groups = static_cast<uint64_t>(tokens) * 2 * cache.kv_heads * lanes_of(cache.head_dim) / kThreads;
     return groups >= 64 * static_cast<uint64_t>(compute_units) ? load<8>(stream, cache, type, keys, values, slots, tokens) : load<1>(stream, cache, type, keys, values, slots, tokens);
 }

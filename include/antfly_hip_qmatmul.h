@@ -528,7 +528,8 @@ afhip_status afhip_launch_quantized_load(void *stream, const afhip_quantized_cac
  * type: of query and key; out_type: of the arrays that are written (F32, F16 or BF16 each; sums and products in f32, one
  * rounding at the end).  head_dim a multiple of 8 up to 256, rotary_dim a multiple of 8 up to head_dim, 1 <= axes <= 16; strides
  * in elements, multiples of 4, base addresses 16-byte (f32) or 8-byte aligned (else AFHIP_ERR_INVALID_STATE; head_dim > 256:
- * AFHIP_ERR_OP_UNSUPPORTED, as are 2^24 tokens and 2^19 heads).  heads == 0: no queries.  out_query and out_key may be query and key themselves (the same buffer,
+ * AFHIP_ERR_OP_UNSUPPORTED, as are 2^24 tokens and more of at least 32 (16, 8) heads of up to 64 (128, 256) in all, of queries, keys and
+ * stored values, more tokens of fewer heads, and more than 65535 times as many heads).  heads == 0: no queries.  out_query and out_key may be query and key themselves (the same buffer,
  * strides and type); otherwise nothing that is written overlaps what is read. */
 typedef struct afhip_head_rotation {
     int type, out_type, interleaved;
@@ -558,12 +559,13 @@ afhip_status afhip_launch_rotated_store(void *stream, const afhip_head_rotation 
  * row whose seen scores are all minus infinity, or whose query holds an infinity or no number, is no numbers.
  * query and out: F32, F16 or BF16, both of `type`, [tokens][heads][head_dim], strides in elements (multiples of 4 for F32, of 8
  * otherwise; 16-byte aligned).  Codes are multiplied as bf16, which holds each of them; queries, and the weights beside the values,
- * as three terms of bf16 for F32 (24 bits), two for F16 (16 bits) and one for BF16.  Sums are f32.
+ * as three terms of bf16 for F32 (24 bits), two for F16 (16 bits) and one for BF16; on an I8 cache queries are three digits of a
+ * whole number instead, 2^-22 of their row's largest value, and their products with the codes are exact.  Sums are f32.
  * max_query_len and max_key_len bound what the batch holds (new tokens; context plus new tokens) and choose the launch's
  * shape; tokens past the first and keys past the second are left out.  slopes f32 [heads], optional (.ptr == 0).  heads is a multiple of
  * kv_heads (else AFHIP_ERR_INVALID_STATE); requests <= 65535, max_key_len * block_size < 2^32, max_query_len * heads < 2^31 and a grid
- * of fewer than 2^32 threads (256 or 512 for every 16 of a request's max_query_len * heads / kv_heads rows and every key head, or as
- * many as the units hold), else AFHIP_ERR_OP_UNSUPPORTED.
+ * of fewer than 2^32 threads (256 or 512 for every 16 or 32 of a request's max_query_len * heads / kv_heads rows and every key head,
+ * and twice the units' number of such workgroups where keys are shared out), else AFHIP_ERR_OP_UNSUPPORTED.
  * `workspace` (256-byte aligned, afhip_quantized_attention_workspace_bytes) holds the parts of rows whose keys are shared out over
  * workgroups; less than asked for is refused (AFHIP_ERR_INVALID_STATE). */
 typedef struct afhip_quantized_attention {

@@ -117,6 +117,14 @@ def test_bounds_of_the_launch():
     assert attend(b, most=(6, 0)).abs().max() == 0
 
 
+def test_many_requests():
+    """More requests than a wavefront has lanes, a few of them long, some without new tokens; and more than are shared out."""
+    rng = np.random.default_rng(14)
+    new = [int(n) for n in rng.integers(0, 3, 150)]
+    check(a_batch(rng, [3000 if r % 41 == 7 else int(rng.integers(0, 60)) for r in range(150)], new, 16, 4, 2, 64, "f32", "e4m3"))
+    check(a_batch(rng, [1100 if r == 1050 else r % 3 for r in range(1100)], [1] * 1100, 16, 2, 1, 64, "bf16", "i8", garbage=False))
+
+
 def test_single_scores():
     """A scale of zero, a negative one, scores far apart, and a row whose scores all overflow to minus infinity."""
     rng = np.random.default_rng(10)

@@ -103,6 +103,23 @@ def test_load(out, stored, tokens, block, heads, dim, outside):
     assert same_numbers(to64(wide), to64(want))
 
 
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens,heads,dim", [(18001, 8, 128), (60003, 8, 48), (9001, 9, 240)])
+def test_load_many(out, tokens, heads, dim):
+    rng = np.random.default_rng(tokens)
+    cache = a_cache(rng, 20, 16, heads, dim, "i8", False)
+    slots = rng.integers(-3, 330, tokens).astype(np.int32)
+    k, v = (torch.full((tokens + 1, heads, dim), -7.0, dtype=R.DTYPES[out], device=G.DEV) for _ in "kv")
+    paged.launchQuantizedLoad(G.stream(), paged.quantizedCache(*cache), k[:-1], v[:-1], G.to_dev(slots))
+    torch.cuda.synchronize()
+    there = np.append((slots >= 0) & (slots < 320), False)
+    at = torch.from_numpy(np.where(there, np.append(slots, 0), 0)).long()
+    for which, got in enumerate((k, v)):
+        numbers = (cache[which].cpu().float() * cache[2 + which].cpu()[..., None]).view(320, heads, dim).to(R.DTYPES[out])
+        want = torch.where(torch.from_numpy(there)[:, None, None], numbers[at], torch.tensor(-7.0, dtype=R.DTYPES[out]))
+        assert torch.equal(got.cpu(), want)
+
+
 ROTATIONS = [(1, 32, 8, 128, 128, False, 1), (37, 5, 1, 96, 48, True, 3), (130, 4, 4, 64, 64, True, 1), (7, 3, 3, 256, 256, False, 2), (3, 16, 2, 80, 40, False, 3),
              (600, 2, 1, 112, 56, False, 1), (5, 7, 1, 192, 96, True, 1), (11, 2, 2, 8, 8, False, 1), (4, 1, 1, 40, 0, False, 1), (2000, 28, 4, 128, 64, False, 2)]
 

@@ -159,3 +159,37 @@ def test_replayed():
         torch.cuda.synchronize()
         want = draw(logits, u.cpu().numpy(), k=k.cpu().numpy(), p=p.cpu().numpy())[0]
         assert tokens.cpu().numpy().tolist() == want.tolist(), turn
+
+
+def test_streams_and_shared_workspaces():
+    """Two captured calls on one workspace, of other shapes, in turn with eager ones, on a stream that is not the first."""
+    rng = np.random.default_rng(5)
+    side, workspace = torch.cuda.Stream(), None
+    calls = []
+    for rows, vocab, kind in ((2, 32000, "f32"), (40, 7001, "bf16")):
+        logits, u = some_logits(rng, rows, vocab, kind, 2.0), torch.rand(rows, device=G.DEV)
+        p = torch.full((rows,), 0.9, device=G.DEV)
+        calls.append((logits, u, p, sampling.sample(logits, torch.empty(rows, dtype=torch.int32, device=G.DEV), u, top_p=p)))
+    workspace = torch.full((max(sampling.sampleWorkspaceBytes(c[3]) for c in calls),), 0xFF, dtype=torch.uint8, device=G.DEV)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for c in calls:
+            sampling.launchSample(G.stream(), c[3], workspace)
+        side.synchronize()
+        graphs = []
+        for c in calls:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                sampling.launchSample(G.stream(), c[3], workspace)
+            graphs.append(graph)
+        for turn in range(4):
+            for graph, (logits, u, p, call) in zip(graphs, calls):
+                u.uniform_()
+                graph.replay()
+                got = call.arrays[1].clone()
+                call.arrays[1].zero_()
+                if turn % 2:
+                    sampling.launchSample(G.stream(), call, workspace)
+                    assert torch.equal(call.arrays[1], got)
+                side.synchronize()
+                assert got.cpu().numpy().tolist() == [R.sample(row, x, p=np.float32(0.9))[0] for row, x in zip(to64(logits), u.cpu().numpy())], turn
