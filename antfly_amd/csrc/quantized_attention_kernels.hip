@@ -14,16 +14,18 @@
 // Codes come from memory straight into a ring of tiles in LDS that each wavefront has for itself (no barrier anywhere), and go to
 // bf16, which holds every one of them exactly, as they are read from there; of values the bytes of two keys are put side by side
 // before.  A tile's stage is requested anew as soon as its codes are in registers, so two tiles are on their way while a third is
-// worked on.  F32 queries and the weights beside them are three terms of bf16, f16 two, each a product of its own.  On whole
-// numbers the queries are three digits to the base 256, and K Q^T is on the i8 instructions: the codes as they are, sums exact.
+// worked on.  F32 queries and the weights beside them are three terms of bf16, f16 two, each a product of its own; bf16 queries are
+// one, but their weights two (one term of 8 bits would be the largest error of all; the second costs 0.6 us of 61 on 2 requests of
+// 131000 keys).  On whole numbers the queries are three digits to the base 256, and K Q^T is on the i8 instructions: the codes as
+// they are, sums exact.
 //
 // Wavefronts of a workgroup have parts of its keys and add up in LDS; long contexts are shared out over workgroups by the lengths
 // that the device holds, and a second kernel joins the parts.
 //
-// Bound by the cache's bytes where keys are many: 64 requests of 100 to 4000 keys, 8 heads of 128 in whole numbers, 76 us, 3.8 TB/s;
+// Bound by the cache's bytes where keys are many: 64 requests of 100 to 4000 keys, 8 heads of 128 in whole numbers, 68 us, 4.2 TB/s;
 // 2 requests of 99001 to 131000 keys, 4 heads of 128 e4m3, 52 us (4.6 TB/s) and 8 for the join.  The rest is the start: lengths, block
 // table, then the first tiles, 4 to 7 us one after the other, so that one request of 700 keys takes 13 us, of which a launch is 4.
-// Where a wavefront has few tiles (16 requests of 3 to 7 new tokens: 42 us, and 9 for the join) they are most of the time.
+// Where a wavefront has few tiles (16 requests of 3 to 7 new tokens: 42 us with the join's 9) they are most of the time.
 #include "quantized_launch.h"
 
 #include <hip/hip_runtime.h>
@@ -287,11 +289,11 @@ constexpr int wave_lds(int dim, int rows) {
     return ((ring > sums ? ring : sums) + 1023) / 1024 * 1024;
 }
 
-// kDim: the head's values, rounded up to a size that is here (the rest are zeros).  kTerms: 1 bf16, 2 f16, 3 f32 queries.  kQ:
+// kDim: the head's values, rounded up to a size that is here (the rest are zeros).  kTerms: of the queries, 1 bf16, 2 f16, 3 f32.  kQ:
 // sixteens of rows.
 template <int kDim, bool kE4m3, int kTerms, int kQ>
 __global__ __launch_bounds__(64 * most_waves(kDim)) void quantized_attention_kernel(QuantizedAttentionArgs a, Plan plan, float* part_out, Part* parts) {
-    constexpr int kSteps = kDim / 32, kVec = kDim / 16, kWords = kVec / 4, kPieces = kDim / 16, kRows = 16 * kQ;
+    constexpr int kWeights = kTerms > 2 ? kTerms : 2, kSteps = kDim / 32, kVec = kDim / 16, kWords = kVec / 4, kPieces = kDim / 16, kRows = 16 * kQ;
     constexpr int kLoads = kTile * kPieces / 64, kRowsALoad = 64 / kPieces;  // of keys, and of values: 1 KiB each
     typedef typename Bytes<kVec>::type Value;
     constexpr int kStages = stages_of(kDim), kWaveLds = wave_lds(kDim, kRows);
@@ -368,6 +370,9 @@ __global__ __launch_bounds__(64 * most_waves(kDim)) void quantized_attention_ker
     // Where a lane's bytes of load i lie behind its first row's, where the rows of a load are in one block; whether there are any (the
     // ring holds zeros for what is past a head's end).
     const bool in_one = a.block_size.by % kRowsALoad == 0 && a.cache.slot_stride < (1u << 20);
+    // (Loads that turn lanes off cost: 64 requests of 100 to 4000 keys take 75 us instead of 68 with them, so whole heads do without.
+    // Every load has rows' first pieces, so that none is left out and the waits below count them all.)
+    const bool whole_heads = head_dim == kDim;
     uint32_t lane_at[kLoads];
     bool has[kLoads];
 #pragma unroll
@@ -395,7 +400,10 @@ __global__ __launch_bounds__(64 * most_waves(kDim)) void quantized_attention_ker
                 const uint32_t key = first_key + i * kRowsALoad, column_of = divide(key, a.block_size);
                 const uint32_t block = __builtin_amdgcn_readlane(window, column_of - window_at);
                 const uint32_t place = block * a.cache.block_stride + (key - column_of * a.block_size.by) * a.cache.slot_stride + head_at;
-                if (has[i]) {
+                if (whole_heads) {
+                    load_to_lds(to + i * 1024, a.cache.keys + place, lane_at[i]);
+                    load_to_lds(to + kTile * kDim + i * 1024, a.cache.values + place, lane_at[i]);
+                } else if (has[i]) {
                     load_to_lds(to + i * 1024, a.cache.keys + place, lane_at[i]);
                     load_to_lds(to + kTile * kDim + i * 1024, a.cache.values + place, lane_at[i]);
                 }
@@ -407,7 +415,10 @@ __global__ __launch_bounds__(64 * most_waves(kDim)) void quantized_attention_ker
                 const uint32_t key = first_key + row, column_of = divide(key, a.block_size);
                 const uint32_t block = static_cast<uint32_t>(__shfl(static_cast<int>(window), static_cast<int>(column_of - window_at)));
                 const uint32_t place = block * a.cache.block_stride + (key - column_of * a.block_size.by) * a.cache.slot_stride + head_at + piece;
-                if (has[i]) {
+                if (whole_heads) {
+                    load_to_lds(to + i * 1024, a.cache.keys + place);
+                    load_to_lds(to + kTile * kDim + i * 1024, a.cache.values + place);
+                } else if (has[i]) {
                     load_to_lds(to + i * 1024, a.cache.keys + place);
                     load_to_lds(to + kTile * kDim + i * 1024, a.cache.values + place);
                 }
@@ -571,7 +582,7 @@ __global__ __launch_bounds__(64 * most_waves(kDim)) void quantized_attention_ker
             }
         }
         uint32_t seen[kQ];
-        bf16x8 weight[kQ][kTerms];
+        bf16x8 weight[kQ][kWeights];
 #pragma unroll
         for (int qt = 0; qt < kQ; ++qt) {
             float x[8], by[8];
@@ -622,7 +633,7 @@ __global__ __launch_bounds__(64 * most_waves(kDim)) void quantized_attention_ker
                 sum[qt] += p;
                 float rest = p * by[j];
 #pragma unroll
-                for (int term = 0; term < kTerms; ++term) {
+                for (int term = 0; term < kWeights; ++term) {
                     weight[qt][term][j] = static_cast<__bf16>(rest);
                     rest -= static_cast<float>(weight[qt][term][j]);
                 }
@@ -685,7 +696,7 @@ __global__ __launch_bounds__(64 * most_waves(kDim)) void quantized_attention_ker
             for (int i = 0; i < 4; ++i) {
                 const bf16x8 v = __builtin_bit_cast(bf16x8, u32x4{operand[i][0], operand[i][1], operand[i][2], operand[i][3]});
 #pragma unroll
-                for (int term = kTerms - 1; term >= 0; --term) {
+                for (int term = kWeights - 1; term >= 0; --term) {
 #pragma unroll
                     for (int qt = 0; qt < kQ; ++qt) out[qt][4 * w + i] = product(v, weight[qt][term], out[qt][4 * w + i]);
                 }
@@ -825,9 +836,22 @@ Shape shape_of(const QuantizedAttentionArgs& a, int compute_units) {
     s.plan.row_tiles = static_cast<uint32_t>(most_row_tiles);
     s.plan.least = 8;
     s.plan.target = 0;
-    const uint64_t resident = 2 * static_cast<uint64_t>(compute_units < 512 ? compute_units : 512);
-    if (a.requests <= kMostShared && (base < resident || tiles > 160) && tiles > 32) s.plan.target = static_cast<uint32_t>(resident);
-    else if (base < static_cast<uint64_t>(compute_units)) s.waves = most_waves(s.dim);
+    // Contexts are shared out where row tiles would leave units idle, or where long ones of few requests would be waited for: 64
+    // requests of 100 to 8000 keys and 8 heads take 132 us instead of 156, of 100 to 3000 keys 66 instead of 65; 200 requests of 500 to
+    // 8000 keys 395 instead of 366.  With few requests and heads a unit has two workgroups of four wavefronts (2 requests of 131000 keys
+    // and 4 heads: 61 us, 65 of twice as many, 64 of pairs of wavefronts); with more of them workgroups of unequal work even out when
+    // there are twice as many (30 requests of 3000 to 9000 keys and 8 heads: 91 us instead of 105), and where each would have a few
+    // tiles a wavefront, wavefronts in pairs (16 requests of 300 to 9000 keys and 4 heads: 43 us instead of 49 in fours and 49 with
+    // two workgroups of them a unit; but 64 requests of 1000 keys and 1 head 17 us instead of 15).  Of heads of 256 a unit's LDS holds four wavefronts: as two pairs (2 requests of 60000 to 90000
+    // keys 78 us instead of 84).
+    const uint64_t units = static_cast<uint64_t>(compute_units < 256 ? compute_units : 256), pairs = static_cast<uint64_t>(a.requests) * a.cache.kv_heads;
+    if (a.requests <= kMostShared && tiles > 32 && (base < 2 * units || (base < 4 * units && tiles > 160))) {
+        const bool many = pairs >= units / 8 && base * tiles >= 16 * units;
+        s.plan.target = static_cast<uint32_t>(many ? 4 * units : 2 * units);
+        if (s.dim == 256 || (many && pairs < units / 2)) s.waves = 2;
+    } else if (base < units) {
+        s.waves = most_waves(s.dim);
+    }
     s.groups = s.plan.target == 0 ? a.requests * most_row_tiles * a.cache.kv_heads : base + s.plan.target;
     s.plan.slots = s.plan.target == 0 ? 0 : static_cast<uint32_t>(s.groups);
     const uint64_t together = 8 * most_row_tiles * a.cache.kv_heads;

@@ -559,13 +559,13 @@ afhip_status afhip_launch_rotated_store(void *stream, const afhip_head_rotation 
  * row whose seen scores are all minus infinity, or whose query holds an infinity or no number, is no numbers.
  * query and out: F32, F16 or BF16, both of `type`, [tokens][heads][head_dim], strides in elements (multiples of 4 for F32, of 8
  * otherwise; 16-byte aligned).  Codes are multiplied as bf16, which holds each of them; queries, and the weights beside the values,
- * as three terms of bf16 for F32 (24 bits), two for F16 (16 bits) and one for BF16; on an I8 cache queries are three digits of a
+ * as three terms of bf16 for F32 (24 bits), two for F16 (16 bits), and for BF16 one and two; on an I8 cache queries are three digits of a
  * whole number instead, 2^-22 of their row's largest value, and their products with the codes are exact.  Sums are f32.
  * max_query_len and max_key_len bound what the batch holds (new tokens; context plus new tokens) and choose the launch's
  * shape; tokens past the first and keys past the second are left out.  slopes f32 [heads], optional (.ptr == 0).  heads is a multiple of
  * kv_heads (else AFHIP_ERR_INVALID_STATE); requests <= 65535, max_key_len * block_size < 2^32, max_query_len * heads < 2^31 and a grid
  * of fewer than 2^32 threads (256 or 512 for every 16 or 32 of a request's max_query_len * heads / kv_heads rows and every key head,
- * and twice the units' number of such workgroups where keys are shared out), else AFHIP_ERR_OP_UNSUPPORTED.
+ * and up to four times the units' number of workgroups where keys are shared out), else AFHIP_ERR_OP_UNSUPPORTED.
  * `workspace` (256-byte aligned, afhip_quantized_attention_workspace_bytes) holds the parts of rows whose keys are shared out over
  * workgroups; less than asked for is refused (AFHIP_ERR_INVALID_STATE). */
 typedef struct afhip_quantized_attention {

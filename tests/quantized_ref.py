@@ -61,12 +61,12 @@ def attend(q, keys, values, key_scales, value_scales, scale, starts, context, ta
     `digits`: queries are whole numbers of 22 bits beside their row's largest value, at least 2^21: half a unit is 2^-22 of that.
     A score is off by its f32 sums (dim additions of exact products, 2^-23 each of the absolute ones), three roundings, and with a cap or
     slopes by tanh's 2^-20 of the cap and one rounding of the bias; a weight by exp's argument, exp2 (2^-22) and by its terms: half a
-    step of 8, 16 or 24 bits; the sum over keys by one rounding of 2^-23 a tile of 32 keys, 32 inside it and two a join; the
+    step of 16 (f16, bf16) or 24 bits; the sum over keys by one rounding of 2^-23 a tile of 32 keys, 32 inside it and two a join; the
     result by half a step of its own type."""
     tokens, heads, dim = q.shape
     group = heads // keys.shape[2]
     out, off = np.full(q.shape, np.nan), np.zeros(q.shape)
-    kept = {"f32": 2.0 ** -23, "f16": 2.0 ** -15, "bf16": 2.0 ** -8}[kind]
+    kept = {"f32": 2.0 ** -23, "f16": 2.0 ** -15, "bf16": 2.0 ** -15}[kind]
     for r in range(len(context)):
         n, c = min(int(starts[r + 1] - starts[r]), most_query), max(int(context[r]), 0)
         total = min(c + n, table.shape[1] * block, most_keys)
