@@ -136,7 +136,8 @@ afhip_status attention_args(const afhip_quantized_attention* t, QuantizedAttenti
         t->softcap < 0.0f || isinf(t->softcap))
         return AFHIP_ERR_INVALID_STATE;
     size_t most, rows;
-    if (t->requests > 65535 || !checked_mul(t->max_key_len, t->cache.block_size, &most) || most >= (size_t{1} << 32) ||
+    // (a tile's keys are divided by the block size as far as 31 behind the last one)
+    if (t->requests > 65535 || !checked_mul(t->max_key_len + 32, t->cache.block_size, &most) || most >= (size_t{1} << 32) ||
         !checked_mul(t->max_query_len, t->heads, &rows) || rows > kInt32Max)
         return AFHIP_ERR_OP_UNSUPPORTED;
     *empty = t->requests == 0 || t->tokens == 0 || t->max_query_len == 0;

@@ -320,7 +320,7 @@ __global__ __launch_bounds__(64 * most_waves(kDim)) void quantized_attention_ker
     const int keys = static_cast<int>(min(static_cast<unsigned long long>(last_position) + 1, most));  // seen by none from here on
     const uint32_t limit = a.window != 0 ? a.window : 0x80000000u;                                      // a key is seen where position - key is below
     int tile = share.first_tile + static_cast<int>(split * share.each);
-    int end = min(min(tile + static_cast<int>(share.each), share.first_tile + share.tiles), (keys + kTile - 1) / kTile);
+    int end = min(min(tile + static_cast<int>(share.each), share.first_tile + share.tiles), static_cast<int>((static_cast<uint32_t>(keys) + kTile - 1) / kTile));
     if (a.window != 0 && first_position >= static_cast<int>(a.window)) tile = max(tile, (first_position - static_cast<int>(a.window) + 1) / kTile);
     if (end > tile) {
         const int each = (end - tile + waves - 1) / waves;

@@ -563,7 +563,7 @@ afhip_status afhip_launch_rotated_store(void *stream, const afhip_head_rotation 
  * whole number instead, 2^-22 of their row's largest value, and their products with the codes are exact.  Sums are f32.
  * max_query_len and max_key_len bound what the batch holds (new tokens; context plus new tokens) and choose the launch's
  * shape; tokens past the first and keys past the second are left out.  slopes f32 [heads], optional (.ptr == 0).  heads is a multiple of
- * kv_heads (else AFHIP_ERR_INVALID_STATE); requests <= 65535, max_key_len * block_size < 2^32, max_query_len * heads < 2^31 and a grid
+ * kv_heads (else AFHIP_ERR_INVALID_STATE); requests <= 65535, (max_key_len + 32) * block_size < 2^32, max_query_len * heads < 2^31 and a grid
  * of fewer than 2^32 threads (256 or 512 for every 16 or 32 of a request's max_query_len * heads / kv_heads rows and every key head,
  * and up to four times the units' number of workgroups where keys are shared out), else AFHIP_ERR_OP_UNSUPPORTED.
  * `workspace` (256-byte aligned, afhip_quantized_attention_workspace_bytes) holds the parts of rows whose keys are shared out over

@@ -96,6 +96,17 @@ def test_greedy():
 
 
 @pytest.mark.parametrize("vocab", [300, 30000])
+def test_far_temperatures(vocab):
+    """Where all tokens weigh the same, whatever their logits, and where only the largest weighs."""
+    rng = np.random.default_rng(7)
+    logits = some_logits(rng, 8, vocab, "f32", 3.0)
+    t = [np.inf, 1e30, 1e-30, 1e-45, 3e38, np.inf, 1e30, 1e6]
+    check(logits, rng.random(8), t=t)
+    check(logits, rng.random(8), t=t, k=[0, 100, 5, 0, 7000, 20, 1, 290])
+    check(logits, rng.random(8), t=t, p=[0.9, 0.5, 0.9, 0.1, 0.99, 0.01, 0.9, 0.5], m=[0.0, 0.1, 0.5, 1.0, 0.2, 0.0, 1.0, 0.9])
+
+
+@pytest.mark.parametrize("vocab", [300, 30000])
 def test_numbers_that_are_none(vocab):
     rng = np.random.default_rng(2)
     x = rng.standard_normal((8, vocab))

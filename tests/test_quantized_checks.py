@@ -128,7 +128,7 @@ def test_attention():
                    {"type": _lib.TYPE_F16, "query_token_stride": 260}):
         refused(_lib.InvalidHipState, attend, attention(**change))
     refused(_lib.UnsupportedTensorType, attend, attention(type=_lib.TYPE_I8))
-    for change in ({"max_key_len": 1 << 28}, {"requests": 65536}, {"max_query_len": 1 << 30}):
+    for change in ({"max_key_len": 1 << 28}, {"max_key_len": (1 << 28) - 32}, {"requests": 65536}, {"max_query_len": 1 << 30}):
         refused(_lib.HipOpUnsupported, attend, attention(**change))
     huge = Buffer(0x1000, 1 << 46)
     refused(_lib.HipOpUnsupported, attend, attention(cache=a_cache(kv_heads=64, block_stride=1 << 16, slot_stride=1 << 12, scale_block_stride=1 << 10, scale_slot_stride=64),
