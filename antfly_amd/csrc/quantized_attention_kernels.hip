@@ -23,9 +23,9 @@
 // that the device holds, and a second kernel joins the parts.
 //
 // Bound by the cache's bytes where keys are many: 64 requests of 100 to 4000 keys, 8 heads of 128 in whole numbers, 68 us, 4.2 TB/s;
-// 2 requests of 99001 to 131000 keys, 4 heads of 128 e4m3, 52 us (4.6 TB/s) and 8 for the join.  The rest is the start: lengths, block
+// 2 requests of 99001 to 131000 keys, 4 heads of 128 e4m3, 52 us (4.6 TB/s) and 6 for the join.  The rest is the start: lengths, block
 // table, then the first tiles, 4 to 7 us one after the other, so that one request of 700 keys takes 13 us, of which a launch is 4.
-// Where a wavefront has few tiles (16 requests of 3 to 7 new tokens: 42 us with the join's 9) they are most of the time.
+// Where a wavefront has few tiles (16 requests of 3 to 7 new tokens: 38 us with the join's 6) they are most of the time.
 #include "quantized_launch.h"
 
 #include <hip/hip_runtime.h>
@@ -750,8 +750,11 @@ __global__ __launch_bounds__(64 * most_waves(kDim)) void quantized_attention_ker
     }
 }
 
-// A workgroup has a row, all its parts: their weights first, then every group of lanes has parts in turn, a lane four values.
+// Of a few parts a wavefront has a row, of more a workgroup: their weights first, then every group of lanes has parts in turn, a lane
+// four values.  The first parts' sums are asked for before their weights are known: one way to memory instead of two (64 parts of 56
+// rows 5.5 us instead of 7.3; 16 parts or so of 16 x 140 rows 5.6 us by wavefronts, 11.2 by workgroups).
 constexpr uint32_t kMostParts = 1100;  // of a request: plan.target is 1024 at most
+constexpr uint32_t kFewParts = 32;
 __global__ __launch_bounds__(256) void join_quantized_parts_kernel(QuantizedAttentionArgs a, Plan plan, int rows_a_tile, const float* part_out, const Part* parts) {
     __shared__ float by[kMostParts];
     __shared__ float numbers[8];
@@ -763,10 +766,60 @@ __global__ __launch_bounds__(256) void join_quantized_parts_kernel(QuantizedAtte
     const uint32_t tid = threadIdx.x, rows = static_cast<uint32_t>(share.tokens) * a.group, splits = min(share.splits, kMostParts);
     // (starts that fall, which no batch has, could count rows twice and ask for more parts than there is room for)
     if (share.first_slot + static_cast<uint64_t>(share.row_tiles) * splits * heads > plan.slots) return;
+    const uint32_t lane = tid % lanes;
+    constexpr uint32_t kAhead = 8;
+    f32x4 ahead[kAhead], x;
+    const auto take = [&](f32x4 y, float w) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(w == 0.0f ? 0.0f : y[j], w, x[j]);
+    };
+    const auto put = [&](uint32_t kv_head, uint32_t row, float all, float highest) {
+        store4(a, static_cast<size_t>(share.begin) + row / a.group, kv_head * a.group + row % a.group, static_cast<int>(4 * lane), x, all, highest != -__builtin_inff());
+    };
+    const auto first_part = [&](uint32_t kv_head, uint32_t row) {
+        return (share.first_slot + static_cast<size_t>(kv_head) * share.row_tiles + row / rows_a_tile) * rows_a_tile + row % rows_a_tile;
+    };
+    const size_t apart = static_cast<size_t>(heads) * share.row_tiles * rows_a_tile;
+    if (splits <= kFewParts) {
+        const uint32_t at = tid & 63, first = at / lanes, in_wave = 64 / lanes;
+        for (uint32_t number = blockIdx.x * 4 + (tid >> 6); number < rows * heads; number += gridDim.x * 4) {
+            const uint32_t kv_head = number / rows, row = number % rows;
+            const size_t part = first_part(kv_head, row);
+            const auto sums_at = [&](uint32_t s) {
+                return lane < fours && s < splits ? *reinterpret_cast<const f32x4*>(part_out + (part + s * apart) * a.cache.head_dim + 4 * lane) : f32x4{0, 0, 0, 0};
+            };
+            const Part own = at < splits ? parts[part + at * apart] : Part{-__builtin_inff(), 0.0f};
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead; ++i) ahead[i] = sums_at(first + i * in_wave);
+            float highest = own.most;
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) highest = fmaxf(highest, __shfl_xor(highest, d));
+            const float weight = own.most == -__builtin_inff() ? 0.0f : exp2_between(own.most, highest);
+            float all = own.sum * weight;  // (a part that saw nothing has a sum of zero)
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
+            x = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead; ++i) take(ahead[i], __shfl(weight, static_cast<int>(first + i * in_wave)));  // (below 64; zero from `splits` on)
+            for (uint32_t s = first + kAhead * in_wave; s - first < splits; s += in_wave) take(sums_at(s), __shfl(weight, static_cast<int>(s)));
+            for (uint32_t d = lanes; d < 64; d *= 2) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float v = x[j];
+                    x[j] = v + __shfl_xor(v, static_cast<int>(d));
+                }
+            }
+            if (at < fours) put(kv_head, row, all, highest);
+        }
+        return;
+    }
     for (uint32_t number = blockIdx.x; number < rows * heads; number += gridDim.x) {
-        const uint32_t kv_head = number / rows, row = number % rows, row_tile = row / rows_a_tile, r = row % rows_a_tile;
-        const size_t first_slot = share.first_slot + static_cast<size_t>(kv_head) * share.row_tiles + row_tile;
-        const auto part_at = [&](uint32_t s) { return (first_slot + static_cast<size_t>(s) * heads * share.row_tiles) * rows_a_tile + r; };
+        const uint32_t kv_head = number / rows, row = number % rows, first = tid / lanes;
+        const size_t part = first_part(kv_head, row);
+        const auto part_at = [&](uint32_t s) { return part + s * apart; };
+        const auto sums_at = [&](uint32_t s) { return *reinterpret_cast<const f32x4*>(part_out + part_at(s) * a.cache.head_dim + 4 * lane); };
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) ahead[i] = lane < fours && first + i * groups < splits ? sums_at(first + i * groups) : f32x4{0, 0, 0, 0};
         constexpr uint32_t kOwn = (kMostParts + 255) / 256;
         Part own[kOwn];
         float highest = -__builtin_inff(), all = 0.0f;
@@ -790,22 +843,18 @@ __global__ __launch_bounds__(256) void join_quantized_parts_kernel(QuantizedAtte
         if ((tid & 63) == 0) numbers[4 + (tid >> 6)] = all;
         __syncthreads();
         all = (numbers[4] + numbers[5]) + (numbers[6] + numbers[7]);
-        const uint32_t lane = tid % lanes, first = tid / lanes;
-        f32x4 x{0, 0, 0, 0};
+        x = f32x4{0, 0, 0, 0};
         if (lane < fours) {
-#pragma unroll 4
-            for (uint32_t s = first; s < splits; s += groups) {
-                const f32x4 y = *reinterpret_cast<const f32x4*>(part_out + part_at(s) * a.cache.head_dim + 4 * lane);
-                const float w = by[s];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(w == 0.0f ? 0.0f : y[j], w, x[j]);
-            }
+            for (uint32_t i = 0; i < kAhead; ++i) take(ahead[i], first + i * groups < splits ? by[first + i * groups] : 0.0f);
+#pragma unroll 4
+            for (uint32_t s = first + kAhead * groups; s < splits; s += groups) take(sums_at(s), by[s]);
         }
         sums[tid] = x;
         __syncthreads();
         if (tid < fours) {
             for (uint32_t g = 1; g < groups; ++g) x += sums[g * lanes + tid];
-            store4(a, static_cast<size_t>(share.begin) + row / a.group, kv_head * a.group + row % a.group, static_cast<int>(4 * tid), x, all, highest != -__builtin_inff());
+            put(kv_head, row, all, highest);
         }
         __syncthreads();
     }
@@ -838,14 +887,16 @@ Shape shape_of(const QuantizedAttentionArgs& a, int compute_units) {
     s.plan.target = 0;
     // Contexts are shared out where row tiles would leave units idle, or where long ones of few requests would be waited for: 64
     // requests of 100 to 8000 keys and 8 heads take 132 us instead of 156, of 100 to 3000 keys 66 instead of 65; 200 requests of 500 to
-    // 8000 keys 395 instead of 366.  With few requests and heads a unit has two workgroups of four wavefronts (2 requests of 131000 keys
+    // 8000 keys 395 instead of 366; 30 requests of 4000 keys 51 instead of 52, of 2500 keys 36 instead of 34; 8 requests of 4 to 8 new
+    // tokens, 500 to 1000 keys and 8 heads 20 instead of 22, 16 of 500 to 900 keys and 4 heads 11.2 instead of 10.5.  With few requests and heads a unit has two workgroups of four wavefronts (2 requests of 131000 keys
     // and 4 heads: 61 us, 65 of twice as many, 64 of pairs of wavefronts); with more of them workgroups of unequal work even out when
     // there are twice as many (30 requests of 3000 to 9000 keys and 8 heads: 91 us instead of 105), and where each would have a few
     // tiles a wavefront, wavefronts in pairs (16 requests of 300 to 9000 keys and 4 heads: 43 us instead of 49 in fours and 49 with
     // two workgroups of them a unit; but 64 requests of 1000 keys and 1 head 17 us instead of 15).  Of heads of 256 a unit's LDS holds four wavefronts: as two pairs (2 requests of 60000 to 90000
     // keys 78 us instead of 84).
     const uint64_t units = static_cast<uint64_t>(compute_units < 256 ? compute_units : 256), pairs = static_cast<uint64_t>(a.requests) * a.cache.kv_heads;
-    if (a.requests <= kMostShared && tiles > 32 && (base < 2 * units || (base < 4 * units && tiles > 160))) {
+    const uint64_t enough = base < units / 2 ? 24 : base < 2 * units ? 100 : 160;  // tiles of the longest context
+    if (a.requests <= kMostShared && base < 4 * units && tiles > enough) {
         const bool many = pairs >= units / 8 && base * tiles >= 16 * units;
         s.plan.target = static_cast<uint32_t>(many ? 4 * units : 2 * units);
         if (s.dim == 256 || (many && pairs < units / 2)) s.waves = 2;
@@ -857,6 +908,7 @@ Shape shape_of(const QuantizedAttentionArgs& a, int compute_units) {
     const uint64_t together = 8 * most_row_tiles * a.cache.kv_heads;
     s.groups = (s.groups + together - 1) / together * together;
     s.join_groups = rows * a.cache.kv_heads;
+    if (base * 16 >= s.plan.target) s.join_groups = (s.join_groups + 3) / 4;  // (mostly few parts: rows by wavefronts)
     if (s.join_groups > 4096) s.join_groups = 4096;
     return s;
 }

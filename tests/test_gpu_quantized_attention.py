@@ -98,6 +98,15 @@ def test_capped_biased_windowed(kind, stored, cap, window, bias):
         check(b, cap=cap, window=window, slopes=slopes)
 
 
+@pytest.mark.parametrize("kind,stored", [("f32", "e4m3"), ("bf16", "i8"), ("f16", "e4m3")])
+@pytest.mark.parametrize("context,new,block,heads,kv_heads,dim", [([140000], [1], 64, 2, 1, 64), ([20000], [1], 16, 2, 1, 256), ([3000, 700, 2500], [1, 2, 1], 16, 8, 8, 256),
+                                                                  ([1000 + 50 * r for r in range(16)], [3] * 16, 24, 20, 4, 96), ([3300] * 17, [1] * 17, 16, 8, 8, 32)])
+def test_shared_out(kind, stored, context, new, block, heads, kv_heads, dim):
+    """Keys over hundreds of workgroups, over tens, and wavefronts in pairs."""
+    print(f"case: shared out {kind} on {stored} context={context[:4]} new={new[:4]} heads={heads}/{kv_heads} dim={dim}", flush=True)
+    check(a_batch(np.random.default_rng(dim), context, new, block, heads, kv_heads, dim, kind, stored))
+
+
 def test_bounds_of_the_launch():
     """New tokens past max_query_len and keys past max_key_len are left out; lengths below zero count as zero; a table that is
     too short, and blocks that there are not, are not seen."""
