@@ -6,9 +6,12 @@
 //
 // A head is a group of 8, 16 or 32 lanes with eight values each: its sum of squares and its maximum are three to five exchanges of
 // registers.  A lane's eight values are four pairs of the rotation (two runs of four values), so a pair never leaves its lane.  The
-// angles of a lane's four pairs are the same for all heads of a token: it makes them once and takes several heads.
-// Bound by the bytes: 7500 tokens of 32 and 8 heads of 128, f32 in, bf16 queries out, keys and values to e4m3, 64 us, 4.1 TB/s; 4000
-// tokens of 8 heads of 128 stored and 30001 loaded, 58 us, 3.9 TB/s.  A few tokens cost a launch (one: 4.0 us).
+// angles are the same for all heads of a token: a workgroup's threads make one each, while the first heads' values are on their way,
+// and every lane keeps those of its four pairs for the heads it takes (made by each lane, 2111 tokens of 32 heads took 14.7 us
+// instead of 14.0).  Registers are kept to eight wavefronts a SIMD: 7500 tokens of 48 heads take 60 us instead of 64 with seven, the
+// 2111 14.4 instead of 14.0.
+// Bound by the bytes: 7500 tokens of 32 and 8 heads of 128, f32 in, bf16 queries out, keys and values to e4m3, 60 us, 4.3 TB/s; 4000
+// tokens of 8 heads of 128 stored and 30001 loaded, 57 us, 4.0 TB/s.  A few tokens cost a launch (one: 3.7 us).
 #include "quantized_launch.h"
 
 #include <hip/hip_runtime.h>
@@ -130,28 +133,52 @@ __device__ __forceinline__ Codes quantize(f32x4 a, f32x4 b, bool e4m3) {
 // Items of a token: its queries' heads, its keys', its values'.  A workgroup has tokens_a_group tokens and groups_a_token groups of
 // lanes for each, which take the items of its chunk (blockIdx.y) in turn.
 template <int kType, int kLanes>
-__global__ __launch_bounds__(kThreads) void heads_kernel(HeadsArgs a) {
-    const uint32_t lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-    const uint32_t token = blockIdx.x * a.tokens_a_group + group / a.groups_a_token;
-    if (group >= a.tokens_a_group * a.groups_a_token || token >= a.tokens) return;
+__global__ __launch_bounds__(kThreads, 8) void heads_kernel(HeadsArgs a) {
+    __shared__ float2 turned[kThreads * 4];  // sines and cosines of [token][pair]: 32, 16 or 8 tokens of up to 32, 64 or 128
+    const uint32_t lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, own_token = group / a.groups_a_token;
+    const uint32_t token = blockIdx.x * a.tokens_a_group + own_token;
+    const bool idle = group >= a.tokens_a_group * a.groups_a_token || token >= a.tokens;
     const uint32_t items = a.heads + a.kv_heads + a.value_heads;
     const uint32_t last = min(items, (blockIdx.y + 1) * a.chunk);
     // the lane's two runs of four values, and its four pairs
     const uint32_t rotary = a.rotary_dim, first_pair = 4 * lane;
     const bool works = 8 * lane < a.head_dim, turns = 8 * lane < rotary;
     const uint32_t d0 = turns && !a.interleaved ? 4 * lane : 8 * lane, d1 = turns && !a.interleaved ? rotary / 2 + 4 * lane : 8 * lane + 4;
-    float sine[4], cosine[4];
-    if (turns && a.positions != nullptr) {
-        int position[4];
-        const Four frequency = *reinterpret_cast<const Four*>(a.frequencies + first_pair);
-        if (a.one_axis) {
-            position[0] = position[1] = position[2] = position[3] = a.positions[token];
-        } else {
-#pragma unroll
-            for (int p = 0; p < 4; ++p) position[p] = a.positions[static_cast<size_t>(a.pair_axes[first_pair + p]) * a.tokens + token];
+    // a head's values, asked for before the angles are formed
+    f32x4 next_x{0, 0, 0, 0}, next_y{0, 0, 0, 0};
+    const auto request = [&](uint32_t item) {
+        const bool is_query = item < a.heads, is_value = item >= a.heads + a.kv_heads;
+        const uint32_t head = is_query ? item : is_value ? item - a.heads - a.kv_heads : item - a.heads;
+        const HeadRows& from = is_query ? a.query : is_value ? a.value : a.key;
+        const size_t at = static_cast<size_t>(token) * from.token_stride + static_cast<size_t>(head) * from.head_stride;
+        if (works && item < last) {
+            next_x = load4<kType>(from.data, at + d0);
+            next_y = load4<kType>(from.data, at + d1);
         }
+    };
+    const uint32_t first_item = blockIdx.y * a.chunk + group % a.groups_a_token;
+    if (!idle) request(first_item);
+    if (a.positions != nullptr) {
+        const uint32_t pairs = rotary / 2;
+        for (uint32_t i = threadIdx.x; i < a.tokens_a_group * pairs; i += kThreads) {
+            const uint32_t of = a.tokens_a_group == 1 ? 0 : i / pairs, pair = i - of * pairs, its = blockIdx.x * a.tokens_a_group + of;
+            if (its >= a.tokens) break;
+            const int position = a.positions[a.one_axis ? its : static_cast<size_t>(a.pair_axes[pair]) * a.tokens + its];
+            float2 both;
+            sine_cosine(position, a.frequencies[pair], &both.x, &both.y);
+            turned[i] = both;
+        }
+        __syncthreads();
+    }
+    if (idle) return;
+    float sine[4], cosine[4];
+    if (turns) {
 #pragma unroll
-        for (int p = 0; p < 4; ++p) sine_cosine(position[p], frequency.v[p], &sine[p], &cosine[p]);
+        for (int p = 0; p < 4; ++p) {
+            const float2 both = turned[own_token * (rotary / 2) + first_pair + p];
+            sine[p] = both.x;
+            cosine[p] = both.y;
+        }
     }
     const float inverse_dim = 1.0f / static_cast<float>(a.head_dim);
     const int target = static_cast<int>(a.target);
@@ -163,16 +190,11 @@ __global__ __launch_bounds__(kThreads) void heads_kernel(HeadsArgs a) {
         inside = slot - block * block_size;
         there = block < (target >= static_cast<int>(HeadTarget::i8_cache) ? a.quantized.blocks : a.cache.blocks);
     }
-    for (uint32_t item = blockIdx.y * a.chunk + group % a.groups_a_token; item < last; item += a.groups_a_token) {
+    for (uint32_t item = first_item; item < last; item += a.groups_a_token) {
         const bool is_query = item < a.heads, is_value = item >= a.heads + a.kv_heads;
         const uint32_t head = is_query ? item : is_value ? item - a.heads - a.kv_heads : item - a.heads;
-        const HeadRows& from = is_query ? a.query : is_value ? a.value : a.key;
-        const size_t at = static_cast<size_t>(token) * from.token_stride + static_cast<size_t>(head) * from.head_stride;
-        f32x4 x{0, 0, 0, 0}, y{0, 0, 0, 0};
-        if (works) {
-            x = load4<kType>(from.data, at + d0);
-            y = load4<kType>(from.data, at + d1);
-        }
+        f32x4 x = next_x, y = next_y;
+        request(item + a.groups_a_token);
         if (!is_value) {
             const float* weight = is_query ? a.query_weight : a.key_weight;
             if (weight != nullptr) {
