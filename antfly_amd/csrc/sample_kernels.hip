@@ -26,12 +26,14 @@
 
 #include <hip/hip_runtime.h>
 
+#include "sample_search.h"
+
 namespace afhip {
 
 namespace {
 
-constexpr int kThreads = 512, kWaves = kThreads / 64;
-constexpr uint32_t kBins = 1024, kListed = 4096;
+constexpr int kThreads = kSampleThreads, kWaves = kThreads / 64;
+constexpr uint32_t kBins = kSampleBins, kListed = 4096;
 constexpr uint32_t kMostParts = 32, kGroups = kThreads / 4;  // parts of a row, and groups of threads of a part with a largest logit of their own
 constexpr double kLog2e = 1.4426950408889634;
 typedef unsigned long long u64;
@@ -145,17 +147,6 @@ __device__ __forceinline__ void block_before(uint32_t count, u64 sum, Shared& s,
     *count_before = c;
     *sum_before = m;
 }
-
-// What passes: the count, or the sum in 64-bit floating point, up to and with a token.
-struct Target {
-    uint32_t count;   // at least so many tokens, where not zero
-    double sum;       // otherwise: at least, or more than, this sum
-    bool more;
-    __device__ __forceinline__ bool passed(uint32_t c, u64 m) const {
-        if (count != 0) return c >= count;
-        return more ? static_cast<double>(m) > sum : static_cast<double>(m) >= sum;
-    }
-};
 
 // Tokens [begin, end) of a row (begin a multiple of eight) by f(values, first), runs of four or eight, a thread's own in rising
 // order; no numbers are minus infinity, and so is what fills up the last run.
@@ -426,20 +417,6 @@ __device__ __forceinline__ void scan_bins(Shared& s, uint32_t* all_count, u64* a
         sum_before += sums[j];
     }
     __syncthreads();
-}
-
-// The bin in which the target is passed (kBins: none), behind the counts and sums of those before it.
-__device__ __forceinline__ uint32_t find_bin(const Target& target, uint32_t count0, u64 sum0, uint32_t all_count, u64 all_sum, Shared& s) {
-    if (threadIdx.x == 0) s.found_bin = kBins;
-    __syncthreads();
-    for (uint32_t b = threadIdx.x; b < kBins; b += kThreads) {
-        const uint32_t c = s.counts[b], next_c = b + 1 < kBins ? s.counts[b + 1] : all_count;
-        const u64 m = s.sums[b], next_m = b + 1 < kBins ? s.sums[b + 1] : all_sum;
-        const bool holds = target.count != 0 ? next_c > c : next_m > m, is_first = target.count != 0 ? c == 0 : m == 0;  // (counts may be left out)
-        if (holds && target.passed(count0 + next_c, sum0 + next_m) && (is_first || !target.passed(count0 + c, sum0 + m))) s.found_bin = b;
-    }
-    __syncthreads();
-    return s.found_bin;
 }
 
 // The first token of the row at which the target is passed (found_*), by the histogram's bins; false: none.  The bins are
@@ -879,7 +856,6 @@ __global__ __launch_bounds__(kThreads) void spread_kernel(SampleArgs a, Scratch 
     }
     if (wishes.has_p) {
         const uint32_t first = bin_of(wishes.nucleus(low));
-        __syncthreads();
         const uint32_t last = low == high ? first : bin_of(wishes.nucleus(high));
         of_p = wanted(first, last);
         low = before(first);
@@ -891,9 +867,7 @@ __global__ __launch_bounds__(kThreads) void spread_kernel(SampleArgs a, Scratch 
     }
     low = max(low, one);
     high = max(high, one);
-    __syncthreads();
     const uint32_t first = bin_of(wishes.draw(low));
-    __syncthreads();
     const uint32_t last = low == high ? first : bin_of(wishes.draw(high));
     if (tid == 0) {
         state->of_k = of_k;
