@@ -769,9 +769,10 @@ __global__ __launch_bounds__(256) void join_quantized_parts_kernel(QuantizedAtte
     const uint32_t lane = tid % lanes;
     constexpr uint32_t kAhead = 8;
     f32x4 ahead[kAhead], x;
+    // (also of a part without weight: a value that is no number shows whichever part has it; parts that saw nothing hold zeros)
     const auto take = [&](f32x4 y, float w) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(w == 0.0f ? 0.0f : y[j], w, x[j]);
+        for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(y[j], w, x[j]);
     };
     const auto put = [&](uint32_t kv_head, uint32_t row, float all, float highest) {
         store4(a, static_cast<size_t>(share.begin) + row / a.group, kv_head * a.group + row % a.group, static_cast<int>(4 * lane), x, all, highest != -__builtin_inff());

@@ -1,0 +1,33 @@
+"""Values that are no numbers under weights that vanish, in attention over the 8-bit paged cache, through the C ABI."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from tests.test_gpu_quantized_attention import a_batch, attend, check  # noqa: E402
+from tests.paged_ref import to64  # noqa: E402
+
+
+@pytest.mark.parametrize("kind,stored", [("f32", "i8"), ("bf16", "e4m3"), ("f16", "e4m3")])
+@pytest.mark.parametrize("context", [500, 5000, 140000])  # by one workgroup, a few parts, hundreds of them
+def test_seen_value_without_weight(kind, stored, context):
+    """A seen value that is no number makes its rows none, however far its score lies below the others and whichever
+    workgroup has its key: scores fall by one a key, so that the key's weight is zero in f32."""
+    print(f"case: seen value without weight {kind} on {stored} context={context}", flush=True)
+    rng = np.random.default_rng(context)
+    b = a_batch(rng, [context], [2], 16, 4, 2, 64, kind, stored, garbage=False)
+    slopes = np.ones(4, np.float32)
+    check(b, slopes=slopes)
+    clean = attend(b, slopes=slopes)
+    values = b["tensors"][3]  # the scales of the values
+    for key in (3, context // 2):
+        place = (int(b["table"][0, key // 16]), key % 16, 1)
+        held = float(values[place])
+        values[place] = float("nan")
+        check(b, slopes=slopes)
+        got = attend(b, slopes=slopes)
+        assert torch.isnan(got[:, 2:]).all() and torch.equal(got[:, :2], clean[:, :2])
+        values[place] = held
+    assert np.isfinite(to64(clean)).all()
