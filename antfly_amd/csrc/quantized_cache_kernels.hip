@@ -80,12 +80,17 @@ __device__ __forceinline__ void store4(void* base, size_t element, f32x4 v, int 
     else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + element) = uint2{pack16(v[0], v[1], type == 30), pack16(v[2], v[3], type == 30)};
 }
 
-// sin and cos of position * frequency.  The turn's quarters are taken off in 64 bits (a position of 31 bits times a frequency of 24
-// has 55), what is left, at most an eighth of a turn, is good to f32's last bit.  Then the two Taylor series in quarter turns,
-// whose first terms left out are below 2e-9 and 2e-10.
+// sin and cos of position * frequency.  The product with 1 / (2 pi) is held in two 64-bit numbers (a position of 31 bits times a
+// frequency of 24 has 55, and 28 of the quotient's go with the whole turns: in one number the angle is off by 8 steps of 2^-24 at
+// positions of 2^31), so that what is left of the turn, at most an eighth, is good to f32's last bit.  Then the two Taylor series in
+// quarter turns, whose first terms left out are below 2e-9 and 2e-10.
 __device__ __forceinline__ void sine_cosine(int position, float frequency, float* sine, float* cosine) {
-    const double turns = static_cast<double>(position) * (static_cast<double>(frequency) * 0.15915494309189533577);  // 1 / (2 pi)
-    const double quarters = 4.0 * (turns - __builtin_rint(turns)), whole = __builtin_rint(quarters);
+    constexpr double kTurn = 0x1.45f306dc9c883p-3, kTurnRest = -0x1.6b01ec5417056p-57;  // 1 / (2 pi)
+    const double f = static_cast<double>(frequency), p = static_cast<double>(position);
+    const double step = f * kTurn, step_rest = __builtin_fma(f, kTurn, -step) + f * kTurnRest;
+    const double turns = p * step, turns_rest = __builtin_fma(p, step, -turns) + p * step_rest;
+    const double rest = (turns - __builtin_rint(turns)) + turns_rest;
+    const double quarters = 4.0 * (rest - __builtin_rint(rest)), whole = __builtin_rint(quarters);
     const float x = static_cast<float>(quarters - whole), z = x * x;
     const int quarter = static_cast<int>(whole);
     // (pi / 2)^n / n!

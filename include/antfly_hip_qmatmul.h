@@ -524,7 +524,8 @@ afhip_status afhip_launch_quantized_load(void *stream, const afhip_quantized_cac
  *
  * A pair is (y[p], y[p + rotary_dim / 2]), or with `interleaved` (y[2 p], y[2 p + 1]); dimensions from rotary_dim on stay.
  * position is positions[pair_axes[p]][token], int32 [axes][tokens] (time, height and width of an image's tokens, or one axis: all
- * pair_axes zero); the angle is formed and reduced in 64 bits, so that far positions keep f32's accuracy.
+ * pair_axes zero); the angle is formed and reduced in two numbers of 64 bits, so that every position keeps
+ * f32's accuracy (sine and cosine to 3 * 2^-24).
  * type: of query and key; out_type: of the arrays that are written (F32, F16 or BF16 each; sums and products in f32, one
  * rounding at the end).  head_dim a multiple of 8 up to 256, rotary_dim a multiple of 8 up to head_dim, 1 <= axes <= 16; strides
  * in elements, multiples of 4, base addresses 16-byte (f32) or 8-byte aligned (else AFHIP_ERR_INVALID_STATE; head_dim > 256:
