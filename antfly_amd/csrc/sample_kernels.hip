@@ -541,15 +541,18 @@ struct Wishes {
         has_least = least > 0.0f;
         if (!(u > 0.0f)) u = 0.0f;
     }
-    // The target of the drawn token among tokens of this sum.
+    // The target of the drawn token among tokens of this sum: more than u of it, for a u of 1 or more all of it.
     __device__ __forceinline__ Target draw(u64 kept) const {
-        return u >= 1.0f ? Target{0, static_cast<double>(kept), false} : Target{0, static_cast<double>(u) * static_cast<double>(kept), true};
+        return Target{0, u >= 1.0f ? kept : static_cast<u64>(static_cast<double>(u) * static_cast<double>(kept)) + 1};
     }
     // What a token has to weigh for min-p, as a whole number.
     __device__ __forceinline__ u64 least_sum(u64 one) const {
         return !has_least ? 0 : least >= 1.0f ? (least > 1.0f ? one + 1 : one) : static_cast<u64>(__builtin_ceil(static_cast<double>(least) * static_cast<double>(one)));
     }
-    __device__ __forceinline__ Target nucleus(u64 kept) const { return Target{0, static_cast<double>(p) * static_cast<double>(kept), false}; }
+    // At least p of this sum (nothing of it: the first token passes).
+    __device__ __forceinline__ Target nucleus(u64 kept) const {
+        return Target{0, p > 0.0f ? static_cast<u64>(__builtin_ceil(static_cast<double>(p) * static_cast<double>(kept))) : 0};
+    }
 };
 
 __device__ __forceinline__ Weights weights_of(float top, float temperature, uint32_t vocab) {
@@ -849,7 +852,7 @@ __global__ __launch_bounds__(kThreads) void spread_kernel(SampleArgs a, Scratch 
     Wanted of_k = none, of_p = none;
     u64 low = all, high = all;  // between which the sum of what is kept so far lies
     if (wishes.k != 0 && wishes.k < all_count) {
-        const uint32_t b = bin_of(Target{wishes.k, 0.0, false});
+        const uint32_t b = bin_of(Target{wishes.k, 0});
         of_k = wanted(b, b);
         low = before(b);
         high = before(b + 1);
@@ -916,7 +919,7 @@ __device__ __forceinline__ void draw_wide(const SampleArgs& a, uint32_t r, float
         if (step == 0) kept = all;
         if (step == 2) kept = max(wishes.has_least ? min(kept, weighty) : kept, one);
         if ((step == 0 && (wishes.k == 0 || wishes.k >= all_count)) || (step == 1 && !wishes.has_p)) continue;
-        const Target target = step == 0 ? Target{wishes.k, 0.0, false} : step == 1 ? wishes.nucleus(kept) : wishes.draw(kept);
+        const Target target = step == 0 ? Target{wishes.k, 0} : step == 1 ? wishes.nucleus(kept) : wishes.draw(kept);
         found = locate<kType>(row, a.vocab, histogram, all_count, all, target, weights, s, &fresh);
         if (found && step < 2) kept = s.found_sum;
         __syncthreads();
@@ -971,7 +974,7 @@ __global__ __launch_bounds__(kThreads, 4) void settle_kernel(SampleArgs a, Scrat
     };
     u64 kept = state->all;
     if (of_k.first <= of_k.last) {
-        if (find(of_k, Target{wishes.k, 0.0, false})) kept = s.found_sum;
+        if (find(of_k, Target{wishes.k, 0})) kept = s.found_sum;
         __syncthreads();
     }
     if (wishes.has_p) {

@@ -9,15 +9,12 @@ namespace afhip {
 constexpr int kSampleThreads = 512;
 constexpr uint32_t kSampleBins = 1024;
 
-// What passes: the count, or the sum in 64-bit floating point, up to and with a token.
+// What passes: the count, or the sum, up to and with a token.  Sums are compared as the whole numbers that they are: the last token of a
+// long one can weigh less than its 53rd bit.
 struct Target {
-    uint32_t count;   // at least so many tokens, where not zero
-    double sum;       // otherwise: at least, or more than, this sum
-    bool more;
-    __device__ __forceinline__ bool passed(uint32_t c, unsigned long long m) const {
-        if (count != 0) return c >= count;
-        return more ? static_cast<double>(m) > sum : static_cast<double>(m) >= sum;
-    }
+    uint32_t count;          // at least so many tokens, where not zero
+    unsigned long long sum;  // otherwise at least this sum
+    __device__ __forceinline__ bool passed(uint32_t c, unsigned long long m) const { return count != 0 ? c >= count : m >= sum; }
 };
 
 // The bin in which the target is passed (kSampleBins: none), behind the counts and sums of those before it.

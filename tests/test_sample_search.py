@@ -54,7 +54,7 @@ int main() {
         s.sums[b] = 15 * b;
     }
     pthread_barrier_init(&barrier, nullptr, kSampleThreads);
-    const Target targets[] = {{3 * 700 + 1, 0.0, false}, {0, 15.0 * 40, true}, {0, 15.0 * 40, false}, {0, 15.0 * 1023 + 1, false}, {0, 1e9, false}, {1, 0.0, false}};
+    const Target targets[] = {{3 * 700 + 1, 0}, {0, 15 * 40 + 1}, {0, 15 * 40}, {0, 15 * 1023 + 1}, {0, 1000000000}, {1, 0}};
     const uint32_t bins[] = {700, 40, 39, 1023, kSampleBins, 0};
     std::atomic<int> wrong{0};
     std::vector<std::thread> threads;
