@@ -494,7 +494,8 @@ __device__ bool locate(const void* row, uint32_t vocab, const Histogram& histogr
         const uint32_t from = high - (b << shift);
         low = max(low, from - ((1u << shift) - 1));  // (the bin's lowest key)
         high = from;
-        n = gather<kType>(row, 0, vocab, s, value_of(low), value_of(high), [](float v) { return v > -__builtin_inff(); });
+        // (by keys: the value of a highest key right below zero's compares as zero)
+        n = gather<kType>(row, 0, vocab, s, value_of(low), value_of(high), [&](float v) { return key_of(v) >= low && key_of(v) <= high && v > -__builtin_inff(); });
         if (n <= kListed) {
             sort_list(n, s);
             return Listed(n, weights, s).find(0, n, count0, sum0, target, s);

@@ -41,3 +41,16 @@ def test_last_token_of_long_sums(vocab):
         assert tokens.tolist() == [5, 5, 5, vocab - 1, vocab - 1, 5]
         assert (np.abs(probabilities - share) <= share * 2.0 ** -23).all()
     assert draw(logits, [1.0] * 6, k=[vocab - 1] * 6)[0].tolist() == [vocab - 1, 5, 5, 5, vocab - 2, vocab - 1]
+
+
+def test_zeros_beside_tiny_logits():
+    """Too many logits in one bin for a list, among them zeros of both signs and some below zero by less than a normal number: where
+    the bin is narrowed down to these, the zeros do not count among them."""
+    rng = np.random.default_rng(6)
+    x = np.concatenate([[np.nextafter(1.0, 0.0, dtype=np.float32)],  # (the narrower bins begin at this largest logit: one ends at the zeros)
+                        np.zeros(700), np.full(800, -0.0), -rng.integers(1, 1 << 20, 1500) * 2.0 ** -149, rng.uniform(-1.0, -0.5, 7000)]).astype(np.float32)
+    logits = G.to_dev(np.stack([x[rng.permutation(len(x))] for _ in range(6)]))
+    t, u = [1000.0] * 6, np.array([0.05, 0.16, 0.2, 0.25, 0.29, 0.9])
+    check(logits, u, t=t)
+    check(logits, 4 * u / 3.7, t=t, p=[0.9, 0.9, 0.8, 0.9, 0.9, 0.22])
+    check(logits, 2 * u, t=t, k=[5000] * 6)
