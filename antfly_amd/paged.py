@@ -305,7 +305,7 @@ def headRotation(query, key, out_query, out_key, positions, frequencies, query_w
         packed = _ONE_AXIS
     else:
         try:
-            packed = bytes(pair_axes)
+            packed = bytes(list(pair_axes))  # (bytes of a number alone would be that many zeros)
         except (TypeError, ValueError):
             raise _bad_number() from None
         if len(packed) != pairs:
