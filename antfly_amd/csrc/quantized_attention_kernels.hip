@@ -30,6 +30,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include "xcd_order.h"
+
 namespace afhip {
 
 namespace {
@@ -126,6 +128,7 @@ struct Plan {
     uint32_t target;     // workgroups that the tiles are shared out over, before each request's are rounded up; 0: one part a request
     uint32_t least;      // tiles of a part at least
     uint32_t slots;      // parts that there is room for
+    uint32_t chunk;      // shares that lie on one XCD side by side
 };
 
 __device__ __forceinline__ Share lengths_of(const QuantizedAttentionArgs& a, uint32_t request, int rows_a_tile) {
@@ -299,10 +302,7 @@ __global__ __launch_bounds__(64 * most_waves(kDim)) void quantized_attention_ker
     constexpr int kStages = stages_of(kDim), kWaveLds = wave_lds(kDim, kRows);
     extern __shared__ __attribute__((aligned(1024))) char lds[];
 
-    // workgroups go round the eight XCDs in turn: the row tiles of a part, which share its keys, and the key heads beside them, whose
-    // scales share its lines of memory, lie on one and share its L2
-    const uint32_t together = plan.row_tiles * a.cache.kv_heads, turn = blockIdx.x >> 3;
-    const uint32_t number = (turn / together * 8 + (blockIdx.x & 7)) * together + turn % together;
+    const uint32_t number = xcd_share(blockIdx.x, plan.chunk);
     uint32_t request;
     Share share;
     if (!find_share<false>(a, plan, kRows, number, &request, &share)) return;
@@ -906,8 +906,9 @@ Shape shape_of(const QuantizedAttentionArgs& a, int compute_units) {
     }
     s.groups = s.plan.target == 0 ? a.requests * most_row_tiles * a.cache.kv_heads : base + s.plan.target;
     s.plan.slots = s.plan.target == 0 ? 0 : static_cast<uint32_t>(s.groups);
-    const uint64_t together = 8 * most_row_tiles * a.cache.kv_heads;
-    s.groups = (s.groups + together - 1) / together * together;
+    const uint64_t chunk = xcd_chunk(most_row_tiles, a.cache.kv_heads, s.groups);
+    s.plan.chunk = static_cast<uint32_t>(chunk);
+    s.groups = (s.groups + 8 * chunk - 1) / (8 * chunk) * (8 * chunk);
     s.join_groups = rows * a.cache.kv_heads;
     if (base * 16 >= s.plan.target) s.join_groups = (s.join_groups + 3) / 4;  // (mostly few parts: rows by wavefronts)
     if (s.join_groups > 4096) s.join_groups = 4096;

@@ -31,3 +31,12 @@ def test_seen_value_without_weight(kind, stored, context):
         assert torch.isnan(got[:, 2:]).all() and torch.equal(got[:, :2], clean[:, :2])
         values[place] = held
     assert np.isfinite(to64(clean)).all()
+
+
+@pytest.mark.parametrize("kind,stored", [("f32", "i8"), ("bf16", "e4m3")])
+@pytest.mark.parametrize("context,new,heads,kv_heads,dim", [([0], [1200], 8, 8, 64), ([300, 0, 40], [5, 700, 33], 15, 5, 48), ([600], [1], 40, 40, 16),
+                                                            ([5000], [90], 8, 1, 128), ([9, 0, 700], [400, 1, 9], 16, 8, 32)])
+def test_prompts(kind, stored, context, new, heads, kv_heads, dim):
+    """Long prompts beside short ones and alone, and single tokens of many key heads: shares go round the XCDs by heads and by tiles."""
+    print(f"case: prompts {kind} on {stored} context={context} new={new} heads={heads}/{kv_heads} dim={dim}", flush=True)
+    check(a_batch(np.random.default_rng(dim), context, new, 16, heads, kv_heads, dim, kind, stored))
