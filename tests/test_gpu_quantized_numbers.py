@@ -40,3 +40,22 @@ def test_prompts(kind, stored, context, new, heads, kv_heads, dim):
     """Long prompts beside short ones and alone, and single tokens of many key heads: shares go round the XCDs by heads and by tiles."""
     print(f"case: prompts {kind} on {stored} context={context} new={new} heads={heads}/{kv_heads} dim={dim}", flush=True)
     check(a_batch(np.random.default_rng(dim), context, new, 16, heads, kv_heads, dim, kind, stored))
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("stored", ["i8", "e4m3"])
+@pytest.mark.parametrize("dim", [48, 64, 96, 128, 256])
+def test_keys_without_a_block(kind, stored, dim):
+    """Keys that the table does not name, any of a tile's 32 and between others that are seen, and a bound of the keys at any place of a
+    tile: of rows in sixteens and of more, under a window too."""
+    print(f"case: keys without a block {kind} on {stored} dim={dim}", flush=True)
+    rng = np.random.default_rng(dim)
+    for heads, new, block in ((4, 2, 1), (16, 9, 1), (16, 5, 3)):
+        b = a_batch(rng, [150, 40, 7], [new, 1, new], block, heads, 1, dim, kind, stored)
+        b["table"][rng.random(b["table"].shape) < 0.3] = -1
+        b["table"][2, :2] = b["blocks"]
+        check(b)
+        check(b, window=37)
+    b = a_batch(rng, [70], [9], 16, 16, 1, dim, kind, stored)
+    for most in range(60, 79):
+        check(b, most=(9, most))
