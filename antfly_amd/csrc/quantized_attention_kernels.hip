@@ -23,9 +23,11 @@
 // that the device holds, and a second kernel joins the parts.
 //
 // Bound by the cache's bytes where keys are many: 64 requests of 100 to 4000 keys, 8 heads of 128 in whole numbers, 68 us, 4.2 TB/s;
-// 2 requests of 99001 to 131000 keys, 4 heads of 128 e4m3, 52 us (4.6 TB/s) and 6 for the join.  The rest is the start: lengths, block
+// 2 requests of 99001 to 131000 keys, 4 heads of 128 e4m3, 53 us (4.5 TB/s) and 6 for the join.  The rest is the start: lengths, block
 // table, then the first tiles, 4 to 7 us one after the other, so that one request of 700 keys takes 13 us, of which a launch is 4.
-// Where a wavefront has few tiles (16 requests of 3 to 7 new tokens: 38 us with the join's 6) they are most of the time.
+// Where a wavefront has few tiles (16 requests of 3 to 7 new tokens: 36 us with the join's 6) they are most of the time.  Prompts are bound
+// by what is done for every tile of keys again by each 32 rows (4000 tokens, 32 heads on 8 of 128, bf16: 381 us on whole numbers, 332 on
+// e4m3; 16 of 200 tokens 80 and 70, mostly starts).
 #include "quantized_launch.h"
 
 #include <hip/hip_runtime.h>
@@ -879,6 +881,9 @@ Shape shape_of(const QuantizedAttentionArgs& a, int compute_units) {
     s.dim = a.cache.head_dim <= 64 ? 64 : a.cache.head_dim <= 128 ? 128 : 256;
     s.waves = 4;
     const uint64_t rows = static_cast<uint64_t>(a.max_query_len) * a.group;
+    // In 32 rows a key is read once for twice as many; with no more than sixteen of them half the products are idle (16 requests of 4 tokens, 4
+    // heads a key head, on 1000 keys: 16.8 us in sixteens, 20.7 in 32 rows; of 8 tokens on 500 keys 13.2 and 17.4; of 3 to 7 tokens, 5 heads, on 300
+    // to 9000 keys 43.1 and 42.7).
     s.sixteens = rows <= 16 || s.dim == 256 ? 1 : 2;
     const uint64_t tile_rows = s.rows_a_tile(), most_row_tiles = (rows + tile_rows - 1) / tile_rows;
     uint64_t row_tiles = static_cast<uint64_t>(a.tokens) * a.group / tile_rows + a.requests;  // of the batch: a request's last may be part empty
@@ -888,17 +893,21 @@ Shape shape_of(const QuantizedAttentionArgs& a, int compute_units) {
     if (a.window != 0 && keys > static_cast<uint64_t>(a.window) + a.max_query_len) keys = static_cast<uint64_t>(a.window) + a.max_query_len;
     const uint64_t tiles = keys / kTile + 2;
     s.plan.row_tiles = static_cast<uint32_t>(most_row_tiles);
-    s.plan.least = 8;
+    s.plan.least = 8;  // (of 4, 8 and 16: 1 request of 4000 keys and 8 key heads 15.0, 13.4 and 15.9 us, of 1000 12.0, 13.2 and 15.8; 8 of 6 tokens on 1000 24, 19 and 22)
     s.plan.target = 0;
-    // Contexts are shared out where row tiles would leave units idle, or where long ones of few requests would be waited for: 64
-    // requests of 100 to 8000 keys and 8 heads take 132 us instead of 156, of 100 to 3000 keys 66 instead of 65; 200 requests of 500 to
-    // 8000 keys 395 instead of 366; 30 requests of 4000 keys 51 instead of 52, of 2500 keys 36 instead of 34; 8 requests of 4 to 8 new
-    // tokens, 500 to 1000 keys and 8 heads 20 instead of 22, 16 of 500 to 900 keys and 4 heads 11.2 instead of 10.5.  With few requests and heads a unit has two workgroups of four wavefronts (2 requests of 131000 keys
-    // and 4 heads: 61 us, 65 of twice as many, 64 of pairs of wavefronts); with more of them workgroups of unequal work even out when
-    // there are twice as many (30 requests of 3000 to 9000 keys and 8 heads: 91 us instead of 105), and where each would have a few
-    // tiles a wavefront, wavefronts in pairs (16 requests of 300 to 9000 keys and 4 heads: 43 us instead of 49 in fours and 49 with
-    // two workgroups of them a unit; but 64 requests of 1000 keys and 1 head 17 us instead of 15).  Of heads of 256 a unit's LDS holds four wavefronts: as two pairs (2 requests of 60000 to 90000
-    // keys 78 us instead of 84).
+    // Contexts are shared out where row tiles would leave units idle, or where long ones of few requests would be waited for.  In one part
+    // and shared out (heads of 128, 8 key heads and 1 token where no others are named, bf16 on whole numbers): 2 requests of 700 keys
+    // 12.8 and 13.2 us, of 900 14.9 and 13.1; 16 of 500 to 900 keys and 4 key heads 14.7 and 13.5; 8 of 4 to 8 tokens on 500 to 1000 keys 21.5
+    // and 19.7; 30 of 2500 keys 38 and 43, of 4000 55 and 58; 64 of 100 to 3000 keys 52 and 51, of 100 to 8000 152 and 128; 100 of 300 to 3000
+    // keys 90 and 87, of 300 to 5500 159 and 148; 200 of 500 to 8000 keys in random order 368 and 381, in rising order 386 and 372.
+    //
+    // Workgroups that keys are shared out over, one, two, four and eight a unit: 2 requests of 131000 keys and 4 key heads
+    // 56, 61, 62 and 71 us; 30 requests of 3000 to 9000 keys 120, 101, 90 and 90; 16 of 300 to 9000 keys and 4 key heads 43, 31, 31 and 36: two with few
+    // requests and heads, four with many and enough tiles, whose unequal work evens out (16 tiles a unit; 30 requests of 4000 keys and
+    // 2 key heads 25 us with four, 30 with two; 16 of 1000 keys and 4 16.2 and 13.6).  Then, below half as many heads as units, wavefronts in
+    // pairs, since a part has few tiles for each (alone, in pairs, in fours: 16 requests of 3 to 7 tokens on 300 to 9000 keys, 4 key heads,
+    // 54, 43 and 49 us without a window; 30 of 3000 to 9000 keys, 8 key heads, 105, 98 and 89; 2 of 131000, 4 key heads, 87, 65 and 60).
+    // Of heads of 256 a unit's LDS holds four wavefronts: as two pairs (2 requests of 60000 to 90000 keys 69 us, in fours 75).
     const uint64_t units = static_cast<uint64_t>(compute_units < 256 ? compute_units : 256), pairs = static_cast<uint64_t>(a.requests) * a.cache.kv_heads;
     const uint64_t enough = base < units / 2 ? 24 : base < 2 * units ? 100 : 160;  // tiles of the longest context
     if (a.requests <= kMostShared && base < 4 * units && tiles > enough) {
@@ -914,7 +923,9 @@ Shape shape_of(const QuantizedAttentionArgs& a, int compute_units) {
     s.plan.chunk = static_cast<uint32_t>(chunk);
     s.groups = (s.groups + 8 * chunk - 1) / (8 * chunk) * (8 * chunk);
     s.join_groups = rows * a.cache.kv_heads;
-    if (base * 16 >= s.plan.target) s.join_groups = (s.join_groups + 3) / 4;  // (mostly few parts: rows by wavefronts)
+    // Mostly few parts: a workgroup has four rows, one a wavefront (8 requests of 6 tokens on 3000 keys 31.3 us, with four times the workgroups
+    // 32.3).  Of many parts a row is a workgroup's (1 request of 60000 keys 37 us, 45 with a quarter of them; of 1 key head 23 and 52).
+    if (base * 16 >= s.plan.target) s.join_groups = (s.join_groups + 3) / 4;
     if (s.join_groups > 4096) s.join_groups = 4096;
     return s;
 }

@@ -19,9 +19,9 @@
 // A list that would not hold what it has to (thousands of equal logits, mostly) leaves the row to one workgroup, which narrows the
 // bins down and counts equal ones.
 //
-// Large calls are bound by reading the logits twice and by the 64-bit weights of those that may count (256 rows of 128000 f32 logits:
-// 140 us, 131 MB of them are 26 at the rate of a copy); small ones by the three launches and the ways from workgroup to workgroup
-// (one row of 32000: 18 us).
+// Large calls are bound by reading the logits twice and by the 64-bit weights of those that may count (256 rows of 128000 f32 logits,
+// a filter set each: 144 to 148 us, 131 MB of them are 26 at the rate of a copy); small ones by the three launches and the ways from
+// workgroup to workgroup (one row of 32000 with top-k and top-p: 17 to 28 us by their values).
 #include "quantized_launch.h"
 
 #include <hip/hip_runtime.h>
@@ -584,7 +584,7 @@ __device__ __forceinline__ void put_drawn(const SampleArgs& a, uint32_t r, u64 r
 
 // What a row's workgroups tell one another within a launch goes past the caches that they do not share (relaxed atomics of the
 // device's scope): a fence for all else that they wrote would write back and drop an XCD's whole L2 (the second launch
-// over 256 rows of 128000 takes 519 us with such fences, 98 without).
+// over 256 rows of 128000 takes five times as long with such fences).
 template <typename T>
 __device__ __forceinline__ void tell(T* to, T v) { __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 template <typename T>
@@ -754,7 +754,10 @@ __global__ __launch_bounds__(kThreads) void spread_kernel(SampleArgs a, Scratch 
             cut = fmaxf(cut, value_of(found));
         }
         if (by_weight) cut = fmaxf(cut, cut_at(wishes.least >= 1.0f ? 0.0 : static_cast<double>(__builtin_log2f(wishes.least)) - 1e-4));
-        // Of tokens that lie above the cut at random, a group of many has one with 1 - exp(-their share): no more than a list holds.
+        // Of tokens that lie above the cut at random, a group of many has one with 1 - exp(-their share): no more than a list holds, with room
+        // for chance.  Lists of up to 1000 tokens or so are the shorter way, longer ones than these 0.7 let pass are not, and some of what lies
+        // between would do better without: 24 rows of 100003 with a min-p that 800 tokens pass take 31 us, that 1600 pass 44 by lists and 33 by
+        // histograms, 2200 70 and 33; 64 rows of 64000 33, 48 and 35, 80 and 36.
         const uint32_t at_cut = key_of(fmaxf(cut, -3.402823466e38f)), with[3] = {at_cut, at_cut, at_cut};
         uint32_t over_cut[3];
         reach(with, over_cut);

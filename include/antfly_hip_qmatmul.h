@@ -591,7 +591,7 @@ afhip_status afhip_launch_quantized_attention(void *stream, const afhip_quantize
  * weighs nothing; where the largest is infinite, the infinite ones weigh 1 and others nothing; where no logit is above minus
  * infinity, the token is -1 and the probability 0.  A uniform below 0 or no number counts as 0, one of 1 or more draws the last kept token that weighs
  * anything.
- * Weights are formed in 64 bits and summed as whole numbers (multiples of 2^-46 for up to 65536 tokens, 2^-45 for 131072, one bit less
+ * Weights are formed in 64 bits, compared with min_p and summed as whole numbers (multiples of 2^-46 for up to 65536 tokens, 2^-45 for 131072, one bit less
  * for every doubling), so neither the sums nor the token hang on an order of additions.
  * temperatures, top_p, min_p, uniforms f32 [rows], top_k int32 [rows]; all but uniforms optional (.ptr == 0: 1, none, none, none).
  * tokens int32 [rows], probabilities f32 [rows] (optional).  vocab from 1 to 2^24, rows up to 65535 (else AFHIP_ERR_OP_UNSUPPORTED; vocab 0:
